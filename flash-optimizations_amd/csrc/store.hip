@@ -15,6 +15,7 @@
 //      scale byte e + 127, code = e4m3_rne(n / 2^e);
 //   4. codes of kept coordinates in ascending order, MSB-first bitmap words;
 //      the record is K codes + 64 bitmap bytes + 8 scales (K + 72 bytes).
+#include "mx4_device.h"
 #include "remnant_device.h"
 #include "remnant_mi355x.h"
 
@@ -687,6 +688,81 @@ __device__ __forceinline__ void native_store_row(const RowRaw& raw, const float 
                     (u32x2*)(page + kPageRecords * kNativeDataBytes + row * kScaleBytes));
 }
 
+// 4-bit records: one row, RMS-normalised, its tail rotated, and coded by a wave
+// (lane l: coordinates 8l..8l+7, one dword of codes; four lanes share a scale).
+// The arithmetic up to the rotated BF16 row is the Native store's; the group
+// maximum is taken after the rotation, on the BF16 values' bits, where integer
+// order is float order with infinity and NaN on top.
+template <bool kBf16, bool kStream>
+__device__ __forceinline__ void mx4_store_row(const RowRaw& raw, const float (&w)[8], float eps,
+                                              int64_t slot, int64_t pos, const float* freqs,
+                                              uint8_t* pool) {
+  const int lane = wave_lane();
+  const bool rotated = freqs && lane >= kNopeDim / 8;
+  f32x4 fa = {1.f, 0.f, 1.f, 0.f}, fb = fa;
+  if (rotated) {
+    const float* f = freqs + (pos * 4) * (2 * kRopePairs) + 8 * (lane - kNopeDim / 8);
+    fa = *(const f32x4*)f;
+    fb = *(const f32x4*)(f + 4);
+  }
+  float v[8];
+  unpack_raw<kBf16>(raw, v);
+  float p = v[0] * v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    float sq = v[i] * v[i];
+    p = p + sq;
+  }
+  const float r = inv_rms(wave_tree_sum(p), eps);
+  bf16x2 nb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = v[2 * i] * r, b = v[2 * i + 1] * r;
+    a = a * w[2 * i];
+    b = b * w[2 * i + 1];
+    nb[i] = bf16_pair(a, b);
+  }
+  if (rotated) {
+    const float cs[8] = {fa[0], fa[1], fa[2], fa[3], fb[0], fb[1], fb[2], fb[3]};
+    float nf[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nf[i] = (float)nb[i / 2][i % 2];
+    rope4(nf, cs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) nb[i] = bf16_pair(nf[2 * i], nf[2 * i + 1]);
+  }
+  int top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t d = __builtin_bit_cast(uint32_t, nb[i]);
+    top = max(top, (int)max(d & 0x7fffu, (d >> 16) & 0x7fffu));
+  }
+  top = max(top, __builtin_amdgcn_update_dpp(0, top, kDppXor1, 0xf, 0xf, false));
+  top = max(top, __builtin_amdgcn_update_dpp(0, top, kDppXor2, 0xf, 0xf, false));
+  const bool special = top >= 0x7f80;  // an infinity or NaN in the group
+  const int e = mx4_exponent(bf16_to_f32((uint32_t)top));
+  const float scale = exp2i(e);
+  uint32_t code = fp4_pair<0>(0, nb[0], scale);
+  code = fp4_pair<1>(code, nb[1], scale);
+  code = fp4_pair<2>(code, nb[2], scale);
+  code = fp4_pair<3>(code, nb[3], scale);
+  code = special ? 0 : code;
+  // scale bytes of the row's four groups, one dword in the first of its 16 lanes
+  int byte = special ? kMx4NanScale : e + 127;
+  byte |= __builtin_amdgcn_update_dpp(0, byte, 0x104, 0xf, 0xf, true) << 8;   // row_shl:4
+  byte |= __builtin_amdgcn_update_dpp(0, byte, 0x108, 0xf, 0xf, true) << 16;  // row_shl:8
+  uint8_t* const rec = pool + slot * kMx4RecordBytes;
+  uint32_t* const at = (uint32_t*)(rec + 4 * lane);
+  uint32_t* const scales = (uint32_t*)(rec + kMx4CodeBytes + 4 * (lane >> 4));
+  if constexpr (kStream) {
+    __builtin_nontemporal_store(code, at);
+    if ((lane & 15) == 0) __builtin_nontemporal_store((uint32_t)byte, scales);
+  } else {
+    *at = code;
+    if ((lane & 15) == 0) *scales = (uint32_t)byte;
+  }
+}
+
 // A skipped row's data is not read: calls often skip many rows (padding), and
 // with every next row loaded ahead of its slot such calls took up to five times
 // as long (131,072 FP32 rows, a quarter stored, 28.7 us with each row waiting
@@ -710,7 +786,8 @@ __device__ __forceinline__ void native_store_row(const RowRaw& raw, const float 
 // and reductions on small ones.
 constexpr int64_t kAheadRows = 8192;
 constexpr int64_t kNativeBlocks = 256 * 16;
-template <bool kBf16, bool kOne, bool kStream>
+// kMx4: the rows become 4-bit records instead of Native ones.
+template <bool kBf16, bool kOne, bool kStream, bool kMx4>
 __global__ __launch_bounds__(256) void native_store_kernel(
     const void* __restrict__ x, int64_t stride, const float* __restrict__ weight, float eps,
     const int32_t* __restrict__ slots, const int32_t* __restrict__ position,
@@ -734,7 +811,10 @@ __global__ __launch_bounds__(256) void native_store_kernel(
     for (int i = 0; i < 8; ++i) w[i] = weight[8 * lane + i];
     if (!stored(slot, pos)) return;
     if (!ahead) next = load_raw<kBf16, kStream>(x, rec, stride, lane);
-    native_store_row<kBf16, kStream>(next, w, eps, slot, pos, freqs, pool);
+    if constexpr (kMx4)
+      mx4_store_row<kBf16, kStream>(next, w, eps, slot, pos, freqs, pool);
+    else
+      native_store_row<kBf16, kStream>(next, w, eps, slot, pos, freqs, pool);
     return;
   }
 #pragma unroll
@@ -756,8 +836,12 @@ __global__ __launch_bounds__(256) void native_store_kernel(
       const RowRaw raw = next;
       todo &= todo - 1;
       if (todo != 0) load_first();
-      native_store_row<kBf16, kStream>(raw, w, eps, __builtin_amdgcn_readlane(my_slot, at),
-                                       __builtin_amdgcn_readlane(my_pos, at), freqs, pool);
+      const int slot = __builtin_amdgcn_readlane(my_slot, at);
+      const int pos = __builtin_amdgcn_readlane(my_pos, at);
+      if constexpr (kMx4)
+        mx4_store_row<kBf16, kStream>(raw, w, eps, slot, pos, freqs, pool);
+      else
+        native_store_row<kBf16, kStream>(raw, w, eps, slot, pos, freqs, pool);
     }
   }
 }
@@ -885,11 +969,13 @@ extern "C" int rm_pack_rows_planes(const void* x, int x_dtype, int64_t x_row_str
                   PackedDst{values, (uint8_t*)bitmaps, scales}, true, rows, keep_count, stream);
 }
 
-extern "C" int rm_native_store_rows(const void* x, int x_dtype, int64_t x_row_stride,
-                                    const float* weight, float eps, const int32_t* dst_slot,
-                                    const int32_t* position, const float* freqs,
-                                    int64_t freq_rows, int64_t n, uint8_t* pool,
-                                    int64_t pool_pages, void* stream) {
+namespace {
+
+// Argument checks and launch of the full-row stores (Native and 4-bit records).
+template <bool kMx4>
+int store_rows(const void* x, int x_dtype, int64_t x_row_stride, const float* weight, float eps,
+               const int32_t* dst_slot, const int32_t* position, const float* freqs,
+               int64_t freq_rows, int64_t n, uint8_t* pool, int64_t pool_pages, void* stream) {
   if (n < 0 || pool_pages < 0 || freq_rows < 0) return RM_ERR_SHAPE;
   if (n == 0) return RM_OK;
   if (!x || !weight || !dst_slot || !pool || (freqs && !position)) return RM_ERR_NULL;
@@ -905,12 +991,33 @@ extern "C" int rm_native_store_rows(const void* x, int x_dtype, int64_t x_row_st
   const int64_t cap = n > kStreamRows ? kMaxBlocks : kNativeBlocks;
   const auto kern =
       n > kStreamRows
-          ? (bf16 ? native_store_kernel<true, false, true> : native_store_kernel<false, false, true>)
+          ? (bf16 ? native_store_kernel<true, false, true, kMx4> : native_store_kernel<false, false, true, kMx4>)
       : n > kNativeBlocks * kWaves
-          ? (bf16 ? native_store_kernel<true, false, false> : native_store_kernel<false, false, false>)
-          : (bf16 ? native_store_kernel<true, true, false> : native_store_kernel<false, true, false>);
+          ? (bf16 ? native_store_kernel<true, false, false, kMx4> : native_store_kernel<false, false, false, kMx4>)
+          : (bf16 ? native_store_kernel<true, true, false, kMx4> : native_store_kernel<false, true, false, kMx4>);
   hipLaunchKernelGGL(kern, dim3(grid_for(n, cap)), dim3(256), 0, s, x, x_row_stride, weight, eps,
                      dst_slot, position, freqs, freq_rows, n, rows_per_wave(bf16, n, cap), pool,
                      rows);
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" int rm_native_store_rows(const void* x, int x_dtype, int64_t x_row_stride,
+                                    const float* weight, float eps, const int32_t* dst_slot,
+                                    const int32_t* position, const float* freqs,
+                                    int64_t freq_rows, int64_t n, uint8_t* pool,
+                                    int64_t pool_pages, void* stream) {
+  return store_rows<false>(x, x_dtype, x_row_stride, weight, eps, dst_slot, position, freqs,
+                           freq_rows, n, pool, pool_pages, stream);
+}
+
+extern "C" int rm_mx4_store_rows(const void* x, int x_dtype, int64_t x_row_stride,
+                                 const float* weight, float eps, const int32_t* dst_slot,
+                                 const int32_t* position, const float* freqs, int64_t freq_rows,
+                                 int64_t n, uint8_t* pool, int64_t pool_pages, void* stream) {
+  if (pool_pages > ((int64_t)1 << 25)) return RM_ERR_SHAPE;  // int32 slots
+  if (weight && ((uintptr_t)weight & 15)) return RM_ERR_ALIGN;
+  return store_rows<true>(x, x_dtype, x_row_stride, weight, eps, dst_slot, position, freqs,
+                          freq_rows, n, pool, pool_pages, stream);
 }

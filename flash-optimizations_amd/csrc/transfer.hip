@@ -6,13 +6,14 @@
 // (coordinated transfers, 256 survivors only; third_party/README.md:261). Here
 // a Packed record is one contiguous (K + 72)-byte span, so one unit moves all
 // three planes; a Native record is its 576-byte data row plus its 8-byte scale
-// row. Either pool may live in device memory or in pinned host memory (both
+// row; a 4-bit record is one 272-byte span. Either pool may live in device memory or in pinned host memory (both
 // are addressable from the GPU), so the same kernel backs up (device -> host)
 // and restores (host -> device).
 //
 // One wave per (record, layer): lane l moves 8-byte piece l (and piece 64 + l
 // where a record has more than 64 pieces), so a wave issues the whole record
 // at once and consecutive waves stream consecutive records.
+#include "mx4_device.h"
 #include "remnant_device.h"
 #include "remnant_mi355x.h"
 
@@ -70,14 +71,16 @@ extern "C" int rm_copy_records(const uint8_t* src, int64_t src_pages, int64_t sr
                                int64_t dst_layer_bytes, const int32_t* dst_slots, int64_t n,
                                int64_t layers, int format, int keep_count, void* stream) {
   if (n < 0 || layers < 0 || src_pages < 0 || dst_pages < 0) return RM_ERR_SHAPE;
-  if (format != RM_FORMAT_PACKED && format != RM_FORMAT_NATIVE) return RM_ERR_DTYPE;
+  if (format != RM_FORMAT_PACKED && format != RM_FORMAT_NATIVE && format != RM_FORMAT_MX4)
+    return RM_ERR_DTYPE;
   if (format == RM_FORMAT_PACKED && (keep_count < 64 || keep_count > 448 || keep_count % 64))
     return RM_ERR_SHAPE;
   if (n == 0 || layers == 0) return RM_OK;
   if (!src || !dst || !src_slots || !dst_slots) return RM_ERR_NULL;
   Geometry g;
-  if (format == RM_FORMAT_PACKED) {
-    g.data_bytes = keep_count + kBitmapBytes + kScaleBytes;
+  if (format != RM_FORMAT_NATIVE) {  // one contiguous span a record
+    g.data_bytes = format == RM_FORMAT_MX4 ? kMx4RecordBytes
+                                           : keep_count + kBitmapBytes + kScaleBytes;
     g.page_bytes = (int64_t)kPageRecords * g.data_bytes;
     g.scale_at = 0;
     g.pieces = g.data_bytes / 8;

@@ -73,6 +73,18 @@ SIGNATURES = {
     "rm_native_sparse_decode_swa_fwd": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64,
                                                _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64,
                                                _vp, _vp, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "rm_mx4_store_rows": (_i32, [_vp, _i32, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _vp,
+                                 _i64, _vp]),
+    "rm_mx4_gather_bf16": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "rm_mx4_sparse_decode_workspace": (_i32, [_i64, _i64, _i64, _i64,
+                                              ctypes.POINTER(ctypes.c_int32),
+                                              ctypes.POINTER(ctypes.c_size_t)]),
+    "rm_mx4_sparse_decode_fwd": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp,
+                                        _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _f32,
+                                        _vp, _vp, _vp, _sz, _vp]),
+    "rm_append_slots": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                               _vp, _vp, _vp, _vp]),
+    "rm_window_slots": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
 }
 
 _lib = None

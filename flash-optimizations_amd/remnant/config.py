@@ -46,8 +46,13 @@ PACKED_PAGE_BYTES = PAGE_RECORDS * PACKED_RECORD_BYTES       # 20992
 NATIVE_DATA_BYTES = NOPE_DIM + 2 * ROPE_DIM                  # 576
 NATIVE_RECORD_BYTES = NATIVE_DATA_BYTES + 8                  # 584
 NATIVE_PAGE_BYTES = PAGE_RECORDS * NATIVE_RECORD_BYTES       # 37376
+MX4_GROUP = 32
+MX4_CODE_BYTES = HEAD_DIM // 2                               # 256
+MX4_RECORD_BYTES = MX4_CODE_BYTES + HEAD_DIM // MX4_GROUP    # 272
+MX4_PAGE_BYTES = PAGE_RECORDS * MX4_RECORD_BYTES             # 17408
+MAX_SLOT_BATCH = 8192                                        # requests of an append_slots call
 
-FORMATS = ("native", "direct")
+FORMATS = ("native", "direct", "mx4")
 DECODE_IMPLS = ("kernel", "reconstruct")
 
 
@@ -161,7 +166,7 @@ class PackedProfile:
 
 @dataclasses.dataclass(frozen=True)
 class CacheFormat:
-    fmt: str = "native"              # "native" | "remnant" (= direct)
+    fmt: str = "native"              # "native" | "remnant" (= direct) | "mx4"
     decode_impl: str = "kernel"      # "kernel" = Direct reader, "reconstruct"
     store_impl: str = "kernel"       # fused store
     profile: PackedProfile = PackedProfile()
@@ -178,6 +183,8 @@ class CacheFormat:
         return self.profile.count_for(layer_id)
 
     def record_bytes_for(self, layer_id: int | None = None) -> int:
+        if self.fmt == "mx4":
+            return MX4_RECORD_BYTES
         if not self.packed:
             return NATIVE_RECORD_BYTES
         return packed_record_bytes(self.keep_count_for(layer_id))
@@ -197,8 +204,9 @@ _current = CacheFormat()
 def configure_cache_format(fmt: str, decode_impl: str = "kernel", store_impl: str | None = None,
                            keep_count: int = KEEP_COUNT, layer_keep_counts=None,
                            compression_ratios=None) -> CacheFormat:
-    """Select the C4 cache format. ``fmt`` is ``native`` or ``remnant``
-    (``direct`` is accepted as the v0.5.22 spelling of Packed + Direct).
+    """Select the C4 cache format. ``fmt`` is ``native``, ``remnant``
+    (``direct`` is accepted as the v0.5.22 spelling of Packed + Direct) or
+    ``mx4`` (4-bit records, which keep every coordinate: no survivor counts).
     ``decode_impl`` is ``kernel`` (the Direct reader) or ``reconstruct`` (gather
     + dequantize + RoPE rows for a dense reader; ``triton`` is the reference's
     name for it). ``compression_ratios`` is the model's per-layer
@@ -208,7 +216,7 @@ def configure_cache_format(fmt: str, decode_impl: str = "kernel", store_impl: st
     global _current
     if fmt == "direct":
         fmt = "remnant"
-    if fmt not in ("native", "remnant"):
+    if fmt not in ("native", "remnant", "mx4"):
         raise ValueError(f"unsupported cache format: {fmt!r}")
     if decode_impl == "triton":
         decode_impl = "reconstruct"
@@ -233,6 +241,9 @@ def configure_cache_format(fmt: str, decode_impl: str = "kernel", store_impl: st
             if layer >= len(ratios) or ratios[layer] != C4_RATIO:
                 raise ValueError(f"layer {layer} is not a C4 layer of the model; overrides "
                                  "must name C4 layers")
+    if fmt == "mx4" and (decode_impl != "kernel" or keep_count != KEEP_COUNT or overrides):
+        raise ValueError("4-bit records keep every coordinate and are read by their own decode "
+                         "kernel: no survivor counts, no reconstruct reader")
     profile = PackedProfile(keep_count, overrides, ratios)
     if fmt == "remnant" and decode_impl == "kernel" and \
             any(c != KEEP_COUNT for c in profile.counts()):
@@ -266,7 +277,8 @@ def add_cli_arguments(parser: argparse.ArgumentParser) -> None:
     C4_LAYER_KEEP_COUNTS)."""
     parser.add_argument("--kv-cache-format", choices=FORMATS, default=None,
                         help="native: 584-byte records; direct: Packed 328-byte records "
-                             "read by the Direct decode kernel (default native)")
+                             "read by the Direct decode kernel; mx4: 4-bit 272-byte records "
+                             "(default native)")
     parser.add_argument("--dsv4-c4-cache-format", choices=LEGACY_FORMATS, default=None,
                         help="v0.5.18 spelling of the format: remnant = Packed records")
     parser.add_argument("--dsv4-c4-cache-implementation", choices=LEGACY_DECODE_IMPLS,

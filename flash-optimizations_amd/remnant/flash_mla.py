@@ -238,9 +238,12 @@ def native_sparse_decode_fwd(q, pool, block_table, indices, *, seqlens=None, top
 
 
 def sparse_decode_fwd(q, pool, block_table, indices, **kwargs):
-    """Dispatch on the configured ``--kv-cache-format`` (native | direct)."""
+    """Dispatch on the configured ``--kv-cache-format`` (native | direct | mx4)."""
     if config.current().packed:
         return remnant_sparse_decode_fwd(q, pool, block_table, indices, **kwargs)
     kwargs.pop("freqs_cis", None)
     kwargs.pop("rope_inv_freq", None)
+    if config.current().fmt == "mx4":
+        from .mx4 import mx4_sparse_decode_fwd
+        return mx4_sparse_decode_fwd(q, pool, block_table, indices, **kwargs)
     return native_sparse_decode_fwd(q, pool, block_table, indices, **kwargs)

@@ -5,7 +5,8 @@ Reference: SGLang's host pool ``srt/mem_cache/memory_pool_host.py`` with the
 hybrid pool assembler (third_party/README.md:261): a Packed record's value,
 bitmap and scale planes move together, indexed by token slots on each side.
 Here a Packed record is one contiguous span, so one transfer unit carries all
-three planes; Native records move their data and scale rows together.
+three planes; Native records move their data and scale rows together; a 4-bit
+record is one span.
 
 The host pool has the device pool's geometry ([layers, pages, page_bytes],
 64-record pages) in pinned memory (``torch.empty(..., pin_memory=True)``,
@@ -106,7 +107,7 @@ def copy_records(src, src_slots: torch.Tensor, dst, dst_slots: torch.Tensor, *,
                              "memory")
     sbuf = src.buffer if layer_id is None else src.buffer[layer_id]
     dbuf = dst.buffer if layer_id is None else dst.buffer[layer_id]
-    fmt = 0 if sfmt == "remnant" else 1
+    fmt = {"remnant": 0, "native": 1, "mx4": 4}[sfmt]
     _lib.check(_lib.load().rm_copy_records(
         sbuf.data_ptr(), spages, spages * spb, src_slots.data_ptr(), dbuf.data_ptr(), dpages,
         dpages * dpb, dst_slots.data_ptr(), n, slayers if layer_id is None else 1, fmt, skeep,

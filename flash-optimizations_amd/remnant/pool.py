@@ -18,6 +18,9 @@ A Packed pool may hold a survivor profile other than 256 (``keep_count`` 64..448
 in steps of 64, docs/agents/numerical-and-validation.md:10-14): its records are
 ``keep_count + 72`` bytes with the same code/bitmap/scale order, 64 to a page.
 One pool holds one profile; per-layer profiles use one pool per layer.
+
+A 4-bit pool (``fmt="mx4"``) holds 64 contiguous 272-byte records a page: 256 bytes
+of E2M1 codes, two coordinates a byte, then 16 UE8M0 scale bytes.
 """
 
 from __future__ import annotations
@@ -32,13 +35,14 @@ class LatentPool:
                  keep_count: int = config.KEEP_COUNT):
         if fmt == "direct":
             fmt = "remnant"
-        if fmt not in ("remnant", "native"):
+        if fmt not in ("remnant", "native", "mx4"):
             raise ValueError(f"unsupported cache format: {fmt!r}")
         if pages < 0 or layers < 1:
             raise ValueError("pages must be >= 0 and layers >= 1")
         config.check_keep_count(keep_count)
-        if fmt == "native" and keep_count != config.KEEP_COUNT:
-            raise ValueError("Native records keep every coordinate; keep_count is Packed-only")
+        if fmt != "remnant" and keep_count != config.KEEP_COUNT:
+            raise ValueError(f"{'Native' if fmt == 'native' else '4-bit'} records keep every "
+                             "coordinate; keep_count is Packed-only")
         self.fmt = fmt
         self.pages = pages
         self.layers = layers
@@ -46,6 +50,9 @@ class LatentPool:
         if fmt == "remnant":
             self.page_bytes = config.packed_page_bytes(keep_count)
             self.data_bytes = keep_count + 8 * config.BITMAP_WORDS
+        elif fmt == "mx4":
+            self.page_bytes = config.MX4_PAGE_BYTES
+            self.data_bytes = config.MX4_CODE_BYTES
         else:
             self.page_bytes = config.NATIVE_PAGE_BYTES
             self.data_bytes = config.NATIVE_DATA_BYTES
@@ -62,13 +69,13 @@ class LatentPool:
 
     @property
     def record_bytes(self) -> int:
-        return self.data_bytes + 8
+        return self.data_bytes + (16 if self.fmt == "mx4" else 8)
 
     def layer(self, layer_id: int | None = None) -> torch.Tensor:
         return self.buffer[0 if layer_id is None else layer_id]
 
     def _data_rows(self, layer_id):
-        if self.packed:  # contiguous records: data = all but the last 8 bytes of each
+        if self.fmt != "native":  # contiguous records: data = all but the scales of each
             pg = self.layer(layer_id).reshape(self.pages, config.PAGE_RECORDS,
                                               self.record_bytes)
             return pg[..., : self.data_bytes]
@@ -76,8 +83,8 @@ class LatentPool:
         return pg.reshape(self.pages, config.PAGE_RECORDS, self.data_bytes)
 
     def scales(self, layer_id: int | None = None) -> torch.Tensor:
-        """Scale plane view [pages, 64, 8] u8."""
-        if self.packed:
+        """Scale plane view [pages, 64, 8] u8 (4-bit: [pages, 64, 16])."""
+        if self.fmt != "native":
             pg = self.layer(layer_id).reshape(self.pages, config.PAGE_RECORDS,
                                               self.record_bytes)
             return pg[..., self.data_bytes:]
@@ -85,14 +92,17 @@ class LatentPool:
         return pg.reshape(self.pages, config.PAGE_RECORDS, 8)
 
     def values(self, layer_id: int | None = None) -> torch.Tensor:
-        """Code plane view: Packed [pages, 64, keep_count] u8, Native [pages, 64, 448] u8."""
-        width = self.keep_count if self.packed else config.NOPE_DIM
+        """Code plane view: Packed [pages, 64, keep_count] u8, Native [pages, 64, 448] u8,
+        4-bit [pages, 64, 256] u8 (two codes a byte)."""
+        width = (self.keep_count if self.packed else config.MX4_CODE_BYTES if self.fmt == "mx4"
+                 else config.NOPE_DIM)
         return self._data_rows(layer_id)[..., :width]
 
     def bitmaps(self, layer_id: int | None = None) -> torch.Tensor:
         """Bitmap plane view [pages, 64, 64] u8 (8 little-endian MSB-first uint64 words)."""
         if not self.packed:
-            raise ValueError("Native records carry no bitmap")
+            raise ValueError(f"{'Native' if self.fmt == 'native' else '4-bit'} records carry no "
+                             "bitmap")
         return self._data_rows(layer_id)[..., self.keep_count:self.data_bytes]
 
     def records(self, slots: torch.Tensor, layer_id: int | None = None) -> torch.Tensor:
@@ -112,5 +122,6 @@ class LatentPool:
 def records_fitting(nbytes: int, fmt: str = "remnant", keep_count: int = config.KEEP_COUNT) -> int:
     """Records (whole pages of 64) that fit in ``nbytes`` of HBM."""
     fmt = "remnant" if fmt == "direct" else fmt
-    page = config.packed_page_bytes(keep_count) if fmt == "remnant" else config.NATIVE_PAGE_BYTES
+    page = (config.packed_page_bytes(keep_count) if fmt == "remnant" else config.MX4_PAGE_BYTES
+            if fmt == "mx4" else config.NATIVE_PAGE_BYTES)
     return (nbytes // page) * config.PAGE_RECORDS

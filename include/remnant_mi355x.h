@@ -64,6 +64,11 @@
  * bytes (K + 72 bytes, 8-byte aligned), 64 records per page (64 * (K + 72) B).
  * The sparse decode reads the 256-survivor format only.
  *
+ * 4-bit records (no counterpart in the reference): an MX4 page (17,408 B) is 64
+ * contiguous 272-byte records: 256 bytes of E2M1 codes (coordinate 2i in the low
+ * half of byte i) and 16 UE8M0 scale bytes, one per 32 coordinates, value =
+ * code * 2^(byte - 127). The tail is stored rotated. Every coordinate is kept.
+ *
  * Plane form: the same records held as three row-aligned planes, slot s being
  * row s of each: values [rows, K] u8 (codes, ascending coordinate), bitmaps
  * [rows, 8] u64 (the bitmap words as above) and scales [rows, 8] u8. Byte for
@@ -91,7 +96,7 @@ enum rm_status {
 
 enum rm_dtype { RM_F32 = 0, RM_BF16 = 1 };
 
-enum rm_format { RM_FORMAT_PACKED = 0, RM_FORMAT_NATIVE = 1 };
+enum rm_format { RM_FORMAT_PACKED = 0, RM_FORMAT_NATIVE = 1, RM_FORMAT_MX4 = 4 };
 
 #define RM_HEAD_DIM 512
 #define RM_NOPE_DIM 448
@@ -104,6 +109,9 @@ enum rm_format { RM_FORMAT_PACKED = 0, RM_FORMAT_NATIVE = 1 };
 #define RM_NATIVE_DATA_BYTES 576
 #define RM_NATIVE_RECORD_BYTES 584
 #define RM_NATIVE_PAGE_BYTES 37376
+#define RM_MX4_RECORD_BYTES 272
+#define RM_MX4_PAGE_BYTES 17408
+#define RM_MAX_SLOT_BATCH 8192
 
 /* Library version (major * 10000 + minor * 100 + patch). */
 int rm_version(void);
@@ -203,7 +211,8 @@ int rm_packed_to_native_planes(const uint8_t* values, const uint64_t* bitmaps,
  * l of `src` is copied to record dst_slots[i] of layer l of `dst` -- the whole
  * Packed record (codes, bitmap and scales together; format RM_FORMAT_PACKED
  * with its keep_count) or the Native data row and scale row
- * (RM_FORMAT_NATIVE). Pairs with a slot < 0 or beyond its pool are skipped.
+ * (RM_FORMAT_NATIVE) or the 4-bit record (RM_FORMAT_MX4; keep_count is not
+ * looked at). Pairs with a slot < 0 or beyond its pool are skipped.
  * Layer l of a pool starts l * layer_bytes after its base. Either pool may be
  * device memory or pinned host memory (hipHostMalloc). 8-byte alignment. */
 int rm_copy_records(const uint8_t* src, int64_t src_pages, int64_t src_layer_bytes,
@@ -332,6 +341,77 @@ int rm_native_sparse_decode_swa_fwd(const uint16_t* q, int64_t batch, int64_t q_
                                     const float* sink, float softmax_scale, uint16_t* out,
                                     float* lse, void* workspace, size_t workspace_bytes,
                                     void* stream);
+
+/* ---- 4-bit latent records (RM_FORMAT_MX4) and slot maps: no counterpart in the
+ * reference. ---- */
+
+/* Store: rows as rm_native_store_rows takes them (RMSNorm, BF16 rounding, tail
+ * rotated by freqs row position[i] * 4 and rounded to BF16; freqs NULL = no
+ * rotation) as 4-bit records. Per 32 coordinates the scale is 2^e, the smallest
+ * e with max(amax, 1e-4) <= 6 * 2^e and at most 32; codes are n / 2^e rounded to
+ * nearest even, magnitudes above 6 to 6. A group with an infinity or NaN gets
+ * scale byte 255 and reads as 32 NaN. Skipped rows as rm_native_store_rows.
+ * weight 16-byte aligned. */
+int rm_mx4_store_rows(const void* x, int x_dtype, int64_t x_row_stride, const float* weight,
+                      float eps, const int32_t* dst_slot, const int32_t* position,
+                      const float* freqs, int64_t freq_rows, int64_t n, uint8_t* pool,
+                      int64_t pool_pages, void* stream);
+
+/* Reader: out row q * selected_k + k (512 BF16 values, contiguous) = record
+ * slots[q, k], exact; zeros unless k < lengths[q] (NULL = selected_k) and
+ * 0 <= slot < pool_pages * 64. Strides are in int32 elements. */
+int rm_mx4_gather_bf16(const uint8_t* pool, int64_t pool_pages, const int32_t* slots,
+                       int64_t slots_stride_q, int64_t slots_stride_k, const int32_t* lengths,
+                       int64_t length_stride, int64_t n_queries, int64_t selected_k,
+                       uint16_t* out, void* stream);
+
+/* Split planning for the decode below: as rm_sparse_decode_workspace_swa.
+ * heads 0..1024 (any count), topk <= 2^20, swa_topk <= 512, tokens <= 65535. */
+int rm_mx4_sparse_decode_workspace(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk,
+                                   int32_t* num_splits, size_t* workspace_bytes);
+
+/* Sparse-MLA decode over 4-bit records: the contract of
+ * rm_native_sparse_decode_swa_fwd (list, lengths, block table, sink, window rows
+ * of a Native pool; swa_topk 0 = none, the window arguments may then be NULL)
+ * with any number of heads. A row with no valid entry and no sink gives zeros
+ * and lse -inf. Scale bytes of the records are the store's. */
+int rm_mx4_sparse_decode_fwd(const uint16_t* q, int64_t batch, int64_t q_len, int64_t heads,
+                             const uint8_t* pool, int64_t pool_pages, const int32_t* block_table,
+                             int64_t block_table_stride, int64_t max_blocks,
+                             const int32_t* seqlens, const int32_t* indices, int64_t topk,
+                             const int32_t* topk_length, const uint8_t* swa_pool,
+                             int64_t swa_pool_pages, const int32_t* swa_indices,
+                             int64_t swa_topk, const int32_t* swa_length, const float* sink,
+                             float softmax_scale, uint16_t* out, float* lse, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Block tables and slots of a step. Request b (batch <= RM_MAX_SLOT_BATCH) goes
+ * from o = old_lengths[b] / ratio records to n = max(new_lengths[b] / ratio, o)
+ * (lengths in tokens; negative ones count as 0). It takes ceil(n / 64) -
+ * ceil(o / 64) pages, the requests in order, from the front of free_pages:
+ * written to its new columns of block_table [batch, max_blocks] (-1 past the
+ * free list; columns past max_blocks are not written). Its new records are
+ * consecutive rows of the step, the requests in order: loc[i] = page * 64 +
+ * r % 64 of row i's record r (-1 where no page in 0..2^25 - 1 is mapped) and
+ * positions[i] = r; rows past the last record get -1 and 0, records past `rows`
+ * are not written. row_starts [batch + 1]: first row of each request, then
+ * their number; seqlens [batch]: n; pages_taken [1]: pages needed (more than
+ * n_free: the free list was short). Sums saturate at 2^31 - 1. The outputs and
+ * the table must not overlap the inputs or each other (RM_ERR_SHAPE). */
+int rm_append_slots(int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                    const int32_t* old_lengths, const int32_t* new_lengths, int64_t batch,
+                    int64_t ratio, const int32_t* free_pages, int64_t n_free, int64_t rows,
+                    int32_t* loc, int32_t* positions, int32_t* row_starts, int32_t* seqlens,
+                    int32_t* pages_taken, void* stream);
+
+/* Visible slots per query token: query j of request b sits at p = lengths[b] -
+ * q_len + j and sees tokens 0 .. f - 1 with f = min(first, p + 1), then
+ * max(f, p + 1 - window) .. p. slots [batch, q_len, first + window]: their
+ * pool slots in that order (-1 where the table maps no page), then -1;
+ * counts [batch * q_len]: their number (0 where p < 0). */
+int rm_window_slots(const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                    const int32_t* lengths, int64_t batch, int64_t q_len, int64_t window,
+                    int64_t first, int32_t* slots, int32_t* counts, void* stream);
 
 #ifdef __cplusplus
 }
