@@ -93,7 +93,10 @@ def decode(q, pool, table, indices, seqlens=None, topk_length=None, sink=None, s
     products and moves by at most 520 * 2^-24 of the sum of their magnitudes (the sum,
     and the scaling, each rounded), which moves a weight by that factor and lse by that
     much; exp2, log2 and the float32 sums are held to 2^-18 altogether, relative to the
-    sum of the terms' magnitudes."""
+    sum of the terms' magnitudes. Weights are BF16 numbers in units of a record's scale
+    over 2^32, the largest scale there is, and one below 2^-126 of the unit may become
+    zero: at most 2^-126 * 2^32 * 6 < 2^-91 of a coordinate for each record, over a sum of
+    weights of at least 1/2 (the largest weight is in (1/2, 1])."""
     b, sq, h, _ = q.shape
     scale = 512 ** -0.5 if scale is None else scale
     qd = q.double().numpy()
@@ -135,7 +138,8 @@ def decode(q, pool, table, indices, seqlens=None, topk_length=None, sink=None, s
             move = 520 * 2.0 ** -24 * terms
             spread = weight @ np.abs(rows)
             tol[i, j] = 2.0 ** -8 * (spread + np.abs(out[i, j])) \
-                + (2 * move + 2.0 ** -18)[:, None] * spread * (1 + 2.0 ** -8)
+                + (2 * move + 2.0 ** -18)[:, None] * spread * (1 + 2.0 ** -8) \
+                + 2.0 ** -90 * rows.shape[0]
             ltol[i, j] = move + 2.0 ** -18 * (1 + np.abs(lse[i, j]))
     return out, lse, tol, ltol
 
