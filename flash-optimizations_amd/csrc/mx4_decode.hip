@@ -4,27 +4,28 @@
 //   l_j = (q_h . K_j) * scale, Z = sum_j exp(l_j) + exp(sink_h),
 //   out = sum_j exp(l_j) K_j / Z, lse = ln Z.
 //
-// A workgroup of kWaves waves owns (split of a list, token, 16 heads) and walks its
-// share in rounds of 32 records a wave. A round has two halves with a barrier
-// between:
-//   * scores: a wave holds its 32 records as the A operands of S^T = K Q^T
-//     (v_mfma_f32_16x16x32_bf16; lane (r, g) loads 64 contiguous code bytes of
-//     record r straight from its row, four scale groups, so Q, in registers, is
-//     ordered to match). It leaves in LDS the raw code bytes, the weights P
-//     = 2^(s - m) as BF16, m = ceil of its 32 scores' maximum, and each record's
-//     scale exponents.
-//   * values: a wave owns 512 / kWaves output coordinates of O^T += V^T P^T over
-//     all the round's records. The codes come out of LDS transposed
-//     (ds_read_b64_tr_b4: 8 records of 32 coordinates a lane pair) and become BF16
-//     without their scales; the scales are powers of two that differ by record and
-//     group, so they go to the weights instead, and so does the step from the
-//     wave's m to the running maximum: an integer subtraction on the BF16
-//     exponents, two weights an instruction, saturating at zero (v_pk_sub_u16
-//     clamp), against the largest scale the store writes, 2^32; O is in units of it.
-//     A weight that a scale takes below 2^-126 becomes zero: less than 2^-71 of the
-//     largest weight at that scale.
-// Both operands keep the order of the score tile: P^T in LDS is what the lane
-// holding it writes, 16 bytes a lane, with no exchange between lanes.
+// A workgroup of kWaves waves owns (split, token, 16 heads) and takes its share of the
+// list in rounds, 32 records a wave (a chunk; chunks are dealt to the splits and then
+// the waves in turn), then its share of the window, 16 rows a wave. A round has two
+// halves with a barrier between:
+//   * scores: a wave computes S^T = K Q^T of its chunk on v_mfma_f32_16x16x32_bf16, Q in
+//     registers, and leaves in LDS the weights P = 2^(s - m) as BF16, m the whole log2
+//     unit above the chunk's largest score, and each record's scale exponents.
+//   * values: a wave owns 512 / kWaves output coordinates of O^T += V^T P^T over all the
+//     round's records. The codes come out of LDS transposed (ds_read_b64_tr_b4) and
+//     become BF16 without their scales: those are powers of two that differ by record
+//     and group, so they go to the weights, and so does the step from a chunk's m to the
+//     running maximum: integer subtractions on the BF16 exponents, two weights an
+//     instruction, saturating at zero (v_pk_sub_u16 clamp), against the largest scale the
+//     store writes, 2^32; O is in units of it. A weight that a scale takes below 2^-126
+//     becomes zero: less than 2^-71 of the largest weight at that scale.
+// P^T in LDS is what the lane holding it writes, 16 bytes a lane: the order of the
+// records in the second product's long axis is free, and S^T's is taken.
+//
+// A chunk's raw bytes go HBM -> LDS with global_load_lds, a round ahead of their use,
+// consecutive lanes copying consecutive 16-byte pieces of a record (17 a record), so
+// that a copy touches each 128-byte line once. The three loads between a list entry and
+// its record (index, block table, record) are made for kBatch rounds at a time.
 #include <algorithm>
 
 #include "combine.h"
@@ -48,7 +49,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 struct DecodeArgs {
   const uint16_t* q;
-  int q_len, heads;
+  uint64_t q_len_magic;  // ceil(2^32 / q_len): token t < 2^16 is of request t * q_len_magic >> 32
+  int heads;
   const uint8_t* pool;
   int pool_pages;
   const int32_t* block_table;
@@ -65,7 +67,8 @@ struct DecodeArgs {
   const int32_t* swa_length;
   const float* sink;
   float scale_log2;
-  int splits;     // of the list; workgroup x = splits takes the window rows
+  int splits;     // workgroups (along x) that share a token's list and window
+  uint64_t splits_magic;  // ceil(2^32 / splits): x / splits = x * splits_magic >> 32 for x < 2^17
   int ws_splits;  // partial slots a row; 0: finish in place
   uint16_t* out;
   float* lse;
@@ -73,37 +76,69 @@ struct DecodeArgs {
   float* ws_lse;  // [tokens, ws_splits, heads]
 };
 
-// A round's data of one wave. Codes: two tiles of 16 records, 272 bytes apart (4
-// banks), the second tile half a bank row off, so that the transposed reads of a
-// lane group's 2 x 4 records meet no bank twice.
-constexpr int kCodePitch = 272;
-constexpr int kTileBytes = 16 * kCodePitch + 128;
-// Window rows: 16 a wave, the 576 data bytes 592 apart.
-constexpr int kRowPitch = 592;
+// A chunk in LDS: its records 272 bytes apart (4 banks), with 128 bytes between the
+// first 16 and the second, so that the transposed reads of a lane group's 2 x 4 records
+// meet no bank twice. 552 pieces of 16 bytes, 9 copies.
+constexpr int kTilePieces = 16 * 17 + 8;
+constexpr int kTileBytes = 16 * kTilePieces;                     // 4,480
+constexpr int kChunkBytes = kTileBytes + 16 * kMx4RecordBytes;   // 8,832
+constexpr int kCopies = 9;
+constexpr int kLastLanes = 2 * kTilePieces - 8 - 64 * (kCopies - 1);  // of the last copy: 40
+constexpr int kBatch = 8;  // rounds whose slots are resolved together
+// A window chunk: 16 rows, 16-byte piece 4 j + g of row r at 1024 j + 256 g + 16 r, then
+// the scale bytes by group. It takes the room of two chunks.
+constexpr int kWindowScalesAt = 16 * kNativeDataBytes;
+static_assert(kWindowScalesAt + 128 <= 2 * kChunkBytes, "window chunk");
 constexpr int kScaleRef = 127 + kMx4MaxExponent;
 
-struct WaveLds {
-  union {
-    struct {
-      uint8_t codes[2 * kTileBytes];
-      uint16_t shift[16][32];  // [group][record slot]: (159 - scale byte) << 7
-    };
-    struct {
-      uint8_t rows[16 * kRowPitch];
-      uint8_t scales[8][16];   // [group][row]
-    };
-  };
-  u32x4 weight[64];            // by lane; a list: 8 BF16, a window: 4 floats
-  float top[16];               // by head: the exponent the weights are against
+// LDS of a workgroup: two chunks a wave; then the weights (16 bytes a lane; a window
+// chunk: four floats), the scale exponents [16 groups][32 record slots] u16, (159 - scale
+// byte) << 7, and the references of the 16 heads, each by wave. Q passes through the
+// latter three at the start, a head's row every 1,040 bytes (4 banks).
+template <int kWaves>
+struct Lds {
+  static constexpr int kWeights = 2 * kWaves * kChunkBytes;
+  static constexpr int kShifts = kWeights + 1024 * kWaves;
+  static constexpr int kTops = kShifts + 1024 * kWaves;
+  static constexpr int kQPitch = 1040;
+  static constexpr int kEnd = kTops + 64 * kWaves;
+  static constexpr int kBytes = kEnd > kWeights + 16 * kQPitch ? kEnd : kWeights + 16 * kQPitch;
 };
 
+// Copies HBM -> LDS: 16 bytes a lane to lds + 16 lane. The LDS address is a plain number,
+// so that the compiler ties the copies to no array; wait_copies() orders them.
+__device__ __forceinline__ void copy16(const void* src, uint32_t lds) {
+  __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
+                                   16, 0, 0);
+}
+// Until at most kLater vector loads issued since are in flight.
+template <int kLater>
+__device__ __forceinline__ void wait_copies() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (kLater & 15) | ((kLater >> 4) << 14));
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <class T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)(uintptr_t)at;
+}
+template <class T>
+__device__ __forceinline__ void lds_write(uint32_t at, T v) {
+  *(__attribute__((address_space(3))) T*)(uintptr_t)at = v;
+}
+// Over the four lanes that share lane % 16.
 __device__ __forceinline__ float over_groups_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
+  const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+  x = fmaxf(u2f(a[0]), u2f(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+  return fmaxf(u2f(b[0]), u2f(b[1]));
 }
 __device__ __forceinline__ float over_groups_sum(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+  const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+  x = u2f(a[0]) + u2f(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+  return u2f(b[0]) + u2f(b[1]);
 }
 // Barrier that orders LDS accesses only: loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() {
@@ -120,249 +155,347 @@ __device__ __forceinline__ bf16x8 as_bf16x8(u32x4 v) { return __builtin_bit_cast
 
 // 2^(from - to) for running maxima, 1 where both are -inf (nothing yet).
 __device__ __forceinline__ float step_down(float from, float to) {
-  return from == to ? 1.0f : exp2f(from - to);
+  return from == to ? 1.0f : __builtin_amdgcn_exp2f(from - to);
 }
 
 template <int kWaves>
 struct Decode {
+  using L = Lds<kWaves>;
   static constexpr int kTiles = kHeadDim / 16 / kWaves;  // 16-coordinate tiles of O a wave
   const DecodeArgs& a;
-  WaveLds* const lds;  // [kWaves]
+  const uint32_t lds;
   const int lane, wave, row, group;  // row: record of a tile, or head; group: lane / 16
+  const int split;
   const int64_t t;
   const int h0;
-  bf16x8 q[16];     // q[4 j + u]: coordinates 128 group + 32 j + 8 u .. + 7 of head `row`
-  f32x4 o[kTiles];  // coordinate 16 tile + 4 group + i of head `row`
+  bf16x8 q[16];     // q[4 j + u]: coordinates 128 j + 32 group + 8 u .. + 7 of head `row`
+  f32x4 o[kTiles];  // coordinate 16 tile + 4 group + i of the wave's, of head `row`
   float m, l;       // running maximum of head `row` (whole log2 units); this lane's sum
 
-  __device__ __forceinline__ Decode(const DecodeArgs& args, WaveLds* sm)
+  __device__ __forceinline__ Decode(const DecodeArgs& args, uint32_t lds_at)
       : a(args),
-        lds(sm),
+        lds(lds_at),
         lane(wave_lane()),
         wave(uniform((int)(threadIdx.x >> 6))),
         row(lane & 15),
         group(lane >> 4),
+        split((int)blockIdx.x),
         t(blockIdx.y),
-        h0(blockIdx.z * 16) {
-    const uint16_t* src = a.q + (t * a.heads + min(h0 + row, a.heads - 1)) * kHeadDim + 128 * group;
+        h0(blockIdx.z * 16),
+        m(-INFINITY),
+        l(0.0f) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = as_bf16x8(*(const u32x4*)(src + 8 * i));
+    for (int i = 0; i < kTiles; ++i) o[i] = zero_f();
+  }
+  static __device__ __forceinline__ f32x4 zero_f() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+
+  // Q: the waves copy the 16 heads' rows to LDS ...
+  __device__ __forceinline__ void copy_q() const {
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m = -INFINITY;
-    l = 0.0f;
+    for (int i = 0; i < 16 / kWaves; ++i) {
+      const int h = wave * (16 / kWaves) + i;
+      copy16(a.q + (t * a.heads + min(h0 + h, a.heads - 1)) * kHeadDim + 8 * lane,
+             lds + L::kWeights + L::kQPitch * h);
+    }
+  }
+  // ... and, all of it there, take what each lane needs.
+  __device__ __forceinline__ void read_q() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      q[i] = as_bf16x8(lds_read<u32x4>(lds + L::kWeights + L::kQPitch * row + 256 * (i / 4) +
+                                       64 * group + 16 * (i % 4)));
   }
 
-  // Weights of one score tile's four records: against `ref`, zero where bit i of
-  // `live` is off.
+  // s in log2 units, -inf where bit i of `live` is off.
   __device__ __forceinline__ f32x4 scores(f32x4 acc, uint32_t live) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = (live >> i) & 1 ? acc[i] * a.scale_log2 : -INFINITY;
     return acc;
   }
-  // The round's running maximum, from what the waves left; rescales O and l.
-  __device__ __forceinline__ void advance(int waves, float own, float sum) {
-    float top = m;
+  // The round's running maximum, from what the waves left; rescales O and l. down[w]: whole
+  // log2 units from wave w's reference to it, at most 255 (past every exponent).
+  __device__ __forceinline__ void advance(int waves, float own, float sum, int (&down)[kWaves]) {
+    float top = m, of[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) of[w] = lds_read<float>(lds + L::kTops + 64 * w + 4 * row);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w >= waves) of[w] = -INFINITY;
+      top = fmaxf(top, of[w]);
+    }
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
-      if (w < waves) top = fmaxf(top, lds[w].top[row]);
+      down[w] = of[w] == -INFINITY ? 255 : (int)fminf(top - of[w], 255.0f);
     const float f = step_down(m, top);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) o[i] *= f;
     // (sum is zero where own is -inf, and NaN stays NaN)
-    l = l * f + (own == -INFINITY ? sum : sum * exp2f(own - top));
+    l = l * f + (own == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f(own - top));
     m = top;
   }
 
-  // The list's records [begin, end).
-  __device__ __forceinline__ void list(int begin, int end) {
-    const int64_t request = t / a.q_len;
+  // The share of the list: `chunks` chunks of 32 entries, the c-th number c * splits + split.
+  __device__ __forceinline__ void list(int live, int chunks) {
+    const int64_t request = (int64_t)(((uint64_t)t * a.q_len_magic) >> 32);
     const int32_t* const idx = a.indices + t * a.topk;
     const int32_t* const table = a.block_table + request * a.bt_stride;
     const int records = a.seqlens ? a.seqlens[request] : 0x7fffffff;
-    WaveLds& mine = lds[wave];
-    for (int at = begin; at < end; at += 32 * kWaves) {
-      const int waves = min((end - at + 31) / 32, kWaves);
-      float own = -INFINITY, sum = 0.0f;
-      if (wave < waves) {
-        f32x4 s[2];
+    const uint32_t mine = lds + 2 * wave * kChunkBytes;
+    // Copy n takes piece 64 n + lane: of record from / 4 of the chunk, bytes off .. off + 15
+    // (the 8 pieces between the tiles copy some piece again).
+    uint32_t where[kCopies];  // from | off << 8
 #pragma unroll
-        for (int tile = 0; tile < 2; ++tile) {
-          const int k = at + 32 * wave + 16 * tile + row;
-          const int r = k < end ? idx[k] : -1;
-          const int column = r >> 6;
-          const bool inside = r >= 0 && r < records && column < a.max_blocks;
-          const int page = inside ? table[column] : -1;
-          const bool live = page >= 0 && page < a.pool_pages;
-          const int64_t slot = live ? (int64_t)page * kPageRecords + (r & 63) : 0;
-          const uint8_t* rec = a.pool + slot * kMx4RecordBytes;
-          u32x4 code[4];
+    for (int n = 0; n < kCopies; ++n) {
+      const int p = 64 * n + lane, tile = p >= kTilePieces;
+      const int in_tile = min(p - tile * kTilePieces, 16 * 17 - 1);
+      const int r = in_tile * 241 >> 12;  // / 17, for numbers below 272
+      where[n] = (uint32_t)(4 * (16 * tile + r)) | (uint32_t)(16 * (in_tile - 17 * r)) << 8;
+    }
+    for (int first = 0; first * kWaves < chunks; first += kBatch) {
+      const int rounds = min((chunks - first * kWaves + kWaves - 1) / kWaves, kBatch);
+      int slots[kBatch / 2];  // lane: entry lane % 32 of round 2 e + lane / 32; -1: no record
+      {
+        int r[kBatch / 2], page[kBatch / 2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) code[j] = *(const u32x4*)(rec + 64 * group + 16 * j);
-          const uint32_t scale = *(const uint32_t*)(rec + kMx4CodeBytes + 4 * group);
-          const uint32_t mask = (uint32_t)__ballot(live) & 0xffffu;
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-          uint8_t* const dst = mine.codes + tile * kTileBytes + row * kCodePitch + 64 * group;
-          const int rslot = 8 * (row >> 2) + 4 * tile + (row & 3);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            *(u32x4*)(dst + 16 * j) = code[j];
-            const uint32_t byte = (scale >> (8 * j)) & 0xffu;
-            mine.shift[4 * group + j][rslot] = (uint16_t)((kScaleRef - byte) << 7);
-            const float f = mx4_scale(byte);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(fp4x8_to_bf16(code[j][u], f)),
-                                                            q[4 * j + u], acc, 0, 0, 0);
+        for (int e = 0; e < kBatch / 2; ++e) {
+          r[e] = -1;
+          if (2 * e < rounds) {
+            const int c = (first + 2 * e + (lane >> 5)) * kWaves + wave;
+            const int k = 32 * (c * a.splits + split) + (lane & 31);
+            if (k < live) r[e] = idx[k];
           }
-          s[tile] = scores(acc, mask >> (4 * group));
         }
-        float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-        own = ceilf(over_groups_max(top));
-        const float ref = own == -INFINITY ? 0.0f : own;
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = exp2f(s[i / 4][i % 4] - ref);
-          sum += p[i];
+        for (int e = 0; e < kBatch / 2; ++e) {
+          const bool inside = r[e] >= 0 && r[e] < records && (r[e] >> 6) < a.max_blocks;
+          page[e] = inside ? table[r[e] >> 6] : -1;
         }
-        u32x4 w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = __builtin_bit_cast(uint32_t, bf16_pair(p[2 * i], p[2 * i + 1]));
-        mine.weight[lane] = w;
-        if (lane < 16) mine.top[lane] = own;
+        for (int e = 0; e < kBatch / 2; ++e)
+          slots[e] = page[e] >= 0 && page[e] < a.pool_pages
+                         ? page[e] * kPageRecords + (r[e] & 63) : -1;
       }
-      lds_barrier();
-      advance(waves, own, sum);
-#pragma unroll 1
-      for (int w = 0; w < waves; ++w) {
-        const WaveLds& from = lds[w];
-        const float own_w = from.top[row];
-        // (255: past every exponent)
-        const int down = own_w == -INFINITY ? 255 : (int)fminf(m - own_w, 255.0f);
-        u32x4 p = from.weight[lane];
+      auto slots_of = [&](int i) {  // lanes 32 (i % 2) ..: round i's
+        const int s0 = slots[0], s1 = slots[1], s2 = slots[2], s3 = slots[3];
+        return i < 4 ? (i < 2 ? s0 : s1) : (i < 6 ? s2 : s3);
+      };
+      auto copy = [&](int i) {
+        const uint32_t to = mine + (i & 1) * kChunkBytes;
+        const int of = slots_of(i), base = 128 * (i & 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = sub_sat(p[i], (uint32_t)down * 0x00800080u);
-        const uint8_t* codes = from.codes + ((row >> 2) & 1) * kTileBytes +
-                               (4 * group + (row & 3)) * kCodePitch + 8 * (row >> 3);
-#pragma unroll
-        for (int b = 0; b < kTiles / 2; ++b) {
-          const int g = wave * (kTiles / 2) + b;
-          const u32x4 shift = *(const u32x4*)&from.shift[g][8 * group];
-          u32x4 pw;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) pw[i] = sub_sat(p[i], shift[i]);
-          const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(lds_void*)(codes + 16 * g));
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            o[2 * b + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                as_bf16x8(fp4x8_to_bf16((uint32_t)v[i], 1.0f)), as_bf16x8(pw), o[2 * b + i], 0, 0, 0);
+        for (int n = 0; n < kCopies; ++n) {
+          const int slot = __builtin_amdgcn_ds_bpermute(base + (int)(where[n] & 0xff), of);
+          const uint8_t* src =
+              a.pool + ((int64_t)max(slot, 0) * kMx4RecordBytes + (where[n] >> 8));
+          if (n < kCopies - 1 || lane < kLastLanes) copy16(src, to + 1024 * n);
         }
+      };
+      copy(0);
+      if (first == 0) {
+        wait_copies<kCopies>();  // Q
+        lds_barrier();
+        read_q();
+        lds_barrier();
       }
-      lds_barrier();
+      for (int i = 0; i < rounds; ++i) {
+        const int waves = min(chunks - (first + i) * kWaves, kWaves);
+        if (i + 1 < rounds) {
+          copy(i + 1);
+          wait_copies<kCopies>();
+        } else {
+          wait_copies<0>();
+        }
+        float own = -INFINITY, sum = 0.0f;
+        if (wave < waves) {
+          const uint32_t live_now = (uint32_t)(__ballot(slots_of(i) >= 0) >> (32 * (i & 1)));
+          score(mine + (i & 1) * kChunkBytes, live_now, own, sum);
+        }
+        lds_barrier();
+        int down[kWaves];
+        advance(waves, own, sum, down);
+        const uint32_t at = lds + (i & 1) * kChunkBytes;
+        if (waves == kWaves) {
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) values(at, w, down[w]);
+        } else {
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w)
+            if (w < waves) values(at, w, down[w]);
+        }
+        lds_barrier();
+      }
     }
   }
 
-  // The token's window rows [0, end), 16 a wave and round.
-  __device__ __forceinline__ void window(int end) {
+  // Weights of the wave's chunk at `at`; live: bit 16 tile + row.
+  __device__ __forceinline__ void score(uint32_t at, uint32_t live, float& own, float& sum) {
+    f32x4 acc[2][2] = {{zero_f(), zero_f()}, {zero_f(), zero_f()}};
+    u32x4 scale[2];
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile)
+      scale[tile] =
+          lds_read<u32x4>(at + tile * kTileBytes + row * kMx4RecordBytes + kMx4CodeBytes);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        const u32x4 code = lds_read<u32x4>(at + tile * kTileBytes + row * kMx4RecordBytes +
+                                           64 * j + 16 * group);
+        const uint32_t byte = (scale[tile][j] >> (8 * group)) & 0xffu;
+        const float f = mx4_scale(byte);
+        // record slot 8 (row / 4) + 4 tile + row % 4 of group 4 j + group
+        lds_write(lds + L::kShifts + 1024 * wave + 64 * (4 * j + group) +
+                      2 * (8 * (row >> 2) + 4 * tile + (row & 3)),
+                  (uint16_t)((kScaleRef - byte) << 7));
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          acc[tile][u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              as_bf16x8(fp4x8_to_bf16(code[u], f)), q[4 * j + u], acc[tile][u & 1], 0, 0, 0);
+      }
+    f32x4 s[2];
+    float top = -INFINITY;
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      s[tile] = scores(acc[tile][0] + acc[tile][1], live >> (16 * tile + 4 * group));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tile][i]);
+    }
+    own = ceilf(over_groups_max(top));
+    const float ref = own == -INFINITY ? 0.0f : own;
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p0 = __builtin_amdgcn_exp2f(s[i / 2][2 * (i % 2)] - ref);
+      const float p1 = __builtin_amdgcn_exp2f(s[i / 2][2 * (i % 2) + 1] - ref);
+      sum += p0 + p1;
+      w[i] = __builtin_bit_cast(uint32_t, bf16_pair(p0, p1));
+    }
+    lds_write(lds + L::kWeights + 1024 * wave + 16 * lane, w);
+    if (lane < 16) lds_write(lds + L::kTops + 64 * wave + 4 * lane, own);
+  }
+
+  // O += the records of wave w's chunk. at: the round's chunk of wave 0.
+  __device__ __forceinline__ void values(uint32_t at, int w, int down) {
+    u32x4 p = lds_read<u32x4>(lds + L::kWeights + 1024 * w + 16 * lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = sub_sat(p[i], (uint32_t)down * 0x00800080u);
+    const uint32_t codes = at + 2 * w * kChunkBytes + ((row >> 2) & 1) * kTileBytes +
+                           (4 * group + (row & 3)) * kMx4RecordBytes + 8 * (row >> 3);
+#pragma unroll
+    for (int b = 0; b < kTiles / 2; ++b) {
+      const int g = wave * (kTiles / 2) + b;
+      const u32x4 shift = lds_read<u32x4>(lds + L::kShifts + 1024 * w + 64 * g + 16 * group);
+      u32x4 pw;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pw[i] = sub_sat(p[i], shift[i]);
+      const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+          (lds_i32x2*)(lds_void*)(uintptr_t)(codes + 16 * g));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        o[2 * b + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            as_bf16x8(fp4x8_to_bf16((uint32_t)v[i], 1.0f)), as_bf16x8(pw), o[2 * b + i], 0, 0, 0);
+    }
+  }
+
+  // The share of the window: chunks of 16 rows, dealt from the last split down.
+  __device__ __forceinline__ void window(int live, int chunks) {
     const int32_t* const idx = a.swa_indices + t * a.swa_topk;
-    WaveLds& mine = lds[wave];
-    for (int at = 0; at < end; at += 16 * kWaves) {
-      const int waves = min((end - at + 15) / 16, kWaves);
+    const uint32_t at = lds + 2 * wave * kChunkBytes;
+    for (int first = 0; first < chunks; first += kWaves) {
+      const int waves = min(chunks - first, kWaves);
       float own = -INFINITY, sum = 0.0f;
       if (wave < waves) {
-        const int k = at + 16 * wave + row;
-        const int64_t slot = k < end ? idx[k] : -1;
-        const bool live = slot >= 0 && slot < a.swa_rows;
-        const uint8_t* page = a.swa_pool + (live ? slot >> 6 : 0) * kNativePageBytes;
-        const int in_page = live ? (int)(slot & 63) : 0;
+        const int k = 16 * ((first + wave) * a.splits + a.splits - 1 - split) + row;
+        const int64_t slot = k < live ? idx[k] : -1;
+        const bool ok = slot >= 0 && slot < a.swa_rows;
+        const uint8_t* page = a.swa_pool + (ok ? slot >> 6 : 0) * kNativePageBytes;
+        const int in_page = ok ? (int)(slot & 63) : 0;
         const uint8_t* data = page + in_page * kNativeDataBytes;
-        const uint32_t mask = (uint32_t)__ballot(live) & 0xffffu;
-        // The lane's 128 coordinates: 128 codes, or (group 3) 64 codes and the tail. A row
-        // that is no entry becomes zeros: its bytes could be codes or scales of NaN.
-        u32x4 code[8], tail[8];
+        const uint32_t mask = (uint32_t)__ballot(ok) & 0xffffu;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          code[c] = *(const u32x4*)(data + 128 * group + 16 * (group == 3 ? c & 3 : c));
-          tail[c] = *(const u32x4*)(data + kNopeDim + 16 * c);
-        }
-        const u32x2 srow =
-            *(const u32x2*)(page + kPageRecords * kNativeDataBytes + in_page * kScaleBytes);
-        const u32x4 zero = {0, 0, 0, 0};
-        uint8_t* const dst = mine.rows + row * kRowPitch;
+        for (int j = 0; j < 9; ++j) copy16(data + 64 * j + 16 * group, at + 1024 * j);
+        u32x2 srow = *(const u32x2*)(page + kPageRecords * kNativeDataBytes + in_page * kScaleBytes);
+        wait_copies<0>();
+        // A row that is no entry becomes zeros: its bytes could be codes or scales of NaN.
+        if (!ok) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          code[c] = live ? code[c] : zero;
-          tail[c] = live ? tail[c] : zero;
-          if (group < 3 || c < 4) *(u32x4*)(dst + 128 * group + 16 * c) = code[c];
-          if (group == 3) *(u32x4*)(dst + kNopeDim + 16 * c) = tail[c];
+          for (int j = 0; j < 9; ++j) lds_write(at + 1024 * j + 16 * lane, u32x4{0, 0, 0, 0});
+          srow = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
         }
-        const uint32_t sbytes = live ? srow[group >> 1] >> (16 * (group & 1)) : 0x7f7fu;
-        mine.scales[2 * group][row] = (uint8_t)sbytes;
-        mine.scales[2 * group + 1][row] = group == 3 ? 127 : (uint8_t)(sbytes >> 8);  // (tail: none)
-        f32x4 acc = zero_f();
+        srow[1] = (srow[1] & 0x00ffffffu) | 0x7f000000u;  // the tail has no scale
+#pragma unroll
+        for (int i = 0; i < 2; ++i)  // [64-coordinate group][row]
+          lds_write<uint8_t>(at + kWindowScalesAt + 16 * (2 * group + i) + row,
+                             (uint8_t)(srow[group >> 1] >> (16 * (group & 1) + 8 * i)));
+        wave_lds_sync();
+        f32x4 acc[2] = {zero_f(), zero_f()};
+        auto piece = [&](int n) { return at + 1024 * (n >> 2) + 256 * (n & 3) + 16 * row; };
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float f = u2f(((sbytes >> (8 * (j / 2))) & 0xffu) << 23);
+          const float f = u2f(((srow[j / 2] >> (16 * (j % 2) + 8 * (group >> 1))) & 0xffu) << 23);
+          // coordinates 128 j + 32 group: codes, or (448 and up) the BF16 tail
+          const bool tail = j == 3 && group >= 2;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const u32x4 c = code[2 * j + u / 2];
-            const uint32_t lo = c[2 * (u % 2)], hi = c[2 * (u % 2) + 1];
+            const u32x4 c16 = lds_read<u32x4>(piece(tail ? 28 + 4 * (group - 2) + u
+                                                         : 8 * j + 2 * group + u / 2));
+            const uint32_t lo = c16[2 * (u % 2)], hi = c16[2 * (u % 2) + 1];
             u32x4 k8 = {fp8_pair_to_bf16<false>(lo, f), fp8_pair_to_bf16<true>(lo, f),
                         fp8_pair_to_bf16<false>(hi, f), fp8_pair_to_bf16<true>(hi, f)};
-            if (j >= 2) k8 = group == 3 ? tail[4 * (j - 2) + u] : k8;
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k8), q[4 * j + u], acc, 0, 0, 0);
+            if (j == 3) k8 = tail ? c16 : k8;
+            acc[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k8), q[4 * j + u],
+                                                                 acc[u & 1], 0, 0, 0);
           }
         }
-        const f32x4 s = scores(acc, mask >> (4 * group));
+        const f32x4 s = scores(acc[0] + acc[1], mask >> (4 * group));
         own = ceilf(over_groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
         const float ref = own == -INFINITY ? 0.0f : own;
         f32x4 p;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[i] = exp2f(s[i] - ref);
+          p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
           sum += p[i];
         }
-        mine.weight[lane] = __builtin_bit_cast(u32x4, p);
-        if (lane < 16) mine.top[lane] = own;
+        lds_write(lds + L::kWeights + 1024 * wave + 16 * lane, __builtin_bit_cast(u32x4, p));
+        if (lane < 16) lds_write(lds + L::kTops + 64 * wave + 4 * lane, own);
       }
       lds_barrier();
-      advance(waves, own, sum);
+      int down[kWaves];
+      advance(waves, own, sum, down);
 #pragma unroll 1
       for (int w = 0; w < waves; ++w) {
-        const WaveLds& from = lds[w];
-        const float own_w = from.top[row];
-        const float f = own_w == -INFINITY ? 0.0f : exp2f(own_w - m);
-        f32x4 p = __builtin_bit_cast(f32x4, from.weight[lane]);
+        const uint32_t from = lds + 2 * w * kChunkBytes;
+        const float own_w = lds_read<float>(lds + L::kTops + 64 * w + 4 * row);
+        // (O is in units of 2^32)
+        const float f = own_w == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(own_w - m - 32.0f);
+        f32x4 p = lds_read<f32x4>(lds + L::kWeights + 1024 * w + 16 * lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] *= f;
         // 32 coordinates (two tiles) a turn: codes below 448, the BF16 tail above
 #pragma unroll
         for (int b = 0; b < kTiles / 2; ++b) {
-          const int c0 = 32 * (wave * (kTiles / 2) + b);
+          const int g = wave * (kTiles / 2) + b;
           s16x4 v[2];
-          if (c0 < kNopeDim) {
-            const uint8_t* src = from.rows + (4 * group + ((row >> 1) & 3)) * kRowPitch + c0 +
-                                 16 * (row >> 3) + 8 * (row & 1);
-            const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)src);
+          if (32 * g < kNopeDim) {
+            const int x = 32 * g + 16 * (row >> 3) + 8 * (row & 1);
+            const uint32_t src = from + 1024 * (x >> 6) + 256 * ((x >> 4) & 3) +
+                                 16 * (4 * group + ((row >> 1) & 3)) + (x & 8);
+            const i32x2 c8 =
+                __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)(uintptr_t)src);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t lo = fp8_pair_to_bf16<false>((uint32_t)c[i], 1.0f);
-              const uint32_t hi = fp8_pair_to_bf16<true>((uint32_t)c[i], 1.0f);
-              v[i] = __builtin_bit_cast(s16x4, u32x2{lo, hi});
-            }
+            for (int i = 0; i < 2; ++i)
+              v[i] = __builtin_bit_cast(s16x4, u32x2{fp8_pair_to_bf16<false>((uint32_t)c8[i], 1.0f),
+                                                     fp8_pair_to_bf16<true>((uint32_t)c8[i], 1.0f)});
           } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint8_t* src = from.rows + (4 * group + (row >> 2)) * kRowPitch + kNopeDim +
-                                   2 * (c0 - kNopeDim + 16 * i + 4 * (row & 3));
-              v[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)src);
+              const int x = kNopeDim + 2 * (32 * g - kNopeDim + 16 * i) + 8 * (row & 3);
+              const uint32_t src = from + 1024 * (x >> 6) + 256 * ((x >> 4) & 3) +
+                                   16 * (4 * group + (row >> 2)) + (x & 8);
+              v[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)(uintptr_t)src);
             }
           }
-          const uint32_t bytes = *(const uint32_t*)&from.scales[c0 / 64][4 * group];
+          const uint32_t bytes = lds_read<uint32_t>(from + kWindowScalesAt + 16 * (g / 2) + 4 * group);
           f32x4 pw;
 #pragma unroll
           for (int i = 0; i < 4; ++i) pw[i] = p[i] * u2f(((bytes >> (8 * i)) & 0xffu) << 23);
@@ -378,23 +511,20 @@ struct Decode {
       lds_barrier();
     }
   }
-  static __device__ __forceinline__ f32x4 zero_f() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
-  // unit: what O is in units of.
-  __device__ __forceinline__ void finish(int slot, float unit) {
+  __device__ __forceinline__ void finish() {
     l = over_groups_sum(l);
-    if (lane < 16) lds[wave].top[lane] = l;
+    if (lane < 16) lds_write(lds + L::kTops + 64 * wave + 4 * lane, l);
     lds_barrier();
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += lds[w].top[row];
+    for (int w = 0; w < kWaves; ++w) sum += lds_read<float>(lds + L::kTops + 64 * w + 4 * row);
     const int h = h0 + row;
-    const bool write = h < a.heads;
+    if (h >= a.heads) return;
     const int c0 = wave * kTiles * 16 + 4 * group;
     if (a.ws_splits != 0) {
-      const int64_t at = (t * a.ws_splits + slot) * a.heads + h;
-      const float f = sum != 0.0f ? unit / sum : 0.0f;
-      if (!write) return;
+      const int64_t at = (t * a.ws_splits + split) * a.heads + h;
+      const float f = sum != 0.0f ? 0x1p32f / sum : 0.0f;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
         __builtin_nontemporal_store(o[i] * f, (f32x4*)(a.ws_o + at * kHeadDim + c0 + 16 * i));
@@ -403,16 +533,15 @@ struct Decode {
         a.ws_lse[at] = sum != sum ? INFINITY : sum != 0.0f ? m + log2f(sum) : -INFINITY;
       return;
     }
-    const float sink2 = a.sink && write ? a.sink[h] * kLog2e : -INFINITY;
+    const float sink2 = a.sink ? a.sink[h] * kLog2e : -INFINITY;
     const float top = fmaxf(m, sink2);
     float f = 0.0f, lse = -INFINITY;
     if (top != -INFINITY || sum != 0.0f) {
       const float em = m == -INFINITY && sum == 0.0f ? 0.0f : exp2f(m - top);
       const float z = sum * em + exp2f(sink2 - top);
-      f = em * unit / z;
+      f = em * 0x1p32f / z;
       lse = (top + log2f(z)) * kLn2;
     }
-    if (!write) return;
     if (wave == 0 && lane < 16) a.lse[t * a.heads + h] = lse;
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
@@ -426,22 +555,26 @@ struct Decode {
 
 template <int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void mx4_decode_kernel(DecodeArgs a) {
-  __shared__ __attribute__((aligned(16))) WaveLds lds[kWaves];
-  Decode<kWaves> d(a, lds);
-  if ((int)blockIdx.x < a.splits) {
-    int live = a.topk;
-    if (a.topk_length) live = max(min(a.topk_length[d.t], live), 0);
-    // consecutive shares of whole 32-record tiles
-    const int share = ((live + a.splits - 1) / a.splits + 31) & ~31;
-    const int begin = min((int)blockIdx.x * share, live);
-    d.list(begin, min(begin + share, live));
-    d.finish(blockIdx.x, 0x1p32f);
-  } else {
-    int live = a.swa_topk;
-    if (a.swa_length) live = max(min(a.swa_length[d.t], live), 0);
-    d.window(live);
-    d.finish(blockIdx.x, 1.0f);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Lds<kWaves>::kBytes];
+  Decode<kWaves> d(a, (uint32_t)(uintptr_t)(lds_void*)lds);
+  d.copy_q();
+  int live = a.topk, rows = a.swa_topk;
+  if (a.topk_length) live = max(min(a.topk_length[d.t], live), 0);
+  if (a.swa_length) rows = max(min(a.swa_length[d.t], rows), 0);
+  // chunk numbers split, split + splits, ... below the list's
+  const int chunks = (int)(((uint64_t)((live + 31) / 32 - d.split + a.splits - 1) * a.splits_magic) >> 32);
+  const int back = (int)(((uint64_t)((rows + 15) / 16 + d.split) * a.splits_magic) >> 32);
+  if (chunks > 0) {
+    d.list(live, chunks);
+  } else if (back > 0) {
+    wait_copies<0>();
+    lds_barrier();
+    d.read_q();
+    lds_barrier();
   }
+  if (back > 0) d.window(rows, back);
+  wait_copies<0>();  // (of Q, where nothing used it: LDS outlives its copies)
+  d.finish();
 }
 
 bool aligned(const void* p, uintptr_t al) { return ((uintptr_t)p & (al - 1)) == 0; }
@@ -453,21 +586,19 @@ bool bad_sizes(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
 
 struct Plan {
   int waves;   // a workgroup
-  int splits;  // of the list (0: no list)
-  int slots;   // partial slots a row: the splits and the window rows' workgroup
+  int splits;  // workgroups a token and head group
 };
 
 // About one workgroup of eight waves a CU (256): enough splits to reach that, each
-// with a full round of records.
+// with a chunk of records for every wave.
 Plan plan(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
   Plan p;
   p.waves = 8;
   const int64_t base = std::max<int64_t>(tokens * ((heads + 15) / 16), 1);
-  const int64_t rounds = (topk + 32 * p.waves - 1) / (32 * p.waves);
+  const int64_t chunks = (topk + 31) / 32 + (swa_topk + 15) / 16;
   int64_t splits = (256 + base - 1) / base;
-  splits = std::min({splits, rounds, (int64_t)kMaxSplits - 1});
-  p.splits = (int)std::max<int64_t>(splits, topk > 0 || swa_topk == 0 ? 1 : 0);
-  p.slots = p.splits + (swa_topk > 0 ? 1 : 0);
+  splits = std::min({splits, (chunks + p.waves - 1) / p.waves, (int64_t)kMaxSplits});
+  p.splits = (int)std::max<int64_t>(splits, 1);
   return p;
 }
 size_t ws_bytes(int64_t tokens, int64_t heads, int64_t slots) {
@@ -481,8 +612,8 @@ extern "C" int rm_mx4_sparse_decode_workspace(int64_t tokens, int64_t heads, int
                                               size_t* workspace_bytes) {
   if (bad_sizes(tokens, heads, topk, swa_topk)) return RM_ERR_SHAPE;
   const Plan p = plan(tokens, heads, topk, swa_topk);
-  if (num_splits) *num_splits = p.slots;
-  if (workspace_bytes) *workspace_bytes = ws_bytes(tokens, heads, p.slots);
+  if (num_splits) *num_splits = p.splits;
+  if (workspace_bytes) *workspace_bytes = ws_bytes(tokens, heads, p.splits);
   return RM_OK;
 }
 
@@ -508,12 +639,12 @@ extern "C" int rm_mx4_sparse_decode_fwd(
       !aligned(swa_pool, 16))
     return RM_ERR_ALIGN;
   const Plan p = plan(tokens, heads, topk, swa_topk);
-  const size_t bytes = ws_bytes(tokens, heads, p.slots);
+  const size_t bytes = ws_bytes(tokens, heads, p.splits);
   if (bytes > 0 && (!workspace || workspace_bytes < bytes)) return RM_ERR_WORKSPACE;
   if (bytes > 0 && !aligned(workspace, 16)) return RM_ERR_ALIGN;
   DecodeArgs a;
   a.q = q;
-  a.q_len = (int)q_len;
+  a.q_len_magic = (((uint64_t)1 << 32) + q_len - 1) / q_len;
   a.heads = (int)heads;
   a.pool = pool;
   a.pool_pages = (int)pool_pages;
@@ -533,17 +664,18 @@ extern "C" int rm_mx4_sparse_decode_fwd(
   a.sink = sink;
   a.scale_log2 = softmax_scale * kLog2e;
   a.splits = p.splits;
-  a.ws_splits = p.slots > 1 ? p.slots : 0;
+  a.splits_magic = (((uint64_t)1 << 32) + p.splits - 1) / p.splits;
+  a.ws_splits = p.splits > 1 ? p.splits : 0;
   a.out = out;
   a.lse = lse;
   a.ws_o = (float*)workspace;
-  a.ws_lse = bytes ? (float*)workspace + (size_t)tokens * p.slots * heads * kHeadDim : nullptr;
+  a.ws_lse = bytes ? (float*)workspace + (size_t)tokens * p.splits * heads * kHeadDim : nullptr;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)p.slots, (unsigned)tokens, (unsigned)((heads + 15) / 16));
+  const dim3 grid((unsigned)p.splits, (unsigned)tokens, (unsigned)((heads + 15) / 16));
   hipLaunchKernelGGL(mx4_decode_kernel<8>, grid, dim3(64 * p.waves), 0, s, a);
   if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
-  if (p.slots > 1) {
-    launch_combine<true>(a.ws_o, a.ws_lse, sink, p.slots, tokens, heads, out, lse, s);
+  if (p.splits > 1) {
+    launch_combine<true>(a.ws_o, a.ws_lse, sink, p.splits, tokens, heads, out, lse, s);
     if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   }
   return RM_OK;
