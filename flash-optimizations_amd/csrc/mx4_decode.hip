@@ -4,28 +4,33 @@
 //   l_j = (q_h . K_j) * scale, Z = sum_j exp(l_j) + exp(sink_h),
 //   out = sum_j exp(l_j) K_j / Z, lse = ln Z.
 //
-// A workgroup of kWaves waves owns (split, token, 16 heads) and takes its share of the
-// list in rounds, 32 records a wave (a chunk; chunks are dealt to the splits and then
-// the waves in turn), then its share of the window, 16 rows a wave. A round has two
-// halves with a barrier between:
-//   * scores: a wave computes S^T = K Q^T of its chunk on v_mfma_f32_16x16x32_bf16, Q in
-//     registers, and leaves in LDS the weights P = 2^(s - m) as BF16, m the whole log2
-//     unit above the chunk's largest score, and each record's scale exponents.
-//   * values: a wave owns 512 / kWaves output coordinates of O^T += V^T P^T over all the
-//     round's records. The codes come out of LDS transposed (ds_read_b64_tr_b4) and
-//     become BF16 without their scales: those are powers of two that differ by record
-//     and group, so they go to the weights, and so does the step from a chunk's m to the
-//     running maximum: integer subtractions on the BF16 exponents, two weights an
-//     instruction, saturating at zero (v_pk_sub_u16 clamp), against the largest scale the
-//     store writes, 2^32; O is in units of it. A weight that a scale takes below 2^-126
-//     becomes zero: less than 2^-71 of the largest weight at that scale.
-// P^T in LDS is what the lane holding it writes, 16 bytes a lane: the order of the
-// records in the second product's long axis is free, and S^T's is taken.
+// A workgroup owns (split, token, 16 heads) and takes its share of the list in rounds of
+// kWaves / 2 chunks of 32 records (chunks are dealt to the splits and then in turn), then
+// its share of the window, 16 rows a wave and round. kWaves waves compute, half as many
+// more copy; one barrier a round. In the time between two barriers
+//   * a computing wave scores 16 records of round i: S^T = K Q^T on
+//     v_mfma_f32_16x16x32_bf16, Q in registers; it leaves in LDS the weights P = 2^(s -
+//     m) as BF16, m the whole log2 unit above the 16 records' largest score, and the
+//     records' scale exponents;
+//   * and adds all of round i - 1 to the 512 / kWaves output coordinates it owns: O^T +=
+//     V^T P^T. The codes come out of LDS transposed (ds_read_b64_tr_b4) and become BF16
+//     without their scales: those are powers of two that differ by record and group, so
+//     they go to the weights, and so does the step from a tile's m to the running
+//     maximum: integer subtractions on the BF16 exponents, two weights an instruction,
+//     saturating at zero (v_pk_sub_u16 clamp), against the largest scale the store
+//     writes, 2^32; O is in units of it. A weight that a scale takes below 2^-126 becomes
+//     zero: less than 2^-71 of the largest weight at that scale;
+//   * the copying waves fetch round i + 2 into the LDS that round i - 2 has left
+//     (global_load_lds, consecutive lanes taking consecutive 16-byte pieces of a record,
+//     17 a record, so that a copy touches each 128-byte line once), and wait for round
+//     i + 1. Waves that both computed and copied spent 40 % of a round held up at the
+//     issue of copies, with the memory idle for the rest of it.
+// P^T in LDS is what the lane holding it writes: the order of the records in the second
+// product's long axis is free, and S^T's is taken.
 //
-// A chunk's raw bytes go HBM -> LDS with global_load_lds, a round ahead of their use,
-// consecutive lanes copying consecutive 16-byte pieces of a record (17 a record), so
-// that a copy touches each 128-byte line once. The three loads between a list entry and
-// its record (index, block table, record) are made for kBatch rounds at a time.
+// At the start the list's entries, the block-table row (into LDS, up to kTableCache
+// columns), the lengths and Q are all requested together, so that the first records wait
+// for two round trips of memory and not for four.
 #include <algorithm>
 
 #include "combine.h"
@@ -77,32 +82,40 @@ struct DecodeArgs {
 };
 
 // A chunk in LDS: its records 272 bytes apart (4 banks), with 128 bytes between the
-// first 16 and the second, so that the transposed reads of a lane group's 2 x 4 records
-// meet no bank twice. 552 pieces of 16 bytes, 9 copies.
+// first 16 (tile 0) and the second, so that the transposed reads of a lane group's 2 x 4
+// records meet no bank twice. 552 pieces of 16 bytes, 9 copies.
 constexpr int kTilePieces = 16 * 17 + 8;
 constexpr int kTileBytes = 16 * kTilePieces;                     // 4,480
 constexpr int kChunkBytes = kTileBytes + 16 * kMx4RecordBytes;   // 8,832
 constexpr int kCopies = 9;
 constexpr int kLastLanes = 2 * kTilePieces - 8 - 64 * (kCopies - 1);  // of the last copy: 40
-constexpr int kBatch = 8;  // rounds whose slots are resolved together
+constexpr int kBuffers = 4;  // rounds in LDS: being added, being scored, two being copied
+constexpr int kBatch = 16;   // rounds whose slots are looked up together
+constexpr int kTableCache = 1024;  // block-table columns kept in LDS
 // A window chunk: 16 rows, 16-byte piece 4 j + g of row r at 1024 j + 256 g + 16 r, then
-// the scale bytes by group. It takes the room of two chunks.
+// the scale bytes by group.
 constexpr int kWindowScalesAt = 16 * kNativeDataBytes;
-static_assert(kWindowScalesAt + 128 <= 2 * kChunkBytes, "window chunk");
+constexpr int kWindowBytes = kWindowScalesAt + 128;
 constexpr int kScaleRef = 127 + kMx4MaxExponent;
 
-// LDS of a workgroup: two chunks a wave; then the weights (16 bytes a lane; a window
-// chunk: four floats), the scale exponents [16 groups][32 record slots] u16, (159 - scale
-// byte) << 7, and the references of the 16 heads, each by wave. Q passes through the
-// latter three at the start, a head's row every 1,040 bytes (4 banks).
+// LDS of a workgroup: the rounds' chunks (or a window chunk a wave); then, twice (odd and
+// even rounds), by chunk the weights (16 bytes a lane, tile 0's and tile 1's four; a
+// window chunk: four floats) and the scale exponents [16 groups][32 record slots] u16, (159
+// - scale byte) << 7, and by tile the references of the 16 heads; then the block-table row.
+// Q passes through the middle at the start, a head's row every 1,040 bytes (4 banks).
 template <int kWaves>
 struct Lds {
-  static constexpr int kWeights = 2 * kWaves * kChunkBytes;
-  static constexpr int kShifts = kWeights + 1024 * kWaves;
-  static constexpr int kTops = kShifts + 1024 * kWaves;
+  static constexpr int kChunks = kWaves / 2;
+  static constexpr int kRound = kChunks * kChunkBytes;
+  static constexpr int kWeights = kBuffers * kRound;
+  static constexpr int kShifts = kWeights + 2 * kChunks * 1024;
+  static constexpr int kTops = kShifts + 2 * kChunks * 1024;
+  static constexpr int kEnd = kTops + 2 * kWaves * 64;
   static constexpr int kQPitch = 1040;
-  static constexpr int kEnd = kTops + 64 * kWaves;
-  static constexpr int kBytes = kEnd > kWeights + 16 * kQPitch ? kEnd : kWeights + 16 * kQPitch;
+  static constexpr int kTable = kEnd > kWeights + 16 * kQPitch ? kEnd : kWeights + 16 * kQPitch;
+  static constexpr int kLive = kTable + 4 * kTableCache;  // [kBuffers][kChunks] bit masks
+  static constexpr int kBytes = kLive + 4 * kBuffers * kChunks;
+  static_assert(kBytes <= 160 * 1024 && kWaves * kWindowBytes <= kWeights, "LDS of a CU");
 };
 
 // Copies HBM -> LDS: 16 bytes a lane to lds + 16 lane. The LDS address is a plain number,
@@ -110,6 +123,10 @@ struct Lds {
 __device__ __forceinline__ void copy16(const void* src, uint32_t lds) {
   __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
                                    16, 0, 0);
+}
+__device__ __forceinline__ void copy4(const void* src, uint32_t lds) {
+  __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
+                                   4, 0, 0);
 }
 // Until at most kLater vector loads issued since are in flight.
 template <int kLater>
@@ -153,34 +170,174 @@ __device__ __forceinline__ uint32_t sub_sat(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ bf16x8 as_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 
+// What the waves of a workgroup share.
+template <int kWaves>
+struct Share {
+  const DecodeArgs& a;
+  const uint32_t lds;
+  const int lane, wave, split;
+  const int64_t t;
+  int live, rows, records;  // entries of the list and the window; records of the request
+  int chunks, back;         // the split's chunks of the list and the window
+  int rounds;
+
+  __device__ __forceinline__ Share(const DecodeArgs& args, uint32_t lds_at)
+      : a(args),
+        lds(lds_at),
+        lane(wave_lane()),
+        wave(uniform((int)(threadIdx.x >> 6))),
+        split((int)blockIdx.x),
+        t(blockIdx.y) {}
+  __device__ __forceinline__ int64_t request() const {
+    return (int64_t)(((uint64_t)t * a.q_len_magic) >> 32);
+  }
+  __device__ __forceinline__ void lengths() {
+    live = a.topk, rows = a.swa_topk, records = 0x7fffffff;
+    if (a.topk_length) live = max(min(a.topk_length[t], live), 0);
+    if (a.swa_length) rows = max(min(a.swa_length[t], rows), 0);
+    if (a.seqlens) records = a.seqlens[request()];
+    // list chunks split, split + splits, ...; window chunks splits - 1 - split, ...
+    chunks = (int)(((uint64_t)((live + 31) / 32 - split + a.splits - 1) * a.splits_magic) >> 32);
+    back = (int)(((uint64_t)((rows + 15) / 16 + split) * a.splits_magic) >> 32);
+    rounds = (chunks + kWaves / 2 - 1) / (kWaves / 2);
+  }
+};
+
+// A copying wave: chunk `wave - kWaves` of every round.
+template <int kWaves>
+struct Copier : Share<kWaves> {
+  using L = Lds<kWaves>;
+  using S = Share<kWaves>;
+  using S::a, S::lds, S::lane, S::wave, S::split, S::t;
+  const int of;  // the chunk of a round
+  const int32_t *idx, *table;
+  // Copy n takes piece 64 n + lane: of record from / 4 of the chunk, bytes off .. off + 15
+  // (the 8 pieces between the tiles copy some piece again). from | off << 8
+  uint32_t where[kCopies];
+  int slots[kBatch / 2];  // lane: entry lane % 32 of round 2 e + lane / 32; -1: no record
+
+  __device__ __forceinline__ Copier(const DecodeArgs& args, uint32_t lds_at)
+      : S(args, lds_at), of(S::wave - kWaves) {
+    idx = a.indices + t * a.topk;
+    table = a.block_table + this->request() * a.bt_stride;
+  }
+  __device__ __forceinline__ int entry(int first, int e) const {
+    const int c = (first + 2 * e + (lane >> 5)) * (kWaves / 2) + of;
+    return 32 * (c * a.splits + split) + (lane & 31);
+  }
+  // The first batch's entries, as far as the list's capacity goes: the length comes beside.
+  __device__ __forceinline__ void ask() {
+#pragma unroll
+    for (int e = 0; e < kBatch / 2; ++e) {
+      slots[e] = -1;
+      if (e * 32 * kWaves * a.splits < a.topk) slots[e] = idx[min(entry(0, e), a.topk - 1)];
+    }
+#pragma unroll
+    for (int n = 0; n < kCopies; ++n) {
+      const int p = 64 * n + lane, tile = p >= kTilePieces;
+      const int in_tile = min(p - tile * kTilePieces, 16 * 17 - 1);
+      const int r = in_tile * 241 >> 12;  // / 17, for numbers below 272
+      where[n] = (uint32_t)(4 * (16 * tile + r)) | (uint32_t)(16 * (in_tile - 17 * r)) << 8;
+    }
+  }
+  __device__ __forceinline__ void look_up(int first) {
+    const bool cached = a.max_blocks <= kTableCache;
+    int page[kBatch / 2];
+#pragma unroll
+    for (int e = 0; e < kBatch / 2; ++e) {
+      const int k = entry(first, e);
+      if (first > 0) slots[e] = k < this->live ? idx[k] : -1;
+      if (k >= this->live) slots[e] = -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kBatch / 2; ++e) {
+      const int r = slots[e];
+      const bool inside = r >= 0 && r < this->records && (r >> 6) < a.max_blocks;
+      page[e] = -1;
+      if (cached)
+        page[e] = lds_read<int>(lds + L::kTable + 4 * (inside ? r >> 6 : 0));
+      else if (inside)
+        page[e] = table[r >> 6];
+      if (!inside) page[e] = -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kBatch / 2; ++e)
+      slots[e] = page[e] >= 0 && page[e] < a.pool_pages
+                     ? page[e] * kPageRecords + (slots[e] & 63) : -1;
+  }
+  // The chunk of round i; its live records go to LDS.
+  __device__ __forceinline__ void copy(int i) {
+    const int of_round = slots[0];
+    if (i & 1) {  // (rounds come in turn)
+#pragma unroll
+      for (int e = 1; e < kBatch / 2; ++e) slots[e - 1] = slots[e];
+    }
+    const uint32_t to = lds + (i & (kBuffers - 1)) * L::kRound + of * kChunkBytes;
+    const uint32_t live_at = lds + L::kLive + 4 * ((i & (kBuffers - 1)) * L::kChunks + of);
+    const uint32_t mask = (uint32_t)(__ballot(of_round >= 0) >> (32 * (i & 1)));
+    int slot[kCopies];
+#pragma unroll
+    for (int n = 0; n < kCopies; ++n)
+      slot[n] = __builtin_amdgcn_ds_bpermute(128 * (i & 1) + (int)(where[n] & 0xff), of_round);
+    if (lane == 0) lds_write(live_at, mask);
+#pragma unroll
+    for (int n = 0; n < kCopies; ++n) {
+      const uint8_t* src = a.pool + ((int64_t)max(slot[n], 0) * kMx4RecordBytes + (where[n] >> 8));
+      if (n < kCopies - 1 || lane < kLastLanes) copy16(src, to + 1024 * n);
+    }
+  }
+  __device__ __forceinline__ void run() {
+    ask();
+    this->lengths();
+    lds_barrier();  // the block-table row
+    const int rounds = this->rounds;
+    if (rounds > 0) {
+      look_up(0);
+      copy(0);
+      if (rounds > 1) {
+        copy(1);
+        wait_copies<kCopies>();
+      } else {
+        wait_copies<0>();
+      }
+    }
+    lds_barrier();
+    for (int i = 0; i < rounds; ++i) {
+      if (i + 2 < rounds) {
+        if (((i + 2) & (kBatch - 1)) == 0) look_up(i + 2);
+        copy(i + 2);
+        wait_copies<kCopies>();
+      } else {
+        wait_copies<0>();
+      }
+      lds_barrier();
+    }
+  }
+};
+
 // 2^(from - to) for running maxima, 1 where both are -inf (nothing yet).
 __device__ __forceinline__ float step_down(float from, float to) {
   return from == to ? 1.0f : __builtin_amdgcn_exp2f(from - to);
 }
 
+// A computing wave.
 template <int kWaves>
-struct Decode {
+struct Decode : Share<kWaves> {
   using L = Lds<kWaves>;
+  using S = Share<kWaves>;
+  using S::a, S::lds, S::lane, S::wave, S::split, S::t;
   static constexpr int kTiles = kHeadDim / 16 / kWaves;  // 16-coordinate tiles of O a wave
-  const DecodeArgs& a;
-  const uint32_t lds;
-  const int lane, wave, row, group;  // row: record of a tile, or head; group: lane / 16
-  const int split;
-  const int64_t t;
+  const int row, group;  // row: record of a tile, or head; group: lane / 16
   const int h0;
   bf16x8 q[16];     // q[4 j + u]: coordinates 128 j + 32 group + 8 u .. + 7 of head `row`
   f32x4 o[kTiles];  // coordinate 16 tile + 4 group + i of the wave's, of head `row`
   float m, l;       // running maximum of head `row` (whole log2 units); this lane's sum
+  float owns, sums; // reference of the wave's last tile, sum of its weights against it
 
   __device__ __forceinline__ Decode(const DecodeArgs& args, uint32_t lds_at)
-      : a(args),
-        lds(lds_at),
-        lane(wave_lane()),
-        wave(uniform((int)(threadIdx.x >> 6))),
-        row(lane & 15),
-        group(lane >> 4),
-        split((int)blockIdx.x),
-        t(blockIdx.y),
+      : S(args, lds_at),
+        row(S::lane & 15),
+        group(S::lane >> 4),
         h0(blockIdx.z * 16),
         m(-INFINITY),
         l(0.0f) {
@@ -205,6 +362,15 @@ struct Decode {
       q[i] = as_bf16x8(lds_read<u32x4>(lds + L::kWeights + L::kQPitch * row + 256 * (i / 4) +
                                        64 * group + 16 * (i % 4)));
   }
+  __device__ __forceinline__ void copy_table() const {
+    const int32_t* const table = a.block_table + this->request() * a.bt_stride;
+    if (a.max_blocks > kTableCache || a.topk == 0) return;
+#pragma unroll
+    for (int n = 0; n < kTableCache / 64 / kWaves; ++n) {
+      const int c = 64 * (n * kWaves + wave);
+      if (c < a.max_blocks) copy4(table + min(c + lane, a.max_blocks - 1), lds + L::kTable + 4 * c);
+    }
+  }
 
   // s in log2 units, -inf where bit i of `live` is off.
   __device__ __forceinline__ f32x4 scores(f32x4 acc, uint32_t live) const {
@@ -212,20 +378,8 @@ struct Decode {
     for (int i = 0; i < 4; ++i) acc[i] = (live >> i) & 1 ? acc[i] * a.scale_log2 : -INFINITY;
     return acc;
   }
-  // The round's running maximum, from what the waves left; rescales O and l. down[w]: whole
-  // log2 units from wave w's reference to it, at most 255 (past every exponent).
-  __device__ __forceinline__ void advance(int waves, float own, float sum, int (&down)[kWaves]) {
-    float top = m, of[kWaves];
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) of[w] = lds_read<float>(lds + L::kTops + 64 * w + 4 * row);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      if (w >= waves) of[w] = -INFINITY;
-      top = fmaxf(top, of[w]);
-    }
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      down[w] = of[w] == -INFINITY ? 255 : (int)fminf(top - of[w], 255.0f);
+  // Against the new maximum `top`: O, and l with the weights `sum` that are against `own`.
+  __device__ __forceinline__ void advance(float top, float own, float sum) {
     const float f = step_down(m, top);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) o[i] *= f;
@@ -234,179 +388,170 @@ struct Decode {
     m = top;
   }
 
-  // The share of the list: `chunks` chunks of 32 entries, the c-th number c * splits + split.
-  __device__ __forceinline__ void list(int live, int chunks) {
-    const int64_t request = (int64_t)(((uint64_t)t * a.q_len_magic) >> 32);
-    const int32_t* const idx = a.indices + t * a.topk;
-    const int32_t* const table = a.block_table + request * a.bt_stride;
-    const int records = a.seqlens ? a.seqlens[request] : 0x7fffffff;
-    const uint32_t mine = lds + 2 * wave * kChunkBytes;
-    // Copy n takes piece 64 n + lane: of record from / 4 of the chunk, bytes off .. off + 15
-    // (the 8 pieces between the tiles copy some piece again).
-    uint32_t where[kCopies];  // from | off << 8
+  // What the wave reads of its tile to score it.
+  struct Tile {
+    u32x4 code[4], scale;
+    uint32_t bytes, live;
+  };
+  __device__ __forceinline__ void tile(int i, Tile& x) const {
+    const uint32_t at = lds + (i & (kBuffers - 1)) * L::kRound + (wave >> 1) * kChunkBytes +
+                        (wave & 1) * kTileBytes;
+    const uint32_t rec = at + row * kMx4RecordBytes;
 #pragma unroll
-    for (int n = 0; n < kCopies; ++n) {
-      const int p = 64 * n + lane, tile = p >= kTilePieces;
-      const int in_tile = min(p - tile * kTilePieces, 16 * 17 - 1);
-      const int r = in_tile * 241 >> 12;  // / 17, for numbers below 272
-      where[n] = (uint32_t)(4 * (16 * tile + r)) | (uint32_t)(16 * (in_tile - 17 * r)) << 8;
-    }
-    for (int first = 0; first * kWaves < chunks; first += kBatch) {
-      const int rounds = min((chunks - first * kWaves + kWaves - 1) / kWaves, kBatch);
-      int slots[kBatch / 2];  // lane: entry lane % 32 of round 2 e + lane / 32; -1: no record
-      {
-        int r[kBatch / 2], page[kBatch / 2];
-#pragma unroll
-        for (int e = 0; e < kBatch / 2; ++e) {
-          r[e] = -1;
-          if (2 * e < rounds) {
-            const int c = (first + 2 * e + (lane >> 5)) * kWaves + wave;
-            const int k = 32 * (c * a.splits + split) + (lane & 31);
-            if (k < live) r[e] = idx[k];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < kBatch / 2; ++e) {
-          const bool inside = r[e] >= 0 && r[e] < records && (r[e] >> 6) < a.max_blocks;
-          page[e] = inside ? table[r[e] >> 6] : -1;
-        }
-#pragma unroll
-        for (int e = 0; e < kBatch / 2; ++e)
-          slots[e] = page[e] >= 0 && page[e] < a.pool_pages
-                         ? page[e] * kPageRecords + (r[e] & 63) : -1;
-      }
-      auto slots_of = [&](int i) {  // lanes 32 (i % 2) ..: round i's
-        const int s0 = slots[0], s1 = slots[1], s2 = slots[2], s3 = slots[3];
-        return i < 4 ? (i < 2 ? s0 : s1) : (i < 6 ? s2 : s3);
-      };
-      auto copy = [&](int i) {
-        const uint32_t to = mine + (i & 1) * kChunkBytes;
-        const int of = slots_of(i), base = 128 * (i & 1);
-#pragma unroll
-        for (int n = 0; n < kCopies; ++n) {
-          const int slot = __builtin_amdgcn_ds_bpermute(base + (int)(where[n] & 0xff), of);
-          const uint8_t* src =
-              a.pool + ((int64_t)max(slot, 0) * kMx4RecordBytes + (where[n] >> 8));
-          if (n < kCopies - 1 || lane < kLastLanes) copy16(src, to + 1024 * n);
-        }
-      };
-      copy(0);
-      if (first == 0) {
-        wait_copies<kCopies>();  // Q
-        lds_barrier();
-        read_q();
-        lds_barrier();
-      }
-      for (int i = 0; i < rounds; ++i) {
-        const int waves = min(chunks - (first + i) * kWaves, kWaves);
-        if (i + 1 < rounds) {
-          copy(i + 1);
-          wait_copies<kCopies>();
-        } else {
-          wait_copies<0>();
-        }
-        float own = -INFINITY, sum = 0.0f;
-        if (wave < waves) {
-          const uint32_t live_now = (uint32_t)(__ballot(slots_of(i) >= 0) >> (32 * (i & 1)));
-          score(mine + (i & 1) * kChunkBytes, live_now, own, sum);
-        }
-        lds_barrier();
-        int down[kWaves];
-        advance(waves, own, sum, down);
-        const uint32_t at = lds + (i & 1) * kChunkBytes;
-        if (waves == kWaves) {
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) values(at, w, down[w]);
-        } else {
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w)
-            if (w < waves) values(at, w, down[w]);
-        }
-        lds_barrier();
-      }
-    }
+    for (int j = 0; j < 4; ++j) x.code[j] = lds_read<u32x4>(rec + 64 * j + 16 * group);
+    x.scale = lds_read<u32x4>(rec + kMx4CodeBytes);
+    // lane c of a group: scale byte c of the group's four records
+    const i32x2 two = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)(uintptr_t)(
+        at + (4 * group + ((row >> 1) & 3)) * kMx4RecordBytes + kMx4CodeBytes + 8 * (row & 1)));
+    x.bytes = (uint32_t)two[0];
+    x.live = lds_read<uint32_t>(lds + L::kLive +
+                                4 * ((i & (kBuffers - 1)) * L::kChunks + (wave >> 1))) >>
+             (16 * (wave & 1) + 4 * group);
   }
-
-  // Weights of the wave's chunk at `at`; live: bit 16 tile + row.
-  __device__ __forceinline__ void score(uint32_t at, uint32_t live, float& own, float& sum) {
-    f32x4 acc[2][2] = {{zero_f(), zero_f()}, {zero_f(), zero_f()}};
-    u32x4 scale[2];
+  // Round i's weights, scale exponents and reference of the wave's tile, to LDS. between():
+  // run behind the product, when the tile's registers are free.
+  template <class F>
+  __device__ __forceinline__ void score(int i, const Tile& x, const F& between) {
+    const uint32_t chunk = (i & 1) * L::kChunks + (wave >> 1);
+    f32x4 acc[2] = {zero_f(), zero_f()};
 #pragma unroll
-    for (int tile = 0; tile < 2; ++tile)
-      scale[tile] =
-          lds_read<u32x4>(at + tile * kTileBytes + row * kMx4RecordBytes + kMx4CodeBytes);
+    for (int j = 0; j < 4; ++j) {
+      const float f = mx4_scale((x.scale[j] >> (8 * group)) & 0xffu);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int tile = 0; tile < 2; ++tile) {
-        const u32x4 code = lds_read<u32x4>(at + tile * kTileBytes + row * kMx4RecordBytes +
-                                           64 * j + 16 * group);
-        const uint32_t byte = (scale[tile][j] >> (8 * group)) & 0xffu;
-        const float f = mx4_scale(byte);
-        // record slot 8 (row / 4) + 4 tile + row % 4 of group 4 j + group
-        lds_write(lds + L::kShifts + 1024 * wave + 64 * (4 * j + group) +
-                      2 * (8 * (row >> 2) + 4 * tile + (row & 3)),
-                  (uint16_t)((kScaleRef - byte) << 7));
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          acc[tile][u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              as_bf16x8(fp4x8_to_bf16(code[u], f)), q[4 * j + u], acc[tile][u & 1], 0, 0, 0);
-      }
-    f32x4 s[2];
-    float top = -INFINITY;
-#pragma unroll
-    for (int tile = 0; tile < 2; ++tile) {
-      s[tile] = scores(acc[tile][0] + acc[tile][1], live >> (16 * tile + 4 * group));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tile][i]);
+      for (int u = 0; u < 4; ++u)
+        acc[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            as_bf16x8(fp4x8_to_bf16(x.code[j][u], f)), q[4 * j + u], acc[u & 1], 0, 0, 0);
     }
-    own = ceilf(over_groups_max(top));
+    u32x2 shift;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t two = __builtin_amdgcn_perm(0, x.bytes, k ? 0x0c030c02u : 0x0c010c00u);
+      const u16x2 down = u16x2{kScaleRef, kScaleRef} - __builtin_bit_cast(u16x2, two);
+      shift[k] = __builtin_bit_cast(uint32_t, (u16x2)(down << 7));
+    }
+    lds_write(lds + L::kShifts + 1024 * chunk + 64 * row + 16 * group + 8 * (wave & 1), shift);
+    __builtin_amdgcn_sched_barrier(0);
+    between();
+    __builtin_amdgcn_sched_barrier(0);
+    const f32x4 s = scores(acc[0] + acc[1], x.live);
+    const float own = ceilf(over_groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
     const float ref = own == -INFINITY ? 0.0f : own;
-    u32x4 w;
+    owns = own;
+    float p[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float p0 = __builtin_amdgcn_exp2f(s[i / 2][2 * (i % 2)] - ref);
-      const float p1 = __builtin_amdgcn_exp2f(s[i / 2][2 * (i % 2) + 1] - ref);
-      sum += p0 + p1;
-      w[i] = __builtin_bit_cast(uint32_t, bf16_pair(p0, p1));
-    }
-    lds_write(lds + L::kWeights + 1024 * wave + 16 * lane, w);
-    if (lane < 16) lds_write(lds + L::kTops + 64 * wave + 4 * lane, own);
+    for (int k = 0; k < 4; ++k) p[k] = __builtin_amdgcn_exp2f(s[k] - ref);
+    sums = (p[0] + p[1]) + (p[2] + p[3]);
+    lds_write(lds + L::kWeights + 1024 * chunk + 16 * lane + 8 * (wave & 1),
+              u32x2{__builtin_bit_cast(uint32_t, bf16_pair(p[0], p[1])),
+                    __builtin_bit_cast(uint32_t, bf16_pair(p[2], p[3]))});
+    if (lane < 16) lds_write(lds + L::kTops + 64 * ((i & 1) * kWaves + wave) + 4 * lane, own);
+  }
+  // A tile that the round does not have: weights of zero.
+  __device__ __forceinline__ void no_score(int i) {
+    const uint32_t chunk = (i & 1) * L::kChunks + (wave >> 1);
+    owns = -INFINITY;
+    sums = 0.0f;
+    lds_write(lds + L::kWeights + 1024 * chunk + 16 * lane + 8 * (wave & 1), u32x2{0, 0});
+    if (lane < 16) lds_write(lds + L::kTops + 64 * ((i & 1) * kWaves + wave) + 4 * lane, -INFINITY);
   }
 
-  // O += the records of wave w's chunk. at: the round's chunk of wave 0.
-  __device__ __forceinline__ void values(uint32_t at, int w, int down) {
-    u32x4 p = lds_read<u32x4>(lds + L::kWeights + 1024 * w + 16 * lane);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = sub_sat(p[i], (uint32_t)down * 0x00800080u);
-    const uint32_t codes = at + 2 * w * kChunkBytes + ((row >> 2) & 1) * kTileBytes +
+  // What the wave reads of one chunk for its coordinates.
+  struct Operands {
+    u32x4 p, shift[kTiles / 2];
+    i32x2 v[kTiles / 2];
+  };
+  __device__ __forceinline__ void operands(int i, int c, Operands& x) const {
+    const uint32_t chunk = (i & 1) * L::kChunks + c;
+    x.p = lds_read<u32x4>(lds + L::kWeights + 1024 * chunk + 16 * lane);
+    const uint32_t codes = lds + (i & (kBuffers - 1)) * L::kRound + c * kChunkBytes +
+                           ((row >> 2) & 1) * kTileBytes +
                            (4 * group + (row & 3)) * kMx4RecordBytes + 8 * (row >> 3);
 #pragma unroll
     for (int b = 0; b < kTiles / 2; ++b) {
       const int g = wave * (kTiles / 2) + b;
-      const u32x4 shift = lds_read<u32x4>(lds + L::kShifts + 1024 * w + 64 * g + 16 * group);
+      x.shift[b] = lds_read<u32x4>(lds + L::kShifts + 1024 * chunk + 64 * g + 16 * group);
+      x.v[b] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+          (lds_i32x2*)(lds_void*)(uintptr_t)(codes + 16 * g));
+    }
+  }
+  // O += a chunk; of: its tiles' references.
+  __device__ __forceinline__ void values(Operands& x, float of0, float of1) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float of = k ? of1 : of0;
+      // whole log2 units down to the maximum (255: past every exponent)
+      const uint32_t down = of == -INFINITY ? 255 : (uint32_t)(int)fminf(m - of, 255.0f);
+      x.p[2 * k] = sub_sat(x.p[2 * k], down * 0x00800080u);
+      x.p[2 * k + 1] = sub_sat(x.p[2 * k + 1], down * 0x00800080u);
+    }
+#pragma unroll
+    for (int b = 0; b < kTiles / 2; ++b) {
       u32x4 pw;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pw[i] = sub_sat(p[i], shift[i]);
-      const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-          (lds_i32x2*)(lds_void*)(uintptr_t)(codes + 16 * g));
+      for (int i = 0; i < 4; ++i) pw[i] = sub_sat(x.p[i], x.shift[b][i]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         o[2 * b + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            as_bf16x8(fp4x8_to_bf16((uint32_t)v[i], 1.0f)), as_bf16x8(pw), o[2 * b + i], 0, 0, 0);
+            as_bf16x8(fp4x8_to_bf16((uint32_t)x.v[b][i], 1.0f)), as_bf16x8(pw), o[2 * b + i], 0, 0,
+            0);
+    }
+  }
+
+  // The share of the list: chunk c of the split's is number c * splits + split.
+  __device__ __forceinline__ void list() {
+    for (int i = 0; i <= this->rounds; ++i) {
+      const bool scoring = i < this->rounds &&
+                           i * L::kChunks + (wave >> 1) < this->chunks;
+      Tile x;
+      Operands y[2];
+      float of[kWaves];
+      const float own = owns, sum = sums;
+      auto ahead = [&] {
+        if (i == 0) return;
+        operands(i - 1, 0, y[0]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+          of[w] = lds_read<float>(lds + L::kTops + 64 * (((i - 1) & 1) * kWaves + w) + 4 * row);
+      };
+      if (scoring) {
+        tile(i, x);
+        __builtin_amdgcn_sched_barrier(0);
+        score(i, x, ahead);
+      } else {
+        ahead();
+        if (i < this->rounds) no_score(i);
+      }
+      if (i > 0) {
+        float top = m;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, of[w]);
+        advance(top, own, sum);
+#pragma unroll
+        for (int c = 0; c < L::kChunks; ++c) {
+          if (c + 1 < L::kChunks) operands(i - 1, c + 1, y[(c + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          values(y[c & 1], of[2 * c], of[2 * c + 1]);
+        }
+      }
+      if (i < this->rounds) lds_barrier();
     }
   }
 
   // The share of the window: chunks of 16 rows, dealt from the last split down.
-  __device__ __forceinline__ void window(int live, int chunks) {
-    const int32_t* const idx = a.swa_indices + t * a.swa_topk;
-    const uint32_t at = lds + 2 * wave * kChunkBytes;
-    for (int first = 0; first < chunks; first += kWaves) {
-      const int waves = min(chunks - first, kWaves);
+  __device__ __forceinline__ int window_entry(int first) const {
+    return 16 * ((first + wave) * a.splits + a.splits - 1 - split) + row;
+  }
+  __device__ __forceinline__ void window(int early) {
+    const int32_t* const swa = a.swa_indices + t * a.swa_topk;
+    const uint32_t at = lds + wave * kWindowBytes;
+    for (int first = 0; first < this->back; first += kWaves) {
+      const int waves = min(this->back - first, kWaves);
       float own = -INFINITY, sum = 0.0f;
+      lds_barrier();
       if (wave < waves) {
-        const int k = 16 * ((first + wave) * a.splits + a.splits - 1 - split) + row;
-        const int64_t slot = k < live ? idx[k] : -1;
+        const int k = window_entry(first);
+        int64_t slot = first == 0 ? early : k < this->rows ? swa[k] : -1;
+        if (k >= this->rows) slot = -1;
         const bool ok = slot >= 0 && slot < a.swa_rows;
         const uint8_t* page = a.swa_pool + (ok ? slot >> 6 : 0) * kNativePageBytes;
         const int in_page = ok ? (int)(slot & 63) : 0;
@@ -460,11 +605,14 @@ struct Decode {
         if (lane < 16) lds_write(lds + L::kTops + 64 * wave + 4 * lane, own);
       }
       lds_barrier();
-      int down[kWaves];
-      advance(waves, own, sum, down);
+      float top = m;
+#pragma unroll 1
+      for (int w = 0; w < waves; ++w)
+        top = fmaxf(top, lds_read<float>(lds + L::kTops + 64 * w + 4 * row));
+      advance(top, own, sum);
 #pragma unroll 1
       for (int w = 0; w < waves; ++w) {
-        const uint32_t from = lds + 2 * w * kChunkBytes;
+        const uint32_t from = lds + w * kWindowBytes;
         const float own_w = lds_read<float>(lds + L::kTops + 64 * w + 4 * row);
         // (O is in units of 2^32)
         const float f = own_w == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(own_w - m - 32.0f);
@@ -514,6 +662,7 @@ struct Decode {
 
   __device__ __forceinline__ void finish() {
     l = over_groups_sum(l);
+    lds_barrier();
     if (lane < 16) lds_write(lds + L::kTops + 64 * wave + 4 * lane, l);
     lds_barrier();
     float sum = 0.0f;
@@ -554,26 +703,26 @@ struct Decode {
 };
 
 template <int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void mx4_decode_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(96 * kWaves) void mx4_decode_kernel(DecodeArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[Lds<kWaves>::kBytes];
-  Decode<kWaves> d(a, (uint32_t)(uintptr_t)(lds_void*)lds);
-  d.copy_q();
-  int live = a.topk, rows = a.swa_topk;
-  if (a.topk_length) live = max(min(a.topk_length[d.t], live), 0);
-  if (a.swa_length) rows = max(min(a.swa_length[d.t], rows), 0);
-  // chunk numbers split, split + splits, ... below the list's
-  const int chunks = (int)(((uint64_t)((live + 31) / 32 - d.split + a.splits - 1) * a.splits_magic) >> 32);
-  const int back = (int)(((uint64_t)((rows + 15) / 16 + d.split) * a.splits_magic) >> 32);
-  if (chunks > 0) {
-    d.list(live, chunks);
-  } else if (back > 0) {
-    wait_copies<0>();
-    lds_barrier();
-    d.read_q();
-    lds_barrier();
+  const uint32_t at = (uint32_t)(uintptr_t)(lds_void*)lds;
+  if (threadIdx.x >= 64 * kWaves) {  // (s_barrier counts the waves that have not ended)
+    Copier<kWaves>(a, at).run();
+    return;
   }
-  if (back > 0) d.window(rows, back);
-  wait_copies<0>();  // (of Q, where nothing used it: LDS outlives its copies)
+  Decode<kWaves> d(a, at);
+  d.copy_table();
+  d.copy_q();
+  int early = -1;
+  if (a.swa_topk > 0)
+    early = a.swa_indices[d.t * a.swa_topk + min(d.window_entry(0), a.swa_topk - 1)];
+  d.lengths();
+  wait_copies<0>();
+  lds_barrier();
+  d.read_q();
+  lds_barrier();
+  if (d.rounds > 0) d.list();
+  if (d.back > 0) d.window(early);
   d.finish();
 }
 
@@ -589,15 +738,15 @@ struct Plan {
   int splits;  // workgroups a token and head group
 };
 
-// About one workgroup of eight waves a CU (256): enough splits to reach that, each
-// with a chunk of records for every wave.
+// About one workgroup a CU (256): enough splits to reach that, each with a round of its
+// own.
 Plan plan(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
   Plan p;
   p.waves = 8;
   const int64_t base = std::max<int64_t>(tokens * ((heads + 15) / 16), 1);
-  const int64_t chunks = (topk + 31) / 32 + (swa_topk + 15) / 16;
-  int64_t splits = (256 + base - 1) / base;
-  splits = std::min({splits, (chunks + p.waves - 1) / p.waves, (int64_t)kMaxSplits});
+  const int64_t rounds = std::max((topk + 16 * p.waves - 1) / (16 * p.waves),
+                                  (swa_topk + 16 * p.waves - 1) / (16 * p.waves));
+  const int64_t splits = std::min({(256 + base - 1) / base, rounds, (int64_t)kMaxSplits});
   p.splits = (int)std::max<int64_t>(splits, 1);
   return p;
 }
@@ -672,7 +821,7 @@ extern "C" int rm_mx4_sparse_decode_fwd(
   a.ws_lse = bytes ? (float*)workspace + (size_t)tokens * p.splits * heads * kHeadDim : nullptr;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)p.splits, (unsigned)tokens, (unsigned)((heads + 15) / 16));
-  hipLaunchKernelGGL(mx4_decode_kernel<8>, grid, dim3(64 * p.waves), 0, s, a);
+  hipLaunchKernelGGL(mx4_decode_kernel<8>, grid, dim3(96 * p.waves), 0, s, a);
   if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   if (p.splits > 1) {
     launch_combine<true>(a.ws_o, a.ws_lse, sink, p.splits, tokens, heads, out, lse, s);
