@@ -10,13 +10,14 @@
 // more copy; one barrier a round. In the time between two barriers
 //   * a computing wave scores 16 records of round i: S^T = K Q^T on
 //     v_mfma_f32_16x16x32_bf16, Q in registers; it leaves in LDS the weights P = 2^(s -
-//     m) as BF16, m the whole log2 unit above the 16 records' largest score, and the
-//     records' scale exponents;
+//     m) as BF16, m the running maximum (in whole log2 units) as far as the wave knows
+//     it, or where a score passes that by 2^24, the unit above the tile's largest (weights
+//     of up to 2^24 are no loss in a floating format), and the records' scale exponents;
 //   * and adds all of round i - 1 to the 512 / kWaves output coordinates it owns: O^T +=
 //     V^T P^T. The codes come out of LDS transposed (ds_read_b64_tr_b4) and become BF16
 //     without their scales: those are powers of two that differ by record and group, so
-//     they go to the weights, and so does the step from a tile's m to the running
-//     maximum: integer subtractions on the BF16 exponents, two weights an instruction,
+//     they go to the weights, and so does, where the round has any, the step from a
+//     tile's m to the running maximum: integer subtractions on the BF16 exponents, two weights an instruction,
 //     saturating at zero (v_pk_sub_u16 clamp), against the largest scale the store
 //     writes, 2^32; O is in units of it. A weight that a scale takes below 2^-126 becomes
 //     zero: less than 2^-71 of the largest weight at that scale;
@@ -97,6 +98,7 @@ constexpr int kTableCache = 1024;  // block-table columns kept in LDS
 constexpr int kWindowScalesAt = 16 * kNativeDataBytes;
 constexpr int kWindowBytes = kWindowScalesAt + 128;
 constexpr int kScaleRef = 127 + kMx4MaxExponent;
+constexpr float kSlack = 24.0f;  // log2 units a score may pass the running maximum by
 
 // LDS of a workgroup: the rounds' chunks (or a window chunk a wave); then, twice (odd and
 // even rounds), by chunk the weights (16 bytes a lane, tile 0's and tile 1's four; a
@@ -114,7 +116,9 @@ struct Lds {
   static constexpr int kQPitch = 1040;
   static constexpr int kTable = kEnd > kWeights + 16 * kQPitch ? kEnd : kWeights + 16 * kQPitch;
   static constexpr int kLive = kTable + 4 * kTableCache;  // [kBuffers][kChunks] bit masks
-  static constexpr int kBytes = kLive + 4 * kBuffers * kChunks;
+  static constexpr int kMoved = kLive + 4 * kBuffers * kChunks;  // [4]: a round moves m
+  static constexpr int kEarly = kMoved + 16;                     // [kWaves][16] window slots
+  static constexpr int kBytes = kEarly + 64 * kWaves;
   static_assert(kBytes <= 160 * 1024 && kWaves * kWindowBytes <= kWeights, "LDS of a CU");
 };
 
@@ -380,12 +384,15 @@ struct Decode : Share<kWaves> {
   }
   // Against the new maximum `top`: O, and l with the weights `sum` that are against `own`.
   __device__ __forceinline__ void advance(float top, float own, float sum) {
-    const float f = step_down(m, top);
+    if (__ballot(top != m) != 0) {
+      const float f = step_down(m, top);
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) o[i] *= f;
+      for (int i = 0; i < kTiles; ++i) o[i] *= f;
+      l *= f;
+      m = top;
+    }
     // (sum is zero where own is -inf, and NaN stays NaN)
-    l = l * f + (own == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f(own - top));
-    m = top;
+    l += own == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f(own - top);
   }
 
   // What the wave reads of its tile to score it.
@@ -434,8 +441,10 @@ struct Decode : Share<kWaves> {
     between();
     __builtin_amdgcn_sched_barrier(0);
     const f32x4 s = scores(acc[0] + acc[1], x.live);
-    const float own = ceilf(over_groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
+    const float top = over_groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const float own = top > m + kSlack ? ceilf(top) : m;
     const float ref = own == -INFINITY ? 0.0f : own;
+    if (__ballot(own != m) != 0 && lane == 0) lds_write(lds + L::kMoved + 4 * (i & 3), 1);
     owns = own;
     float p[4];
 #pragma unroll
@@ -455,93 +464,132 @@ struct Decode : Share<kWaves> {
     if (lane < 16) lds_write(lds + L::kTops + 64 * ((i & 1) * kWaves + wave) + 4 * lane, -INFINITY);
   }
 
-  // What the wave reads of one chunk for its coordinates.
+  // What the wave reads of a chunk for its coordinates: the weights, and by group (32
+  // coordinates) the scale exponents and codes.
   struct Operands {
-    u32x4 p, shift[kTiles / 2];
-    i32x2 v[kTiles / 2];
+    u32x4 shift;
+    i32x2 v;
   };
-  __device__ __forceinline__ void operands(int i, int c, Operands& x) const {
-    const uint32_t chunk = (i & 1) * L::kChunks + c;
-    x.p = lds_read<u32x4>(lds + L::kWeights + 1024 * chunk + 16 * lane);
-    const uint32_t codes = lds + (i & (kBuffers - 1)) * L::kRound + c * kChunkBytes +
-                           ((row >> 2) & 1) * kTileBytes +
-                           (4 * group + (row & 3)) * kMx4RecordBytes + 8 * (row >> 3);
-#pragma unroll
-    for (int b = 0; b < kTiles / 2; ++b) {
-      const int g = wave * (kTiles / 2) + b;
-      x.shift[b] = lds_read<u32x4>(lds + L::kShifts + 1024 * chunk + 64 * g + 16 * group);
-      x.v[b] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-          (lds_i32x2*)(lds_void*)(uintptr_t)(codes + 16 * g));
-    }
+  // By chunk c at w_at + 1024 c, s_at + 1024 c + 64 b and v_at + kChunkBytes c + 16 b.
+  struct Places {
+    uint32_t w_at, s_at, v_at;
+  };
+  __device__ __forceinline__ Places places(int i) const {
+    const uint32_t odd = (i & 1) * 1024 * L::kChunks;
+    return {lds + L::kWeights + odd + 16 * lane,
+            lds + L::kShifts + odd + 64 * wave * (kTiles / 2) + 16 * group,
+            lds + (i & (kBuffers - 1)) * L::kRound + ((row >> 2) & 1) * kTileBytes +
+                (4 * group + (row & 3)) * kMx4RecordBytes + 8 * (row >> 3) + 16 * wave * (kTiles / 2)};
   }
-  // O += a chunk; of: its tiles' references.
-  __device__ __forceinline__ void values(Operands& x, float of0, float of1) {
+  __device__ __forceinline__ void operands(const Places& at, int c, int b, Operands& x) const {
+    x.shift = lds_read<u32x4>(at.s_at + 1024 * c + 64 * b);
+    x.v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+        (lds_i32x2*)(lds_void*)(uintptr_t)(at.v_at + kChunkBytes * c + 16 * b));
+  }
+  // A chunk's weights against the running maximum; of0, of1: its tiles' references.
+  __device__ __forceinline__ void lower(u32x4& p, float of0, float of1) const {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float of = k ? of1 : of0;
-      // whole log2 units down to the maximum (255: past every exponent)
-      const uint32_t down = of == -INFINITY ? 255 : (uint32_t)(int)fminf(m - of, 255.0f);
-      x.p[2 * k] = sub_sat(x.p[2 * k], down * 0x00800080u);
-      x.p[2 * k + 1] = sub_sat(x.p[2 * k + 1], down * 0x00800080u);
+      // whole log2 units down to the maximum, in both exponents; 255: past every exponent,
+      // also for a tile without a record (of -inf, and the difference perhaps NaN)
+      const uint32_t down = __umul24((uint32_t)fminf(m - (k ? of1 : of0), 255.0f), 0x00800080u);
+      p[2 * k] = sub_sat(p[2 * k], down);
+      p[2 * k + 1] = sub_sat(p[2 * k + 1], down);
     }
+  }
+  // O of group b of the wave's coordinates += a chunk.
+  __device__ __forceinline__ void values(int b, const u32x4& p, const Operands& x) {
+    u32x4 pw;
 #pragma unroll
-    for (int b = 0; b < kTiles / 2; ++b) {
-      u32x4 pw;
+    for (int i = 0; i < 4; ++i) pw[i] = sub_sat(p[i], x.shift[i]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pw[i] = sub_sat(x.p[i], x.shift[b][i]);
+    for (int i = 0; i < 2; ++i)
+      o[2 * b + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+          as_bf16x8(fp4x8_to_bf16((uint32_t)x.v[i], 1.0f)), as_bf16x8(pw), o[2 * b + i], 0, 0, 0);
+  }
+
+  // O += a round, whose first chunk's operands are p and y. kMoved: the tiles' references
+  // `of` are not all the running maximum.
+  template <bool kMoved>
+  __device__ __forceinline__ void add(const Places& at, const float (&of)[kWaves], u32x4 (&p)[2],
+                                      Operands (&y)[2]) {
+    constexpr int kGroups = kTiles / 2, kSteps = L::kChunks * kGroups;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        o[2 * b + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            as_bf16x8(fp4x8_to_bf16((uint32_t)x.v[b][i], 1.0f)), as_bf16x8(pw), o[2 * b + i], 0, 0,
-            0);
+    for (int n = 0; n < kSteps; ++n) {
+      const int c = n / kGroups, b = n % kGroups, next = n + 1;
+      if (next < kSteps) {
+        if (next % kGroups == 0) p[(c + 1) & 1] = lds_read<u32x4>(at.w_at + 1024 * (c + 1));
+        operands(at, next / kGroups, next % kGroups, y[next & 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (kMoved && b == 0) lower(p[c & 1], of[2 * c], of[2 * c + 1]);
+      values(b, p[c & 1], y[n & 1]);
     }
   }
 
+  // Between two barriers: scores of round i (but after the last), O += round i - 1 (but
+  // before the first). before: whether round i - 2 moved the maximum, since when round i -
+  // 1 was scored without knowing.
+  template <bool kFirst, bool kLast>
+  __device__ __forceinline__ void step(int i, bool& before) {
+    Operands y[2];
+    u32x4 p[2];
+    int moved = 0;
+    const float own = owns, sum = sums;
+    const Places at = places(i - 1);
+    auto ahead = [&] {
+      if (kFirst) return;
+      moved = lds_read<int>(lds + L::kMoved + 4 * ((i - 1) & 3));
+      p[0] = lds_read<u32x4>(at.w_at);
+      operands(at, 0, 0, y[0]);
+    };
+    if (kLast) {
+      ahead();
+    } else if (i * L::kChunks + (wave >> 1) < this->chunks) {
+      Tile x;
+      tile(i, x);
+      __builtin_amdgcn_sched_barrier(0);
+      score(i, x, ahead);
+    } else {
+      ahead();
+      no_score(i);
+    }
+    if (!kLast && threadIdx.x == 0) lds_write(lds + L::kMoved + 4 * ((i + 2) & 3), 0);
+    if (kFirst) return;
+    const bool now = uniform(moved) != 0;
+    float of[kWaves];
+    if (now || before) {
+      float top = m;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        of[w] = lds_read<float>(lds + L::kTops + 64 * (((i - 1) & 1) * kWaves + w) + 4 * row);
+        top = fmaxf(top, of[w]);
+      }
+      advance(top, own, sum);
+      add<true>(at, of, p, y);
+    } else {
+      l += sum;
+      add<false>(at, of, p, y);
+    }
+    before = now;
+  }
   // The share of the list: chunk c of the split's is number c * splits + split.
   __device__ __forceinline__ void list() {
-    for (int i = 0; i <= this->rounds; ++i) {
-      const bool scoring = i < this->rounds &&
-                           i * L::kChunks + (wave >> 1) < this->chunks;
-      Tile x;
-      Operands y[2];
-      float of[kWaves];
-      const float own = owns, sum = sums;
-      auto ahead = [&] {
-        if (i == 0) return;
-        operands(i - 1, 0, y[0]);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w)
-          of[w] = lds_read<float>(lds + L::kTops + 64 * (((i - 1) & 1) * kWaves + w) + 4 * row);
-      };
-      if (scoring) {
-        tile(i, x);
-        __builtin_amdgcn_sched_barrier(0);
-        score(i, x, ahead);
-      } else {
-        ahead();
-        if (i < this->rounds) no_score(i);
-      }
-      if (i > 0) {
-        float top = m;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, of[w]);
-        advance(top, own, sum);
-#pragma unroll
-        for (int c = 0; c < L::kChunks; ++c) {
-          if (c + 1 < L::kChunks) operands(i - 1, c + 1, y[(c + 1) & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-          values(y[c & 1], of[2 * c], of[2 * c + 1]);
-        }
-      }
-      if (i < this->rounds) lds_barrier();
+    bool before = false;
+    step<true, false>(0, before);
+    lds_barrier();
+    for (int i = 1; i < this->rounds; ++i) {
+      step<false, false>(i, before);
+      lds_barrier();
     }
+    step<false, true>(this->rounds, before);
   }
 
   // The share of the window: chunks of 16 rows, dealt from the last split down.
   __device__ __forceinline__ int window_entry(int first) const {
     return 16 * ((first + wave) * a.splits + a.splits - 1 - split) + row;
   }
-  __device__ __forceinline__ void window(int early) {
+  __device__ __forceinline__ void window() {
     const int32_t* const swa = a.swa_indices + t * a.swa_topk;
     const uint32_t at = lds + wave * kWindowBytes;
     for (int first = 0; first < this->back; first += kWaves) {
@@ -550,7 +598,8 @@ struct Decode : Share<kWaves> {
       lds_barrier();
       if (wave < waves) {
         const int k = window_entry(first);
-        int64_t slot = first == 0 ? early : k < this->rows ? swa[k] : -1;
+        int64_t slot = first == 0 ? lds_read<int>(lds + L::kEarly + 64 * wave + 4 * row)
+                       : k < this->rows ? swa[k] : -1;
         if (k >= this->rows) slot = -1;
         const bool ok = slot >= 0 && slot < a.swa_rows;
         const uint8_t* page = a.swa_pool + (ok ? slot >> 6 : 0) * kNativePageBytes;
@@ -717,12 +766,15 @@ __global__ __launch_bounds__(96 * kWaves) void mx4_decode_kernel(DecodeArgs a) {
   if (a.swa_topk > 0)
     early = a.swa_indices[d.t * a.swa_topk + min(d.window_entry(0), a.swa_topk - 1)];
   d.lengths();
+  // (kept in LDS: the list's loop needs the registers)
+  if (a.swa_topk > 0) lds_write(at + Lds<kWaves>::kEarly + 64 * d.wave + 4 * d.row, early);
   wait_copies<0>();
   lds_barrier();
   d.read_q();
+  if (threadIdx.x == 0) lds_write(at + Lds<kWaves>::kMoved, u32x2{0, 0});
   lds_barrier();
   if (d.rounds > 0) d.list();
-  if (d.back > 0) d.window(early);
+  if (d.back > 0) d.window();
   d.finish();
 }
 
