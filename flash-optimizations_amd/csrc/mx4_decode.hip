@@ -59,6 +59,7 @@ struct DecodeArgs {
   int heads;
   const uint8_t* pool;
   int pool_pages;
+  bool once;  // the list's records are read with copy16_once()
   const int32_t* block_table;
   int64_t bt_stride;
   int max_blocks;
@@ -73,7 +74,8 @@ struct DecodeArgs {
   const int32_t* swa_length;
   const float* sink;
   float scale_log2;
-  int splits;     // workgroups (along x) that share a token's list and window
+  int splits;        // workgroups (along x) that share a token's list
+  int window_split;  // the one that takes the window: one more, or 0 where there is one only
   uint64_t splits_magic;  // ceil(2^32 / splits): x / splits = x * splits_magic >> 32 for x < 2^17
   int ws_splits;  // partial slots a row; 0: finish in place
   uint16_t* out;
@@ -98,6 +100,9 @@ constexpr int kTableCache = 1024;  // block-table columns kept in LDS
 constexpr int kWindowScalesAt = 16 * kNativeDataBytes;
 constexpr int kWindowBytes = kWindowScalesAt + 128;
 constexpr int kScaleRef = 127 + kMx4MaxExponent;
+constexpr int kSmallPool = 246723;  // pages whose bytes have 32-bit numbers
+static_assert((int64_t)kSmallPool * kPageRecords * kMx4RecordBytes <= 0xffffffff, "4 GiB");
+constexpr int64_t kOnceBytes = 64 << 20;
 constexpr float kSlack = 24.0f;  // log2 units a score may pass the running maximum by
 
 // LDS of a workgroup: the rounds' chunks (or a window chunk a wave); then, twice (odd and
@@ -127,6 +132,13 @@ struct Lds {
 __device__ __forceinline__ void copy16(const void* src, uint32_t lds) {
   __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
                                    16, 0, 0);
+}
+// The same, of data that the caches will not see again: calls whose lists hold kOnceBytes
+// of records or more (256 tokens x 2,048 records, 143 MB, 48.4 -> 46.4 us; 64 tokens, 36 MB,
+// which three calls in turn find in the last-level cache, 22.7 -> 23.4).
+__device__ __forceinline__ void copy16_once(const void* src, uint32_t lds) {
+  __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
+                                   16, 0, 2);
 }
 __device__ __forceinline__ void copy4(const void* src, uint32_t lds) {
   __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
@@ -200,9 +212,10 @@ struct Share {
     if (a.topk_length) live = max(min(a.topk_length[t], live), 0);
     if (a.swa_length) rows = max(min(a.swa_length[t], rows), 0);
     if (a.seqlens) records = a.seqlens[request()];
-    // list chunks split, split + splits, ...; window chunks splits - 1 - split, ...
-    chunks = (int)(((uint64_t)((live + 31) / 32 - split + a.splits - 1) * a.splits_magic) >> 32);
-    back = (int)(((uint64_t)((rows + 15) / 16 + split) * a.splits_magic) >> 32);
+    // list chunks split, split + splits, ...; the window in one workgroup
+    chunks = split < a.splits ? (int)(((uint64_t)((live + 31) / 32 - split + a.splits - 1) *
+                                       a.splits_magic) >> 32) : 0;
+    back = split == a.window_split ? (rows + 15) / 16 : 0;
     rounds = (chunks + kWaves / 2 - 1) / (kWaves / 2);
   }
 };
@@ -225,16 +238,19 @@ struct Copier : Share<kWaves> {
     idx = a.indices + t * a.topk;
     table = a.block_table + this->request() * a.bt_stride;
   }
-  __device__ __forceinline__ int entry(int first, int e) const {
-    const int c = (first + 2 * e + (lane >> 5)) * (kWaves / 2) + of;
+  // Entry of the list that slots[0] of a batch stands for, and how far on slots[1]'s is.
+  __device__ __forceinline__ int entry(int first) const {
+    const int c = (first + (lane >> 5)) * L::kChunks + of;
     return 32 * (c * a.splits + split) + (lane & 31);
   }
+  __device__ __forceinline__ int stride() const { return 64 * L::kChunks * a.splits; }
   // The first batch's entries, as far as the list's capacity goes: the length comes beside.
   __device__ __forceinline__ void ask() {
+    const int k = entry(0);
 #pragma unroll
     for (int e = 0; e < kBatch / 2; ++e) {
       slots[e] = -1;
-      if (e * 32 * kWaves * a.splits < a.topk) slots[e] = idx[min(entry(0, e), a.topk - 1)];
+      if (e * stride() < a.topk) slots[e] = idx[min(k + e * stride(), a.topk - 1)];
     }
 #pragma unroll
     for (int n = 0; n < kCopies; ++n) {
@@ -244,18 +260,20 @@ struct Copier : Share<kWaves> {
       where[n] = (uint32_t)(4 * (16 * tile + r)) | (uint32_t)(16 * (in_tile - 17 * r)) << 8;
     }
   }
+  // slots[kFrom] .. [kTo - 1]: from entries (the first batch's are there) to record numbers.
+  template <int kFrom, int kTo>
   __device__ __forceinline__ void look_up(int first) {
     const bool cached = a.max_blocks <= kTableCache;
+    const int k = entry(first);
     int page[kBatch / 2];
+    if (first > 0) {
 #pragma unroll
-    for (int e = 0; e < kBatch / 2; ++e) {
-      const int k = entry(first, e);
-      if (first > 0) slots[e] = k < this->live ? idx[k] : -1;
-      if (k >= this->live) slots[e] = -1;
+      for (int e = kFrom; e < kTo; ++e)
+        slots[e] = k + e * stride() < this->live ? idx[k + e * stride()] : -1;
     }
 #pragma unroll
-    for (int e = 0; e < kBatch / 2; ++e) {
-      const int r = slots[e];
+    for (int e = kFrom; e < kTo; ++e) {
+      const int r = k + e * stride() < this->live ? slots[e] : -1;
       const bool inside = r >= 0 && r < this->records && (r >> 6) < a.max_blocks;
       page[e] = -1;
       if (cached)
@@ -265,9 +283,20 @@ struct Copier : Share<kWaves> {
       if (!inside) page[e] = -1;
     }
 #pragma unroll
-    for (int e = 0; e < kBatch / 2; ++e)
+    for (int e = kFrom; e < kTo; ++e)
       slots[e] = page[e] >= 0 && page[e] < a.pool_pages
                      ? page[e] * kPageRecords + (slots[e] & 63) : -1;
+  }
+  // The rest of the first batch, when rounds 0 and 1 have been copied and slots moved down.
+  __device__ __forceinline__ void look_up_later() {
+    int rest[kBatch / 2];
+#pragma unroll
+    for (int e = 0; e + 1 < kBatch / 2; ++e) rest[e + 1] = slots[e];
+#pragma unroll
+    for (int e = 1; e < kBatch / 2; ++e) slots[e] = rest[e];
+    look_up<1, kBatch / 2>(0);
+#pragma unroll
+    for (int e = 1; e < kBatch / 2; ++e) slots[e - 1] = slots[e];
   }
   // The chunk of round i; its live records go to LDS.
   __device__ __forceinline__ void copy(int i) {
@@ -279,27 +308,48 @@ struct Copier : Share<kWaves> {
     const uint32_t to = lds + (i & (kBuffers - 1)) * L::kRound + of * kChunkBytes;
     const uint32_t live_at = lds + L::kLive + 4 * ((i & (kBuffers - 1)) * L::kChunks + of);
     const uint32_t mask = (uint32_t)(__ballot(of_round >= 0) >> (32 * (i & 1)));
-    int slot[kCopies];
-#pragma unroll
-    for (int n = 0; n < kCopies; ++n)
-      slot[n] = __builtin_amdgcn_ds_bpermute(128 * (i & 1) + (int)(where[n] & 0xff), of_round);
     if (lane == 0) lds_write(live_at, mask);
+    const int record = max(of_round, 0);
+    const int base = 128 * (i & 1);
+    const bool all = lane < kLastLanes;
+    if (a.pool_pages <= kSmallPool) {  // 32-bit offsets from the pool
+      const int at = record * kMx4RecordBytes;
+      uint32_t off[kCopies];
 #pragma unroll
-    for (int n = 0; n < kCopies; ++n) {
-      const uint8_t* src = a.pool + ((int64_t)max(slot[n], 0) * kMx4RecordBytes + (where[n] >> 8));
-      if (n < kCopies - 1 || lane < kLastLanes) copy16(src, to + 1024 * n);
+      for (int n = 0; n < kCopies; ++n)
+        off[n] = (uint32_t)__builtin_amdgcn_ds_bpermute(base + (int)(where[n] & 0xff), at);
+#pragma unroll
+      for (int n = 0; n < kCopies; ++n) off[n] += where[n] >> 8;
+      if (a.once) {
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n)
+          if (n < kCopies - 1 || all) copy16_once(a.pool + off[n], to + 1024 * n);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n)
+          if (n < kCopies - 1 || all) copy16(a.pool + off[n], to + 1024 * n);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < kCopies; ++n) {
+        const int slot = __builtin_amdgcn_ds_bpermute(base + (int)(where[n] & 0xff), record);
+        if (n < kCopies - 1 || all)
+          copy16_once(a.pool + ((int64_t)slot * kMx4RecordBytes + (where[n] >> 8)), to + 1024 * n);
+      }
     }
   }
   __device__ __forceinline__ void run() {
+    __builtin_amdgcn_s_setprio(3);
     ask();
     this->lengths();
     lds_barrier();  // the block-table row
     const int rounds = this->rounds;
     if (rounds > 0) {
-      look_up(0);
+      look_up<0, 1>(0);  // rounds 0 and 1; the others' while their records are on the way
       copy(0);
       if (rounds > 1) {
         copy(1);
+        if (rounds > 2) look_up_later();
         wait_copies<kCopies>();
       } else {
         wait_copies<0>();
@@ -308,7 +358,7 @@ struct Copier : Share<kWaves> {
     lds_barrier();
     for (int i = 0; i < rounds; ++i) {
       if (i + 2 < rounds) {
-        if (((i + 2) & (kBatch - 1)) == 0) look_up(i + 2);
+        if (((i + 2) & (kBatch - 1)) == 0) look_up<0, kBatch / 2>(i + 2);
         copy(i + 2);
         wait_copies<kCopies>();
       } else {
@@ -585,10 +635,8 @@ struct Decode : Share<kWaves> {
     step<false, true>(this->rounds, before);
   }
 
-  // The share of the window: chunks of 16 rows, dealt from the last split down.
-  __device__ __forceinline__ int window_entry(int first) const {
-    return 16 * ((first + wave) * a.splits + a.splits - 1 - split) + row;
-  }
+  // The window: chunks of 16 rows.
+  __device__ __forceinline__ int window_entry(int first) const { return 16 * (first + wave) + row; }
   __device__ __forceinline__ void window() {
     const int32_t* const swa = a.swa_indices + t * a.swa_topk;
     const uint32_t at = lds + wave * kWindowBytes;
@@ -722,23 +770,27 @@ struct Decode : Share<kWaves> {
     const int c0 = wave * kTiles * 16 + 4 * group;
     if (a.ws_splits != 0) {
       const int64_t at = (t * a.ws_splits + split) * a.heads + h;
-      const float f = sum != 0.0f ? 0x1p32f / sum : 0.0f;
+      const float f = sum != 0.0f ? 0x1p32f * __builtin_amdgcn_rcpf(sum) : 0.0f;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
         __builtin_nontemporal_store(o[i] * f, (f32x4*)(a.ws_o + at * kHeadDim + c0 + 16 * i));
       // (NaN goes on as infinity: the combine's maximum would pass over a NaN)
       if (wave == 0 && lane < 16)
-        a.ws_lse[at] = sum != sum ? INFINITY : sum != 0.0f ? m + log2f(sum) : -INFINITY;
+        a.ws_lse[at] = sum != sum     ? INFINITY
+                       : sum != 0.0f ? m + __builtin_amdgcn_logf(sum)
+                                     : -INFINITY;
       return;
     }
+    // (the sums are in normal range: the hardware's log2, exp2 and reciprocal, each within
+    // an ulp, need no scaling)
     const float sink2 = a.sink ? a.sink[h] * kLog2e : -INFINITY;
     const float top = fmaxf(m, sink2);
     float f = 0.0f, lse = -INFINITY;
     if (top != -INFINITY || sum != 0.0f) {
-      const float em = m == -INFINITY && sum == 0.0f ? 0.0f : exp2f(m - top);
-      const float z = sum * em + exp2f(sink2 - top);
-      f = em * 0x1p32f / z;
-      lse = (top + log2f(z)) * kLn2;
+      const float em = m == -INFINITY && sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+      const float z = sum * em + __builtin_amdgcn_exp2f(sink2 - top);
+      f = em * 0x1p32f * __builtin_amdgcn_rcpf(z);
+      lse = (top + __builtin_amdgcn_logf(z)) * kLn2;
     }
     if (wave == 0 && lane < 16) a.lse[t * a.heads + h] = lse;
 #pragma unroll
@@ -786,20 +838,22 @@ bool bad_sizes(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
 }
 
 struct Plan {
-  int waves;   // a workgroup
-  int splits;  // workgroups a token and head group
+  int waves;   // that compute, a workgroup
+  int slots;   // workgroups a token and 16 heads
+  int splits;  // of them the list's; the window has one of its own where there are several
 };
 
-// About one workgroup a CU (256): enough splits to reach that, each with a round of its
-// own.
+// About one workgroup a CU (256), each with a round of the list of its own. The window's
+// rows are fetched while the list's are where it has a workgroup to itself (16 tokens x 64
+// heads, 317 + 64 rows: 15.0 -> 14.0 us against both in each workgroup).
 Plan plan(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
   Plan p;
   p.waves = 8;
   const int64_t base = std::max<int64_t>(tokens * ((heads + 15) / 16), 1);
-  const int64_t rounds = std::max((topk + 16 * p.waves - 1) / (16 * p.waves),
-                                  (swa_topk + 16 * p.waves - 1) / (16 * p.waves));
-  const int64_t splits = std::min({(256 + base - 1) / base, rounds, (int64_t)kMaxSplits});
-  p.splits = (int)std::max<int64_t>(splits, 1);
+  const int64_t rounds = (topk + 16 * p.waves - 1) / (16 * p.waves), window = swa_topk > 0;
+  p.slots = (int)std::max<int64_t>(
+      std::min({(256 + base - 1) / base, rounds + window, (int64_t)kMaxSplits}), 1);
+  p.splits = (int)std::max<int64_t>(p.slots - window, 1);
   return p;
 }
 size_t ws_bytes(int64_t tokens, int64_t heads, int64_t slots) {
@@ -813,8 +867,8 @@ extern "C" int rm_mx4_sparse_decode_workspace(int64_t tokens, int64_t heads, int
                                               size_t* workspace_bytes) {
   if (bad_sizes(tokens, heads, topk, swa_topk)) return RM_ERR_SHAPE;
   const Plan p = plan(tokens, heads, topk, swa_topk);
-  if (num_splits) *num_splits = p.splits;
-  if (workspace_bytes) *workspace_bytes = ws_bytes(tokens, heads, p.splits);
+  if (num_splits) *num_splits = p.slots;
+  if (workspace_bytes) *workspace_bytes = ws_bytes(tokens, heads, p.slots);
   return RM_OK;
 }
 
@@ -840,7 +894,7 @@ extern "C" int rm_mx4_sparse_decode_fwd(
       !aligned(swa_pool, 16))
     return RM_ERR_ALIGN;
   const Plan p = plan(tokens, heads, topk, swa_topk);
-  const size_t bytes = ws_bytes(tokens, heads, p.splits);
+  const size_t bytes = ws_bytes(tokens, heads, p.slots);
   if (bytes > 0 && (!workspace || workspace_bytes < bytes)) return RM_ERR_WORKSPACE;
   if (bytes > 0 && !aligned(workspace, 16)) return RM_ERR_ALIGN;
   DecodeArgs a;
@@ -856,6 +910,7 @@ extern "C" int rm_mx4_sparse_decode_fwd(
   a.indices = indices;
   // (an entry that is none reads the pool's first record: without one the list is empty)
   a.topk = pool_pages > 0 && max_blocks > 0 ? (int)topk : 0;
+  a.once = tokens * topk * kMx4RecordBytes >= kOnceBytes;
   a.topk_length = topk_length;
   a.swa_pool = swa_pool;
   a.swa_rows = swa_pool_pages * kPageRecords;
@@ -866,17 +921,18 @@ extern "C" int rm_mx4_sparse_decode_fwd(
   a.scale_log2 = softmax_scale * kLog2e;
   a.splits = p.splits;
   a.splits_magic = (((uint64_t)1 << 32) + p.splits - 1) / p.splits;
-  a.ws_splits = p.splits > 1 ? p.splits : 0;
+  a.window_split = p.slots > 1 ? p.splits : 0;
+  a.ws_splits = p.slots > 1 ? p.slots : 0;
   a.out = out;
   a.lse = lse;
   a.ws_o = (float*)workspace;
-  a.ws_lse = bytes ? (float*)workspace + (size_t)tokens * p.splits * heads * kHeadDim : nullptr;
+  a.ws_lse = bytes ? (float*)workspace + (size_t)tokens * p.slots * heads * kHeadDim : nullptr;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)p.splits, (unsigned)tokens, (unsigned)((heads + 15) / 16));
+  const dim3 grid((unsigned)p.slots, (unsigned)tokens, (unsigned)((heads + 15) / 16));
   hipLaunchKernelGGL(mx4_decode_kernel<8>, grid, dim3(96 * p.waves), 0, s, a);
   if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
-  if (p.splits > 1) {
-    launch_combine<true>(a.ws_o, a.ws_lse, sink, p.splits, tokens, heads, out, lse, s);
+  if (p.slots > 1) {
+    launch_combine<true>(a.ws_o, a.ws_lse, sink, p.slots, tokens, heads, out, lse, s);
     if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   }
   return RM_OK;
