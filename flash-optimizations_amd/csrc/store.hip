@@ -693,7 +693,7 @@ __device__ __forceinline__ void native_store_row(const RowRaw& raw, const float 
 // The arithmetic up to the rotated BF16 row is the Native store's; the group
 // maximum is taken after the rotation, on the BF16 values' bits, where integer
 // order is float order with infinity and NaN on top.
-template <bool kBf16, bool kStream>
+template <bool kBf16>
 __device__ __forceinline__ void mx4_store_row(const RowRaw& raw, const float (&w)[8], float eps,
                                               int64_t slot, int64_t pos, const float* freqs,
                                               uint8_t* pool) {
@@ -754,13 +754,8 @@ __device__ __forceinline__ void mx4_store_row(const RowRaw& raw, const float (&w
   uint8_t* const rec = pool + slot * kMx4RecordBytes;
   uint32_t* const at = (uint32_t*)(rec + 4 * lane);
   uint32_t* const scales = (uint32_t*)(rec + kMx4CodeBytes + 4 * (lane >> 4));
-  if constexpr (kStream) {
-    __builtin_nontemporal_store(code, at);
-    if ((lane & 15) == 0) __builtin_nontemporal_store((uint32_t)byte, scales);
-  } else {
-    *at = code;
-    if ((lane & 15) == 0) *scales = (uint32_t)byte;
-  }
+  *at = code;
+  if ((lane & 15) == 0) *scales = (uint32_t)byte;
 }
 
 // A skipped row's data is not read: calls often skip many rows (padding), and
@@ -786,7 +781,7 @@ __device__ __forceinline__ void mx4_store_row(const RowRaw& raw, const float (&w
 // and reductions on small ones.
 constexpr int64_t kAheadRows = 8192;
 constexpr int64_t kNativeBlocks = 256 * 16;
-// kMx4: the rows become 4-bit records instead of Native ones.
+// kMx4: the rows become 4-bit records instead of Native ones (kOne only).
 template <bool kBf16, bool kOne, bool kStream, bool kMx4>
 __global__ __launch_bounds__(256) void native_store_kernel(
     const void* __restrict__ x, int64_t stride, const float* __restrict__ weight, float eps,
@@ -812,7 +807,7 @@ __global__ __launch_bounds__(256) void native_store_kernel(
     if (!stored(slot, pos)) return;
     if (!ahead) next = load_raw<kBf16, kStream>(x, rec, stride, lane);
     if constexpr (kMx4)
-      mx4_store_row<kBf16, kStream>(next, w, eps, slot, pos, freqs, pool);
+      mx4_store_row<kBf16>(next, w, eps, slot, pos, freqs, pool);
     else
       native_store_row<kBf16, kStream>(next, w, eps, slot, pos, freqs, pool);
     return;
@@ -838,10 +833,206 @@ __global__ __launch_bounds__(256) void native_store_kernel(
       if (todo != 0) load_first();
       const int slot = __builtin_amdgcn_readlane(my_slot, at);
       const int pos = __builtin_amdgcn_readlane(my_pos, at);
-      if constexpr (kMx4)
-        mx4_store_row<kBf16, kStream>(raw, w, eps, slot, pos, freqs, pool);
-      else
-        native_store_row<kBf16, kStream>(raw, w, eps, slot, pos, freqs, pool);
+      native_store_row<kBf16, kStream>(raw, w, eps, slot, pos, freqs, pool);
+    }
+  }
+}
+
+// Four rows a wave, sixteen lanes a row: lane j of them owns the pieces of eight
+// coordinates j, 16 + j, 32 + j and 48 + j. The sum of squares keeps the order of the
+// one-row form (eight squares in turn, then the pairwise tree over the 64 pieces:
+// distances 1..8 are the lanes', 16 and 32 the lane's own). The tail is piece 48 + j
+// of the upper eight lanes, rotated once for all four rows, and a scale group is the
+// pieces 16 i + j of four lanes: after their maxima, lane j keeps the one of
+// i = j % 4, forms that group's exponent and hands it to the other three.
+//
+// A wave of one row issues about 200 vector instructions for it, 40 of them the
+// rotation by eight lanes, and 1M rows were bound by them: 333 us (BF16) in the form
+// above (runs of rows, streaming loads and stores). Here it is about 100, and 1M rows
+// are bound by memory: 295 us for 1,024 + 272 bytes each at random slots (4.6 TB/s; a
+// 1 GiB copy moves 5.1), FP32 rows 553 us (4.4 TB/s) after 561.
+//   * up to kOneRows one row a wave: the chain is shorter (24 rows 2.6 us, 2.9 here;
+//     2,048 rows 2.9 and 3.3; 4,096 BF16 / FP32 rows 3.4 / 3.8 either way; 8,192 rows
+//     5.3 / 6.5 and 4.8 / 6.2).
+//   * up to kQuadStreamRows a wave takes four rows, beyond eight, the second four on
+//     their way while the first are coded, and rows are read past the caches (65,536
+//     BF16 rows 22.4 us, eight a wave 21.9, FP32 35.8 and 37.3; 131,072 rows 43.1 /
+//     67.6 and 37.1 / 68.8; 1M rows 334 / 555 and 295 / 553, sixteen a wave 299 / 553).
+//     Records go through the caches, which join a record's 256 + 16 bytes: written
+//     past them 1M BF16 rows took 327 us.
+//   * rows that are not stored are passed over: a wave moves the others together (1M
+//     BF16 rows a quarter stored 155 -> 81 us).
+constexpr int64_t kOneRows = 4096;
+constexpr int64_t kQuadStreamRows = 65536;
+template <bool kBf16>
+struct QuadRaw {
+  u32x4 v[kBf16 ? 4 : 8];
+};
+template <int kCtrl>
+__device__ __forceinline__ int dpp_i(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, kCtrl, 0xf, 0xf, false);
+}
+
+template <bool kBf16, bool kStream, int kLoop>
+__global__ __launch_bounds__(256) void mx4_store_quads_kernel(
+    const void* __restrict__ x, int64_t stride, const float* __restrict__ weight, float eps,
+    const int32_t* __restrict__ slots, const int32_t* __restrict__ position,
+    const float* __restrict__ freqs, int64_t freq_rows, int64_t n, uint8_t* __restrict__ pool,
+    int64_t pool_rows) {
+  const int lane = wave_lane(), j = lane & 15, g = lane >> 4;
+  const int64_t row0 = ((int64_t)blockIdx.x * kWaves + uniform((int)(threadIdx.x >> 6))) * (4 * kLoop);
+  if (row0 >= n) return;
+  // lane i: slot and position of the i-th row of row0 .. that is stored
+  int32_t slot = -1, pos = 0, row = lane;
+  if (lane < 4 * kLoop && row0 + lane < n) {
+    slot = slots[row0 + lane];
+    if (freqs) pos = position[row0 + lane];
+    if (slot >= pool_rows || (freqs && (pos < 0 || (int64_t)pos * 4 >= freq_rows))) slot = -1;
+  }
+  const uint64_t stored = __ballot(slot >= 0);
+  const int count = __popcll(stored);
+  if (count == 0) return;
+  if (stored & (stored + 1)) {  // rows left out in between
+    const int before = __popcll(stored & ((1ull << lane) - 1));
+    const int to = 4 * (slot >= 0 ? before : count + lane - before);
+    slot = __builtin_amdgcn_ds_permute(to, slot);
+    pos = __builtin_amdgcn_ds_permute(to, pos);
+    row = __builtin_amdgcn_ds_permute(to, row);
+  }
+  f32x4 w[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4* const at = (const f32x4*)(weight + 8 * (16 * i + j));
+    w[2 * i] = at[0];
+    w[2 * i + 1] = at[1];
+  }
+  struct Row {
+    int32_t slot, pos;
+    QuadRaw<kBf16> raw;
+  };
+  auto load = [&](int it) {
+    const int from = 4 * (4 * it + g);
+    Row r;
+    r.slot = __builtin_amdgcn_ds_bpermute(from, slot);
+    r.pos = __builtin_amdgcn_ds_bpermute(from, pos);
+    const int64_t at = (row0 + __builtin_amdgcn_ds_bpermute(from, row)) * stride + 8 * j;
+    r.raw = QuadRaw<kBf16>{};
+    if (r.slot >= 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kBf16) {
+          r.raw.v[i] = load16<kStream>((const u32x4*)((const uint16_t*)x + at + 128 * i));
+        } else {
+          const u32x4* const p = (const u32x4*)((const float*)x + at + 128 * i);
+          r.raw.v[2 * i] = load16<kStream>(p);
+          r.raw.v[2 * i + 1] = load16<kStream>(p + 1);
+        }
+      }
+    }
+    return r;
+  };
+  Row next = load(0);
+#pragma unroll
+  for (int it = 0; it < kLoop; ++it) {
+    if (4 * it >= count) break;
+    const int32_t this_slot = next.slot;
+    const QuadRaw<kBf16> cur = next.raw;
+    const bool rotated = freqs && j >= 8 && this_slot >= 0;
+    f32x4 fa = {1.f, 0.f, 1.f, 0.f}, fb = fa;
+    if (rotated) {
+      const float* const f = freqs + ((int64_t)next.pos * 4) * (2 * kRopePairs) + 8 * (j - 8);
+      fa = *(const f32x4*)f;
+      fb = *(const f32x4*)(f + 4);
+    }
+    if (it + 1 < kLoop && 4 * (it + 1) < count) next = load(it + 1);
+    float v[4][8], sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (kBf16) {
+          v[i][2 * c] = u2f(cur.v[i][c] << 16);
+          v[i][2 * c + 1] = u2f(cur.v[i][c] & 0xffff0000u);
+        } else {
+          v[i][c] = u2f(cur.v[2 * i][c]);
+          v[i][4 + c] = u2f(cur.v[2 * i + 1][c]);
+        }
+      }
+      float p = v[i][0] * v[i][0];
+#pragma unroll
+      for (int c = 1; c < 8; ++c) {
+        const float sq = v[i][c] * v[i][c];
+        p = p + sq;
+      }
+      p = p + dpp<kDppXor1>(p);
+      p = p + dpp<kDppXor2>(p);
+      p = p + dpp<kDppHalfMirror>(p);
+      sum[i] = p + dpp<kDppMirror>(p);
+    }
+    const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    const float r = inv_root(all * (1.0f / 512.0f) + eps);
+    bf16x2 nb[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float a = v[i][2 * c] * r, b = v[i][2 * c + 1] * r;
+        a = a * w[2 * i + c / 2][2 * (c % 2)];
+        b = b * w[2 * i + c / 2][2 * (c % 2) + 1];
+        nb[i][c] = bf16_pair(a, b);
+      }
+    if (rotated) {
+      const float cs[8] = {fa[0], fa[1], fa[2], fa[3], fb[0], fb[1], fb[2], fb[3]};
+      float nf[8];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t d = __builtin_bit_cast(uint32_t, nb[3][c]);
+        nf[2 * c] = u2f(d << 16);
+        nf[2 * c + 1] = u2f(d & 0xffff0000u);
+      }
+      rope4(nf, cs);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) nb[3][c] = bf16_pair(nf[2 * c], nf[2 * c + 1]);
+    }
+    int top[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int t = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t d = __builtin_bit_cast(uint32_t, nb[i][c]);
+        t = max(t, (int)max(d & 0x7fffu, (d >> 16) & 0x7fffu));
+      }
+      t = max(t, dpp_i<kDppXor1>(t));
+      top[i] = max(t, dpp_i<kDppXor2>(t));
+    }
+    const int mine = (j & 2) ? ((j & 1) ? top[3] : top[2]) : ((j & 1) ? top[1] : top[0]);
+    const bool special = mine >= 0x7f80;  // an infinity or NaN in the group
+    const int e = mx4_exponent(bf16_to_f32((uint32_t)mine));
+    // what the group's lanes need of it: the scale, 0 for a special group
+    const int scale = special ? 0 : (e + 127) << 23;
+    uint8_t* const rec = pool + (int64_t)max(this_slot, 0) * kMx4RecordBytes;
+    uint32_t code[4];
+    const int scales[4] = {dpp_i<0x00>(scale), dpp_i<0x55>(scale), dpp_i<0xAA>(scale),
+                           dpp_i<0xFF>(scale)};  // lane i of each four
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float s = u2f((uint32_t)scales[i]);
+      uint32_t c = fp4_pair<0>(0, nb[i][0], s);
+      c = fp4_pair<1>(c, nb[i][1], s);
+      c = fp4_pair<2>(c, nb[i][2], s);
+      c = fp4_pair<3>(c, nb[i][3], s);
+      code[i] = scales[i] != 0 ? c : 0;
+    }
+    if (this_slot >= 0) {
+      const uint8_t byte = special ? kMx4NanScale : e + 127;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t* const at = (uint32_t*)(rec + 64 * i + 4 * j);
+        *at = code[i];
+      }
+      uint8_t* const at = rec + kMx4CodeBytes + 4 * (j & 3) + (j >> 2);
+      *at = byte;
     }
   }
 }
@@ -988,16 +1179,35 @@ int store_rows(const void* x, int x_dtype, int64_t x_row_stride, const float* we
   hipStream_t s = (hipStream_t)stream;
   const int64_t rows = pool_pages * kPageRecords;
   const bool bf16 = x_dtype == RM_BF16;
-  const int64_t cap = n > kStreamRows ? kMaxBlocks : kNativeBlocks;
-  const auto kern =
-      n > kStreamRows
-          ? (bf16 ? native_store_kernel<true, false, true, kMx4> : native_store_kernel<false, false, true, kMx4>)
-      : n > kNativeBlocks * kWaves
-          ? (bf16 ? native_store_kernel<true, false, false, kMx4> : native_store_kernel<false, false, false, kMx4>)
-          : (bf16 ? native_store_kernel<true, true, false, kMx4> : native_store_kernel<false, true, false, kMx4>);
-  hipLaunchKernelGGL(kern, dim3(grid_for(n, cap)), dim3(256), 0, s, x, x_row_stride, weight, eps,
-                     dst_slot, position, freqs, freq_rows, n, rows_per_wave(bf16, n, cap), pool,
-                     rows);
+  if constexpr (kMx4) {
+    if (n > kOneRows) {
+      const int64_t rows_a_block = 4 * kWaves * (n > kQuadStreamRows ? 2 : 1);
+      const auto quads =
+          n > kQuadStreamRows
+              ? (bf16 ? mx4_store_quads_kernel<true, true, 2> : mx4_store_quads_kernel<false, true, 2>)
+              : (bf16 ? mx4_store_quads_kernel<true, false, 1> : mx4_store_quads_kernel<false, false, 1>);
+      const int64_t blocks = (n + rows_a_block - 1) / rows_a_block;
+      if (blocks > 0x7fffffff) return RM_ERR_SHAPE;
+      hipLaunchKernelGGL(quads, dim3((unsigned)blocks), dim3(64 * kWaves), 0, s, x, x_row_stride,
+                         weight, eps, dst_slot, position, freqs, freq_rows, n, pool, rows);
+    } else {
+      hipLaunchKernelGGL((bf16 ? native_store_kernel<true, true, false, true>
+                               : native_store_kernel<false, true, false, true>),
+                         dim3(grid_for(n)), dim3(256), 0, s, x, x_row_stride, weight, eps, dst_slot,
+                         position, freqs, freq_rows, n, rows_per_wave(bf16, n), pool, rows);
+    }
+  } else {
+    const int64_t cap = n > kStreamRows ? kMaxBlocks : kNativeBlocks;
+    const auto kern =
+        n > kStreamRows
+            ? (bf16 ? native_store_kernel<true, false, true, false> : native_store_kernel<false, false, true, false>)
+        : n > kNativeBlocks * kWaves
+            ? (bf16 ? native_store_kernel<true, false, false, false> : native_store_kernel<false, false, false, false>)
+            : (bf16 ? native_store_kernel<true, true, false, false> : native_store_kernel<false, true, false, false>);
+    hipLaunchKernelGGL(kern, dim3(grid_for(n, cap)), dim3(256), 0, s, x, x_row_stride, weight, eps,
+                       dst_slot, position, freqs, freq_rows, n, rows_per_wave(bf16, n, cap), pool,
+                       rows);
+  }
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
 }
 

@@ -130,6 +130,38 @@ def test_store_special_rows():
                 assert np.array_equal(got, expect(x, np.arange(16), 1, weight, eps)), eps
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [4097, 4112, 65537, 65552])
+def test_store_special_rows_in_large_calls(rows, dtype):
+    """Each form of the store writes the same record for the same row, also next to an
+    infinity, to rows left out and at the end of the call."""
+    banner(f"store special rows x {rows} {dtype}")
+    base = syn.latents(23, seed=9).float()
+    base[3] = 0.0
+    base[5, 100] = float("inf")
+    base[6, 511] = float("nan")
+    base[8] *= 1e18
+    base[9] *= 1e-18
+    base[10] = torch.arange(512) % 25 * 0.25
+    base = base.to(dtype)
+    freqs = syn.rope_freqs(4 * 23).to(DEV)
+    weight = torch.linspace(0.5, 1.5, 512, device=DEV)
+    ids = torch.arange(rows) % 23
+    pages = rows // 64 + 1
+    slots = torch.arange(rows, dtype=I32)
+    slots[(torch.arange(rows) % 29 == 7) | (torch.arange(rows) // 64 % 5 == 3)] = -1
+    pools = []
+    for take, where in ((ids, slots), (torch.arange(23), torch.arange(23, dtype=I32))):
+        pool = torch.full((pages, 17408), 0x5A, dtype=torch.uint8, device=DEV)
+        remnant.mx4_store_rows(base[take].to(DEV), weight, 1e-6, where.to(DEV),
+                               take.to(I32).to(DEV), freqs, pool)
+        pools.append(pool.cpu().reshape(-1, 272))
+    want = pools[1][:23][ids]
+    want[slots < 0] = 0x5A
+    assert torch.equal(pools[0][:rows], want)
+    assert (pools[0][rows:] == 0x5A).all()
+
+
 def test_store_keeps_bytes_past_4_gib_apart():
     """A pool of 4.6 GB: the last slots' records, beyond 32-bit offsets."""
     banner("store far slots")
