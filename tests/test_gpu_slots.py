@@ -91,6 +91,22 @@ def test_append_extreme_values():
     assert got.positions.tolist() == list(range(300))
 
 
+@pytest.mark.parametrize("ratio", [2, 3, 7, 641, 65537, 2 ** 30 - 1, 2 ** 30 + 1, 2 ** 31 - 1])
+def test_append_divides_exactly(ratio):
+    """old // ratio at the multiples of the ratio, beside them and at the ends of int32."""
+    print(f"[gpu-slots] append ratio {ratio}", flush=True)
+    rng = np.random.default_rng(ratio)
+    big = 2 ** 31 - 1
+    near = rng.integers(0, big // ratio + 1, 300) * ratio
+    new = np.concatenate([near, near - 1, near + 1, [big, big - 1, 0, 1, -1], rng.integers(0, big, 300)])
+    new = np.clip(new, -1, big)
+    got = remnant.append_slots(gpu(np.zeros((len(new), 0))), gpu(new), gpu(new), gpu([]),
+                               ratio=ratio, rows=3)
+    assert np.array_equal(got.seqlens.cpu().numpy(), np.maximum(new, 0) // ratio)
+    assert got.row_starts.max().item() == 0 and got.pages_taken.item() == 0
+    assert got.loc.tolist() == [-1] * 3
+
+
 def test_append_writes_caller_buffers():
     print("[gpu-slots] append out", flush=True)
     out = [torch.full((n,), 55, dtype=I32, device=DEV) for n in (20, 20, 3, 2, 1)]
@@ -124,6 +140,26 @@ def test_window_equals_loops(q_len, window, first):
         want, n = ref.window(table[:, :width], lengths, q_len, window, first)
         assert np.array_equal(slots.cpu().numpy(), want)
         assert np.array_equal(counts.cpu().numpy(), n)
+
+
+@pytest.mark.parametrize("window,first,shift", [(32768, 0, 0), (32764, 4, 0), (32766, 5, 0),
+                                                (32768, 0, 1), (39999, 1, 0)])
+def test_window_long_lists(window, first, shift):
+    """Lists long enough for the form of four entries a thread, rows that do not divide
+    by it and a buffer that is not 16-byte aligned."""
+    print(f"[gpu-slots] window long {window} {first} {shift}", flush=True)
+    rng = np.random.default_rng(window + first)
+    lengths = np.array([0, 1, 63, 20000, 32767, 32770, 39999, 40000, 33000])
+    table = rng.permutation(9 * 626).reshape(9, 626)
+    table[4, 100] = -1
+    n = 9 * (first + window)
+    flat = torch.full((n + shift + 8,), -7, dtype=I32, device=DEV)
+    out = flat[shift:shift + n].view(9, 1, first + window), torch.empty(9, dtype=I32, device=DEV)
+    remnant.window_slots(gpu(table), gpu(lengths), 1, window, first=first, out=out)
+    want, count = ref.window(table, lengths, 1, window, first)
+    assert np.array_equal(out[0].cpu().numpy(), want)
+    assert np.array_equal(out[1].cpu().numpy(), count)
+    assert (flat[:shift] == -7).all() and (flat[shift + n:] == -7).all()
 
 
 def test_window_many_tokens_and_extreme_lengths():
