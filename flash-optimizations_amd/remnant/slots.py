@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, config
-from .mx4 import _launch, _one_device
+from .mx4 import _I32, _launch, _one_device
 
 
 class SlotMap(NamedTuple):
@@ -28,21 +28,22 @@ class SlotMap(NamedTuple):
     pages_taken: torch.Tensor  # int32 [1]: pages needed; beyond the free list: it was short
 
 
-def _vector(name, t, n=None):
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() \
-            or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} must be a contiguous int32 vector"
-                         + ("" if n is None else f" of {n} entries"))
+def _vector(name, t, n):
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector of {n} entries")
 
 
 def _table(block_table):
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    shape, strides = block_table.shape, block_table.stride()
+    if block_table.dtype is not _I32 or len(shape) != 2 or (shape[1] > 1 and strides[1] != 1):
         raise ValueError("block_table must be int32 [batch, max_blocks] with unit inner stride")
-    batch, width = block_table.shape
-    if batch > 1 and block_table.stride(0) < width:
-        raise ValueError("block_table rows must not overlap")
-    return batch, width, max(block_table.stride(0), width) if batch <= 1 else block_table.stride(0)
+    batch, width = shape
+    stride = strides[0]
+    if stride < width:
+        if batch > 1:
+            raise ValueError("block_table rows must not overlap")
+        stride = width
+    return batch, width, stride
 
 
 def append_slots(block_table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: torch.Tensor,
@@ -71,22 +72,31 @@ def append_slots(block_table: torch.Tensor, old_lengths: torch.Tensor, new_lengt
         raise ValueError("ratio must be a positive int")
     _vector("old_lengths", old_lengths, batch)
     _vector("new_lengths", new_lengths, batch)
-    _vector("free_pages", free_pages)
+    free = free_pages.shape
+    if free_pages.dtype is not _I32 or len(free) != 1 or not free_pages.is_contiguous():
+        raise ValueError("free_pages must be a contiguous int32 vector")
+    if rows is None and out is not None:
+        rows = out[0].shape[0] if out[0].dim() == 1 else 0
+    elif type(rows) is not int or not 0 <= rows < 2 ** 31:
+        raise ValueError("rows must be an int, the capacity of the row lists")
     if out is None:
-        if type(rows) is not int or not 0 <= rows < 2 ** 31:
-            raise ValueError("rows must be an int, the capacity of the row lists")
         new = block_table.new_empty
         out = SlotMap(new(rows), new(rows), new(batch + 1), new(batch), new(1))
     else:
-        out = SlotMap(*out)
-        n = out.loc.shape[0] if rows is None else rows
-        for name, t, size in zip(out._fields, out, (n, n, batch + 1, batch, 1)):
-            _vector(name, t, size)
-        rows = n
-    device = _one_device(block_table, old_lengths, new_lengths, free_pages, *out)
+        if type(out) is not SlotMap:
+            out = SlotMap(*out)
+        _vector("loc", out.loc, rows)
+        _vector("positions", out.positions, rows)
+        _vector("row_starts", out.row_starts, batch + 1)
+        _vector("seqlens", out.seqlens, batch)
+        _vector("pages_taken", out.pages_taken, 1)
+    loc, positions, row_starts, seqlens, taken = out
+    device = _one_device(block_table, old_lengths, new_lengths, free_pages, loc, positions,
+                         row_starts, seqlens, taken)
     _launch(device, "rm_append_slots", block_table.data_ptr(), stride, width,
             old_lengths.data_ptr(), new_lengths.data_ptr(), batch, ratio, free_pages.data_ptr(),
-            free_pages.shape[0], rows, *[t.data_ptr() for t in out])
+            free[0], rows, loc.data_ptr(), positions.data_ptr(), row_starts.data_ptr(),
+            seqlens.data_ptr(), taken.data_ptr())
     return out
 
 
@@ -104,15 +114,15 @@ def window_slots(block_table: torch.Tensor, lengths: torch.Tensor, q_len: int, w
     ``swa_indices`` and ``swa_lengths`` of the decodes, or, with a window as long as the
     history, the slot lists of the readers. ``out``: the two tensors to write to."""
     batch, width, stride = _table(block_table)
-    for name, v in (("q_len", q_len), ("window", window), ("first", first)):
-        if type(v) is not int or not 0 <= v < 2 ** 31:
-            raise ValueError(f"{name} must be a non-negative int")
+    if not (type(q_len) is type(window) is type(first) is int and 0 <= q_len < 2 ** 31
+            and 0 <= window < 2 ** 31 and 0 <= first < 2 ** 31):
+        raise ValueError("q_len, window and first must be non-negative ints")
     _vector("lengths", lengths, batch)
     shape = (batch, q_len, first + window)
     if out is None:
         out = block_table.new_empty(shape), block_table.new_empty(batch * q_len)
     slots, counts = out
-    if slots.dtype != torch.int32 or slots.shape != shape or not slots.is_contiguous():
+    if slots.dtype is not _I32 or slots.shape != shape or not slots.is_contiguous():
         raise ValueError(f"slots must be a contiguous int32 {list(shape)} tensor")
     _vector("counts", counts, batch * q_len)
     if batch * q_len == 0:
