@@ -3,6 +3,7 @@
 // their whole input domains, for the GPU tests to compare with the software
 // rounding and with the CPU oracle. Test infrastructure, built into its own
 // library (libremnant_selftest.so); the product library does not contain it.
+#include "mx4_device.h"
 #include "remnant_device.h"
 
 using namespace rm;
@@ -78,6 +79,36 @@ __global__ __launch_bounds__(kThreads) void fp8_decode_kernel(uint16_t* out) {
     r = (uint16_t)(fp8_pair_to_bf16<false>(codes, exp2i(s - 127)) & 0xffffu);
   }
   out[i] = r;
+}
+
+// Scaled FP4 encode: out[(e - e_lo) * 65536 + n] = code of BF16 pattern n at scale 2^e
+// (both halves of every byte of the dword are checked equal).
+__global__ __launch_bounds__(kThreads) void fp4_encode_kernel(int e_lo, int e_count,
+                                                              uint8_t* out,
+                                                              unsigned long long* result) {
+  unsigned long long bad = 0;
+  for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < (uint64_t)e_count * 65536;
+       i += (uint64_t)gridDim.x * kThreads) {
+    const __bf16 v = __builtin_bit_cast(__bf16, (uint16_t)(i & 0xffffu));
+    const float scale = exp2i(e_lo + (int)(i >> 16));
+    uint32_t acc = fp4_pair<0>(0, bf16x2{v, v}, scale);
+    acc = fp4_pair<1>(acc, bf16x2{v, v}, scale);
+    acc = fp4_pair<2>(acc, bf16x2{v, v}, scale);
+    acc = fp4_pair<3>(acc, bf16x2{v, v}, scale);
+    if (acc != (acc & 15u) * 0x11111111u) ++bad;
+    out[i] = (uint8_t)(acc & 15u);
+  }
+  report(result, bad, ~0ull);
+}
+
+// Scaled FP4 decode: out[s * 256 + c] = the two BF16 of byte c at scale byte s, low code
+// in the low half (the four bytes of a dword are checked to read alike).
+__global__ __launch_bounds__(kThreads) void fp4_decode_kernel(uint32_t* out,
+                                                              unsigned long long* result) {
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  const u32x4 v = fp4x8_to_bf16((uint32_t)(i & 255) * 0x01010101u, mx4_scale((uint32_t)i >> 8));
+  out[i] = v[0];
+  report(result, v[1] != v[0] || v[2] != v[0] || v[3] != v[0], ~0ull);
 }
 
 // Neighbouring floats of a positive finite v.
@@ -266,6 +297,22 @@ extern "C" int rmt_fp8_encode_table(int e_lo, int e_hi, uint8_t* out, unsigned l
 // out: device [256 * 256] u16.
 extern "C" int rmt_fp8_decode_table(uint16_t* out, void* stream) {
   hipLaunchKernelGGL(fp8_decode_kernel, dim3(256), dim3(kThreads), 0, (hipStream_t)stream, out);
+  return status();
+}
+
+// out: device [(e_hi - e_lo + 1) * 65536] u8; result as above (dwords whose codes differ).
+extern "C" int rmt_fp4_encode_table(int e_lo, int e_hi, uint8_t* out, unsigned long long* result,
+                                    void* stream) {
+  if (e_lo < -126 || e_hi > 127 || e_hi < e_lo) return -2;
+  hipLaunchKernelGGL(fp4_encode_kernel, dim3(kBlocks), dim3(kThreads), 0, (hipStream_t)stream,
+                     e_lo, e_hi - e_lo + 1, out, result);
+  return status();
+}
+
+// out: device [256 * 256] u32; result as above (bytes read differently).
+extern "C" int rmt_fp4_decode_table(uint32_t* out, unsigned long long* result, void* stream) {
+  hipLaunchKernelGGL(fp4_decode_kernel, dim3(256), dim3(kThreads), 0, (hipStream_t)stream, out,
+                     result);
   return status();
 }
 

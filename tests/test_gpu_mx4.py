@@ -2,6 +2,9 @@
 derived tolerances (mx4_reference.py) of the plain definitions; a serving step that
 runs slot maps, store, window lists and decode together; graphs, streams."""
 
+import ctypes
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -39,6 +42,60 @@ def native_pool(pages, seed):
     remnant.native_store_rows(x.to(DEV), torch.ones(512, device=DEV), 1e-6,
                               torch.arange(pages * 64, dtype=I32, device=DEV), None, None, pool)
     return pool
+
+
+# ---- the conversions ----
+
+@pytest.fixture(scope="module")
+def selftest():
+    path = os.path.join(os.path.dirname(remnant.__file__), "_lib", "libremnant_selftest.so")
+    if not os.path.exists(path):
+        pytest.fail(f"{path} is not built (make -C flash-optimizations_amd/csrc)")
+    lib = ctypes.CDLL(path)
+    vp, i32 = ctypes.c_void_p, ctypes.c_int
+    lib.rmt_fp4_encode_table.argtypes = [i32, i32, vp, vp, vp]
+    lib.rmt_fp4_decode_table.argtypes = [vp, vp, vp]
+    return lib
+
+
+def test_fp4_encode_every_bf16_input_and_scale(selftest):
+    """v_cvt_scalef32_pk_fp4_bf16 at the scales a store writes: the nearest level, a
+    midpoint to the even code, magnitudes above 6 to 6."""
+    banner("fp4 encode: all bf16 x scales -15..32")
+    lo, hi = -15, 32
+    out = torch.empty((hi - lo + 1) * 65536, dtype=torch.uint8, device=DEV)
+    result = torch.tensor([0, -1], dtype=torch.int64, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert selftest.rmt_fp4_encode_table(lo, hi, out.data_ptr(), result.data_ptr(), stream) == 0
+    assert result[0].item() == 0, "the codes of one dword differ"
+    table = out.cpu().numpy().reshape(-1, 65536)
+    bits = np.arange(65536, dtype=np.uint32)
+    with np.errstate(invalid="ignore"):
+        n = (bits << 16).view(np.float32).astype(np.float64)
+    finite = np.isfinite(n)
+    mid = (ref.LEVELS[1:] + ref.LEVELS[:-1]) / 2
+    for e in range(lo, hi + 1):
+        v = np.abs(n[finite]) * 2.0 ** -e
+        code = np.searchsorted(mid, v, side="left")  # a midpoint to the lower level ...
+        tie = np.isin(v, mid)
+        code = np.where(tie & (code % 2 == 1), code + 1, code)  # ... unless that is odd
+        assert np.array_equal(table[e - lo][finite], code + 8 * np.signbit(n[finite])), e
+
+
+def test_fp4_decode_every_byte_and_scale(selftest):
+    """v_cvt_scalef32_pk_bf16_fp4 at the scale bytes a store writes, 255 among them."""
+    banner("fp4 decode: all bytes x scales")
+    out = torch.empty(65536, dtype=torch.int32, device=DEV)
+    result = torch.tensor([0, -1], dtype=torch.int64, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert selftest.rmt_fp4_decode_table(out.data_ptr(), result.data_ptr(), stream) == 0
+    got = out.view(torch.bfloat16).double().cpu().numpy().reshape(256, 256, 2)
+    level = np.concatenate([ref.LEVELS, -ref.LEVELS])
+    codes = np.arange(256)
+    want = np.stack([level[codes & 15], level[codes >> 4]], -1)
+    assert np.isnan(got[255]).all()
+    scales = np.arange(112, 160)
+    assert np.array_equal(got[scales], want * 2.0 ** (scales - 127.0)[:, None, None])
 
 
 # ---- store ----
@@ -307,6 +364,50 @@ def test_decode_batches(batch, q_len, topk):
     check(case.run(), case.want())
 
 
+@pytest.mark.parametrize("batch,heads,topk,window", [
+    (128, 16, 2048, 0),    # records past the caches
+    (64, 64, 5000, 0),     # the same, forty rounds a workgroup, each record for four of them
+    (32, 128, 5000, 40),   # forty rounds through the caches, the window behind them
+    (260, 16, 200, 100),   # more tokens than workgroups at once, the window behind the list
+    (20, 16, 2000, 512),   # splits, and the window in a workgroup of its own
+    (3, 1000, 70, 20), (1, 1024, 300, 0)])
+def test_decode_forms(batch, heads, topk, window):
+    """Sizes at which the kernel shares its work out in another way, some tokens of each
+    against the definition."""
+    banner(f"decode batch {batch} heads {heads} topk {topk} window {window}")
+    case = Case(heads, topk, batch=batch, seed=batch, window=window, context=40)
+    rng = np.random.default_rng(batch)
+    case.pool = random_pool(90, 5)
+    case.table = rng.integers(0, 90, (batch, 31)).astype(np.int32)
+    case.kw["seqlens"] = rng.integers(1500, 31 * 64 + 1, batch).astype(np.int32)
+    case.kw["topk_length"][:] = rng.integers(topk * 3 // 4, topk + 1, batch)
+    case.indices = rng.integers(-20, 31 * 64, case.indices.shape).astype(np.int32)
+    out, lse = case.run()
+    assert out.isfinite().all() and lse.isfinite().all()
+    some = sorted({0, batch // 2, batch - 1})
+    part = {k: v if k in ("sink", "swa_pool") or v is None else v[some] for k, v in case.kw.items()}
+    if window:
+        part["swa_pool"] = case.kw["swa_pool"].layer().cpu().numpy()
+    check((out[some], lse[some]),
+          ref.decode(case.q[some], case.pool, case.table[some], case.indices[some], **part))
+
+
+def test_decode_wide_block_table():
+    """More columns than the kernel keeps at hand, lists that use the last of them."""
+    banner("decode wide table")
+    for columns in (1024, 1025, 3000):
+        case = Case(16, 700, batch=2, seed=columns, context=40, window=30)
+        rng = np.random.default_rng(columns)
+        case.pool = random_pool(40, 6)
+        case.table = rng.integers(0, 40, (2, columns)).astype(np.int32)
+        case.table[:, rng.integers(0, columns, 50)] = -1
+        case.kw["seqlens"][:] = [columns * 64, columns * 64 - 70]
+        case.kw["topk_length"][:] = 700
+        case.indices = rng.integers(0, columns * 64 + 40, case.indices.shape).astype(np.int32)
+        case.indices[..., 5] = columns * 64 - 1
+        check(case.run(), case.want(), f"{columns} columns")
+
+
 def test_decode_rows_with_nothing():
     """Lists and windows that leave no row: zeros, the sink alone, or -inf."""
     banner("decode empty rows")
@@ -389,19 +490,6 @@ def test_decode_nan_group_poisons_its_token_alone():
     assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
     for b in (0, 2):
         assert torch.equal(out[b], before[0][b]) and torch.equal(lse[b], before[1][b])
-    # a list of nothing but such records, with and without a sink, in one split and in many
-    rec[:, 256] = 255
-    for topk in (1, 50):
-        case.indices = case.indices[..., :topk].copy()
-        case.kw["topk_length"][:] = topk
-        for sink in (case.kw["sink"], None):
-            out, lse = case.run(sink=None if sink is None else gpu(sink))
-            assert torch.isnan(out).all() and torch.isnan(lse).all()
-    long = Case(16, 4000, seed=9, full=True, batch=1)
-    long.pool.reshape(-1, 272)[:, 256] = 255
-    for sink in (None, gpu(long.kw["sink"])):
-        out, lse = long.run(sink=sink)
-        assert torch.isnan(out).all() and torch.isnan(lse).all()
     # a list of nothing but such records, with and without a sink, in one split and in many
     rec[:, 256] = 255
     for topk in (1, 50):
