@@ -843,17 +843,26 @@ struct Plan {
   int splits;  // of them the list's; the window has one of its own where there are several
 };
 
-// About one workgroup a CU (256), each with a round of the list of its own. The window's
-// rows are fetched while the list's are where it has a workgroup to itself (16 tokens x 64
-// heads, 317 + 64 rows: 15.0 -> 14.0 us against both in each workgroup).
+// At most one workgroup a CU (256; its LDS allows one at a time), so that all run at once:
+// 96 tokens x 2,048 records 29.4 us with two a token and 44.1 with three, 129 tokens 40.0
+// with one and 52.4 with two, 300 tokens 79.6 and 80.3. No more than the rounds divide by
+// (43 tokens x 16 rounds: 20.8 us with four a token, 21.5 with five), and one alone where
+// splitting saves a round only, which the second kernel costs again (32 tokens x 2 rounds
+// 9.4 and 10.2 us, x 3 rounds 12.4 and 10.9; 1 token x 2 rounds 9.0 both); with more tokens
+// their partial results count too (96 tokens x 4 rounds 15.5 and 16.0). The window's rows
+// are fetched while the list's are where it has a workgroup to itself.
 Plan plan(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
   Plan p;
   p.waves = 8;
+  p.slots = p.splits = 1;
   const int64_t base = std::max<int64_t>(tokens * ((heads + 15) / 16), 1);
   const int64_t rounds = (topk + 16 * p.waves - 1) / (16 * p.waves), window = swa_topk > 0;
-  p.slots = (int)std::max<int64_t>(
-      std::min({(256 + base - 1) / base, rounds + window, (int64_t)kMaxSplits}), 1);
-  p.splits = (int)std::max<int64_t>(p.slots - window, 1);
+  const int64_t most = std::min({256 / base - window, rounds, kMaxSplits - window});
+  if (most < 1) return p;
+  const int64_t each = (rounds + most - 1) / most;
+  if (64 * (rounds + window - std::max(each, window)) < 64 + base) return p;
+  p.splits = (int)((rounds + each - 1) / each);
+  p.slots = p.splits + (int)window;
   return p;
 }
 size_t ws_bytes(int64_t tokens, int64_t heads, int64_t slots) {
@@ -890,9 +899,12 @@ extern "C" int rm_mx4_sparse_decode_fwd(
   if (!q || !out || !lse || (topk > 0 && (!indices || !pool || !block_table)) ||
       (swa_topk > 0 && (!swa_indices || !swa_pool)))
     return RM_ERR_NULL;
-  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(lse, 4) || !aligned(pool, 16) ||
-      !aligned(swa_pool, 16))
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(pool, 16) || !aligned(swa_pool, 16))
     return RM_ERR_ALIGN;
+  for (const void* p : {(const void*)block_table, (const void*)seqlens, (const void*)indices,
+                        (const void*)topk_length, (const void*)swa_indices,
+                        (const void*)swa_length, (const void*)sink, (const void*)lse})
+    if (!aligned(p, 4)) return RM_ERR_ALIGN;
   const Plan p = plan(tokens, heads, topk, swa_topk);
   const size_t bytes = ws_bytes(tokens, heads, p.slots);
   if (bytes > 0 && (!workspace || workspace_bytes < bytes)) return RM_ERR_WORKSPACE;

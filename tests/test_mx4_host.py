@@ -199,7 +199,8 @@ def test_c_entries_refuse_bad_arguments():
                               (16, 513, -2), (14, -1, -2), (0, None, -1), (4, None, -1),
                               (6, None, -1), (10, None, -1), (20, None, -1), (21, None, -1),
                               (16, 4, -1), (0, x + 8, -3), (4, pool + 8, -3), (20, x + 2, -3),
-                              (21, x + 2, -3)):
+                              (21, x + 2, -3), (6, s + 2, -3), (9, s + 2, -3), (10, s + 1, -3),
+                              (12, s + 2, -3), (15, s + 2, -3), (17, s + 2, -3), (18, s + 2, -3)):
         args = list(ok)
         args[at] = value
         assert decode(*args) == status, (at, value)
