@@ -17,10 +17,10 @@
 //     V^T P^T. The codes come out of LDS transposed (ds_read_b64_tr_b4) and become BF16
 //     without their scales: those are powers of two that differ by record and group, so
 //     they go to the weights, and so does, where the round has any, the step from a
-//     tile's m to the running maximum: integer subtractions on the BF16 exponents, two weights an instruction,
-//     saturating at zero (v_pk_sub_u16 clamp), against the largest scale the store
-//     writes, 2^32; O is in units of it. A weight that a scale takes below 2^-126 becomes
-//     zero: less than 2^-71 of the largest weight at that scale;
+//     tile's m to the running maximum: integer subtractions on the BF16 exponents, two
+//     weights an instruction, saturating at zero (v_pk_sub_u16 clamp), against the largest
+//     scale the store writes, 2^32; O is in units of it. A weight that a scale takes below
+//     2^-126 becomes zero: less than 2^-71 of the largest weight at that scale;
 //   * the copying waves fetch round i + 2 into the LDS that round i - 2 has left
 //     (global_load_lds, consecutive lanes taking consecutive 16-byte pieces of a record,
 //     17 a record, so that a copy touches each 128-byte line once), and wait for round
@@ -54,6 +54,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 
 struct DecodeArgs {
+  int first;  // token of workgroups (., 0, .)
   const uint16_t* q;
   uint64_t q_len_magic;  // ceil(2^32 / q_len): token t < 2^16 is of request t * q_len_magic >> 32
   int heads;
@@ -80,8 +81,8 @@ struct DecodeArgs {
   int ws_splits;  // partial slots a row; 0: finish in place
   uint16_t* out;
   float* lse;
-  float* ws_o;    // [tokens, ws_splits, heads, 512]
-  float* ws_lse;  // [tokens, ws_splits, heads]
+  float* ws_o;    // [this launch's tokens, ws_splits, heads, 512]
+  float* ws_lse;  // [the same, ws_splits, heads]
 };
 
 // A chunk in LDS: its records 272 bytes apart (4 banks), with 128 bytes between the
@@ -203,7 +204,7 @@ struct Share {
         lane(wave_lane()),
         wave(uniform((int)(threadIdx.x >> 6))),
         split((int)blockIdx.x),
-        t(blockIdx.y) {}
+        t(args.first + (int)blockIdx.y) {}
   __device__ __forceinline__ int64_t request() const {
     return (int64_t)(((uint64_t)t * a.q_len_magic) >> 32);
   }
@@ -769,7 +770,7 @@ struct Decode : Share<kWaves> {
     if (h >= a.heads) return;
     const int c0 = wave * kTiles * 16 + 4 * group;
     if (a.ws_splits != 0) {
-      const int64_t at = (t * a.ws_splits + split) * a.heads + h;
+      const int64_t at = ((int64_t)blockIdx.y * a.ws_splits + split) * a.heads + h;
       const float f = sum != 0.0f ? 0x1p32f * __builtin_amdgcn_rcpf(sum) : 0.0f;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
@@ -837,36 +838,40 @@ bool bad_sizes(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
          topk > kMaxTopk || swa_topk < 0 || swa_topk > kMaxWindow;
 }
 
+constexpr int kWaves = 8;  // that compute, a workgroup
+
 struct Plan {
-  int waves;   // that compute, a workgroup
-  int slots;   // workgroups a token and 16 heads
-  int splits;  // of them the list's; the window has one of its own where there are several
+  int64_t alone;  // tokens with one workgroup a 16 heads
+  int slots;      // workgroups a 16 heads of each of the others
+  int splits;     // of them the list's; the window, where there is one, has the last
 };
 
 // At most one workgroup a CU (256; its LDS allows one at a time), so that all run at once:
 // 96 tokens x 2,048 records 29.4 us with two a token and 44.1 with three, 129 tokens 40.0
-// with one and 52.4 with two, 300 tokens 79.6 and 80.3. No more than the rounds divide by
-// (43 tokens x 16 rounds: 20.8 us with four a token, 21.5 with five), and one alone where
-// splitting saves a round only, which the second kernel costs again (32 tokens x 2 rounds
-// 9.4 and 10.2 us, x 3 rounds 12.4 and 10.9; 1 token x 2 rounds 9.0 both); with more tokens
-// their partial results count too (96 tokens x 4 rounds 15.5 and 16.0). The window's rows
-// are fetched while the list's are where it has a workgroup to itself.
+// with one and 52.4 with two. No more than the rounds divide by (43 tokens x 16 rounds: 20.8
+// us with four a token, 21.5 with five), and one alone where splitting saves a round only,
+// which the second kernel costs again (32 tokens x 2 rounds 9.4 and 10.2 us, x 3 rounds 12.4
+// and 10.9; 1 token x 2 rounds 9.0 both); with more tokens their partial results count too
+// (96 tokens x 4 rounds 15.5 and 16.0). The window's rows are fetched while the list's are
+// where it has a workgroup to itself.
+// Beyond 256 workgroups it is the tokens of the last, partial turn that are split, in a
+// launch of their own (270 tokens x 2,048 records 78.7 -> 59.4 us, 300 79.5 -> 68.2, 384
+// 83.4 -> 79.3, 520 118.8 -> 100.6; 384 x 512 34.8 both; one launch for both kinds took 2.5
+// less there and 0.2 more on one token, 9.2).
 Plan plan(int64_t tokens, int64_t heads, int64_t topk, int64_t swa_topk) {
-  Plan p;
-  p.waves = 8;
-  p.slots = p.splits = 1;
-  const int64_t base = std::max<int64_t>(tokens * ((heads + 15) / 16), 1);
-  const int64_t rounds = (topk + 16 * p.waves - 1) / (16 * p.waves), window = swa_topk > 0;
+  const int64_t groups = std::max<int64_t>((heads + 15) / 16, 1);
+  const int64_t rounds = (topk + 16 * kWaves - 1) / (16 * kWaves), window = swa_topk > 0;
+  const int64_t alone = tokens * groups / 256 * 256 / groups;
+  const int64_t base = std::max<int64_t>((tokens - alone) * groups, 1);
   const int64_t most = std::min({256 / base - window, rounds, kMaxSplits - window});
-  if (most < 1) return p;
+  if (alone == tokens || most < 1) return {tokens, 1, 1};
   const int64_t each = (rounds + most - 1) / most;
-  if (64 * (rounds + window - std::max(each, window)) < 64 + base) return p;
-  p.splits = (int)((rounds + each - 1) / each);
-  p.slots = p.splits + (int)window;
-  return p;
+  if (64 * (rounds + window - std::max(each, window)) < 64 + base) return {tokens, 1, 1};
+  const int64_t splits = (rounds + each - 1) / each;
+  return {alone, (int)(splits + window), (int)splits};
 }
-size_t ws_bytes(int64_t tokens, int64_t heads, int64_t slots) {
-  return slots > 1 ? (size_t)(tokens * slots * heads) * (kHeadDim + 1) * sizeof(float) : 0;
+size_t ws_bytes(const Plan& p, int64_t tokens, int64_t heads) {
+  return (size_t)((tokens - p.alone) * p.slots * heads) * (kHeadDim + 1) * sizeof(float);
 }
 
 }  // namespace
@@ -877,7 +882,7 @@ extern "C" int rm_mx4_sparse_decode_workspace(int64_t tokens, int64_t heads, int
   if (bad_sizes(tokens, heads, topk, swa_topk)) return RM_ERR_SHAPE;
   const Plan p = plan(tokens, heads, topk, swa_topk);
   if (num_splits) *num_splits = p.slots;
-  if (workspace_bytes) *workspace_bytes = ws_bytes(tokens, heads, p.slots);
+  if (workspace_bytes) *workspace_bytes = ws_bytes(p, tokens, heads);
   return RM_OK;
 }
 
@@ -906,7 +911,7 @@ extern "C" int rm_mx4_sparse_decode_fwd(
                         (const void*)swa_length, (const void*)sink, (const void*)lse})
     if (!aligned(p, 4)) return RM_ERR_ALIGN;
   const Plan p = plan(tokens, heads, topk, swa_topk);
-  const size_t bytes = ws_bytes(tokens, heads, p.slots);
+  const size_t bytes = ws_bytes(p, tokens, heads);
   if (bytes > 0 && (!workspace || workspace_bytes < bytes)) return RM_ERR_WORKSPACE;
   if (bytes > 0 && !aligned(workspace, 16)) return RM_ERR_ALIGN;
   DecodeArgs a;
@@ -931,20 +936,33 @@ extern "C" int rm_mx4_sparse_decode_fwd(
   a.swa_length = swa_length;
   a.sink = sink;
   a.scale_log2 = softmax_scale * kLog2e;
-  a.splits = p.splits;
-  a.splits_magic = (((uint64_t)1 << 32) + p.splits - 1) / p.splits;
-  a.window_split = p.slots > 1 ? p.splits : 0;
-  a.ws_splits = p.slots > 1 ? p.slots : 0;
   a.out = out;
   a.lse = lse;
-  a.ws_o = (float*)workspace;
-  a.ws_lse = bytes ? (float*)workspace + (size_t)tokens * p.slots * heads * kHeadDim : nullptr;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)p.slots, (unsigned)tokens, (unsigned)((heads + 15) / 16));
-  hipLaunchKernelGGL(mx4_decode_kernel<8>, grid, dim3(96 * p.waves), 0, s, a);
-  if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
-  if (p.slots > 1) {
-    launch_combine<true>(a.ws_o, a.ws_lse, sink, p.slots, tokens, heads, out, lse, s);
+  const unsigned groups = (unsigned)((heads + 15) / 16);
+  if (p.alone > 0) {
+    a.first = 0;
+    a.splits = 1;
+    a.splits_magic = (uint64_t)1 << 32;
+    a.window_split = a.ws_splits = 0;
+    a.ws_o = a.ws_lse = nullptr;
+    hipLaunchKernelGGL(mx4_decode_kernel<kWaves>, dim3(1, (unsigned)p.alone, groups),
+                       dim3(96 * kWaves), 0, s, a);
+    if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
+  }
+  const int64_t rest = tokens - p.alone;
+  if (rest > 0) {
+    a.first = (int)p.alone;
+    a.splits = a.window_split = p.splits;
+    a.splits_magic = (((uint64_t)1 << 32) + p.splits - 1) / p.splits;
+    a.ws_splits = p.slots;
+    a.ws_o = (float*)workspace;
+    a.ws_lse = (float*)workspace + (size_t)rest * p.slots * heads * kHeadDim;
+    hipLaunchKernelGGL(mx4_decode_kernel<kWaves>, dim3((unsigned)p.slots, (unsigned)rest, groups),
+                       dim3(96 * kWaves), 0, s, a);
+    if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
+    launch_combine<true>(a.ws_o, a.ws_lse, sink, p.slots, rest, heads,
+                         out + p.alone * heads * kHeadDim, lse + p.alone * heads, s);
     if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   }
   return RM_OK;

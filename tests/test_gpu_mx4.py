@@ -369,6 +369,7 @@ def test_decode_batches(batch, q_len, topk):
     (64, 64, 5000, 0),     # the same, forty rounds a workgroup, each record for four of them
     (32, 128, 5000, 40),   # forty rounds through the caches, the window behind them
     (260, 16, 200, 100),   # more tokens than workgroups at once, the window behind the list
+    (300, 16, 1000, 0), (300, 16, 1000, 30), (90, 48, 700, 5),  # the last of them split
     (20, 16, 2000, 512),   # splits, and the window in a workgroup of its own
     (3, 1000, 70, 20), (1, 1024, 300, 0)])
 def test_decode_forms(batch, heads, topk, window):
