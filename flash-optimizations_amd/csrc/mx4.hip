@@ -42,14 +42,8 @@ __global__ __launch_bounds__(256) void mx4_gather_kernel(GatherArgs a) {
     const int64_t r = r0 + lane;
     int32_t slot = -1;  // lane i: the slot of row r0 + i
     if (lane < kRows && r < a.rows) {
-      int64_t q, k;
-      if (a.rows <= 0xffffffffll) {
-        q = (uint32_t)r / (uint32_t)a.k;
-        k = (uint32_t)r - (uint32_t)q * (uint32_t)a.k;
-      } else {
-        q = r / a.k;
-        k = r - q * a.k;
-      }
+      const int64_t q = (uint32_t)r / (uint32_t)a.k;
+      const int64_t k = r - q * a.k;
       const int64_t live = a.lengths ? a.lengths[q * a.length_stride] : a.k;
       if (k < live) slot = a.slots[q * a.stride_q + k * a.stride_k];
       if (slot >= a.pool_rows) slot = -1;
@@ -84,7 +78,7 @@ extern "C" int rm_mx4_gather_bf16(const uint8_t* pool, int64_t pool_pages, const
                                   void* stream) {
   if (n_queries < 0 || selected_k < 0 || pool_pages < 0 || pool_pages > ((int64_t)1 << 25))
     return RM_ERR_SHAPE;
-  if (selected_k > 0 && n_queries > ((int64_t)1 << 40) / selected_k) return RM_ERR_SHAPE;
+  if (selected_k > 0 && n_queries > 0xffffffffll / selected_k) return RM_ERR_SHAPE;
   if (n_queries == 0 || selected_k == 0) return RM_OK;
   if (!pool || !slots || !out) return RM_ERR_NULL;
   if (!aligned(pool, 16) || !aligned(out, 16) || !aligned(slots, 4) || !aligned(lengths, 4))

@@ -82,8 +82,9 @@ def mx4_store_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, loc: torch
     slots ``loc`` [n] int32: RMSNorm with ``weight``, BF16 rounding, the tail rotated
     with frequency row ``positions * 4`` (``freqs_cis=None``: not rotated) and rounded
     to BF16, then E2M1 codes under one scale per 32 coordinates. Slots outside the
-    pool, and rows whose frequency row is outside the table, are skipped. A group of 32
-    with an infinity or NaN reads back as NaN."""
+    pool, and rows whose frequency row is outside the table, are skipped; those stored
+    must differ (two rows for one slot leave a mixture of both). A group of 32 with an
+    infinity or NaN reads back as NaN."""
     buf, pages, n_pages = _pages(pool, layer_id)
     shape, strides, dtype = x.shape, x.stride(), x.dtype
     if len(shape) != 2 or shape[1] != config.HEAD_DIM or strides[1] != 1:

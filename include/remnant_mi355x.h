@@ -350,7 +350,8 @@ int rm_native_sparse_decode_swa_fwd(const uint16_t* q, int64_t batch, int64_t q_
  * rotation) as 4-bit records. Per 32 coordinates the scale is 2^e, the smallest
  * e with max(amax, 1e-4) <= 6 * 2^e and at most 32; codes are n / 2^e rounded to
  * nearest even, magnitudes above 6 to 6. A group with an infinity or NaN gets
- * scale byte 255 and reads as 32 NaN. Skipped rows as rm_native_store_rows.
+ * scale byte 255 and reads as 32 NaN. Skipped rows as rm_native_store_rows; the
+ * slots of the others must differ (two rows at once leave a mixture of both).
  * weight 16-byte aligned. */
 int rm_mx4_store_rows(const void* x, int x_dtype, int64_t x_row_stride, const float* weight,
                       float eps, const int32_t* dst_slot, const int32_t* position,
@@ -359,7 +360,8 @@ int rm_mx4_store_rows(const void* x, int x_dtype, int64_t x_row_stride, const fl
 
 /* Reader: out row q * selected_k + k (512 BF16 values, contiguous) = record
  * slots[q, k], exact; zeros unless k < lengths[q] (NULL = selected_k) and
- * 0 <= slot < pool_pages * 64. Strides are in int32 elements. */
+ * 0 <= slot < pool_pages * 64. Strides are in int32 elements; fewer than 2^32
+ * rows. */
 int rm_mx4_gather_bf16(const uint8_t* pool, int64_t pool_pages, const int32_t* slots,
                        int64_t slots_stride_q, int64_t slots_stride_k, const int32_t* lengths,
                        int64_t length_stride, int64_t n_queries, int64_t selected_k,

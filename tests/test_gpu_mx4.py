@@ -409,6 +409,27 @@ def test_decode_wide_block_table():
         check(case.run(), case.want(), f"{columns} columns")
 
 
+@pytest.mark.parametrize("pages", [130000, 246723, 246724, 300000])
+def test_decode_and_reader_far_in_the_pool(pages):
+    """Records past 2 and 4 GiB, by either way of forming their addresses: the bits of the
+    same records in a small pool."""
+    banner(f"decode far, {pages} pages")
+    case = Case(16, 400, batch=2, seed=11, context=2000, full=True)
+    near = case.pool.shape[0]
+    pool = torch.zeros(pages, 17408, dtype=torch.uint8, device=DEV)
+    pool[pages - near:] = gpu(case.pool)
+    want = case.run()
+    check(want, case.want())
+    kw = {k: gpu(v) for k, v in case.kw.items()}
+    table = gpu(np.where(case.table >= 0, case.table + pages - near, -1))
+    got = remnant.mx4_sparse_decode_fwd(case.q.to(DEV), pool, table, gpu(case.indices), **kw)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    slots = torch.arange(near * 64, dtype=I32, device=DEV)[None]
+    far = remnant.mx4_gather_bf16(pool, slots + (pages - near) * 64, None)
+    assert torch.equal(far, remnant.mx4_gather_bf16(gpu(case.pool), slots, None))
+
+
 def test_decode_rows_with_nothing():
     """Lists and windows that leave no row: zeros, the sink alone, or -inf."""
     banner("decode empty rows")

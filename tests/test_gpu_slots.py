@@ -162,6 +162,20 @@ def test_window_long_lists(window, first, shift):
     assert (flat[:shift] == -7).all() and (flat[shift + n:] == -7).all()
 
 
+def test_window_more_than_32_bits_of_entries():
+    print("[gpu-slots] window 4.3e9 entries", flush=True)
+    tokens, window = 33000, 131073
+    table = torch.arange(tokens, dtype=I32, device=DEV)[:, None] + torch.arange(2, dtype=I32,
+                                                                                device=DEV)
+    table = table.contiguous()
+    lengths = torch.arange(tokens, dtype=I32, device=DEV) % 140 + 1
+    slots, counts = remnant.window_slots(table, lengths, 1, window)
+    assert torch.equal(counts, lengths)
+    some = [0, 1, 139, 20000, 32767, 32768, 32999]
+    want, _ = ref.window(table[some].cpu().numpy(), lengths[some].cpu().numpy(), 1, window, 0)
+    assert np.array_equal(slots[some].cpu().numpy(), want)
+
+
 def test_window_many_tokens_and_extreme_lengths():
     print("[gpu-slots] window many", flush=True)
     lengths = torch.full((70000,), 3, dtype=I32, device=DEV)
