@@ -8,10 +8,12 @@ missing, every operator raises instead of computing anything on the CPU.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libremnant_mi355x.so")
+OPS_PATH = os.path.join(_HERE, "_lib", "remnant_ops.so")
 
 STATUS = {
     0: "ok",
@@ -108,6 +110,36 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_ops = None
+
+
+def ops():
+    """Module of csrc/ops.cpp: checks and launches of the 4-bit operators and the slot
+    maps, over the entry points of ``load()``."""
+    return _ops or _load_ops()
+
+
+def _load_ops():
+    global _ops
+    import torch
+
+    from .flash_mla import _native_pages
+    from .pool import LatentPool
+    lib = load()
+    if not os.path.exists(OPS_PATH):
+        raise RemnantLibraryMissing(f"{OPS_PATH} is not built; run __graft_entry__.build() "
+                                    "(or make -C flash-optimizations_amd/csrc)")
+    spec = importlib.util.spec_from_file_location("remnant_ops", OPS_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.setup(tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        "rm_mx4_store_rows", "rm_mx4_gather_bf16", "rm_mx4_sparse_decode_workspace",
+        "rm_mx4_sparse_decode_fwd", "rm_append_slots", "rm_window_slots")),
+        LatentPool, torch._C._cuda_getCurrentRawStream, check, _native_pages)
+    _ops = module
+    return module
 
 
 def check(status: int, what: str) -> None:

@@ -49,15 +49,21 @@ def _plan(tokens: int, heads: int, topk: int, swa_topk: int) -> tuple[int, int]:
     return splits.value, nbytes.value
 
 
+def _native_pages(swa_pool):
+    """Page tensor of the Native pool of the window rows."""
+    pages, packed, _ = _as_pool(swa_pool, None)
+    if packed:
+        raise ValueError("the window rows are read from a Native pool")
+    return pages
+
+
 def _swa_args(swa_pool, swa_indices, swa_lengths, batch, q_len):
     """Validate the window inputs: (pool pages, indices, lengths, W)."""
     if swa_pool is None and swa_indices is None:
         return None, None, None, 0
     if swa_pool is None or swa_indices is None:
         raise ValueError("swa_pool and swa_indices are given together")
-    sbuf, spacked, _ = _as_pool(swa_pool, None)
-    if spacked:
-        raise ValueError("the window rows are read from a Native pool")
+    sbuf = _native_pages(swa_pool)
     if swa_indices.dtype != torch.int32 or swa_indices.dim() != 3 \
             or swa_indices.shape[:2] != (batch, q_len) or not swa_indices.is_contiguous():
         raise ValueError("swa_indices must be a contiguous int32 [batch, q_len, W] tensor")

@@ -14,8 +14,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib, config
-from .mx4 import _I32, _launch, _one_device
+from . import _lib
 
 
 class SlotMap(NamedTuple):
@@ -26,24 +25,6 @@ class SlotMap(NamedTuple):
     row_starts: torch.Tensor   # int32 [batch + 1]
     seqlens: torch.Tensor      # int32 [batch]: records after the step
     pages_taken: torch.Tensor  # int32 [1]: pages needed; beyond the free list: it was short
-
-
-def _vector(name, t, n):
-    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 vector of {n} entries")
-
-
-def _table(block_table):
-    shape, strides = block_table.shape, block_table.stride()
-    if block_table.dtype is not _I32 or len(shape) != 2 or (shape[1] > 1 and strides[1] != 1):
-        raise ValueError("block_table must be int32 [batch, max_blocks] with unit inner stride")
-    batch, width = shape
-    stride = strides[0]
-    if stride < width:
-        if batch > 1:
-            raise ValueError("block_table rows must not overlap")
-        stride = width
-    return batch, width, stride
 
 
 def append_slots(block_table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: torch.Tensor,
@@ -65,39 +46,13 @@ def append_slots(block_table: torch.Tensor, old_lengths: torch.Tensor, new_lengt
     past the capacity are left out. Where the free list or the table's columns run out,
     slots are -1; ``pages_taken`` tells how many pages were needed. ``out``: a
     ``SlotMap`` (or five tensors) to write to instead of new ones."""
-    batch, width, stride = _table(block_table)
-    if batch > config.MAX_SLOT_BATCH:
-        raise ValueError(f"at most {config.MAX_SLOT_BATCH} requests a call")
-    if type(ratio) is not int or not 1 <= ratio < 2 ** 31:
-        raise ValueError("ratio must be a positive int")
-    _vector("old_lengths", old_lengths, batch)
-    _vector("new_lengths", new_lengths, batch)
-    free = free_pages.shape
-    if free_pages.dtype is not _I32 or len(free) != 1 or not free_pages.is_contiguous():
-        raise ValueError("free_pages must be a contiguous int32 vector")
-    if rows is None and out is not None:
-        rows = out[0].shape[0] if out[0].dim() == 1 else 0
-    elif type(rows) is not int or not 0 <= rows < 2 ** 31:
-        raise ValueError("rows must be an int, the capacity of the row lists")
+    append = _lib.ops().append
     if out is None:
-        new = block_table.new_empty
-        out = SlotMap(new(rows), new(rows), new(batch + 1), new(batch), new(1))
-    else:
-        if type(out) is not SlotMap:
-            out = SlotMap(*out)
-        _vector("loc", out.loc, rows)
-        _vector("positions", out.positions, rows)
-        _vector("row_starts", out.row_starts, batch + 1)
-        _vector("seqlens", out.seqlens, batch)
-        _vector("pages_taken", out.pages_taken, 1)
-    loc, positions, row_starts, seqlens, taken = out
-    device = _one_device(block_table, old_lengths, new_lengths, free_pages, loc, positions,
-                         row_starts, seqlens, taken)
-    _launch(device, "rm_append_slots", block_table.data_ptr(), stride, width,
-            old_lengths.data_ptr(), new_lengths.data_ptr(), batch, ratio, free_pages.data_ptr(),
-            free[0], rows, loc.data_ptr(), positions.data_ptr(), row_starts.data_ptr(),
-            seqlens.data_ptr(), taken.data_ptr())
-    return out
+        return SlotMap._make(append(block_table, old_lengths, new_lengths, free_pages, ratio, rows,
+                                    None))
+    if type(out) is not SlotMap:
+        out = SlotMap(*out)
+    return append(block_table, old_lengths, new_lengths, free_pages, ratio, rows, out)
 
 
 def window_slots(block_table: torch.Tensor, lengths: torch.Tensor, q_len: int, window: int, *,
@@ -113,21 +68,4 @@ def window_slots(block_table: torch.Tensor, lengths: torch.Tensor, q_len: int, w
     order, -1 behind them (and where no page is mapped), and their number -- the
     ``swa_indices`` and ``swa_lengths`` of the decodes, or, with a window as long as the
     history, the slot lists of the readers. ``out``: the two tensors to write to."""
-    batch, width, stride = _table(block_table)
-    if not (type(q_len) is type(window) is type(first) is int and 0 <= q_len < 2 ** 31
-            and 0 <= window < 2 ** 31 and 0 <= first < 2 ** 31):
-        raise ValueError("q_len, window and first must be non-negative ints")
-    _vector("lengths", lengths, batch)
-    shape = (batch, q_len, first + window)
-    if out is None:
-        out = block_table.new_empty(shape), block_table.new_empty(batch * q_len)
-    slots, counts = out
-    if slots.dtype is not _I32 or slots.shape != shape or not slots.is_contiguous():
-        raise ValueError(f"slots must be a contiguous int32 {list(shape)} tensor")
-    _vector("counts", counts, batch * q_len)
-    if batch * q_len == 0:
-        return slots, counts
-    device = _one_device(block_table, lengths, slots, counts)
-    _launch(device, "rm_window_slots", block_table.data_ptr(), stride, width, lengths.data_ptr(),
-            batch, q_len, window, first, slots.data_ptr(), counts.data_ptr())
-    return slots, counts
+    return _lib.ops().window(block_table, lengths, q_len, window, first, out)

@@ -606,6 +606,25 @@ def test_decode_outputs_in_place_and_workspace():
         assert torch.equal(a, b)
 
 
+def test_tensors_of_two_devices_are_refused():
+    banner("two devices")
+    pool = remnant.LatentPool(2, fmt="mx4", device=DEV)
+    x, w, n = torch.zeros(4, 512), torch.ones(512), torch.zeros(4, dtype=I32)
+    with pytest.raises(ValueError, match="same GPU"):
+        remnant.mx4_store_rows(x.to(DEV), w, 1e-6, n.to(DEV), None, None, pool)
+    with pytest.raises(ValueError, match="same GPU"):
+        remnant.mx4_gather_bf16(pool, n[None], None)
+    with pytest.raises(ValueError, match="same GPU"):
+        remnant.window_slots(n[None].to(DEV), n[:1], 1, 4)
+    with pytest.raises(ValueError, match="same GPU"):
+        remnant.append_slots(n[None].to(DEV), n[:1].to(DEV), n[:1].to(DEV), n, rows=2)
+    case = Case(16, 20, batch=1, seed=1)
+    with pytest.raises(ValueError, match="same GPU"):
+        case.run(sink=torch.zeros(16))
+    with pytest.raises(ValueError, match="same GPU"):
+        case.run(workspace=torch.zeros(1 << 20, dtype=torch.uint8))
+
+
 def test_configured_dispatch_reaches_the_4bit_decode():
     banner("dispatch")
     case = Case(16, 64, seed=18)

@@ -3,6 +3,7 @@ against torch casts and closed forms, and the calls that are refused before anyt
 is launched. No kernel runs here."""
 
 import ctypes
+import sys
 
 import numpy as np
 import pytest
@@ -296,6 +297,41 @@ def test_store_and_gather_refuse():
         with pytest.raises(ValueError):
             remnant.mx4_gather_bf16(**(good | change))
     assert remnant.mx4_gather_bf16(pool, slots[:, :0], None).shape == (0, 512)
+
+
+def test_lazily_negated_and_sparse_tensors_are_refused():
+    """Views whose memory does not hold their values."""
+    negated = torch.zeros(4, 512, dtype=torch.complex64).conj().imag
+    assert negated.is_neg()
+    pool = remnant.LatentPool(2, fmt="mx4", device="cpu")
+    loc, w = torch.zeros(4, dtype=I32), torch.ones(512)
+    for x in (negated, torch.zeros(4, 512).to_sparse()):
+        with pytest.raises(ValueError, match="strided"):
+            remnant.mx4_store_rows(x, w, 1e-6, loc, None, None, pool)
+    with pytest.raises(TypeError):
+        remnant.mx4_store_rows(None, w, 1e-6, loc, None, None, pool)
+    with pytest.raises(TypeError):
+        remnant.mx4_store_rows(torch.zeros(4, 512), w, "1e-6", loc, None, None, pool)
+
+
+def test_calls_hold_no_references():
+    pool = remnant.LatentPool(2, fmt="mx4", device="cpu")
+    slots = torch.zeros(2, 0, dtype=I32)
+    t, n = torch.zeros(3, 4, dtype=I32), torch.zeros(3, dtype=I32)
+    held = [pool, pool.buffer, slots, t, n]
+    counts = [sys.getrefcount(x) for x in held]
+    for _ in range(50):
+        out = remnant.mx4_gather_bf16(pool, slots, None)
+        assert remnant.mx4_gather_bf16(pool, slots, None, out) is out
+        assert sys.getrefcount(out) == 2
+        a, b = remnant.window_slots(t, n, 0, 4)
+        assert sys.getrefcount(a) == 2 and sys.getrefcount(b) == 2
+        with pytest.raises(ValueError):
+            remnant.append_slots(t, n, n, n, rows=4)
+        with pytest.raises(ValueError):
+            remnant.mx4_gather_bf16(pool, t, n[:2])
+    del a, b, out
+    assert [sys.getrefcount(x) for x in held] == counts
 
 
 def test_slot_maps_refuse():
