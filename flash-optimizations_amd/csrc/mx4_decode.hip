@@ -307,6 +307,16 @@ struct Copier : Share<kWaves> {
 #pragma unroll
     for (int e = 1; e < kBatch / 2; ++e) slots[e - 1] = slots[e];
   }
+  // Chunks that the last round does not have are neither copied nor added (1 token x 129
+  // records 8.4 -> 7.7 us, 16 tokens x 64 heads x 317 13.4 -> 12.8).
+  __device__ __forceinline__ bool has(int i) const { return i * L::kChunks + of < this->chunks; }
+  // Until round i has landed, of which round i + 1's copies, if there are any, came later.
+  __device__ __forceinline__ void landed(int i) const {
+    if (has(i + 1))
+      wait_copies<kCopies>();
+    else
+      wait_copies<0>();
+  }
   // The chunk of round i; its live records go to LDS.
   __device__ __forceinline__ void copy(int i) {
     const int of_round = slots[0];
@@ -318,6 +328,7 @@ struct Copier : Share<kWaves> {
     const uint32_t live_at = lds + L::kLive + 4 * ((i & (kBuffers - 1)) * L::kChunks + of);
     const uint32_t mask = (uint32_t)(__ballot(of_round >= 0) >> (32 * (i & 1)));
     if (lane == 0) lds_write(live_at, mask);
+    if (!has(i)) return;
     const int record = max(of_round, 0);
     const int base = 128 * (i & 1);
     const bool all = lane < kLastLanes;
@@ -359,7 +370,7 @@ struct Copier : Share<kWaves> {
       if (rounds > 1) {
         copy(1);
         if (rounds > 2) look_up_later();
-        wait_copies<kCopies>();
+        landed(0);
       } else {
         wait_copies<0>();
       }
@@ -369,7 +380,7 @@ struct Copier : Share<kWaves> {
       if (i + 2 < rounds) {
         if (((i + 2) & (kBatch - 1)) == 0) look_up<0, kBatch / 2>(i + 2);
         copy(i + 2);
-        wait_copies<kCopies>();
+        landed(i + 1);
       } else {
         wait_copies<0>();
       }
@@ -568,14 +579,15 @@ struct Decode : Share<kWaves> {
   }
 
   // O += a round, whose first chunk's operands are p and y. kMoved: the tiles' references
-  // `of` are not all the running maximum.
-  template <bool kMoved>
+  // `of` are not all the running maximum. kLast: the round has `here` chunks.
+  template <bool kMoved, bool kLast>
   __device__ __forceinline__ void add(const Places& at, const float (&of)[kWaves], u32x4 (&p)[2],
-                                      Operands (&y)[2]) {
+                                      Operands (&y)[2], int here) {
     constexpr int kGroups = kTiles / 2, kSteps = L::kChunks * kGroups;
 #pragma unroll
     for (int n = 0; n < kSteps; ++n) {
       const int c = n / kGroups, b = n % kGroups, next = n + 1;
+      if (kLast && b == 0 && c > 0 && c >= here) break;
       if (next < kSteps) {
         if (next % kGroups == 0) p[(c + 1) & 1] = lds_read<u32x4>(at.w_at + 1024 * (c + 1));
         operands(at, next / kGroups, next % kGroups, y[next & 1]);
@@ -616,6 +628,7 @@ struct Decode : Share<kWaves> {
     if (!kLast && threadIdx.x == 0) lds_write(lds + L::kMoved + 4 * ((i + 2) & 3), 0);
     if (kFirst) return;
     const bool now = uniform(moved) != 0;
+    const int here = kLast ? this->chunks - (i - 1) * L::kChunks : L::kChunks;
     float of[kWaves];
     if (now || before) {
       float top = m;
@@ -625,10 +638,10 @@ struct Decode : Share<kWaves> {
         top = fmaxf(top, of[w]);
       }
       advance(top, own, sum);
-      add<true>(at, of, p, y);
+      add<true, kLast>(at, of, p, y, here);
     } else {
       l += sum;
-      add<false>(at, of, p, y);
+      add<false, kLast>(at, of, p, y, here);
     }
     before = now;
   }
