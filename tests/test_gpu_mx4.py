@@ -393,6 +393,21 @@ def test_decode_forms(batch, heads, topk, window):
           ref.decode(case.q[some], case.pool, case.table[some], case.indices[some], **part))
 
 
+@pytest.mark.parametrize("copies", [1, 3, 40, 700])
+def test_decode_of_one_record_is_that_record(copies):
+    """Weights of one record alone, also many times over, cancel: its values, exactly."""
+    banner(f"decode one record x {copies}")
+    case = Case(16, copies, batch=2, seed=copies, full=True, q=1.0)
+    case.kw["seqlens"][:] = 500
+    case.indices[:] = 37
+    case.kw["sink"] = None
+    out, lse = case.run()
+    rec = case.pool.reshape(-1, 272)[case.table[:, 0] * 64 + 37]
+    want = np.broadcast_to(ref.decode_rows(rec)[:, None, None], out.shape)
+    assert np.array_equal(out.double().cpu().numpy(), want)
+    check((out, lse), case.want())
+
+
 def test_decode_wide_block_table():
     """More columns than the kernel keeps at hand, lists that use the last of them."""
     banner("decode wide table")
