@@ -23,7 +23,7 @@ using at::Tensor;
 
 // The C entry points of the loaded library and what is needed of Python, from setup().
 struct {
-  decltype(&rm_mx4_store_rows) store;
+  decltype(&rm_mx4_store_rows_ratio) store;
   decltype(&rm_mx4_gather_bf16) gather;
   decltype(&rm_mx4_sparse_decode_workspace) plan;
   decltype(&rm_mx4_sparse_decode_fwd) decode;
@@ -37,6 +37,7 @@ struct {
 } lib;
 
 constexpr int64_t kInt32 = (int64_t)1 << 31;
+constexpr const char* kRatio = "ratio must be a positive int";
 
 // ---- arguments ----
 
@@ -184,10 +185,10 @@ PyObject* same(PyObject* o) {
 #define ARGUMENTS(n) \
   TORCH_CHECK_TYPE(count == n, "expected ", n, " arguments, not ", count)
 
-// x, weight, eps, loc, positions, freqs_cis, pool, layer_id
+// x, weight, eps, loc, positions, freqs_cis, pool, layer_id, ratio
 PyObject* store(PyObject*, PyObject* const* v, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  ARGUMENTS(8);
+  ARGUMENTS(9);
   const Pages pool = mx4_pages(v[6], v[7]);
   const Tensor &x = tensor(v[0], "x"), &weight = tensor(v[1], "weight"), &loc = tensor(v[3], "loc");
   TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == RM_HEAD_DIM && x.stride(1) == 1,
@@ -202,6 +203,7 @@ PyObject* store(PyObject*, PyObject* const* v, Py_ssize_t count) {
                         weight.size(0) == RM_HEAD_DIM && weight.is_contiguous(),
                     "weight must be a contiguous float32 [512] tensor");
   const float eps = number(v[2]);
+  const int64_t ratio = integer(v[8], 1, kInt32, kRatio);
   const Tensor* const freqs = maybe(v[5], "freqs_cis");
   const Tensor* const positions = freqs ? maybe(v[4], "positions") : nullptr;
   int64_t freq_rows = 0;
@@ -215,10 +217,10 @@ PyObject* store(PyObject*, PyObject* const* v, Py_ssize_t count) {
     freq_rows = freqs->numel() / ((RM_HEAD_DIM - RM_NOPE_DIM) / 2);
   }
   if (rows == 0 || (freqs && freq_rows == 0)) return none();
-  launch(one_device(x, &weight, &loc, positions, freqs, &pool.buffer), "rm_mx4_store_rows",
+  launch(one_device(x, &weight, &loc, positions, freqs, &pool.buffer), "rm_mx4_store_rows_ratio",
          lib.store, x.const_data_ptr(), bf16 ? (int)RM_BF16 : (int)RM_F32, x.stride(0),
          (const float*)weight.const_data_ptr(), eps, i32(loc), i32(positions),
-         freqs ? (const float*)freqs->const_data_ptr() : nullptr, freq_rows, rows, pool.at,
+         freqs ? (const float*)freqs->const_data_ptr() : nullptr, freq_rows, ratio, rows, pool.at,
          pool.pages);
   return none();
   END_HANDLE_TH_ERRORS
@@ -356,7 +358,7 @@ PyObject* append(PyObject*, PyObject* const* v, Py_ssize_t count) {
   const Table table = slot_table(v[0]);
   const int64_t batch = table.batch;
   TORCH_CHECK_VALUE(batch <= RM_MAX_SLOT_BATCH, "at most ", RM_MAX_SLOT_BATCH, " requests a call");
-  const int64_t ratio = integer(v[4], 1, kInt32, "ratio must be a positive int");
+  const int64_t ratio = integer(v[4], 1, kInt32, kRatio);
   const Tensor &before = tensor(v[1], "old_lengths"), &after = tensor(v[2], "new_lengths"),
                &free = tensor(v[3], "free_pages");
   vector(before, batch, "old_lengths");

@@ -36,6 +36,8 @@ SIGNATURES = {
                                    _i32, _vp]),
     "rm_native_store_rows": (_i32, [_vp, _i32, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _vp,
                                     _i64, _vp]),
+    "rm_native_store_rows_ratio": (_i32, [_vp, _i32, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _i64,
+                                          _i64, _vp, _i64, _vp]),
     "rm_unpack_gather_bf16_planes": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp, _i64, _i64, _vp,
                                             _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp,
                                             _vp]),
@@ -77,6 +79,8 @@ SIGNATURES = {
                                                _vp, _vp, _f32, _vp, _vp, _vp, _sz, _vp]),
     "rm_mx4_store_rows": (_i32, [_vp, _i32, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _vp,
                                  _i64, _vp]),
+    "rm_mx4_store_rows_ratio": (_i32, [_vp, _i32, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _i64,
+                                       _i64, _vp, _i64, _vp]),
     "rm_mx4_gather_bf16": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp]),
     "rm_mx4_sparse_decode_workspace": (_i32, [_i64, _i64, _i64, _i64,
                                               ctypes.POINTER(ctypes.c_int32),
@@ -135,7 +139,7 @@ def _load_ops():
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     module.setup(tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-        "rm_mx4_store_rows", "rm_mx4_gather_bf16", "rm_mx4_sparse_decode_workspace",
+        "rm_mx4_store_rows_ratio", "rm_mx4_gather_bf16", "rm_mx4_sparse_decode_workspace",
         "rm_mx4_sparse_decode_fwd", "rm_append_slots", "rm_window_slots")),
         LatentPool, torch._C._cuda_getCurrentRawStream, check, _native_pages)
     _ops = module

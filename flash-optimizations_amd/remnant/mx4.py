@@ -19,20 +19,21 @@ import functools
 
 import torch
 
-from . import _lib
+from . import _lib, config
 
 
 def mx4_store_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, loc: torch.Tensor,
                    positions: torch.Tensor | None, freqs_cis: torch.Tensor | None, pool, *,
-                   layer_id: int | None = None) -> None:
+                   layer_id: int | None = None, ratio: int = config.C4_RATIO) -> None:
     """Write raw C4 rows ``x`` [n, 512] (float32 or bfloat16) as 4-bit records at pool
     slots ``loc`` [n] int32: RMSNorm with ``weight``, BF16 rounding, the tail rotated
-    with frequency row ``positions * 4`` (``freqs_cis=None``: not rotated) and rounded
+    with frequency row ``positions * ratio`` (``ratio``: tokens a position stands for, as
+    ``native_store_rows``; ``freqs_cis=None``: not rotated) and rounded
     to BF16, then E2M1 codes under one scale per 32 coordinates. Slots outside the
     pool, and rows whose frequency row is outside the table, are skipped; those stored
     must differ (two rows for one slot leave a mixture of both). A group of 32 with an
     infinity or NaN reads back as NaN."""
-    _lib.ops().store(x, weight, eps, loc, positions, freqs_cis, pool, layer_id)
+    _lib.ops().store(x, weight, eps, loc, positions, freqs_cis, pool, layer_id, ratio)
 
 
 def mx4_gather_bf16(pool, slots: torch.Tensor, lengths: torch.Tensor | None,

@@ -176,9 +176,14 @@ def pack_rows_fused(x: torch.Tensor, weight: torch.Tensor, eps: float, loc: torc
 
 def native_store_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, loc: torch.Tensor,
                       positions: torch.Tensor | None, freqs_cis: torch.Tensor | None, pool,
-                      *, layer_id: int | None = None) -> None:
+                      *, layer_id: int | None = None, ratio: int = config.C4_RATIO) -> None:
     """Native 584-byte control store (unpruned RMSNorm, tail rotated with
-    frequency row positions * 4)."""
+    frequency row positions * ratio). ``ratio`` is the number of tokens a position
+    stands for: 4 where positions are record numbers of the C4 pool, 1 where they are
+    token positions (the window pool). Rows whose frequency row is outside the table
+    are skipped."""
+    if type(ratio) is not int or not 1 <= ratio < 2 ** 31:
+        raise ValueError("ratio must be a positive int")
     pages, n_pages, planes, packed, _, tensors = _operand(pool, layer_id)
     if planes is not None:
         raise ValueError("this operator reads contiguous pages, not plane buffers")
@@ -208,10 +213,10 @@ def native_store_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, loc: to
     if rows == 0:
         return
     _check_cuda(x, weight, loc, *tensors, freqs_cis, positions if freqs_cis is not None else None)
-    _lib.check(_lib.load().rm_native_store_rows(
+    _lib.check(_lib.load().rm_native_store_rows_ratio(
         x.data_ptr(), 1 if dtype == torch.bfloat16 else 0, strides[0], weight.data_ptr(),
-        float(eps), loc.data_ptr(), pos_ptr, freq_ptr, freq_rows, rows, pages, n_pages,
-        _stream()), "rm_native_store_rows")
+        float(eps), loc.data_ptr(), pos_ptr, freq_ptr, freq_rows, ratio, rows, pages, n_pages,
+        _stream()), "rm_native_store_rows_ratio")
 
 
 def unpack_gather_bf16(packed_buffers, physical_indices: torch.Tensor,

@@ -21,7 +21,7 @@ class SlotMap(NamedTuple):
     """The rows of a step: row ``row_starts[b] + i`` is record ``seqlens`` before the
     step plus i of request b."""
     loc: torch.Tensor          # int32 [rows]: pool slot, -1 past the step's records
-    positions: torch.Tensor    # int32 [rows]: record number within its request
+    positions: torch.Tensor    # int32 [rows]: record number within its request, 0 past them
     row_starts: torch.Tensor   # int32 [batch + 1]
     seqlens: torch.Tensor      # int32 [batch]: records after the step
     pages_taken: torch.Tensor  # int32 [1]: pages needed; beyond the free list: it was short
@@ -38,8 +38,10 @@ def append_slots(block_table: torch.Tensor, old_lengths: torch.Tensor, new_lengt
     adds none). The pages it lacks are taken, the requests in order, from the front of
     ``free_pages`` (int32 [n]) and written to the next columns of its row of
     ``block_table`` (int32 [batch, max_blocks], updated in place). Its new records are
-    consecutive rows of the step, the requests in order: ``loc`` and ``positions`` are
-    what ``pack_rows_fused`` / ``native_store_rows`` / ``mx4_store_rows`` take.
+    consecutive rows of the step, the requests in order: ``loc`` is what the stores take
+    (``pack_rows_fused``, ``native_store_rows``, ``mx4_store_rows``), and ``positions``,
+    numbers of records of ``ratio`` tokens each, what the rotating ones take with the same
+    ``ratio`` (theirs is 4 unless given).
 
     ``rows`` is the capacity of the two row lists (in a captured graph: the largest
     step); rows past the step's records get slot -1, which the stores skip, and records

@@ -150,6 +150,17 @@ int rm_native_store_rows(const void* x, int x_dtype, int64_t x_row_stride,
                          const int32_t* position, const float* freqs, int64_t freq_rows,
                          int64_t n, uint8_t* pool, int64_t pool_pages, void* stream);
 
+/* The same with freqs row position[i] * ratio (1 <= ratio < 2^31; above it is 4):
+ * ratio is the number of tokens a position stands for, 4 where positions are
+ * record numbers of the C4 pool, 1 where they are token positions (the window
+ * pool), as rm_append_slots gives them for its ratio. Rows whose position * ratio
+ * is outside [0, freq_rows) are skipped. */
+int rm_native_store_rows_ratio(const void* x, int x_dtype, int64_t x_row_stride,
+                               const float* weight, float eps, const int32_t* dst_slot,
+                               const int32_t* position, const float* freqs, int64_t freq_rows,
+                               int64_t ratio, int64_t n, uint8_t* pool, int64_t pool_pages,
+                               void* stream);
+
 /* Reconstruct: out row (q, k) (row index q * selected_k + k, 512 BF16 values,
  * contiguous) = dequantized record physical[q, k], tail rotated by freqs row
  * raw[q, k] * 4. A row is zero unless k < lengths[q], 0 <= physical < pool rows
@@ -357,6 +368,12 @@ int rm_mx4_store_rows(const void* x, int x_dtype, int64_t x_row_stride, const fl
                       float eps, const int32_t* dst_slot, const int32_t* position,
                       const float* freqs, int64_t freq_rows, int64_t n, uint8_t* pool,
                       int64_t pool_pages, void* stream);
+
+/* The same with freqs row position[i] * ratio, as rm_native_store_rows_ratio. */
+int rm_mx4_store_rows_ratio(const void* x, int x_dtype, int64_t x_row_stride, const float* weight,
+                            float eps, const int32_t* dst_slot, const int32_t* position,
+                            const float* freqs, int64_t freq_rows, int64_t ratio, int64_t n,
+                            uint8_t* pool, int64_t pool_pages, void* stream);
 
 /* Reader: out row q * selected_k + k (512 BF16 values, contiguous) = record
  * slots[q, k], exact; zeros unless k < lengths[q] (NULL = selected_k) and

@@ -355,3 +355,26 @@ def test_slot_maps_refuse():
             remnant.window_slots(**(good | change))
     slots, counts = remnant.window_slots(t, n, 0, 4)
     assert slots.shape == (3, 0, 4) and counts.shape == (0,)
+
+
+def test_stores_refuse_ratios():
+    """Frequency rows a position: a positive int of 31 bits."""
+    x, w, loc = torch.zeros(4, 512), torch.ones(512), torch.zeros(4, dtype=I32)
+    f = torch.zeros(8, 32, dtype=torch.complex64)
+    for store, fmt in ((remnant.mx4_store_rows, "mx4"), (remnant.native_store_rows, "native")):
+        pool = remnant.LatentPool(2, fmt=fmt, device="cpu")
+        for ratio in (0, -4, 2 ** 31, 2.0, True, None):
+            with pytest.raises(ValueError, match="ratio"):
+                store(x, w, 1e-6, loc, loc, f, pool, ratio=ratio)
+        with pytest.raises(ValueError, match="GPU"):
+            store(x, w, 1e-6, loc, loc, f, pool, ratio=2 ** 31 - 1)
+    lib = _lib.load()
+    hold = [buf(4096) for _ in range(4)]
+    x, w, s, pool = [a for _, a in hold]
+    for store in (lib.rm_mx4_store_rows_ratio, lib.rm_native_store_rows_ratio):
+        ok = [x, 1, 512, w, 1e-6, s, s, w, 8, 1, 4, pool, 1, None]
+        for at, value, status in ((10, 0, 0), (9, 0, -2), (9, -1, -2), (9, 1 << 31, -2),
+                                  (6, None, -1), (11, None, -1), (2, 100, -2)):
+            args = list(ok)
+            args[at] = value
+            assert store(*args) == status, (at, value)
