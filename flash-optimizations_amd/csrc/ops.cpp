@@ -167,7 +167,7 @@ struct Table {
 Table slot_table(PyObject* o) {
   const Tensor& t = tensor(o, "block_table");
   TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 2 &&
-                        (t.size(1) <= 1 || t.stride(1) == 1),
+                        (t.size(1) <= 1 || t.stride(1) == 1 || t.numel() == 0),
                     "block_table must be int32 [batch, max_blocks] with unit inner stride");
   const int64_t batch = t.size(0), width = t.size(1);
   TORCH_CHECK_VALUE(batch <= 1 || t.stride(0) >= width, "block_table rows must not overlap");

@@ -378,3 +378,12 @@ def test_stores_refuse_ratios():
             args = list(ok)
             args[at] = value
             assert store(*args) == status, (at, value)
+
+
+def test_empty_tables_have_no_strides_to_refuse():
+    """A batch of nothing, its table's strides whatever they are (numpy's are zero)."""
+    none = torch.zeros(0, dtype=I32)
+    for strides in ((0, 0), (9, 1), (1, 2)):
+        table = torch.empty_strided((0, 9), strides, dtype=I32)
+        slots, counts = remnant.window_slots(table, none, 2, 4)
+        assert slots.shape == (0, 2, 4) and counts.shape == (0,)
