@@ -27,7 +27,7 @@ struct {
   decltype(&rm_mx4_gather_bf16) gather;
   decltype(&rm_mx4_sparse_decode_workspace) plan;
   decltype(&rm_mx4_sparse_decode_fwd) decode;
-  decltype(&rm_append_slots) append;
+  decltype(&rm_append_slots_after) append;
   decltype(&rm_window_slots) window;
   PyObject* pool_type;    // LatentPool
   PyObject* get_stream;   // device index -> raw current stream
@@ -351,10 +351,11 @@ PyObject* decode(PyObject*, PyObject* const* v, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// block_table, old_lengths, new_lengths, free_pages, ratio, rows, out -> the five outputs
+// block_table, old_lengths, new_lengths, free_pages, ratio, rows, out, taken -> the five
+// outputs
 PyObject* append(PyObject*, PyObject* const* v, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  ARGUMENTS(7);
+  ARGUMENTS(8);
   const Table table = slot_table(v[0]);
   const int64_t batch = table.batch;
   TORCH_CHECK_VALUE(batch <= RM_MAX_SLOT_BATCH, "at most ", RM_MAX_SLOT_BATCH, " requests a call");
@@ -365,6 +366,8 @@ PyObject* append(PyObject*, PyObject* const* v, Py_ssize_t count) {
   vector(after, batch, "new_lengths");
   TORCH_CHECK_VALUE(free.scalar_type() == at::kInt && free.dim() == 1 && free.is_contiguous(),
                     "free_pages must be a contiguous int32 vector");
+  const Tensor* const taken = maybe(v[7], "taken");
+  if (taken) vector(*taken, 1, "taken");
   static const char* const names[5] = {"loc", "positions", "row_starts", "seqlens", "pages_taken"};
   Tensor made[5];
   const Tensor* out[5];
@@ -385,9 +388,9 @@ PyObject* append(PyObject*, PyObject* const* v, Py_ssize_t count) {
     const int64_t sizes[5] = {rows, rows, batch + 1, batch, 1};
     for (int i = 0; i < 5; ++i) vector(*out[i], sizes[i], names[i]);
   }
-  launch(one_device(table.t, &before, &after, &free, out[0], out[1], out[2], out[3], out[4]),
-         "rm_append_slots", lib.append, i32_out(table.t), table.stride, table.width, i32(before),
-         i32(after), batch, ratio, i32(free), free.size(0), rows, i32_out(*out[0]),
+  launch(one_device(table.t, &before, &after, &free, taken, out[0], out[1], out[2], out[3], out[4]),
+         "rm_append_slots_after", lib.append, i32_out(table.t), table.stride, table.width, i32(before),
+         i32(after), batch, ratio, i32(free), free.size(0), i32(taken), rows, i32_out(*out[0]),
          i32_out(*out[1]), i32_out(*out[2]), i32_out(*out[3]), i32_out(*out[4]));
   if (v[6] != Py_None) return same(v[6]);
   THPObjectPtr r(PyTuple_New(5));

@@ -8,7 +8,9 @@
 //   the requests in order, from the front of the free list: column c of row b,
 //   P(o) <= c < P(n), becomes free[base_b + c - P(o)], base_b the exclusive sum
 //   of the pages taken. Its new records o .. n - 1 follow those of the requests
-//   before it in the rows of the step.
+//   before it in the rows of the step. With a count of pages that steps before have
+//   taken, the list starts behind them and the step's are counted on top: a step's
+//   count is the next one's, so that steps need no host between them.
 // window: query j of a request of L tokens sits at p = L - q_len + j and sees
 //   tokens 0 .. f - 1, f = min(first, p + 1), and max(f, p + 1 - window) .. p.
 //
@@ -44,6 +46,7 @@ struct AppendArgs {
   int32_t* row_starts;
   int32_t* seqlens;
   int32_t* pages_taken;
+  const int32_t* taken;  // of kAfter: pages that the steps before took
 };
 
 // Tokens to records, a negative length as 0: floor(x / ratio) for x < 2^31 by a
@@ -102,9 +105,10 @@ __device__ __forceinline__ int request_of(const int32_t* end, int batch, int32_t
 // and 4,096 to 262,144 rows 1.0 us more; with table columns by a wave a request 12.4.
 // 1,024 threads a workgroup sum more than kNarrowBatch requests in less time (8,192
 // requests 17.9 -> 9.1 us, 1,024 5.1 -> 4.6, 512 4.1 -> 4.0; 256 threads are quicker
-// below: 16 requests 3.3 and 3.5).
+// below: 16 requests 3.3 and 3.5). kAfter: behind the pages that steps before took (one
+// kernel for both took 0.05 us more of a step's 3.4).
 constexpr int64_t kNarrowBatch = 256;
-template <int kSize>
+template <int kSize, bool kAfter>
 __global__ __launch_bounds__(kSize) void append_slots_kernel(AppendArgs a) {
   extern __shared__ int32_t sm[];
   const int batch = (int)a.batch;
@@ -113,6 +117,7 @@ __global__ __launch_bounds__(kSize) void append_slots_kernel(AppendArgs a) {
   int32_t* const held = sm + 2 * batch;     // [batch] records before the step
   __shared__ uint32_t wave_sum[2][kSize / 64];
   const int tid = threadIdx.x, lane = wave_lane(), wave = uniform(tid >> 6);
+  const uint32_t gone = kAfter ? (uint32_t)max(*a.taken, 0) : 0;
   // each wave sums its share of the requests, 64 at a time
   const int span = ((batch + kSize - 1) / kSize) * 64;
   const int b0 = min(wave * span, batch), b1 = min(b0 + span, batch);
@@ -157,8 +162,11 @@ __global__ __launch_bounds__(kSize) void append_slots_kernel(AppendArgs a) {
   all_pages = min(all_pages, kSat);
   if (blockIdx.x == 0 && tid == 0) {
     a.row_starts[0] = 0;
-    *a.pages_taken = (int32_t)all_pages;
+    *a.pages_taken = (int32_t)(kAfter ? min(add_sat(gone, all_pages), kSat) : all_pages);
   }
+  const int64_t skip = kAfter ? min((int64_t)gone, a.n_free) : 0;
+  const int32_t* const free_pages = a.free_pages + skip;
+  const int64_t n_free = a.n_free - skip;
   __syncthreads();
   // the rows
   const int64_t step = (int64_t)gridDim.x * kSize;
@@ -174,8 +182,8 @@ __global__ __launch_bounds__(kSize) void append_slots_kernel(AppendArgs a) {
       if (column < a.width) {
         if (column < own)
           from = a.table + b * a.table_stride + column;
-        else if (at < a.n_free)
-          from = a.free_pages + at;
+        else if (at < n_free)
+          from = free_pages + at;
       }
     }
     a.loc[i] = from ? slot_in(*from, record) : -1;
@@ -183,18 +191,18 @@ __global__ __launch_bounds__(kSize) void append_slots_kernel(AppendArgs a) {
   }
   // the pages, from the last workgroup on: each to its request's next column
   const int64_t first = (int64_t)(gridDim.x - 1 - blockIdx.x) * kSize + tid;
-  for (int64_t i = first; i < min((int64_t)all_pages, a.n_free); i += step) {
+  for (int64_t i = first; i < min((int64_t)all_pages, n_free); i += step) {
     const int b = request_of(page_end, batch, (int32_t)i);
     const int64_t c = (int64_t)pages_of(held[b]) + i - (b > 0 ? page_end[b - 1] : 0);
-    if (c < a.width) a.table[b * a.table_stride + c] = a.free_pages[i];
+    if (c < a.width) a.table[b * a.table_stride + c] = free_pages[i];
   }
-  if (all_pages > a.n_free) {  // too few: -1 in the columns left over, a wave a request
+  if (all_pages > n_free) {  // too few: -1 in the columns left over, a wave a request
     for (int64_t b = first / 64; b < batch; b += step / 64) {
       const uint32_t o = held[b];
       const int64_t base = b > 0 ? page_end[b - 1] : 0;
       const uint32_t n = max(records_of(a, a.new_len[b]), o);
       const int64_t from = pages_of(o), to = min((int64_t)pages_of(n), a.width);
-      for (int64_t c = from + max(a.n_free - base, (int64_t)0) + lane; c < to; c += 64)
+      for (int64_t c = from + max(n_free - base, (int64_t)0) + lane; c < to; c += 64)
         a.table[b * a.table_stride + c] = -1;
     }
   }
@@ -263,12 +271,13 @@ bool overlap(const int32_t* p, int64_t n, const int32_t* q, int64_t m) {
 
 }  // namespace
 
-extern "C" int rm_append_slots(int32_t* block_table, int64_t block_table_stride,
-                               int64_t max_blocks, const int32_t* old_lengths,
-                               const int32_t* new_lengths, int64_t batch, int64_t ratio,
-                               const int32_t* free_pages, int64_t n_free, int64_t rows,
-                               int32_t* loc, int32_t* positions, int32_t* row_starts,
-                               int32_t* seqlens, int32_t* pages_taken, void* stream) {
+extern "C" int rm_append_slots_after(int32_t* block_table, int64_t block_table_stride,
+                                     int64_t max_blocks, const int32_t* old_lengths,
+                                     const int32_t* new_lengths, int64_t batch, int64_t ratio,
+                                     const int32_t* free_pages, int64_t n_free,
+                                     const int32_t* taken, int64_t rows, int32_t* loc,
+                                     int32_t* positions, int32_t* row_starts, int32_t* seqlens,
+                                     int32_t* pages_taken, void* stream) {
   if (batch < 0 || batch > kMaxBatch || max_blocks < 0 || n_free < 0 || rows < 0 || rows > kSat ||
       max_blocks > kSat || n_free > kSat || ratio < 1 || ratio > kSat ||
       (batch > 1 && block_table_stride < max_blocks))
@@ -279,18 +288,19 @@ extern "C" int rm_append_slots(int32_t* block_table, int64_t block_table_stride,
     return RM_ERR_NULL;
   for (const void* p : {(const void*)block_table, (const void*)old_lengths, (const void*)new_lengths,
                         (const void*)free_pages, (const void*)loc, (const void*)positions,
-                        (const void*)row_starts, (const void*)seqlens, (const void*)pages_taken})
+                        (const void*)row_starts, (const void*)seqlens, (const void*)pages_taken,
+                        (const void*)taken})
     if (!aligned(p, 4)) return RM_ERR_ALIGN;
   // what is written must be apart from what other workgroups still read, and from each other
   const int64_t table_n = batch > 0 ? (batch - 1) * block_table_stride + max_blocks : 0;
   const struct {
     const int32_t* p;
     int64_t n;
-  } in[3] = {{old_lengths, batch}, {new_lengths, batch}, {free_pages, n_free}},
+  } in[4] = {{old_lengths, batch}, {new_lengths, batch}, {free_pages, n_free}, {taken, taken ? 1 : 0}},
     out[6] = {{block_table, table_n}, {loc, rows},       {positions, rows},
               {row_starts, batch + 1}, {seqlens, batch}, {pages_taken, 1}};
   for (int i = 0; i < 6; ++i) {
-    for (int j = 0; j < 3; ++j)
+    for (int j = 0; j < 4; ++j)
       if (overlap(out[i].p, out[i].n, in[j].p, in[j].n)) return RM_ERR_SHAPE;
     for (int j = 0; j < i; ++j)
       if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return RM_ERR_SHAPE;
@@ -300,17 +310,30 @@ extern "C" int rm_append_slots(int32_t* block_table, int64_t block_table_stride,
   const uint32_t m = (uint32_t)((((uint64_t)1 << (31 + log2)) + ratio - 1) / ratio);
   AppendArgs a{block_table, block_table_stride, max_blocks, old_lengths, new_lengths, batch, m,
                31 + log2, free_pages, n_free, rows, loc, positions, row_starts, seqlens,
-               pages_taken};
+               pages_taken, taken};
   const bool wide = batch > kNarrowBatch;
   const int64_t threads = wide ? 1024 : kThreads;
   const int64_t lds = batch * 3 * sizeof(int32_t);
   // as many as run at once
   const int64_t most = 256 * std::min<int64_t>(2048 / threads / 2, 160 * 1024 / (lds + 1024));
   const int64_t blocks = std::min<int64_t>((rows + threads - 1) / threads + 1, most);
-  hipLaunchKernelGGL((wide ? append_slots_kernel<1024> : append_slots_kernel<kThreads>),
-                     dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)lds,
+  const auto kern =
+      wide ? (taken ? append_slots_kernel<1024, true> : append_slots_kernel<1024, false>)
+           : (taken ? append_slots_kernel<kThreads, true> : append_slots_kernel<kThreads, false>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)lds,
                      (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
+}
+
+extern "C" int rm_append_slots(int32_t* block_table, int64_t block_table_stride,
+                               int64_t max_blocks, const int32_t* old_lengths,
+                               const int32_t* new_lengths, int64_t batch, int64_t ratio,
+                               const int32_t* free_pages, int64_t n_free, int64_t rows,
+                               int32_t* loc, int32_t* positions, int32_t* row_starts,
+                               int32_t* seqlens, int32_t* pages_taken, void* stream) {
+  return rm_append_slots_after(block_table, block_table_stride, max_blocks, old_lengths,
+                               new_lengths, batch, ratio, free_pages, n_free, nullptr, rows, loc,
+                               positions, row_starts, seqlens, pages_taken, stream);
 }
 
 extern "C" int rm_window_slots(const int32_t* block_table, int64_t block_table_stride,

@@ -90,6 +90,8 @@ SIGNATURES = {
                                         _vp, _vp, _vp, _sz, _vp]),
     "rm_append_slots": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
                                _vp, _vp, _vp, _vp]),
+    "rm_append_slots_after": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+                                     _vp, _vp, _vp, _vp, _vp, _vp]),
     "rm_window_slots": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
 }
 
@@ -140,7 +142,7 @@ def _load_ops():
     spec.loader.exec_module(module)
     module.setup(tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
         "rm_mx4_store_rows_ratio", "rm_mx4_gather_bf16", "rm_mx4_sparse_decode_workspace",
-        "rm_mx4_sparse_decode_fwd", "rm_append_slots", "rm_window_slots")),
+        "rm_mx4_sparse_decode_fwd", "rm_append_slots_after", "rm_window_slots")),
         LatentPool, torch._C._cuda_getCurrentRawStream, check, _native_pages)
     _ops = module
     return module

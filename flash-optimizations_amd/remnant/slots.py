@@ -2,9 +2,11 @@
 
 What the store (``loc``, ``positions``), the readers (slot lists) and the decodes
 (``block_table``, ``seqlens``, ``swa_indices``) take, without a round trip to the
-host: a step's pages are taken from a list of free ones, and the lists of visible
+host: a step's pages are taken from a list of free ones, behind those that the steps
+before have taken (a count on the GPU), and the lists of visible
 slots are derived from the table. One launch a call, on the current stream of the
-tensors' device; all of it can be captured in a HIP graph. No counterpart in the
+tensors' device; all of it can be captured in a HIP graph, which then stands for one
+step a replay where lengths and count are carried on in it. No counterpart in the
 reference's tree (its allocator and index builders live in the un-vendored forks).
 """
 
@@ -24,12 +26,12 @@ class SlotMap(NamedTuple):
     positions: torch.Tensor    # int32 [rows]: record number within its request, 0 past them
     row_starts: torch.Tensor   # int32 [batch + 1]
     seqlens: torch.Tensor      # int32 [batch]: records after the step
-    pages_taken: torch.Tensor  # int32 [1]: pages needed; beyond the free list: it was short
+    pages_taken: torch.Tensor  # int32 [1]: pages needed so far; beyond the free list: it was short
 
 
 def append_slots(block_table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: torch.Tensor,
                  free_pages: torch.Tensor, *, ratio: int = 1, rows: int | None = None,
-                 out=None) -> SlotMap:
+                 out=None, taken: torch.Tensor | None = None) -> SlotMap:
     """Give a step's new records their pages and slots.
 
     Request b grows from ``old_lengths[b]`` to ``new_lengths[b]`` tokens (int32
@@ -47,14 +49,21 @@ def append_slots(block_table: torch.Tensor, old_lengths: torch.Tensor, new_lengt
     step); rows past the step's records get slot -1, which the stores skip, and records
     past the capacity are left out. Where the free list or the table's columns run out,
     slots are -1; ``pages_taken`` tells how many pages were needed. ``out``: a
-    ``SlotMap`` (or five tensors) to write to instead of new ones."""
+    ``SlotMap`` (or five tensors) to write to instead of new ones.
+
+    ``taken`` (int32 [1]): pages that earlier steps have taken from the front of
+    ``free_pages``, the ``pages_taken`` of the step before; this step takes those behind
+    them and counts on. Without it every call starts at the front, each replay of a
+    captured one too: the pages it took have to be off the list by then. A graph that is
+    a step a replay ends with ``taken.copy_(map.pages_taken)`` (``taken`` is read while
+    the outputs are written, and must not be one of them) and the same of the lengths."""
     append = _lib.ops().append
     if out is None:
         return SlotMap._make(append(block_table, old_lengths, new_lengths, free_pages, ratio, rows,
-                                    None))
+                                    None, taken))
     if type(out) is not SlotMap:
         out = SlotMap(*out)
-    return append(block_table, old_lengths, new_lengths, free_pages, ratio, rows, out)
+    return append(block_table, old_lengths, new_lengths, free_pages, ratio, rows, out, taken)
 
 
 def window_slots(block_table: torch.Tensor, lengths: torch.Tensor, q_len: int, window: int, *,

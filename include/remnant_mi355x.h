@@ -423,6 +423,18 @@ int rm_append_slots(int32_t* block_table, int64_t block_table_stride, int64_t ma
                     int32_t* loc, int32_t* positions, int32_t* row_starts, int32_t* seqlens,
                     int32_t* pages_taken, void* stream);
 
+/* The same for a step behind others on one free list, without the host between
+ * them: taken [1] is the number of pages that the steps before have taken from its
+ * front (their pages_taken; negative: 0), the step takes those behind them, and its
+ * pages_taken counts both. taken is an input that must not be an output of the same
+ * call (RM_ERR_SHAPE); NULL is a first step. */
+int rm_append_slots_after(int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                          const int32_t* old_lengths, const int32_t* new_lengths, int64_t batch,
+                          int64_t ratio, const int32_t* free_pages, int64_t n_free,
+                          const int32_t* taken, int64_t rows, int32_t* loc, int32_t* positions,
+                          int32_t* row_starts, int32_t* seqlens, int32_t* pages_taken,
+                          void* stream);
+
 /* Visible slots per query token: query j of request b sits at p = lengths[b] -
  * q_len + j and sees tokens 0 .. f - 1 with f = min(first, p + 1), then
  * max(f, p + 1 - window) .. p. slots [batch, q_len, first + window]: their

@@ -211,3 +211,70 @@ def test_window_lists_feed_the_readers():
     rows = torch.empty(384, 512, dtype=torch.bfloat16, device=DEV)
     remnant.unpack_gather_bf16(packed, slots[:, 0], None, counts, None, rows)
     assert torch.equal(rows.view(2, 192, 512)[0, :150], remnant.unpack_rows(packed, loc[:150]))
+
+
+@pytest.mark.parametrize("batch", [0, 5, 300])
+@pytest.mark.parametrize("gone", [-7, 0, 1, 40, 100000, 2 ** 31 - 1])
+def test_append_takes_pages_behind_those_taken(gone, batch):
+    """The list starts behind `taken`, the count goes on from it (and saturates)."""
+    print(f"[gpu-slots] append {batch} after {gone}", flush=True)
+    rng = np.random.default_rng(batch)
+    old = rng.integers(0, 300, batch)
+    new = old + rng.integers(0, 200, batch)
+    table = rng.integers(0, 1000, (batch, 9))
+    free = rng.permutation(5000)
+    for n_free in (5000, 60, 40, 0):
+        dev, taken = gpu(table), gpu([gone])
+        got = remnant.append_slots(dev, gpu(old), gpu(new), gpu(free[:n_free]), rows=500, taken=taken)
+        want = ref.append(table, old, new, free[:n_free][max(gone, 0):], 1, 500)
+        pages = min(int(want[4][0]) + max(gone, 0), 2 ** 31 - 1)
+        assert got.pages_taken.tolist() == [pages] and taken.tolist() == [gone]
+        for name, a, b in zip(got._fields[:4], got, want):
+            assert np.array_equal(a.cpu().numpy(), b), name
+        assert np.array_equal(dev.cpu().numpy(), want[5])
+
+
+def test_captured_steps_take_pages_of_their_own():
+    """One captured step replayed again and again: lengths and the count of pages are
+    carried on in the graph. Every replay against loops on the host, until the list is
+    short; eager work of the same tensors' values between the replays."""
+    print("[gpu-slots] captured steps", flush=True)
+    rng = np.random.default_rng(3)
+    table, free = np.full((6, 8), -1), rng.permutation(30)
+    grow = gpu([1, 64, 0, 33, 3, 70])
+    dev = dict(table=gpu(table), old=gpu(np.zeros(6)), new=gpu(np.zeros(6)), free=gpu(free),
+               taken=gpu([0]))
+
+    def step(d):
+        torch.add(d["old"], grow, out=d["new"])
+        m = remnant.append_slots(d["table"], d["old"], d["new"], d["free"], rows=200,
+                                 taken=d["taken"])
+        d["taken"].copy_(m.pages_taken)
+        d["old"].copy_(d["new"])
+        return m
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step({k: t.clone() for k, t in dev.items()})
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(dev)
+    eager = {k: t.clone() for k, t in dev.items()}
+    old, taken = np.zeros(6, np.int64), 0
+    for i in range(13):
+        new = old + grow.cpu().numpy()
+        want = ref.append(table, old, new, free[taken:], 1, 200)
+        taken, table, old = taken + int(want[4][0]), want[5], new
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        same = step(eager)
+        for name, a, b, c in zip(got._fields[:4], got, want, same):
+            assert np.array_equal(a.cpu().numpy(), b) and torch.equal(a, c), (i, name)
+        assert got.pages_taken.tolist() == [taken] == dev["taken"].tolist()
+        assert np.array_equal(dev["table"].cpu().numpy(), table)
+        mapped = table[table >= 0]
+        assert len(np.unique(mapped)) == len(mapped)
+    assert taken > 30

@@ -387,3 +387,24 @@ def test_empty_tables_have_no_strides_to_refuse():
         table = torch.empty_strided((0, 9), strides, dtype=I32)
         slots, counts = remnant.window_slots(table, none, 2, 4)
         assert slots.shape == (0, 2, 4) and counts.shape == (0,)
+
+
+def test_slot_maps_refuse_counts_of_taken_pages():
+    t, n, f = torch.zeros(3, 4, dtype=I32), torch.zeros(3, dtype=I32), torch.zeros(5, dtype=I32)
+    for taken in (f, f[:0], f[0], f[:1].long(), f[:1].float(), f.view(1, 5)[:, :1]):
+        with pytest.raises(ValueError, match="taken"):
+            remnant.append_slots(t, n, n, f, rows=8, taken=taken)
+    with pytest.raises(TypeError):
+        remnant.append_slots(t, n, n, f, rows=8, taken=3)
+    with pytest.raises(ValueError, match="GPU"):
+        remnant.append_slots(t, n, n, f, rows=8, taken=f[:1])
+    raw, base = buf(8192)
+    t, old, new, free, loc, pos, starts, lens, pages, taken = (base + 512 * i for i in range(10))
+    #     0  1  2  3    4    5  6  7     8  9      10 11   12   13      14    15
+    ok = [t, 8, 8, old, new, 4, 4, free, 8, taken, 8, loc, pos, starts, lens, pages, None]
+    for at, value, status in ((9, taken + 2, -3), (9, pages, -2), (9, t + 4, -2), (9, loc + 28, -2),
+                              (9, lens, -2), (9, starts + 16, -2), (8, -1, -2), (7, None, -1),
+                              (10, -1, -2)):
+        args = list(ok)
+        args[at] = value
+        assert _lib.load().rm_append_slots_after(*args) == status, (at, value)
