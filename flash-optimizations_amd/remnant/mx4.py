@@ -71,7 +71,10 @@ def mx4_sparse_decode_fwd(q, pool, block_table, indices, *, seqlens=None, topk_l
     """Sparse-MLA decode over 4-bit records: ``native_sparse_decode_fwd``'s contract
     (logical record indices through the block table, lengths, sink, window rows of a
     Native ``swa_pool`` in the same softmax; returns (out [B, Sq, H, 512] bf16, lse
-    [B, Sq, H])) for any number of heads up to 1024."""
+    [B, Sq, H])) for any number of heads up to 1024. Scale bytes of up to 159 (2^32, the
+    largest that ``mx4_store_rows`` writes) are read exactly; records written elsewhere
+    with a larger one read as NaN, like those the store marks with 255, where
+    ``mx4_gather_bf16`` gives their values."""
     return _lib.ops().decode(q, pool, block_table, indices, seqlens, topk_length, sink,
                              softmax_scale, out, lse, workspace, layer_id, swa_pool, swa_indices,
                              swa_lengths)

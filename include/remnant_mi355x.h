@@ -393,7 +393,9 @@ int rm_mx4_sparse_decode_workspace(int64_t tokens, int64_t heads, int64_t topk, 
  * rm_native_sparse_decode_swa_fwd (list, lengths, block table, sink, window rows
  * of a Native pool; swa_topk 0 = none, the window arguments may then be NULL)
  * with any number of heads. A row with no valid entry and no sink gives zeros
- * and lse -inf. Scale bytes of the records are the store's. */
+ * and lse -inf. Scale bytes up to 159 (2^32, the store's largest) are exact; a
+ * listed record with a larger one reads as NaN, as with the store's 255: outputs
+ * and lse of its token are NaN. */
 int rm_mx4_sparse_decode_fwd(const uint16_t* q, int64_t batch, int64_t q_len, int64_t heads,
                              const uint8_t* pool, int64_t pool_pages, const int32_t* block_table,
                              int64_t block_table_stride, int64_t max_blocks,

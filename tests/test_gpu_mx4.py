@@ -848,3 +848,42 @@ def test_two_streams_at_once():
         for o in outs:
             for a, b in zip(o, want):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("byte", [0, 1, 111, 112, 159])
+def test_decode_reads_scale_bytes_up_to_the_reference(byte):
+    """Bytes the store does not write, below its own: exact, as the reader gives them."""
+    banner(f"decode scale byte {byte}")
+    case = Case(16, 300, seed=17, full=True, q=2.0 ** -33 if byte == 159 else 0.5)
+    rec = case.pool.reshape(-1, 272)
+    rng = np.random.default_rng(byte)
+    rec[::3, 256 + rng.integers(0, 16, len(rec[::3]))] = byte
+    check(case.run(), case.want())
+
+
+@pytest.mark.parametrize("byte", [160, 191, 223, 254, 255])
+def test_decode_of_scales_past_the_reference_is_nan(byte):
+    """In any group, in either half of a chunk, by itself or among others: the token is
+    NaN, the others are as before."""
+    banner(f"decode scale byte {byte}")
+    case = Case(16, 64, seed=18, full=True)
+    case.kw["seqlens"][:] = 500
+    case.indices[:] = np.random.default_rng(18).permutation(64)  # mapped for every request
+    rec = case.pool.reshape(-1, 272)
+    before = [t.clone() for t in case.run()]
+    plain = rec.copy()
+    for group in range(16):
+        rec[:] = plain
+        rec[int(case.table[1, 0]) * 64 + int(case.indices[1, 0, (37 * group) % 64]), 256 + group] = byte
+        out, lse = case.run()
+        assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all(), group
+        for b in (0, 2):
+            assert torch.equal(out[b], before[0][b]) and torch.equal(lse[b], before[1][b])
+    # in many splits, whatever the codes are (also zero), with and without a sink
+    long = Case(16, 4000, seed=19, full=True, batch=1)
+    at = long.pool.reshape(-1, 272)[int(long.table[0, 0]) * 64 + 5]
+    long.indices[0, 0, 1234] = 5
+    at[:256], at[256 + 7] = 0, byte
+    for sink in (None, gpu(long.kw["sink"])):
+        out, lse = long.run(sink=sink)
+        assert torch.isnan(out).all() and torch.isnan(lse).all()
