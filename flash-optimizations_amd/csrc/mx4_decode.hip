@@ -35,11 +35,12 @@
 // P^T in LDS is what the lane holding it writes: the order of the records in the second
 // product's long axis is free, and S^T's is taken.
 //
-// 256 tokens x 2,048 records at random places: 46 us (143 MB of records, 3.1 TB/s; a kernel
+// 256 tokens x 2,048 records at random places: 45 us (143 MB of records, 3.2 TB/s; a kernel
 // that does nothing but gather them takes 32 to 34). About 8 us are the start; the rest is
-// bound by that gather, with the vector pipes issuing in 47 % of the cycles (22.6
+// bound by that gather, with the vector pipes issuing in 50 % of the cycles (23.5
 // instructions a record, a third of them the two conversions of its codes) and the matrix
-// pipes busy in 17 %. 64 tokens x 2,048: 19.5 us and 3.4 the combine, 1 token 7.0 and 2.2.
+// pipes busy in 17 %. 64 tokens x 2,048: 19.3 us and 4.1 the combine, 1 token 7.1 and 3.0
+// (traced).
 // Before the copying waves had their own turn: 58; with one accumulator of all coordinates
 // a wave, merged at the end: 57.9; with records prefetched into registers: 77.
 //

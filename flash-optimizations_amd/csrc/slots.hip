@@ -99,9 +99,9 @@ __device__ __forceinline__ int request_of(const int32_t* end, int batch, int32_t
 // request by a binary search in LDS; pages from the last workgroup on, so that a step
 // of few rows has them done beside its rows (256 requests, 1 row each: 4.0 -> 3.5 us).
 //
-// Bound by its chain (lengths, sums, the page's look-up, the row) on a step: 3.5 us in
+// Bound by its chain (lengths, sums, the page's look-up, the row) on a step: 3.4 us in
 // a graph whose empty kernels take 2.4; by that and the 8 MB written for 1,048,576
-// rows of 16 requests: 5.6 us. With four rows a thread written as one piece these took 5.5
+// rows of 16 requests: 5.4 us. With four rows a thread written as one piece these took 5.5
 // and 4,096 to 262,144 rows 1.0 us more; with table columns by a wave a request 12.4.
 // 1,024 threads a workgroup sum more than kNarrowBatch requests in less time (8,192
 // requests 17.9 -> 9.1 us, 1,024 5.1 -> 4.6, 512 4.1 -> 4.0; 256 threads are quicker
@@ -218,9 +218,9 @@ struct WindowArgs {
 };
 
 // A thread takes kVec entries of one token and asks for their pages at once. Bound by
-// the chain length, page, entry on a step (256 requests x 2 tokens x 132 entries 3.0 us,
+// the chain length, page, entry on a step (256 requests x 2 tokens x 132 entries 2.8 us,
 // 2.4 an empty kernel), by the written bytes on long lists (8 x 131,072 entries, 4 MB,
-// 4.2 us; 64 x 131,072, 34 MB, 15). Four entries a thread from kFourEntries on where
+// 4.0 us; 64 x 131,072, 34 MB, 15). Four entries a thread from kFourEntries on where
 // rows divide: 131,072 entries 2.8 us with one and 3.2 with four, 262,144 3.4 and 3.2,
 // 1,048,576 6.2 and 4.2.
 constexpr int64_t kFourEntries = 1 << 18;

@@ -8,7 +8,8 @@ so readers take no positions. No counterpart in the reference.
 
 The calls mirror their siblings' (``native_store_rows``, ``unpack_gather_bf16``,
 ``native_sparse_decode_fwd``): shape and type mistakes raise ``ValueError`` before
-anything is launched, empty inputs launch nothing, and work runs asynchronously on
+anything is launched (``TypeError`` where a tensor or a number is something else
+altogether), empty inputs launch nothing, and work runs asynchronously on
 the current stream of the tensors' device.
 """
 
