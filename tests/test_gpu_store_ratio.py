@@ -122,3 +122,74 @@ def test_window_rows_of_a_step_are_rotated_by_their_tokens():
         widx[b, 0, :len(seen)] = 256 * b + seen
     check(got, ref.decode(q, rec.reshape(12, -1), np.arange(12).reshape(3, 4), idx, new // 4,
                           swa_pool=win, swa_indices=widx))
+
+
+def test_captured_steps_carry_on():
+    """One captured serving step -- both appends behind the pages taken, both stores with
+    their rotation, window lists, decode -- replayed as one step after another, beside the
+    same steps run eagerly: all outputs, tables and pools equal after every replay."""
+    print("[gpu-ratio] captured steps", flush=True)
+    freqs, ones = syn.rope_freqs(400).to(DEV), torch.ones(512, device=DEV)
+    sink = torch.linspace(-1, 1, 16, device=DEV)
+    grow = gpu([1, 4, 7], I32)
+
+    class State:
+        def __init__(self):
+            self.pools = [remnant.LatentPool(9, fmt="mx4", device=DEV),
+                          remnant.LatentPool(9, fmt="native", device=DEV)]
+            self.tables = [torch.full((3, 3), -1, dtype=I32, device=DEV) for _ in range(2)]
+            self.free = [gpu(np.random.default_rng(i).permutation(9), I32) for i in range(2)]
+            self.taken = [torch.zeros(1, dtype=I32, device=DEV) for _ in range(2)]
+            self.old, self.new = (torch.zeros(3, dtype=I32, device=DEV) for _ in range(2))
+            self.x = [torch.zeros(n, 512, dtype=torch.bfloat16, device=DEV) for n in (6, 12)]
+            self.q = torch.zeros(3, 1, 16, 512, dtype=torch.bfloat16, device=DEV)
+            self.idx = torch.zeros(3, 1, 40, dtype=I32, device=DEV)
+
+        def feed(self, seed):
+            g = torch.Generator().manual_seed(seed)
+            for t in (*self.x, self.q):
+                t.copy_(torch.randn(t.shape, generator=g))
+            self.idx.copy_(torch.randint(-1, 40, self.idx.shape, generator=g))
+
+        def step(self):
+            torch.add(self.old, grow, out=self.new)
+            maps = []
+            for i, (ratio, store) in enumerate(((4, remnant.mx4_store_rows),
+                                                (1, remnant.native_store_rows))):
+                m = remnant.append_slots(self.tables[i], self.old, self.new, self.free[i],
+                                         ratio=ratio, rows=self.x[i].shape[0], taken=self.taken[i])
+                store(self.x[i], ones, 1e-6, m.loc, m.positions, freqs, self.pools[i], ratio=ratio)
+                self.taken[i].copy_(m.pages_taken)
+                maps.append(m)
+            slots, counts = remnant.window_slots(self.tables[1], self.new, 1, 16, first=2)
+            out, lse = remnant.mx4_sparse_decode_fwd(
+                self.q, self.pools[0], self.tables[0], self.idx, seqlens=maps[0].seqlens, sink=sink,
+                swa_pool=self.pools[1], swa_indices=slots, swa_lengths=counts)
+            self.old.copy_(self.new)
+            return [*maps[0], *maps[1], slots, counts, out, lse]
+
+        def held(self):
+            return [*self.tables, *self.taken, self.old] + [p.buffer for p in self.pools]
+
+    side, warm = torch.cuda.Stream(), State()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm.step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphed, eager, graph = State(), State(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = graphed.step()
+    for seed in range(25):
+        graphed.feed(seed)
+        eager.feed(seed)
+        graph.replay()
+        if seed % 2:
+            torch.cuda.synchronize()
+        want = eager.step()
+        for i, (a, b) in enumerate(zip(got + graphed.held(), want + eager.held())):
+            assert torch.equal(a, b), (seed, i)
+    assert graphed.old.tolist() == [25, 100, 175]
+    assert [t.tolist() for t in graphed.taken] == [[3], [6]]
+    for t in graphed.tables:
+        pages = [p for p in t.flatten().tolist() if p >= 0]
+        assert len(set(pages)) == len(pages)
