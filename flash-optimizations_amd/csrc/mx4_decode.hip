@@ -50,6 +50,7 @@
 #include <algorithm>
 
 #include "combine.h"
+#include "lds.h"
 #include "mx4_device.h"
 #include "remnant_mi355x.h"
 
@@ -60,14 +61,6 @@ namespace {
 constexpr int kMaxTopk = 1 << 20;
 constexpr int kMaxWindow = 512;
 constexpr int kMaxHeads = 1024;
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef __attribute__((address_space(3))) void lds_void;
 
 struct DecodeArgs {
   int first;  // token of workgroups (., 0, .)
@@ -144,38 +137,12 @@ struct Lds {
   static_assert(kBytes <= 160 * 1024 && kWaves * kWindowBytes <= kWeights, "LDS of a CU");
 };
 
-// Copies HBM -> LDS: 16 bytes a lane to lds + 16 lane. The LDS address is a plain number,
-// so that the compiler ties the copies to no array; wait_copies() orders them.
-__device__ __forceinline__ void copy16(const void* src, uint32_t lds) {
-  __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
-                                   16, 0, 0);
-}
-// The same, of data that the caches will not see again: calls whose lists hold kOnceBytes
+// copy16() of data that the caches will not see again: calls whose lists hold kOnceBytes
 // of records or more (256 tokens x 2,048 records, 143 MB, 48.4 -> 46.4 us; 64 tokens, 36 MB,
 // which three calls in turn find in the last-level cache, 22.7 -> 23.4).
 __device__ __forceinline__ void copy16_once(const void* src, uint32_t lds) {
   __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
                                    16, 0, 2);
-}
-__device__ __forceinline__ void copy4(const void* src, uint32_t lds) {
-  __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)__builtin_amdgcn_readfirstlane(lds),
-                                   4, 0, 0);
-}
-// Until at most kLater vector loads issued since are in flight.
-template <int kLater>
-__device__ __forceinline__ void wait_copies() {
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (kLater & 15) | ((kLater >> 4) << 14));
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-  __builtin_amdgcn_sched_barrier(0);
-}
-template <class T>
-__device__ __forceinline__ T lds_read(uint32_t at) {
-  return *(const __attribute__((address_space(3))) T*)(uintptr_t)at;
-}
-template <class T>
-__device__ __forceinline__ void lds_write(uint32_t at, T v) {
-  *(__attribute__((address_space(3))) T*)(uintptr_t)at = v;
 }
 // Over the four lanes that share lane % 16.
 __device__ __forceinline__ float over_groups_max(float x) {
@@ -190,19 +157,6 @@ __device__ __forceinline__ float over_groups_sum(float x) {
   const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
   return u2f(b[0]) + u2f(b[1]);
 }
-// Barrier that orders LDS accesses only: loads from memory stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-__device__ __forceinline__ uint32_t sub_sat(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(uint32_t,
-                            __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, a),
-                                                          __builtin_bit_cast(u16x2, b)));
-}
-__device__ __forceinline__ bf16x8 as_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
-
 // What the waves of a workgroup share.
 template <int kWaves>
 struct Share {

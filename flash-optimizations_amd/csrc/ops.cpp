@@ -1,5 +1,5 @@
-// Argument checks and launches of the 4-bit operators and the slot maps, for
-// remnant/mx4.py and remnant/slots.py (module remnant_ops). Small calls are bound by
+// Argument checks and launches of the 4-bit and index operators, the tree attention and
+// the slot maps, for remnant/mx4.py, index.py, tree.py and slots.py (module remnant_ops). Small calls are bound by
 // the host: a launch takes 3.2 us, and the same checks in Python, with ctypes, took 4 to
 // 8 more (a call of a window list 8.2 us, 6.1 here; the slot map of a step 10.0 and 6.3;
 // a decode of one launch with window rows 12.4 and 6.8, of two launches 14.6 and 9.3).
@@ -30,6 +30,12 @@ struct {
   decltype(&rm_mx4_sparse_decode_fwd) decode;
   decltype(&rm_append_slots_after) append;
   decltype(&rm_window_slots) window;
+  decltype(&rm_index_store_rows) index_store;
+  decltype(&rm_index_gather_bf16) index_gather;
+  decltype(&rm_index_scores) scores;
+  decltype(&rm_index_topk) topk;
+  decltype(&rm_tree_decode_workspace) tree_plan;
+  decltype(&rm_tree_decode_fwd) tree;
   PyObject* pool_type;    // LatentPool
   PyObject* get_stream;   // device index -> raw current stream
   PyObject* check;        // (status, name): raises
@@ -129,21 +135,31 @@ struct Pages {
   uint8_t* at;
   int64_t pages;
 };
-Pages mx4_pages(PyObject* pool, PyObject* layer_id) {
+// A record format whose pools the operators here take whole.
+struct Format {
+  const char* name;   // of LatentPool
+  const char* title;
+  int64_t page_bytes, dim;
+};
+constexpr Format kMx4{"mx4", "4-bit (mx4)", RM_MX4_PAGE_BYTES, RM_HEAD_DIM};
+constexpr Format kIndex{"index", "index", RM_INDEX_PAGE_BYTES, RM_INDEX_DIM};
+constexpr Format kNative{"native", "Native", RM_NATIVE_PAGE_BYTES, RM_HEAD_DIM};
+
+Pages pages_of(PyObject* pool, PyObject* layer_id, const Format& f, const char* name = "pool") {
   if (THPVariable_Check(pool)) {
-    const Tensor& t = tensor(pool, "pool");
+    const Tensor& t = tensor(pool, name);
     TORCH_CHECK_VALUE(t.scalar_type() == at::kByte && t.dim() == 2 &&
-                          t.size(1) == RM_MX4_PAGE_BYTES && t.is_contiguous(),
-                      "pool must be a contiguous uint8 [pages, 17408] tensor");
+                          t.size(1) == f.page_bytes && t.is_contiguous(),
+                      name, " must be a contiguous uint8 [pages, ", f.page_bytes, "] tensor");
     return {t, (uint8_t*)t.mutable_data_ptr(), t.size(0)};
   }
-  TORCH_CHECK_VALUE(is_pool(pool), "pool must be a LatentPool or a uint8 page tensor");
-  TORCH_CHECK_VALUE(has_format(pool, "mx4"), "this operator takes a 4-bit (mx4) pool");
+  TORCH_CHECK_VALUE(is_pool(pool), name, " must be a LatentPool or a uint8 page tensor");
+  TORCH_CHECK_VALUE(has_format(pool, f.name), "this operator takes a ", f.title, " pool");
   THPObjectPtr o = attribute(pool, lib.buffer);
   const Tensor& t = tensor(o.get(), "pool.buffer");
   TORCH_CHECK_VALUE(t.scalar_type() == at::kByte && t.dim() == 3 &&
-                        t.size(2) == RM_MX4_PAGE_BYTES && t.is_contiguous(),
-                    "a 4-bit pool's buffer is uint8 [layers, pages, 17408]");
+                        t.size(2) == f.page_bytes && t.is_contiguous(),
+                    "a pool's buffer is uint8 [layers, pages, ", f.page_bytes, "]");
   const int64_t layer =
       layer_id == Py_None ? 0 : integer(layer_id, 0, t.size(0), "layer_id out of range");
   return {t, (uint8_t*)t.mutable_data_ptr() + layer * t.stride(0), t.size(1)};
@@ -165,13 +181,13 @@ struct Table {
   const Tensor& t;
   int64_t batch, width, stride;
 };
-Table slot_table(PyObject* o) {
-  const Tensor& t = tensor(o, "block_table");
+Table slot_table(PyObject* o, const char* name = "block_table") {
+  const Tensor& t = tensor(o, name);
   TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 2 &&
                         (t.size(1) <= 1 || t.stride(1) == 1 || t.numel() == 0),
-                    "block_table must be int32 [batch, max_blocks] with unit inner stride");
+                    name, " must be int32 [batch, max_blocks] with unit inner stride");
   const int64_t batch = t.size(0), width = t.size(1);
-  TORCH_CHECK_VALUE(batch <= 1 || t.stride(0) >= width, "block_table rows must not overlap");
+  TORCH_CHECK_VALUE(batch <= 1 || t.stride(0) >= width, name, " rows must not overlap");
   return {t, batch, width, std::max(t.stride(0), width)};
 }
 
@@ -187,13 +203,15 @@ PyObject* same(PyObject* o) {
   TORCH_CHECK_TYPE(count == n, "expected ", n, " arguments, not ", count)
 
 // x, weight, eps, loc, positions, freqs_cis, pool, layer_id, ratio
-PyObject* store(PyObject*, PyObject* const* v, Py_ssize_t count) {
+template <class F>
+PyObject* store_rows(PyObject* const* v, Py_ssize_t count, const Format& format, const char* name,
+                     F entry) {
   HANDLE_TH_ERRORS
   ARGUMENTS(9);
-  const Pages pool = mx4_pages(v[6], v[7]);
+  const Pages pool = pages_of(v[6], v[7], format);
   const Tensor &x = tensor(v[0], "x"), &weight = tensor(v[1], "weight"), &loc = tensor(v[3], "loc");
-  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == RM_HEAD_DIM && x.stride(1) == 1,
-                    "x must be [rows, 512] with unit inner stride");
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == format.dim && x.stride(1) == 1, "x must be [rows, ",
+                    format.dim, "] with unit inner stride");
   const bool bf16 = x.scalar_type() == at::kBFloat16;
   TORCH_CHECK_VALUE(bf16 || x.scalar_type() == at::kFloat, "x must be float32 or bfloat16");
   const int64_t rows = x.size(0);
@@ -201,8 +219,8 @@ PyObject* store(PyObject*, PyObject* const* v, Py_ssize_t count) {
                         loc.is_contiguous(),
                     "loc must be a contiguous int32 [rows] tensor");
   TORCH_CHECK_VALUE(weight.scalar_type() == at::kFloat && weight.dim() == 1 &&
-                        weight.size(0) == RM_HEAD_DIM && weight.is_contiguous(),
-                    "weight must be a contiguous float32 [512] tensor");
+                        weight.size(0) == format.dim && weight.is_contiguous(),
+                    "weight must be a contiguous float32 [", format.dim, "] tensor");
   const float eps = number(v[2]);
   const int64_t ratio = integer(v[8], 1, kInt32, kRatio);
   const Tensor* const freqs = maybe(v[5], "freqs_cis");
@@ -218,20 +236,27 @@ PyObject* store(PyObject*, PyObject* const* v, Py_ssize_t count) {
     freq_rows = freqs->numel() / ((RM_HEAD_DIM - RM_NOPE_DIM) / 2);
   }
   if (rows == 0 || (freqs && freq_rows == 0)) return none();
-  launch(one_device(x, &weight, &loc, positions, freqs, &pool.buffer), "rm_mx4_store_rows_ratio",
-         lib.store, x.const_data_ptr(), bf16 ? (int)RM_BF16 : (int)RM_F32, x.stride(0),
+  launch(one_device(x, &weight, &loc, positions, freqs, &pool.buffer), name, entry, x.const_data_ptr(), bf16 ? (int)RM_BF16 : (int)RM_F32, x.stride(0),
          (const float*)weight.const_data_ptr(), eps, i32(loc), i32(positions),
          freqs ? (const float*)freqs->const_data_ptr() : nullptr, freq_rows, ratio, rows, pool.at,
          pool.pages);
   return none();
   END_HANDLE_TH_ERRORS
 }
+PyObject* store(PyObject*, PyObject* const* v, Py_ssize_t count) {
+  return store_rows(v, count, kMx4, "rm_mx4_store_rows_ratio", lib.store);
+}
+PyObject* index_store(PyObject*, PyObject* const* v, Py_ssize_t count) {
+  return store_rows(v, count, kIndex, "rm_index_store_rows", lib.index_store);
+}
 
 // pool, slots, lengths, output, layer_id -> output
-PyObject* gather(PyObject*, PyObject* const* v, Py_ssize_t count) {
+template <class F>
+PyObject* gather_rows(PyObject* const* v, Py_ssize_t count, const Format& format, const char* name,
+                      F entry) {
   HANDLE_TH_ERRORS
   ARGUMENTS(5);
-  const Pages pool = mx4_pages(v[0], v[4]);
+  const Pages pool = pages_of(v[0], v[4], format);
   const Tensor& slots = tensor(v[1], "slots");
   TORCH_CHECK_VALUE(slots.scalar_type() == at::kInt && slots.dim() == 2,
                     "slots must be int32 [queries, k]");
@@ -241,19 +266,25 @@ PyObject* gather(PyObject*, PyObject* const* v, Py_ssize_t count) {
                                  lengths->size(0) == queries),
                     "lengths must be int32 [queries]");
   Tensor output = v[3] == Py_None
-                      ? at::empty({rows, RM_HEAD_DIM}, slots.options().dtype(at::kBFloat16))
+                      ? at::empty({rows, format.dim}, slots.options().dtype(at::kBFloat16))
                       : tensor(v[3], "output");
   TORCH_CHECK_VALUE(output.scalar_type() == at::kBFloat16 && output.dim() == 2 &&
-                        output.size(1) == RM_HEAD_DIM && output.is_contiguous(),
-                    "output must be a contiguous bfloat16 [rows, 512] tensor");
+                        output.size(1) == format.dim && output.is_contiguous(),
+                    "output must be a contiguous bfloat16 [rows, ", format.dim, "] tensor");
   TORCH_CHECK_VALUE(output.size(0) >= rows, "output has fewer rows than queries * k");
   if (rows > 0)
-    launch(one_device(pool.buffer, &slots, lengths, &output), "rm_mx4_gather_bf16", lib.gather,
+    launch(one_device(pool.buffer, &slots, lengths, &output), name, entry,
            (const uint8_t*)pool.at, pool.pages, i32(slots), slots.stride(0), slots.stride(1),
            i32(lengths), lengths ? lengths->stride(0) : 0, queries, k,
            (uint16_t*)output.mutable_data_ptr());
   return v[3] == Py_None ? THPVariable_Wrap(std::move(output)) : same(v[3]);
   END_HANDLE_TH_ERRORS
+}
+PyObject* gather(PyObject*, PyObject* const* v, Py_ssize_t count) {
+  return gather_rows(v, count, kMx4, "rm_mx4_gather_bf16", lib.gather);
+}
+PyObject* index_gather(PyObject*, PyObject* const* v, Py_ssize_t count) {
+  return gather_rows(v, count, kIndex, "rm_index_gather_bf16", lib.index_gather);
 }
 
 // q, pool, block_table, indices, seqlens, topk_length, sink, softmax_scale, out, lse,
@@ -261,7 +292,7 @@ PyObject* gather(PyObject*, PyObject* const* v, Py_ssize_t count) {
 PyObject* decode(PyObject*, PyObject* const* v, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   ARGUMENTS(15);
-  const Pages pool = mx4_pages(v[1], v[11]);
+  const Pages pool = pages_of(v[1], v[11], kMx4);
   const Tensor &q = tensor(v[0], "q"), &table = tensor(v[2], "block_table"),
                &indices = tensor(v[3], "indices");
   TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == RM_HEAD_DIM &&
@@ -443,19 +474,206 @@ PyObject* window(PyObject*, PyObject* const* v, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// (six entry points' addresses), LatentPool, get_stream, check, native_pages
+// q, weights, pool, block_table, lengths, out, layer_id -> out
+PyObject* scores(PyObject*, PyObject* const* v, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  ARGUMENTS(7);
+  const Pages pool = pages_of(v[2], v[6], kIndex);
+  const Tensor &q = tensor(v[0], "q"), &weights = tensor(v[1], "weights"),
+               &lengths = tensor(v[4], "lengths");
+  const Table table = slot_table(v[3]);
+  TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == RM_INDEX_DIM &&
+                        q.scalar_type() == at::kBFloat16 && q.is_contiguous(),
+                    "q must be a contiguous bfloat16 [batch, q_len, heads, 128] tensor");
+  const int64_t batch = q.size(0), q_len = q.size(1), heads = q.size(2), tokens = batch * q_len;
+  TORCH_CHECK_VALUE(heads <= RM_MAX_INDEX_HEADS, "at most ", RM_MAX_INDEX_HEADS, " heads");
+  TORCH_CHECK_VALUE(weights.sizes() == q.sizes().slice(0, 3) && weights.scalar_type() == at::kFloat &&
+                        weights.is_contiguous(),
+                    "weights must be a contiguous float32 [batch, q_len, heads] tensor");
+  TORCH_CHECK_VALUE(table.batch == batch, "block_table must have a row for each request");
+  TORCH_CHECK_VALUE(lengths.scalar_type() == at::kInt && lengths.numel() == tokens &&
+                        lengths.is_contiguous(),
+                    "lengths must be a contiguous int32 tensor of ", tokens, " entries");
+  Tensor out = v[5] == Py_None ? at::empty({batch, q_len, table.width * RM_PAGE_RECORDS},
+                                           q.options().dtype(at::kFloat))
+                               : tensor(v[5], "out");
+  TORCH_CHECK_VALUE(out.dim() == 3 && out.size(0) == batch && out.size(1) == q_len &&
+                        out.scalar_type() == at::kFloat && out.is_contiguous(),
+                    "out must be a contiguous float32 [batch, q_len, records] tensor");
+  if (tokens > 0 && out.size(2) > 0)
+    launch(one_device(q, &weights, &pool.buffer, &table.t, &lengths, &out), "rm_index_scores",
+           lib.scores, (const uint16_t*)q.const_data_ptr(), batch, q_len, heads,
+           (const float*)weights.const_data_ptr(), (const uint8_t*)pool.at, pool.pages,
+           i32(table.t), table.stride, table.width, i32(lengths), out.size(2),
+           (float*)out.mutable_data_ptr());
+  return v[5] == Py_None ? THPVariable_Wrap(std::move(out)) : same(v[5]);
+  END_HANDLE_TH_ERRORS
+}
+
+// scores, lengths, k, out -> (indices, counts)
+PyObject* topk(PyObject*, PyObject* const* v, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  ARGUMENTS(4);
+  const Tensor& scores = tensor(v[0], "scores");
+  TORCH_CHECK_VALUE(scores.scalar_type() == at::kFloat && (scores.dim() == 2 || scores.dim() == 3),
+                    "scores must be float32 [rows, records] or [batch, q_len, records]");
+  const int64_t width = scores.size(-1), outer = scores.dim() == 3 ? scores.size(0) : 1,
+                inner = scores.size(-2), rows = outer * inner;
+  // rows at one distance from each other
+  const int64_t stride = inner > 1 ? scores.stride(-2) : outer > 1 ? scores.stride(0) : width;
+  TORCH_CHECK_VALUE(scores.numel() == 0 ||
+                        ((width == 1 || scores.stride(-1) == 1) && (rows == 1 || stride >= width) &&
+                         (outer == 1 || inner == 1 || scores.stride(0) == inner * stride)),
+                    "scores must have unit inner stride and rows at one distance");
+  const int64_t k = integer(v[2], 0, (int64_t)RM_MAX_INDEX_WIDTH + 1, "k must be an int of 0 to 2^20");
+  TORCH_CHECK_VALUE(width <= RM_MAX_INDEX_WIDTH, "at most 2^20 records a row");
+  const Tensor* const lengths = maybe(v[1], "lengths");
+  TORCH_CHECK_VALUE(!lengths || (lengths->scalar_type() == at::kInt && lengths->numel() == rows &&
+                                 lengths->is_contiguous()),
+                    "lengths must be a contiguous int32 tensor of ", rows, " entries");
+  Tensor indices, counts;
+  at::DimVector shape(scores.sizes().begin(), scores.sizes().end());
+  shape.back() = k;
+  if (v[3] == Py_None) {
+    const auto options = scores.options().dtype(at::kInt);
+    indices = at::empty(shape, options);
+    counts = at::empty({rows}, options);
+  } else {
+    THPObjectPtr pair(PySequence_Tuple(v[3]));
+    if (!pair) throw python_error();
+    TORCH_CHECK_VALUE(PyTuple_GET_SIZE(pair.get()) == 2, "out must be two tensors");
+    indices = tensor(PyTuple_GET_ITEM(pair.get(), 0), "indices");
+    counts = tensor(PyTuple_GET_ITEM(pair.get(), 1), "counts");
+    TORCH_CHECK_VALUE(indices.scalar_type() == at::kInt && indices.sizes() == shape &&
+                          indices.is_contiguous(),
+                      "indices must be a contiguous int32 tensor shaped like scores, with ", k,
+                      " entries a row");
+    vector(counts, rows, "counts");
+  }
+  if (rows > 0)
+    launch(one_device(scores, lengths, &indices, &counts), "rm_index_topk", lib.topk,
+           (const float*)scores.const_data_ptr(), stride, i32(lengths), rows, width, k,
+           i32_out(indices), i32_out(counts));
+  THPObjectPtr i(THPVariable_Wrap(std::move(indices))), c(THPVariable_Wrap(std::move(counts)));
+  if (!i || !c) throw python_error();
+  return PyTuple_Pack(2, i.get(), c.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// q, pool, block_table, lengths, parents, window, history_pool, history_table,
+// history_lengths, sink, softmax_scale, out, lse, workspace, layer_id, history_layer_id ->
+// (out, lse)
+PyObject* tree(PyObject*, PyObject* const* v, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  ARGUMENTS(16);
+  const Pages pool = pages_of(v[1], v[14], kNative);
+  const Tensor &q = tensor(v[0], "q"), &lengths = tensor(v[3], "lengths"),
+               &parents = tensor(v[4], "parents");
+  const Table table = slot_table(v[2]);
+  TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == RM_HEAD_DIM &&
+                        q.scalar_type() == at::kBFloat16 && q.is_contiguous(),
+                    "q must be a contiguous bfloat16 [batch, nodes, heads, 512] tensor");
+  const int64_t batch = q.size(0), nodes = q.size(1), heads = q.size(2);
+  TORCH_CHECK_VALUE(nodes <= RM_MAX_TREE_NODES, "at most ", RM_MAX_TREE_NODES, " nodes a tree");
+  TORCH_CHECK_VALUE(table.batch == batch, "block_table must have a row for each request");
+  vector(lengths, batch, "lengths");
+  TORCH_CHECK_VALUE(parents.scalar_type() == at::kInt && parents.dim() == 2 &&
+                        parents.size(0) == batch && parents.size(1) == nodes &&
+                        parents.is_contiguous(),
+                    "parents must be a contiguous int32 [batch, nodes] tensor");
+  const int64_t window =
+      v[5] == Py_None ? 0 : integer(v[5], 1, kInt32, "window must be a positive int");
+  Pages past{};
+  const Tensor* past_lengths = nullptr;
+  const Tensor* past_table = nullptr;
+  int64_t past_blocks = 0, past_stride = 0;
+  if (v[6] != Py_None || v[7] != Py_None || v[8] != Py_None) {
+    TORCH_CHECK_VALUE(v[6] != Py_None && v[7] != Py_None && v[8] != Py_None,
+                      "history_pool, history_table and history_lengths are given together");
+    past = pages_of(v[6], v[15], kNative, "history_pool");
+    const Table t = slot_table(v[7], "history_table");
+    TORCH_CHECK_VALUE(t.batch == batch, "history_table must have a row for each request");
+    past_lengths = &tensor(v[8], "history_lengths");
+    vector(*past_lengths, batch, "history_lengths");
+    past_table = &t.t;
+    past_blocks = t.width;
+    past_stride = t.stride;
+  }
+  const Tensor* const sink = maybe(v[9], "sink");
+  TORCH_CHECK_VALUE(!sink || (sink->scalar_type() == at::kFloat && sink->dim() == 1 &&
+                              sink->size(0) == heads && sink->is_contiguous()),
+                    "sink must be a contiguous float32 [heads] tensor");
+  const float scale = v[10] == Py_None ? 0.04419417382415922f : number(v[10]);  // 1 / sqrt(512)
+  Tensor out = v[11] == Py_None ? at::empty(q.sizes(), q.options()) : tensor(v[11], "out");
+  Tensor lse = v[12] == Py_None
+                   ? at::empty({batch, nodes, heads}, q.options().dtype(at::kFloat))
+                   : tensor(v[12], "lse");
+  TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == at::kBFloat16 &&
+                        out.is_contiguous(),
+                    "out must be a contiguous bfloat16 tensor shaped like q");
+  TORCH_CHECK_VALUE(lse.sizes() == q.sizes().slice(0, 3) && lse.scalar_type() == at::kFloat &&
+                        lse.is_contiguous(),
+                    "lse must be a contiguous float32 [batch, nodes, heads] tensor");
+  const Tensor* workspace = maybe(v[13], "workspace");
+  TORCH_CHECK_VALUE(!workspace ||
+                        (workspace->scalar_type() == at::kByte && workspace->is_contiguous()),
+                    "workspace must be a contiguous uint8 tensor on the GPU");
+  if (q.numel() > 0) {
+    size_t need = 0;
+    Tensor own;
+    // (sizes it refuses, the launch refuses too)
+    if (lib.tree_plan(batch, nodes, heads, table.width, window, past_blocks, nullptr, &need) == RM_OK &&
+        need > 0 && (!workspace || (size_t)workspace->numel() < need)) {
+      own = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+      workspace = &own;
+    }
+    launch(one_device(q, &pool.buffer, &table.t, &lengths, &parents,
+                      past_lengths ? &past.buffer : nullptr, past_table, past_lengths, sink, &out,
+                      &lse, workspace),
+           "rm_tree_decode_fwd", lib.tree, (const uint16_t*)q.const_data_ptr(), batch, nodes, heads,
+           (const uint8_t*)pool.at, pool.pages, i32(table.t), table.stride, table.width,
+           i32(lengths), i32(parents), window, (const uint8_t*)past.at, past.pages, i32(past_table),
+           past_stride, past_blocks, i32(past_lengths),
+           sink ? (const float*)sink->const_data_ptr() : nullptr, scale,
+           (uint16_t*)out.mutable_data_ptr(), (float*)lse.mutable_data_ptr(),
+           workspace ? workspace->mutable_data_ptr() : nullptr,
+           workspace ? (size_t)workspace->numel() : (size_t)0);
+  }
+  THPObjectPtr o(v[11] == Py_None ? THPVariable_Wrap(std::move(out)) : same(v[11]));
+  THPObjectPtr s(v[12] == Py_None ? THPVariable_Wrap(std::move(lse)) : same(v[12]));
+  if (!o || !s) throw python_error();
+  return PyTuple_Pack(2, o.get(), s.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// (entry points' addresses in the order of `lib`), LatentPool, get_stream, check, native_pages
 PyObject* setup(PyObject*, PyObject* args) {
-  unsigned long long at[6];
-  PyObject *pool_type, *get_stream, *check, *pages;
-  if (!PyArg_ParseTuple(args, "(KKKKKK)OOOO", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5],
-                        &pool_type, &get_stream, &check, &pages))
+  constexpr int kEntries = 12;
+  PyObject *entries, *pool_type, *get_stream, *check, *pages;
+  if (!PyArg_ParseTuple(args, "O!OOOO", &PyTuple_Type, &entries, &pool_type, &get_stream, &check,
+                        &pages))
     return nullptr;
-  lib.store = (decltype(lib.store))(uintptr_t)at[0];
-  lib.gather = (decltype(lib.gather))(uintptr_t)at[1];
-  lib.plan = (decltype(lib.plan))(uintptr_t)at[2];
-  lib.decode = (decltype(lib.decode))(uintptr_t)at[3];
-  lib.append = (decltype(lib.append))(uintptr_t)at[4];
-  lib.window = (decltype(lib.window))(uintptr_t)at[5];
+  void* at[kEntries];
+  if (PyTuple_GET_SIZE(entries) != kEntries) {
+    PyErr_SetString(PyExc_ValueError, "entry points missing");
+    return nullptr;
+  }
+  for (int i = 0; i < kEntries; ++i) {
+    at[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(entries, i));
+    if (!at[i] && PyErr_Occurred()) return nullptr;
+  }
+  lib.store = (decltype(lib.store))at[0];
+  lib.gather = (decltype(lib.gather))at[1];
+  lib.plan = (decltype(lib.plan))at[2];
+  lib.decode = (decltype(lib.decode))at[3];
+  lib.append = (decltype(lib.append))at[4];
+  lib.window = (decltype(lib.window))at[5];
+  lib.index_store = (decltype(lib.index_store))at[6];
+  lib.index_gather = (decltype(lib.index_gather))at[7];
+  lib.scores = (decltype(lib.scores))at[8];
+  lib.topk = (decltype(lib.topk))at[9];
+  lib.tree_plan = (decltype(lib.tree_plan))at[10];
+  lib.tree = (decltype(lib.tree))at[11];
   lib.pool_type = same(pool_type);
   lib.get_stream = same(get_stream);
   lib.check = same(check);
@@ -467,8 +685,10 @@ PyObject* setup(PyObject*, PyObject* args) {
 
 #define FAST(f) \
   { #f, (PyCFunction)(void*)f, METH_FASTCALL, nullptr }
-PyMethodDef methods[] = {FAST(store),  FAST(gather), FAST(decode),
-                         FAST(append), FAST(window), {"setup", setup, METH_VARARGS, nullptr},
+PyMethodDef methods[] = {FAST(store),        FAST(gather), FAST(decode), FAST(append),
+                         FAST(window),       FAST(index_store),
+                         FAST(index_gather), FAST(scores), FAST(topk),   FAST(tree),
+                         {"setup", setup, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "remnant_ops", nullptr, -1, methods};
 

@@ -211,4 +211,14 @@ __device__ __forceinline__ void rope4(float* v, const float* cs) {
   }
 }
 
+// Row position * ratio of the frequency table, ratio the tokens that a position stands for
+// (4: records of the C4 pool, 1: tokens). As a kernel argument it comes behind those that
+// find the row: between them it cost 8,192 Native rows 0.2 of 5.7 us, one more dependent load.
+__device__ __forceinline__ bool has_freq_row(int32_t pos, uint32_t ratio, int64_t freq_rows) {
+  return pos >= 0 && (uint64_t)(uint32_t)pos * ratio < (uint64_t)freq_rows;
+}
+__device__ __forceinline__ const float* freq_row(const float* freqs, int32_t pos, uint32_t ratio) {
+  return freqs + (uint64_t)(uint32_t)pos * ratio * (2 * kRopePairs);
+}
+
 }  // namespace rm

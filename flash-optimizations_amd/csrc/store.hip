@@ -571,16 +571,6 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(
   }
 }
 
-// Row position * ratio of the frequency table, ratio the tokens that a position stands for
-// (4: records of the C4 pool, 1: tokens). As a kernel argument it comes behind those that
-// find the row: between them it cost 8,192 Native rows 0.2 of 5.7 us, one more dependent load.
-__device__ __forceinline__ bool has_freq_row(int32_t pos, uint32_t ratio, int64_t freq_rows) {
-  return pos >= 0 && (uint64_t)(uint32_t)pos * ratio < (uint64_t)freq_rows;
-}
-__device__ __forceinline__ const float* freq_row(const float* freqs, int32_t pos, uint32_t ratio) {
-  return freqs + (uint64_t)(uint32_t)pos * ratio * (2 * kRopePairs);
-}
-
 // Native records: one row, RMS-normalised and encoded by a wave. The conversions
 // are the hardware's (identical to the software rounding for every finite value
 // in range; a row with anything else takes the software rounding), and the group

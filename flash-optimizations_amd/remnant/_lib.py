@@ -93,6 +93,19 @@ SIGNATURES = {
     "rm_append_slots_after": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
                                      _vp, _vp, _vp, _vp, _vp, _vp]),
     "rm_window_slots": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "rm_index_store_rows": (_i32, [_vp, _i32, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _i64,
+                                   _vp, _i64, _vp]),
+    "rm_index_gather_bf16": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp,
+                                    _vp]),
+    "rm_index_scores": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64,
+                               _vp, _vp]),
+    "rm_index_topk": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "rm_tree_decode_workspace": (_i32, [_i64, _i64, _i64, _i64, _i64, _i64,
+                                        ctypes.POINTER(ctypes.c_int32),
+                                        ctypes.POINTER(ctypes.c_size_t)]),
+    "rm_tree_decode_fwd": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp,
+                                  _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _f32, _vp, _vp, _vp,
+                                  _sz, _vp]),
 }
 
 _lib = None
@@ -122,8 +135,8 @@ _ops = None
 
 
 def ops():
-    """Module of csrc/ops.cpp: checks and launches of the 4-bit operators and the slot
-    maps, over the entry points of ``load()``."""
+    """Module of csrc/ops.cpp: checks and launches of the 4-bit and index operators, the
+    tree attention and the slot maps, over the entry points of ``load()``."""
     return _ops or _load_ops()
 
 
@@ -142,7 +155,9 @@ def _load_ops():
     spec.loader.exec_module(module)
     module.setup(tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
         "rm_mx4_store_rows_ratio", "rm_mx4_gather_bf16", "rm_mx4_sparse_decode_workspace",
-        "rm_mx4_sparse_decode_fwd", "rm_append_slots_after", "rm_window_slots")),
+        "rm_mx4_sparse_decode_fwd", "rm_append_slots_after", "rm_window_slots",
+        "rm_index_store_rows", "rm_index_gather_bf16", "rm_index_scores", "rm_index_topk",
+        "rm_tree_decode_workspace", "rm_tree_decode_fwd")),
         LatentPool, torch._C._cuda_getCurrentRawStream, check, _native_pages)
     _ops = module
     return module

@@ -50,6 +50,9 @@ MX4_GROUP = 32
 MX4_CODE_BYTES = HEAD_DIM // 2                               # 256
 MX4_RECORD_BYTES = MX4_CODE_BYTES + HEAD_DIM // MX4_GROUP    # 272
 MX4_PAGE_BYTES = PAGE_RECORDS * MX4_RECORD_BYTES             # 17408
+INDEX_DIM = 128
+INDEX_RECORD_BYTES = INDEX_DIM + 4                           # 132
+INDEX_PAGE_BYTES = PAGE_RECORDS * INDEX_RECORD_BYTES         # 8448
 MAX_SLOT_BATCH = 8192                                        # requests of an append_slots call
 
 FORMATS = ("native", "direct", "mx4")

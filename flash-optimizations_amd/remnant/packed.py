@@ -87,6 +87,8 @@ def _as_source(buffers, layer_id) -> tuple[RemnantBuffers | torch.Tensor, bool, 
     if isinstance(buffers, LatentPool):
         if buffers.fmt == "mx4":
             raise ValueError("4-bit (mx4) records are read and written by the mx4_ operators")
+        if buffers.fmt == "index":
+            raise ValueError("index records are read and written by the index_ operators")
         pages = buffers.layer(layer_id)
         if not buffers.packed:
             return pages, False, config.KEEP_COUNT
@@ -110,7 +112,7 @@ def _operand(buffers, layer_id):
     """What a launch needs of a pool: (pages address, page count, plane buffers
     or None, packed, survivor count, tensors to check). A LatentPool's layer is
     addressed in its buffer, without making the layer's view."""
-    if type(buffers) is LatentPool and buffers.fmt != "mx4":
+    if type(buffers) is LatentPool and buffers.fmt in ("remnant", "native"):
         buf, i = buffers.buffer, 0 if layer_id is None else layer_id
         shape = buf.shape
         if type(i) is int and len(shape) == 3 and 0 <= i < shape[0] and shape[1] > 0:

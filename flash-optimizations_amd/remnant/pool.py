@@ -21,6 +21,9 @@ One pool holds one profile; per-layer profiles use one pool per layer.
 
 A 4-bit pool (``fmt="mx4"``) holds 64 contiguous 272-byte records a page: 256 bytes
 of E2M1 codes, two coordinates a byte, then 16 UE8M0 scale bytes.
+
+An index pool (``fmt="index"``) holds the index keys of as many records: 64 rows of 128
+E4M3 codes a page, then their 64 float32 scales.
 """
 
 from __future__ import annotations
@@ -30,19 +33,22 @@ import torch
 from . import config
 
 
+_TITLES = {"native": "Native", "mx4": "4-bit", "index": "Index"}
+
+
 class LatentPool:
     def __init__(self, pages: int, layers: int = 1, fmt: str = "remnant", device="cuda",
                  keep_count: int = config.KEEP_COUNT):
         if fmt == "direct":
             fmt = "remnant"
-        if fmt not in ("remnant", "native", "mx4"):
+        if fmt not in ("remnant", "native", "mx4", "index"):
             raise ValueError(f"unsupported cache format: {fmt!r}")
         if pages < 0 or layers < 1:
             raise ValueError("pages must be >= 0 and layers >= 1")
         config.check_keep_count(keep_count)
         if fmt != "remnant" and keep_count != config.KEEP_COUNT:
-            raise ValueError(f"{'Native' if fmt == 'native' else '4-bit'} records keep every "
-                             "coordinate; keep_count is Packed-only")
+            raise ValueError(f"{_TITLES[fmt]} records keep every coordinate; keep_count is "
+                             "Packed-only")
         self.fmt = fmt
         self.pages = pages
         self.layers = layers
@@ -53,6 +59,9 @@ class LatentPool:
         elif fmt == "mx4":
             self.page_bytes = config.MX4_PAGE_BYTES
             self.data_bytes = config.MX4_CODE_BYTES
+        elif fmt == "index":
+            self.page_bytes = config.INDEX_PAGE_BYTES
+            self.data_bytes = config.INDEX_DIM
         else:
             self.page_bytes = config.NATIVE_PAGE_BYTES
             self.data_bytes = config.NATIVE_DATA_BYTES
@@ -69,13 +78,22 @@ class LatentPool:
 
     @property
     def record_bytes(self) -> int:
-        return self.data_bytes + (16 if self.fmt == "mx4" else 8)
+        return self.data_bytes + self._scale_bytes
+
+    @property
+    def _scale_bytes(self) -> int:
+        return {"mx4": 16, "index": 4}.get(self.fmt, 8)
+
+    @property
+    def _scales_apart(self) -> bool:
+        """Whether a page's scales stand behind its 64 data rows."""
+        return self.fmt in ("native", "index")
 
     def layer(self, layer_id: int | None = None) -> torch.Tensor:
         return self.buffer[0 if layer_id is None else layer_id]
 
     def _data_rows(self, layer_id):
-        if self.fmt != "native":  # contiguous records: data = all but the scales of each
+        if not self._scales_apart:  # contiguous records: data = all but the scales of each
             pg = self.layer(layer_id).reshape(self.pages, config.PAGE_RECORDS,
                                               self.record_bytes)
             return pg[..., : self.data_bytes]
@@ -83,26 +101,26 @@ class LatentPool:
         return pg.reshape(self.pages, config.PAGE_RECORDS, self.data_bytes)
 
     def scales(self, layer_id: int | None = None) -> torch.Tensor:
-        """Scale plane view [pages, 64, 8] u8 (4-bit: [pages, 64, 16])."""
-        if self.fmt != "native":
+        """Scale plane view [pages, 64, 8] u8 (4-bit: [pages, 64, 16], index: [pages, 64,
+        4], the bytes of a float32)."""
+        if not self._scales_apart:
             pg = self.layer(layer_id).reshape(self.pages, config.PAGE_RECORDS,
                                               self.record_bytes)
             return pg[..., self.data_bytes:]
         pg = self.layer(layer_id)[:, config.PAGE_RECORDS * self.data_bytes:]
-        return pg.reshape(self.pages, config.PAGE_RECORDS, 8)
+        return pg.reshape(self.pages, config.PAGE_RECORDS, self._scale_bytes)
 
     def values(self, layer_id: int | None = None) -> torch.Tensor:
         """Code plane view: Packed [pages, 64, keep_count] u8, Native [pages, 64, 448] u8,
-        4-bit [pages, 64, 256] u8 (two codes a byte)."""
-        width = (self.keep_count if self.packed else config.MX4_CODE_BYTES if self.fmt == "mx4"
-                 else config.NOPE_DIM)
+        4-bit [pages, 64, 256] u8 (two codes a byte), index [pages, 64, 128] u8."""
+        width = (self.keep_count if self.packed else config.NOPE_DIM if self.fmt == "native"
+                 else self.data_bytes)
         return self._data_rows(layer_id)[..., :width]
 
     def bitmaps(self, layer_id: int | None = None) -> torch.Tensor:
         """Bitmap plane view [pages, 64, 64] u8 (8 little-endian MSB-first uint64 words)."""
         if not self.packed:
-            raise ValueError(f"{'Native' if self.fmt == 'native' else '4-bit'} records carry no "
-                             "bitmap")
+            raise ValueError(f"{_TITLES[self.fmt]} records carry no bitmap")
         return self._data_rows(layer_id)[..., self.keep_count:self.data_bytes]
 
     def records(self, slots: torch.Tensor, layer_id: int | None = None) -> torch.Tensor:
@@ -122,6 +140,7 @@ class LatentPool:
 def records_fitting(nbytes: int, fmt: str = "remnant", keep_count: int = config.KEEP_COUNT) -> int:
     """Records (whole pages of 64) that fit in ``nbytes`` of HBM."""
     fmt = "remnant" if fmt == "direct" else fmt
-    page = (config.packed_page_bytes(keep_count) if fmt == "remnant" else config.MX4_PAGE_BYTES
-            if fmt == "mx4" else config.NATIVE_PAGE_BYTES)
+    page = (config.packed_page_bytes(keep_count) if fmt == "remnant" else
+            {"mx4": config.MX4_PAGE_BYTES, "index": config.INDEX_PAGE_BYTES}.get(
+                fmt, config.NATIVE_PAGE_BYTES))
     return (nbytes // page) * config.PAGE_RECORDS

@@ -69,6 +69,9 @@
  * half of byte i) and 16 UE8M0 scale bytes, one per 32 coordinates, value =
  * code * 2^(byte - 127). The tail is stored rotated. Every coordinate is kept.
  *
+ * Index records (no counterpart in the reference): an index page (8,448 B) is 64 rows
+ * of 128 E4M3 codes, then 64 float32 scales, one a row; value = code * scale.
+ *
  * Plane form: the same records held as three row-aligned planes, slot s being
  * row s of each: values [rows, K] u8 (codes, ascending coordinate), bitmaps
  * [rows, 8] u64 (the bitmap words as above) and scales [rows, 8] u8. Byte for
@@ -96,7 +99,8 @@ enum rm_status {
 
 enum rm_dtype { RM_F32 = 0, RM_BF16 = 1 };
 
-enum rm_format { RM_FORMAT_PACKED = 0, RM_FORMAT_NATIVE = 1, RM_FORMAT_MX4 = 4 };
+enum rm_format { RM_FORMAT_PACKED = 0, RM_FORMAT_NATIVE = 1, RM_FORMAT_MX4 = 4,
+                 RM_FORMAT_INDEX = 5 };
 
 #define RM_HEAD_DIM 512
 #define RM_NOPE_DIM 448
@@ -112,6 +116,12 @@ enum rm_format { RM_FORMAT_PACKED = 0, RM_FORMAT_NATIVE = 1, RM_FORMAT_MX4 = 4 }
 #define RM_MX4_RECORD_BYTES 272
 #define RM_MX4_PAGE_BYTES 17408
 #define RM_MAX_SLOT_BATCH 8192
+#define RM_INDEX_DIM 128
+#define RM_INDEX_RECORD_BYTES 132
+#define RM_INDEX_PAGE_BYTES 8448
+#define RM_MAX_INDEX_HEADS 128
+#define RM_MAX_INDEX_WIDTH 1048576
+#define RM_MAX_TREE_NODES 64
 
 /* Library version (major * 10000 + minor * 100 + patch). */
 int rm_version(void);
@@ -222,8 +232,8 @@ int rm_packed_to_native_planes(const uint8_t* values, const uint64_t* bitmaps,
  * l of `src` is copied to record dst_slots[i] of layer l of `dst` -- the whole
  * Packed record (codes, bitmap and scales together; format RM_FORMAT_PACKED
  * with its keep_count) or the Native data row and scale row
- * (RM_FORMAT_NATIVE) or the 4-bit record (RM_FORMAT_MX4; keep_count is not
- * looked at). Pairs with a slot < 0 or beyond its pool are skipped.
+ * (RM_FORMAT_NATIVE) or the 4-bit record (RM_FORMAT_MX4) or the index row and its
+ * scale (RM_FORMAT_INDEX); keep_count is looked at for Packed records alone. Pairs with a slot < 0 or beyond its pool are skipped.
  * Layer l of a pool starts l * layer_bytes after its base. Either pool may be
  * device memory or pinned host memory (hipHostMalloc). 8-byte alignment. */
 int rm_copy_records(const uint8_t* src, int64_t src_pages, int64_t src_layer_bytes,
@@ -445,6 +455,73 @@ int rm_append_slots_after(int32_t* block_table, int64_t block_table_stride, int6
 int rm_window_slots(const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
                     const int32_t* lengths, int64_t batch, int64_t q_len, int64_t window,
                     int64_t first, int32_t* slots, int32_t* counts, void* stream);
+
+/* ---- Index records (RM_FORMAT_INDEX) and tree attention: no counterpart in the
+ * reference. ---- */
+
+/* Store: rows [n, 128] (dtype, strides and alignment as rm_mx4_store_rows) as index
+ * records: RMSNorm over 128, BF16 rounding, coordinates 64 .. 127 rotated by freqs row
+ * position[i] * ratio and rounded to BF16 (freqs NULL = no rotation), then E4M3 codes
+ * n / 2^e rounded to nearest even under the smallest e with max(amax, 1e-4) <= 448 *
+ * 2^e; the scale is 2^e. A row with an infinity or NaN gets scale NaN and reads as 128
+ * NaN. Skipped rows and slots as rm_mx4_store_rows. */
+int rm_index_store_rows(const void* x, int x_dtype, int64_t x_row_stride, const float* weight,
+                        float eps, const int32_t* dst_slot, const int32_t* position,
+                        const float* freqs, int64_t freq_rows, int64_t ratio, int64_t n,
+                        uint8_t* pool, int64_t pool_pages, void* stream);
+
+/* Reader: as rm_mx4_gather_bf16 with rows of 128: code * scale rounded to BF16. */
+int rm_index_gather_bf16(const uint8_t* pool, int64_t pool_pages, const int32_t* slots,
+                         int64_t slots_stride_q, int64_t slots_stride_k, const int32_t* lengths,
+                         int64_t length_stride, int64_t n_queries, int64_t selected_k,
+                         uint16_t* out, void* stream);
+
+/* Scores of cached index records: out [batch * q_len, width], for token t of request b and
+ * record r < min(lengths[t], width, max_blocks * 64) whose page block_table[b, r / 64]
+ * is one of the pool's,
+ *   scale_r * sum_h weights[t, h] c_h max(0, sum_d Q8_h[d] K8_r[d]),
+ * Q8_h and c_h being q[t, h] [128] BF16 coded as the store codes a row; -inf elsewhere.
+ * A NaN in a record, a query or a weight gives NaN. heads <= RM_MAX_INDEX_HEADS, batch <=
+ * 65535, batch * q_len <= 2^20, q and pool 16-byte aligned. */
+int rm_index_scores(const uint16_t* q, int64_t batch, int64_t q_len, int64_t heads,
+                    const float* weights, const uint8_t* pool, int64_t pool_pages,
+                    const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                    const int32_t* lengths, int64_t width, float* out, void* stream);
+
+/* Selection: indices [rows, k] = the numbers of the counts[row] = min(k, lengths[row],
+ * width) highest of the row's first lengths[row] scores (NULL = width; negative: 0), in
+ * ascending order, -1 behind them. Equal scores go to the lowest numbers, NaN counts as
+ * -inf. scores: rows row_stride floats apart. width, k <= RM_MAX_INDEX_WIDTH. */
+int rm_index_topk(const float* scores, int64_t row_stride, const int32_t* lengths, int64_t rows,
+                  int64_t width, int64_t k, int32_t* indices, int32_t* counts, void* stream);
+
+/* Split planning for the decode below (window 0 = none). nodes <= RM_MAX_TREE_NODES,
+ * heads <= 1024, batch * nodes <= 65535, blocks <= 2^24. */
+int rm_tree_decode_workspace(int64_t batch, int64_t nodes, int64_t heads, int64_t max_blocks,
+                             int64_t window, int64_t history_blocks, int32_t* num_splits,
+                             size_t* workspace_bytes);
+
+/* Attention of drafted trees over a Native pool. Request b holds lengths[b] committed
+ * rows at positions 0 .. lengths[b] - 1 of its block_table row, and node j's own row at
+ * position lengths[b] + j. parents [batch, nodes]: a node's parent, a node before it,
+ * or -1 for a child of the committed text; any other number is padding, and so are its
+ * descendants: they see nothing. A node at depth d (0: child of the committed text)
+ * stands at lengths[b] + d and sees, in one softmax with the sink, the committed rows
+ * and nodes on its path that stand no more than window - 1 before it (window 0: all),
+ * itself among them, and the first history_lengths[b] records of history_table's row
+ * in history_pool (history_blocks 0: none). Positions whose page is not one of the pool's
+ * are not seen. out [batch, nodes, heads, 512], lse [batch, nodes, heads] as
+ * rm_native_sparse_decode_fwd. A row with an infinity or NaN makes outputs NaN only for
+ * nodes that see it. */
+int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t nodes, int64_t heads,
+                       const uint8_t* pool, int64_t pool_pages, const int32_t* block_table,
+                       int64_t block_table_stride, int64_t max_blocks, const int32_t* lengths,
+                       const int32_t* parents, int64_t window, const uint8_t* history_pool,
+                       int64_t history_pages, const int32_t* history_table,
+                       int64_t history_table_stride, int64_t history_blocks,
+                       const int32_t* history_lengths, const float* sink, float softmax_scale,
+                       uint16_t* out, float* lse, void* workspace, size_t workspace_bytes,
+                       void* stream);
 
 #ifdef __cplusplus
 }
