@@ -24,7 +24,7 @@
 // weights and values. m is a whole number of log2 units, kept 16 above the largest score of
 // the round that set it, so that it hardly ever moves again; a unit with a score above it
 // takes its own for that round, and the waves then agree on the highest: integer
-// subtractions on the weights' exponents, and O rescaled.
+// subtractions on the weights' exponents, O rescaled and one barrier more.
 // The output is divided by the sum of the weights as they were rounded, and lse takes the
 // sum of the exact ones: roundings that a row's weights have in common cancel.
 //
@@ -94,13 +94,11 @@ struct TreeArgs {
 __device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
   return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * lane, (int)x);
 }
-// Whether one of the dword's four E4M3 codes is NaN (0x7f or 0xff).
-__device__ __forceinline__ uint32_t nan_codes(uint32_t x) {
-  return ~(((x & 0x7f7f7f7fu) ^ 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u;
-}
-// Whether one of the dword's two BF16 is an infinity or NaN.
-__device__ __forceinline__ uint32_t special_bf16(uint32_t x) {
-  return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+// Nonzero where one of the dword's four E4M3 codes is NaN (0x7f or 0xff), or one of its two
+// BF16 an infinity or NaN.
+__device__ __forceinline__ uint32_t special(uint32_t x, bool bf16) {
+  return ((x & (bf16 ? 0x7f807f80u : 0x7f7f7f7fu)) + (bf16 ? 0x00800080u : 0x01010101u)) &
+         (bf16 ? 0x80008000u : 0x80808080u);
 }
 // Eight codes times a scale -> eight BF16.
 __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi, float scale) {
@@ -119,7 +117,8 @@ __device__ __forceinline__ float over_groups(float x, bool is_max) {
 struct Tree {
   const TreeArgs& a;
   const uint32_t lds;
-  const int lane, row, group, wave, b;
+  int lane, row, group;
+  const int wave, b;
   // the request
   int held, past, first, past_units, units;
   // by half of the query rows, lane % 16: what the row's node sees, and its softmax
@@ -138,6 +137,14 @@ struct Tree {
         group(lane >> 4),
         wave(uniform((int)(threadIdx.x >> 6))),
         b(request) {}
+
+  // What follows from the lane is worked out again in each round: kept, it would push Q out
+  // of the registers.
+  __device__ __forceinline__ void again() {
+    asm volatile("" : "+v"(lane));
+    row = lane & 15;
+    group = lane >> 4;
+  }
 
   // Coordinates 64 s + 16 group .. + 15 as two operands, then the tail's 32 t + 8 group.
   __device__ __forceinline__ void load_q(int first_row) {
@@ -238,23 +245,25 @@ struct Tree {
   // Piece j of row r goes to place j ^ turn(r) of the row, within its four.
   __device__ __forceinline__ static int turn(int r) { return (r >> 1) & 3; }
   __device__ __forceinline__ void copy(const Unit& x, uint32_t to) const {
-    uint32_t from = lane;
-    asm volatile("" : "+v"(from));  // (nine offsets are not worth nine registers)
 #pragma unroll
     for (int n = 0; n < kCopies; ++n) {
-      const uint32_t p = 64 * n + from, r = p / 36, j = p - 36 * r;
+      const uint32_t p = 64 * n + lane, r = p / 36, j = p - 36 * r;
       copy16(x.rows + (576 * r + 16 * (j ^ turn(r))), to + 1024 * n);
     }
   }
 
+  // Where the lane leaves the weights of the wave's unit.
+  __device__ __forceinline__ uint32_t weights_at(int c) const {
+    return lds + kWeightsAt + 2048 * (wave >> 1) + 1024 * c + 16 * lane + 8 * (wave & 1);
+  }
   // Scores and weights of the unit, in LDS at `at`.
   template <bool kWhole>
-  __device__ __forceinline__ void score(const Unit& x, uint32_t at, int odd, float (&own)[2],
-                                        float (&sum)[2], float (&rsum)[2]) {
+  __device__ __forceinline__ void score(const Unit& x, uint32_t at, float (&own)[2], float (&sum)[2],
+                                        float (&rsum)[2]) {
     u32x2 bytes = x.scales;
     // rows of the unit that count
     const int stop = min(x.past ? past - x.at : held + a.nodes - x.at, kUnit);
-    uint32_t special = 0;
+    uint32_t odd = 0;  // rows with an infinity or NaN
     if (!kWhole) {
       // row `row`, pieces 9 group .. + 8: an infinity or NaN in it?
       const uint32_t mine = at + kNativeDataBytes * row + 144 * group;
@@ -265,14 +274,14 @@ struct Tree {
         // (pieces 28 and up are the tail)
         const bool tail = 9 * group + n >= 28;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) bad |= tail ? special_bf16(v[k]) : nan_codes(v[k]);
+        for (int k = 0; k < 4; ++k) bad |= special(v[k], tail);
       }
 #pragma unroll
       for (int g = 0; g < 7; ++g)
         bad |= ((bytes[g / 4] >> (8 * (g % 4))) & 0xffu) == 0xffu;
       const uint64_t found = __ballot(bad != 0);
-      special = (uint32_t)(found | found >> 16 | found >> 32 | found >> 48) & 0xffffu;
-      if (!x.mapped || row >= stop || ((special >> row) & 1u)) {
+      odd = (uint32_t)(found | found >> 16 | found >> 32 | found >> 48) & 0xffffu;
+      if (!x.mapped || row >= stop || ((odd >> row) & 1u)) {
 #pragma unroll
         for (int n = 0; n < 9; ++n) lds_write(mine + 16 * n, u32x4{0, 0, 0, 0});
         bytes = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
@@ -282,7 +291,7 @@ struct Tree {
     {
       const uint32_t two = (group >= 2 ? bytes[1] : bytes[0]) >> (16 * (group & 1));
       const uint32_t to = lds + kShiftsAt + 512 * (wave >> 1) + 128 * group + 16 * (row >> 2) +
-                          2 * (4 * odd + (row & 3));
+                          2 * (4 * (wave & 1) + (row & 3));
       lds_write<uint16_t>(to, (uint16_t)((254u - (two & 0xffu)) << 7));
       lds_write<uint16_t>(to + 64, (uint16_t)((254u - ((two >> 8) & 0xffu)) << 7));
     }
@@ -322,7 +331,7 @@ struct Tree {
           const bool on_path = ((word >> (node & 31)) & 1u) != 0;
           const bool see = live[c] & x.mapped & (n < stop) &
                            (x.past | (node < 0 ? p >= lowest[c] : on_path));
-          s[i] = (special >> n) & 1u ? NAN : s[i];
+          s[i] = (odd >> n) & 1u ? NAN : s[i];
           s[i] = see ? s[i] : -INFINITY;
         }
       }
@@ -344,53 +353,34 @@ struct Tree {
       for (int i = 0; i < 4; ++i)
         rsum[c] = __builtin_fmaf(i & 1 ? u2f(d[i / 2] & 0xffff0000u) : u2f(d[i / 2] << 16),
                                  0x1p-127f, rsum[c]);
-      lds_write(lds + kWeightsAt + 2048 * (wave >> 1) + 1024 * c + 16 * lane + 8 * odd, d);
+      lds_write(weights_at(c), d);
     }
   }
 
-  // O += the round's units, at `at`. kTail: the wave with the BF16 coordinates. kMoved: the
-  // units' references are not all m.
-  template <bool kTail, bool kMoved>
-  __device__ __forceinline__ void add(uint32_t at, int here) {
+  // O += the round's units, at `at`.
+  __device__ __forceinline__ void add(uint32_t at) {
+    const bool tail = wave == kWaves - 1;  // the BF16 coordinates
     const int pair = row >> 1;  // transposed reads: row 4 group + pair % 4 of unit pair / 4
     const int of = 4 * group + (pair & 3);
-    uint32_t v_at[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v_at[e] = at + kUnitBytes * (pair >> 2) + kNativeDataBytes * of + 64 * wave +
-                16 * (e ^ turn(of)) + 8 * (row & 1);
+    const uint32_t v_at = at + kUnitBytes * (pair >> 2) + kNativeDataBytes * of + 64 * wave +
+                          8 * (row & 1);
     const int tail_of = 4 * group + (row >> 2);
     const uint32_t t_at = at + kNativeDataBytes * tail_of + kNopeDim + 8 * (row & 1);
 #pragma unroll
     for (int v = 0; v < kWaves / 2; ++v) {
-      if (2 * v >= here) break;
       u32x4 p[2], shift = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
-      if (!kTail) shift = lds_read<u32x4>(lds + kShiftsAt + 512 * v + 64 * wave + 16 * group);
+      bf16x8 x[4];
+      if (!tail) {
+        shift = lds_read<u32x4>(lds + kShiftsAt + 512 * v + 64 * wave + 16 * group);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        p[c] = lds_read<u32x4>(lds + kWeightsAt + 2048 * v + 1024 * c + 16 * lane);
-        if (kMoved) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float ref = lds_read<float>(lds + kRefsAt + 4 * (kRows * (2 * v + k) + 16 * c + row));
-            // whole log2 units down to m, in both exponents; 255: past every exponent, also
-            // for a unit without a row (of -inf, and the difference perhaps NaN)
-            const uint32_t down = __umul24((uint32_t)fminf(m[c] - ref, 255.0f), 0x00800080u);
-            p[c][2 * k] = sub_sat(p[c][2 * k], down);
-            p[c][2 * k + 1] = sub_sat(p[c][2 * k + 1], down);
-          }
+        for (int u = 0; u < 4; ++u) {
+          const i32x2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)(
+              uintptr_t)(v_at + 16 * (u ^ turn(of)) + 2 * kUnitBytes * v));
+          x[u] = codes8((uint32_t)codes[0], (uint32_t)codes[1], 1.0f);
         }
+      } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) p[c][k] = sub_sat(p[c][k], shift[k]);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        bf16x8 x;
-        if (!kTail) {
-          const i32x2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (lds_i32x2*)(lds_void*)(uintptr_t)(v_at[u] + 2 * kUnitBytes * v));
-          x = codes8((uint32_t)codes[0], (uint32_t)codes[1], 1.0f);
-        } else {
+        for (int u = 0; u < 4; ++u) {
           u32x2 part[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k)  // pieces 28 + 2 u and + 1
@@ -398,12 +388,20 @@ struct Tree {
                 u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)(uintptr_t)(
                            t_at + kUnitBytes * (2 * v + k) + 64 * (u >> 1) +
                            16 * ((2 * (u & 1) + ((row & 3) >> 1)) ^ turn(tail_of)))));
-          x = as_bf16x8(u32x4{part[0][0], part[0][1], part[1][0], part[1][1]});
+          x[u] = as_bf16x8(u32x4{part[0][0], part[0][1], part[1][0], part[1][1]});
         }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        p[c] = lds_read<u32x4>(lds + kWeightsAt + 2048 * v + 1024 * c + 16 * lane);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[c][k] = sub_sat(p[c][k], shift[k]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          o[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, as_bf16x8(p[c]), o[c][u], 0, 0, 0);
-      }
+          o[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], as_bf16x8(p[c]), o[c][u], 0, 0, 0);
     }
   }
 
@@ -426,8 +424,8 @@ struct Tree {
     if (begin + kWaves + wave < end) page = page_of(begin + kWaves + wave);
     int odd = 0;  // round
     for (int i = begin + wave; i - wave < end; i += kWaves, odd ^= 1) {
-      const int here = min(end - (i - wave), kWaves);
       const uint32_t at = lds + odd * kWaves * kUnitBytes;
+      again();
       wait_copies<0>();
       lds_barrier();
       if (i + kWaves < end) {
@@ -439,15 +437,14 @@ struct Tree {
       const uint32_t mine = at + wave * kUnitBytes;
       if (i < end) {
         if (whole(x))
-          score<true>(x, mine, wave & 1, own, sum, rsum);
+          score<true>(x, mine, own, sum, rsum);
         else
-          score<false>(x, mine, wave & 1, own, sum, rsum);
-      } else if (wave == here && (here & 1)) {  // the other half of the last pair: nothing
+          score<false>(x, mine, own, sum, rsum);
+      } else {  // the round's last units: nothing
 #pragma unroll
         for (int n = 0; n < kCopies; ++n) lds_write(mine + 1024 * n + 16 * lane, u32x4{0, 0, 0, 0});
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          lds_write(lds + kWeightsAt + 2048 * (wave >> 1) + 1024 * c + 16 * lane + 8, u32x2{0, 0});
+        for (int c = 0; c < 2; ++c) lds_write(weights_at(c), u32x2{0, 0});
       }
       if (lane < kUnit) {
 #pragma unroll
@@ -459,6 +456,7 @@ struct Tree {
       if (threadIdx.x == 0) lds_write(lds + kMovedAt + 4 * (odd ^ 1), 0);
       lds_barrier();
       if (uniform(lds_read<int>(lds + kMovedAt + 4 * odd)) != 0) {
+        // the highest reference is everyone's: O, the sums and the unit's weights go down to it
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float top = m[c];
@@ -469,23 +467,24 @@ struct Tree {
           const float f = m[c] == top ? 1.0f : __builtin_amdgcn_exp2f(m[c] - top);
           const float g = own[c] == top ? 1.0f : __builtin_amdgcn_exp2f(own[c] - top);
           m[c] = top;
-          l[c] = l[c] * f + sum[c] * g;
-          r[c] = r[c] * f + rsum[c] * g;
+          l[c] *= f;
+          r[c] *= f;
+          sum[c] *= g;
+          rsum[c] *= g;
 #pragma unroll
           for (int u = 0; u < 4; ++u) o[c][u] *= f;
+          // whole log2 units, in both exponents; 255: past every exponent, also for a
+          // difference that is NaN (infinities: the sum is NaN then)
+          const uint32_t down = __umul24((uint32_t)fminf(top - own[c], 255.0f), 0x00800080u);
+          const u32x2 p = lds_read<u32x2>(weights_at(c));
+          lds_write(weights_at(c), u32x2{sub_sat(p[0], down), sub_sat(p[1], down)});
         }
-        if (wave < kWaves - 1)
-          add<false, true>(at, here);
-        else
-          add<true, true>(at, here);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) l[c] += sum[c], r[c] += rsum[c];
-        if (wave < kWaves - 1)
-          add<false, false>(at, here);
-        else
-          add<true, false>(at, here);
+        lds_barrier();
       }
+      again();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) l[c] += sum[c], r[c] += rsum[c];
+      add(at);
       x = next;
     }
   }
