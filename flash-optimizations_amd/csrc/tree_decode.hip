@@ -7,24 +7,26 @@
 //
 // All nodes and heads of a request read the same rows: row m = node * heads + head of q is
 // one of its nodes * heads query rows. A workgroup takes 32 of them and a share of the
-// request's rows, 128 a round: eight units of 16, one a wave. In a round a wave
-//   * copies its unit of the next round to LDS as it is stored (global_load_lds),
-//   * scores its unit: S^T = K Q^T on v_mfma_f32_16x16x32_bf16 for both halves of the 32
-//     query rows, Q in registers, the codes made BF16 with their scales on the way from LDS
-//     (the conversion's operand), and leaves the weights P^T = 2^(s - m) in LDS,
-//   * adds all eight units to the 64 output coordinates that it owns: O^T += V^T P^T. V^T
-//     comes out of LDS transposed (ds_read_b64_tr_b8), and P^T as the lanes left it: the
-//     order of the rows in that product's long axis is free, and S^T's is taken. The codes
-//     become BF16 without their scales there: a row's scale is a power of two, so it goes
-//     to the weights' exponents, and as the eight waves own one group of 64 coordinates
-//     each, once a weight and wave. Weights stand as P * 2^127 in BF16, and
-//     (254 - scale byte) << 7 is subtracted as integers, saturating at zero: exact for
-//     every byte but 255, whose row has NaN scores; what falls below 2^-126 becomes zero.
-// Two barriers a round: before the copies (everyone is done with the buffer) and between
-// weights and values. m is a whole number of log2 units, kept 16 above the largest score of
+// request's rows, 64 a round: four units of 16. Eight waves, two a SIMD, in two roles, so
+// that one's vector work and waits lie under the other's matrix products:
+//   * four scorers, each with all 32 query rows (Q in registers) and a unit of the round:
+//     S^T = K Q^T on v_mfma_f32_16x16x32_bf16, the codes made BF16 with their scales on the
+//     way from LDS (the conversion's operand), once for both halves of the query rows; they
+//     leave the weights P^T = 2^(s - m) in LDS;
+//   * four adders, each with 128 output coordinates of all 32 query rows (in registers):
+//     O^T += V^T P^T of the round before. V^T comes out of LDS transposed
+//     (ds_read_b64_tr_b8), and P^T as the scorers left it: the order of the rows in that
+//     product's long axis is free, and S^T's is taken. The codes become BF16 without their
+//     scales there: a row's scale is a power of two, so it goes to the weights' exponents,
+//     and as an adder owns two groups of 64 coordinates each, twice a weight and wave.
+//     Weights stand as P * 2^127 in BF16, and (254 - scale byte) << 7 is subtracted as
+//     integers, saturating at zero: exact for every byte but 255, whose row has NaN scores;
+//     what falls below 2^-126 becomes zero. The adders also copy the rows of the round after
+//     next to LDS as they are stored (global_load_lds), in between their products.
+// One barrier a round. m is a whole number of log2 units, kept 16 above the largest score of
 // the round that set it, so that it hardly ever moves again; a unit with a score above it
-// takes its own for that round, and the waves then agree on the highest: integer
-// subtractions on the weights' exponents, O rescaled and one barrier more.
+// takes its own for that round. After it the scorers go on from the highest of the units',
+// and the adders lower that round's weights (integer subtractions on their exponents) and O.
 // The output is divided by the sum of the weights as they were rounded, and lse takes the
 // sum of the exact ones: roundings that a row's weights have in common cancel.
 //
@@ -33,8 +35,8 @@
 // one piece of eight rows meet every bank once.
 //
 // Units that some node does not see whole (the ends of the window and of the committed
-// rows, the drafted rows) are masked by row; rows there that nobody sees, and rows with
-// an infinity or NaN, are set to zero, the latter's scores to NaN where they are seen: a
+// rows, the drafted rows) are masked by row; the adders take zeros for rows there that nobody
+// sees, and for rows with an infinity or NaN, whose scores are NaN where they are seen: a
 // zero weight must not meet them.
 #include <algorithm>
 
@@ -46,25 +48,39 @@ using namespace rm;
 
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kRows = 32;  // query rows of a workgroup
-constexpr int kUnit = 16;  // rows a wave scores in a round
-constexpr int kRound = kWaves * kUnit;
+constexpr int kRows = 32;    // query rows of a workgroup
+constexpr int kUnit = 16;    // rows a scorer takes in a round
+constexpr int kUnits = 4;    // of a round
+constexpr int kRound = kUnits * kUnit;
+constexpr int kScorers = 4;  // unit `wave`
+constexpr int kAdders = 4;   // coordinates 128 (wave - 4) ..
+constexpr int kBuffers = 4;  // rounds in LDS: added, scored, two being copied
 constexpr int kMaxNodes = 64;
 constexpr int kMaxHeads = 1024;
-constexpr int kUnitBytes = kUnit * kNativeDataBytes;  // 9,216
-constexpr int kCopies = kUnitBytes / 1024;            // 9
-constexpr int kWeightsAt = 2 * kWaves * kUnitBytes;   // [4 pairs of units][2][64 lanes] 16 bytes
-constexpr int kShiftsAt = kWeightsAt + 8 * 1024;      // [4][8 groups][4][8] u16
-constexpr int kRefsAt = kShiftsAt + 4 * 8 * 64;       // [8 units][32 query rows] float
-constexpr int kMovedAt = kRefsAt + kWaves * kRows * 4;  // [2]
-constexpr int kLdsBytes = kMovedAt + 16;
-constexpr int kSumsAt = kWeightsAt;  // at the end: [8 waves][32] of l, r
-static_assert(kLdsBytes <= 160 * 1024 && kCopies * 1024 == kUnitBytes, "LDS of a CU");
+constexpr int kUnitBytes = kUnit * kNativeDataBytes;  // 9,216: nine copies of 64 pieces
+constexpr int kScalesAt = kUnits * kUnitBytes;  // the units' scale rows, 8 bytes each
+constexpr int kRoundBytes = kScalesAt + kUnits * kUnit * kScaleBytes;
+constexpr int kCopies = 10;  // an adder and round: a unit and its scales
+// Of odd and even rounds:
+constexpr int kWeightsAt = kBuffers * kRoundBytes;  // [2 pairs of units][2][64 lanes] 16 bytes
+constexpr int kWeightsBytes = 4 * 1024;
+constexpr int kShiftsAt = kWeightsAt + 2 * kWeightsBytes;  // [2][8 groups][4][8] u16
+constexpr int kShiftsBytes = 2 * 8 * 64;
+constexpr int kRefsAt = kShiftsAt + 2 * kShiftsBytes;  // [4 units][32 query rows] float
+constexpr int kRefsBytes = kUnits * kRows * 4;
+constexpr int kGoneAt = kRefsAt + 2 * kRefsBytes;  // [4 units]: bits of rows that are left out
+constexpr int kMovedAt = kGoneAt + 2 * 16;         // [4], by round
+constexpr int kSumsAt = kMovedAt + 16;              // [4 units][32 query rows] of l, r
+constexpr int kLdsBytes = kSumsAt + kUnits * kRows * 8;
+static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr float kHeadroom = 16.0f;
+constexpr float kRounded = 0x1p-100f;  // the rounded weights' sums: times 2^127 and this
+
+typedef __attribute__((address_space(4))) int32_t const_i32;  // scalar loads
 
 struct TreeArgs {
   const uint16_t* q;
+  int batch;
   int nodes, heads;
   int q_rows;  // nodes * heads
   int tiles;   // of 32 of them
@@ -114,20 +130,35 @@ __device__ __forceinline__ float over_groups(float x, bool is_max) {
   return is_max ? fmaxf(u2f(b[0]), u2f(b[1])) : u2f(b[0]) + u2f(b[1]);
 }
 
+// Copies memory -> LDS of 16 or 4 bytes a lane, from base + offset to lds + 16 or 4 lane. As
+// assembly, because the compiler orders the builtin's writes to LDS by waits of its own: it
+// waited for all copies in flight before each transposed read and at each barrier (16 x 16
+// nodes 316 us with the builtin, 292 so, both then). wait_copies() and the barriers order them here.
+__device__ __forceinline__ void copy_ahead16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(offset), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void copy_ahead4(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+               :
+               : "v"(offset), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
+
+// What both roles know.
 struct Tree {
   const TreeArgs& a;
   const uint32_t lds;
   int lane, row, group;
   const int wave, b;
-  // the request
+  // the request: its rows of the block tables, and the pools (the compressed records first)
+  const const_i32* table[2];
+  const uint8_t* pool[2];
+  int pages[2];
   int held, past, first, past_units, units;
-  // by half of the query rows, lane % 16: what the row's node sees, and its softmax
-  bool live[2];
-  int lowest[2];  // committed position
-  uint32_t path[2][2];
-  float m[2], l[2], r[2];
-  u32x4 q[2][16];
-  f32x4 o[2][4];  // coordinates 64 wave + 16 u + 4 group + i
+  int begin, end;                            // the workgroup's units
 
   __device__ __forceinline__ Tree(const TreeArgs& args, uint32_t at, int request)
       : a(args),
@@ -138,6 +169,38 @@ struct Tree {
         wave(uniform((int)(threadIdx.x >> 6))),
         b(request) {}
 
+  __device__ __forceinline__ void request(int split) {
+    held = max(min(((const const_i32*)a.lengths)[b], 0x7fffff00), 0);
+    past = 0;
+    if (a.past_lengths)
+      past = max(min(((const const_i32*)a.past_lengths)[b], a.past_blocks * kPageRecords), 0);
+    first = max(held - a.window + 1, 0) & ~(kUnit - 1);
+    const int stop = (int)min((int64_t)held + a.nodes, (int64_t)a.blocks * kPageRecords);
+    past_units = (past + kUnit - 1) / kUnit;
+    units = past_units + max((stop - first + kUnit - 1) / kUnit, 0);
+    const int share = ((units + a.splits - 1) / a.splits + kUnits - 1) / kUnits * kUnits;
+    begin = min(split * share, units);
+    end = min(begin + share, units);
+    table[0] = (const const_i32*)a.past_table + b * a.past_stride;
+    table[1] = (const const_i32*)a.table + b * a.table_stride;
+    pool[0] = a.past;
+    pool[1] = a.pool;
+    pages[0] = a.past_pages;
+    pages[1] = a.pool_pages;
+    // (kept in registers: chosen between in memory, each unit would wait for them again)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      asm volatile("" : "+s"(table[k]));
+      asm volatile("" : "+s"(pool[k]));
+      asm volatile("" : "+s"(pages[k]));
+    }
+  }
+  // Number of the page that unit i of the request lies in.
+  __device__ __forceinline__ int page_of(int i) const {
+    const bool of_past = i < past_units;
+    const int at = of_past ? i * kUnit : first + (i - past_units) * kUnit;
+    return (of_past ? table[0] : table[1])[(uint32_t)at / kPageRecords];
+  }
   // What follows from the lane is worked out again in each round: kept, it would push Q out
   // of the registers.
   __device__ __forceinline__ void again() {
@@ -145,6 +208,46 @@ struct Tree {
     row = lane & 15;
     group = lane >> 4;
   }
+  struct Unit {
+    const uint8_t* page;
+    int at;       // its first record or position
+    int in_page;  // row there
+    bool past, mapped;
+  };
+  __device__ __forceinline__ Unit unit(int i, int page) const {
+    Unit x;
+    x.past = i < past_units;
+    x.at = x.past ? i * kUnit : first + (i - past_units) * kUnit;
+    x.mapped = (uint32_t)page < (uint32_t)(x.past ? pages[0] : pages[1]);
+    x.page = (x.past ? pool[0] : pool[1]) + (uint64_t)(x.mapped ? page : 0) * kNativePageBytes;
+    x.in_page = x.at & (kPageRecords - 1);
+    return x;
+  }
+  // Piece j of row r goes to place j ^ turn(r) of the row, within its four.
+  __device__ __forceinline__ static int turn(int r) { return (r >> 1) & 3; }
+  __device__ __forceinline__ uint32_t buffer(int round) const {
+    return lds + (round & (kBuffers - 1)) * kRoundBytes;
+  }
+  __device__ __forceinline__ float ref(int round, int unit, int c) const {
+    return lds_read<float>(lds + kRefsAt + (round & 1) * kRefsBytes +
+                           4 * (kRows * unit + 16 * c + row));
+  }
+  __device__ __forceinline__ bool moved(int round) const {
+    return uniform(lds_read<int>(lds + kMovedAt + 4 * (round & 3))) != 0;
+  }
+};
+
+// Unit `wave` of every round. By half c of the query rows, 16 c + lane % 16: what the row's
+// node sees, and its softmax.
+struct Scorer : Tree {
+  const int of;
+  bool live[2];
+  int lowest[2];  // committed position
+  uint32_t path[2][2];
+  float m[2], l[2], r[2];
+  u32x4 q[2][16];
+
+  __device__ __forceinline__ Scorer(const Tree& t) : Tree(t), of(wave) {}
 
   // Coordinates 64 s + 16 group .. + 15 as two operands, then the tail's 32 t + 8 group.
   __device__ __forceinline__ void load_q(int first_row) {
@@ -163,25 +266,11 @@ struct Tree {
     }
   }
 
-  __device__ __forceinline__ void request() {
-    held = max(min(a.lengths[b], 0x7fffff00), 0);
-    past = 0;
-    if (a.past_lengths) past = max(min(a.past_lengths[b], a.past_blocks * kPageRecords), 0);
-    first = max(held - a.window + 1, 0) & ~(kUnit - 1);
-    const int end = (int)min((int64_t)held + a.nodes, (int64_t)a.blocks * kPageRecords);
-    past_units = (past + kUnit - 1) / kUnit;
-    units = past_units + max((end - first + kUnit - 1) / kUnit, 0);
-  }
-
-  // Lane j works out node j's path; each lane then takes its query rows' nodes.
-  __device__ __forceinline__ void tree(int first_row) {
-    int up = -1;
-    bool bad = lane >= a.nodes;
-    if (!bad) {
-      const int p = a.parents[(int64_t)b * a.nodes + lane];
-      bad = p < -1 || p >= lane;
-      up = bad ? -1 : p;
-    }
+  // Lane j works out node j's path (parent: of node lane); each lane then takes its query
+  // row's node.
+  __device__ __forceinline__ void tree(int first_row, int parent) {
+    bool bad = lane >= a.nodes || parent < -1 || parent >= lane;
+    int up = bad ? -1 : parent;
     uint64_t seen = 1ull << lane;
     // twice as many steps up each time
 #pragma unroll
@@ -211,62 +300,44 @@ struct Tree {
     }
   }
 
-  // Number of the page that unit i of the request lies in.
-  __device__ __forceinline__ int page_of(int i) const {
-    const bool of_past = i < past_units;
-    const int at = of_past ? i * kUnit : first + (i - past_units) * kUnit;
-    return of_past ? a.past_table[b * a.past_stride + at / kPageRecords]
-                   : a.table[b * a.table_stride + at / kPageRecords];
-  }
-  struct Unit {
-    const uint8_t* rows;  // of the page: the unit's data
-    int at;               // its first record or position
-    bool past, mapped;
-    u32x2 scales;  // of row lane % 16
-  };
-  __device__ __forceinline__ Unit unit(int i, int page) const {
-    Unit x;
-    x.past = i < past_units;
-    x.at = x.past ? i * kUnit : first + (i - past_units) * kUnit;
-    page = uniform(page);
-    x.mapped = page >= 0 && page < (x.past ? a.past_pages : a.pool_pages);
-    const uint8_t* const from =
-        (x.past ? a.past : a.pool) + (int64_t)(x.mapped ? page : 0) * kNativePageBytes;
-    const int at = x.at & (kPageRecords - 1);
-    x.rows = from + at * kNativeDataBytes;
-    x.scales = *(const u32x2*)(from + kPageRecords * kNativeDataBytes + (at + row) * kScaleBytes);
-    return x;
-  }
   // Whether every live query row sees all of the unit.
   __device__ __forceinline__ bool whole(const Unit& x) const {
-    return x.mapped && (x.past ? x.at + kUnit <= past
-                               : x.at + kUnit <= held && x.at >= held + a.nodes - a.window);
+    return x.mapped & (x.at + kUnit <= (x.past ? past : held)) &
+           (x.past | (x.at >= held + a.nodes - a.window));
   }
-  // Piece j of row r goes to place j ^ turn(r) of the row, within its four.
-  __device__ __forceinline__ static int turn(int r) { return (r >> 1) & 3; }
-  __device__ __forceinline__ void copy(const Unit& x, uint32_t to) const {
-#pragma unroll
-    for (int n = 0; n < kCopies; ++n) {
-      const uint32_t p = 64 * n + lane, r = p / 36, j = p - 36 * r;
-      copy16(x.rows + (576 * r + 16 * (j ^ turn(r))), to + 1024 * n);
-    }
+  __device__ __forceinline__ uint32_t weights_at(int round, int c) const {
+    return lds + kWeightsAt + (round & 1) * kWeightsBytes + 2048 * (of >> 1) + 1024 * c +
+           16 * lane + 8 * (of & 1);
   }
 
-  // Where the lane leaves the weights of the wave's unit.
-  __device__ __forceinline__ uint32_t weights_at(int c) const {
-    return lds + kWeightsAt + 2048 * (wave >> 1) + 1024 * c + 16 * lane + 8 * (wave & 1);
+  __device__ __forceinline__ uint32_t gone_at(int round) const {
+    return lds + kGoneAt + 16 * (round & 1) + 4 * of;
   }
-  // Scores and weights of the unit, in LDS at `at`.
+
+  // The unit of a round: weights to LDS, their sums to l and r, m to the references that they
+  // were taken against.
+  struct Rows {
+    u32x2 bytes;   // scales of the row
+    u32x4 key[9];  // its pieces 4 s + group, as the first product takes them
+  };
+  __device__ __forceinline__ Rows rows(int round) const {
+    Rows x;
+    const uint32_t at = buffer(round);
+    x.bytes = lds_read<u32x2>(at + kScalesAt + kScaleBytes * (kUnit * of + row));
+    const uint32_t k_at = at + kUnitBytes * of + kNativeDataBytes * row + 16 * (group ^ turn(row));
+#pragma unroll
+    for (int s = 0; s < 9; ++s) x.key[s] = lds_read<u32x4>(k_at + 64 * s);
+    return x;
+  }
   template <bool kWhole>
-  __device__ __forceinline__ void score(const Unit& x, uint32_t at, float (&own)[2], float (&sum)[2],
-                                        float (&rsum)[2]) {
-    u32x2 bytes = x.scales;
+  __device__ __forceinline__ void score(const Unit& x, int round, const Rows& in) {
+    const u32x2 bytes = in.bytes;
     // rows of the unit that count
     const int stop = min(x.past ? past - x.at : held + a.nodes - x.at, kUnit);
-    uint32_t odd = 0;  // rows with an infinity or NaN
+    uint32_t odd = 0, gone = 0;  // rows with an infinity or NaN, and with those nobody sees
     if (!kWhole) {
       // row `row`, pieces 9 group .. + 8: an infinity or NaN in it?
-      const uint32_t mine = at + kNativeDataBytes * row + 144 * group;
+      const uint32_t mine = buffer(round) + kUnitBytes * of + kNativeDataBytes * row + 144 * group;
       uint32_t bad = 0;
 #pragma unroll
       for (int n = 0; n < 9; ++n) {
@@ -275,33 +346,28 @@ struct Tree {
         const bool tail = 9 * group + n >= 28;
 #pragma unroll
         for (int k = 0; k < 4; ++k) bad |= special(v[k], tail);
+        if (n % 3 == 2) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int g = 0; g < 7; ++g)
         bad |= ((bytes[g / 4] >> (8 * (g % 4))) & 0xffu) == 0xffu;
       const uint64_t found = __ballot(bad != 0);
       odd = (uint32_t)(found | found >> 16 | found >> 32 | found >> 48) & 0xffffu;
-      if (!x.mapped || row >= stop || ((odd >> row) & 1u)) {
-#pragma unroll
-        for (int n = 0; n < 9; ++n) lds_write(mine + 16 * n, u32x4{0, 0, 0, 0});
-        bytes = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
-      }
+      gone = x.mapped ? odd | (0xffffu << stop & 0xffffu) : 0xffffu;
     }
-    // shifts of row `row` for groups 2 group and 2 group + 1
-    {
+    {  // shifts of row `row` for groups 2 group and 2 group + 1
       const uint32_t two = (group >= 2 ? bytes[1] : bytes[0]) >> (16 * (group & 1));
-      const uint32_t to = lds + kShiftsAt + 512 * (wave >> 1) + 128 * group + 16 * (row >> 2) +
-                          2 * (4 * (wave & 1) + (row & 3));
+      const uint32_t to = lds + kShiftsAt + (round & 1) * kShiftsBytes + 512 * (of >> 1) +
+                          128 * group + 16 * (row >> 2) + 2 * (4 * (of & 1) + (row & 3));
       lds_write<uint16_t>(to, (uint16_t)((254u - (two & 0xffu)) << 7));
       lds_write<uint16_t>(to + 64, (uint16_t)((254u - ((two >> 8) & 0xffu)) << 7));
+      if (lane == 0) lds_write(gone_at(round), gone);
     }
-    if (!kWhole) wave_lds_sync();
     f32x4 acc[2][2] = {};
-    const uint32_t k_at = at + kNativeDataBytes * row + 16 * (group ^ turn(row));
 #pragma unroll
     for (int s = 0; s < 7; ++s) {
       const float f = u2f(((bytes[s / 4] >> (8 * (s % 4))) & 0xffu) << 23);
-      const u32x4 v = lds_read<u32x4>(k_at + 64 * s);
+      const u32x4 v = in.key[s];
       const bf16x8 k0 = codes8(v[0], v[1], f), k1 = codes8(v[2], v[3], f);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -313,7 +379,7 @@ struct Tree {
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const bf16x8 k = as_bf16x8(lds_read<u32x4>(k_at + kNopeDim + 64 * t));
+      const bf16x8 k = as_bf16x8(in.key[7 + t]);
 #pragma unroll
       for (int c = 0; c < 2; ++c)
         acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, as_bf16x8(q[c][14 + t]), acc[c][t],
@@ -336,194 +402,324 @@ struct Tree {
         }
       }
       const float top = over_groups(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), true);
-      own[c] = top > m[c] ? ceilf(top) + kHeadroom : m[c];
-      const float ref = own[c] == -INFINITY ? 0.0f : own[c];
+      if (__ballot(top > m[c]) != 0) advance(c, top > m[c] ? ceilf(top) + kHeadroom : m[c]);
+      const float ref = m[c] == -INFINITY ? 0.0f : m[c];
       f32x4 p;
-      sum[c] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
-        sum[c] += p[i];
-        p[i] *= 0x1p127f;
-      }
-      const u32x2 d = {__builtin_bit_cast(uint32_t, bf16_pair(p[0], p[1])),
-                       __builtin_bit_cast(uint32_t, bf16_pair(p[2], p[3]))};
-      rsum[c] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        rsum[c] = __builtin_fmaf(i & 1 ? u2f(d[i / 2] & 0xffff0000u) : u2f(d[i / 2] << 16),
-                                 0x1p-127f, rsum[c]);
-      lds_write(weights_at(c), d);
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+      l[c] += (p[0] + p[1]) + (p[2] + p[3]);
+      p *= 0x1p127f;
+      const bf16x2 lo = bf16_pair(p[0], p[1]), hi = bf16_pair(p[2], p[3]), one = {(__bf16)kRounded,
+                                                                                  (__bf16)kRounded};
+      r[c] = __builtin_amdgcn_fdot2_f32_bf16(lo, one, r[c], false);
+      r[c] = __builtin_amdgcn_fdot2_f32_bf16(hi, one, r[c], false);
+      const u32x2 d = {__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+      lds_write(weights_at(round, c), d);
     }
   }
-
-  // O += the round's units, at `at`.
-  __device__ __forceinline__ void add(uint32_t at) {
-    const bool tail = wave == kWaves - 1;  // the BF16 coordinates
-    const int pair = row >> 1;  // transposed reads: row 4 group + pair % 4 of unit pair / 4
-    const int of = 4 * group + (pair & 3);
-    const uint32_t v_at = at + kUnitBytes * (pair >> 2) + kNativeDataBytes * of + 64 * wave +
-                          8 * (row & 1);
-    const int tail_of = 4 * group + (row >> 2);
-    const uint32_t t_at = at + kNativeDataBytes * tail_of + kNopeDim + 8 * (row & 1);
-#pragma unroll
-    for (int v = 0; v < kWaves / 2; ++v) {
-      u32x4 p[2], shift = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
-      bf16x8 x[4];
-      if (!tail) {
-        shift = lds_read<u32x4>(lds + kShiftsAt + 512 * v + 64 * wave + 16 * group);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const i32x2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)(
-              uintptr_t)(v_at + 16 * (u ^ turn(of)) + 2 * kUnitBytes * v));
-          x[u] = codes8((uint32_t)codes[0], (uint32_t)codes[1], 1.0f);
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          u32x2 part[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k)  // pieces 28 + 2 u and + 1
-            part[k] = __builtin_bit_cast(
-                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)(uintptr_t)(
-                           t_at + kUnitBytes * (2 * v + k) + 64 * (u >> 1) +
-                           16 * ((2 * (u & 1) + ((row & 3) >> 1)) ^ turn(tail_of)))));
-          x[u] = as_bf16x8(u32x4{part[0][0], part[0][1], part[1][0], part[1][1]});
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        p[c] = lds_read<u32x4>(lds + kWeightsAt + 2048 * v + 1024 * c + 16 * lane);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) p[c][k] = sub_sat(p[c][k], shift[k]);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          o[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], as_bf16x8(p[c]), o[c][u], 0, 0, 0);
-    }
+  // The sums go on against `to`. (Equal references may both be infinite.)
+  __device__ __forceinline__ void advance(int c, float to) {
+    const float f = m[c] == to ? 1.0f : __builtin_amdgcn_exp2f(m[c] - to);
+    l[c] *= f;
+    r[c] *= f;
+    m[c] = to;
   }
-
-  // Units [begin, end).
-  __device__ __forceinline__ void run(int begin, int end) {
+  // The highest reference of a round's units.
+  __device__ __forceinline__ void agree(int round) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[c] = -INFINITY;
-      l[c] = r[c] = 0.0f;
+      float top = m[c];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) o[c][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    if (threadIdx.x == 0) lds_write(lds + kMovedAt, u32x2{0, 0});
-    Unit x{}, next{};
-    int page = 0;
-    if (begin + wave < end) {
-      x = unit(begin + wave, page_of(begin + wave));
-      copy(x, lds + wave * kUnitBytes);
-    }
-    if (begin + kWaves + wave < end) page = page_of(begin + kWaves + wave);
-    int odd = 0;  // round
-    for (int i = begin + wave; i - wave < end; i += kWaves, odd ^= 1) {
-      const uint32_t at = lds + odd * kWaves * kUnitBytes;
-      again();
-      wait_copies<0>();
-      lds_barrier();
-      if (i + kWaves < end) {
-        next = unit(i + kWaves, page);
-        copy(next, lds + (odd ^ 1) * kWaves * kUnitBytes + wave * kUnitBytes);
-        if (i + 2 * kWaves < end) page = page_of(i + 2 * kWaves);
-      }
-      float own[2] = {m[0], m[1]}, sum[2] = {0.f, 0.f}, rsum[2] = {0.f, 0.f};
-      const uint32_t mine = at + wave * kUnitBytes;
-      if (i < end) {
-        if (whole(x))
-          score<true>(x, mine, own, sum, rsum);
-        else
-          score<false>(x, mine, own, sum, rsum);
-      } else {  // the round's last units: nothing
-#pragma unroll
-        for (int n = 0; n < kCopies; ++n) lds_write(mine + 1024 * n + 16 * lane, u32x4{0, 0, 0, 0});
-#pragma unroll
-        for (int c = 0; c < 2; ++c) lds_write(weights_at(c), u32x2{0, 0});
-      }
-      if (lane < kUnit) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          lds_write(lds + kRefsAt + 4 * (kRows * wave + 16 * c + row), own[c]);
-      }
-      if (__ballot(own[0] != m[0] || own[1] != m[1]) != 0 && lane == 0)
-        lds_write(lds + kMovedAt + 4 * odd, 1);
-      if (threadIdx.x == 0) lds_write(lds + kMovedAt + 4 * (odd ^ 1), 0);
-      lds_barrier();
-      if (uniform(lds_read<int>(lds + kMovedAt + 4 * odd)) != 0) {
-        // the highest reference is everyone's: O, the sums and the unit's weights go down to it
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float top = m[c];
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w)
-            top = fmaxf(top, lds_read<float>(lds + kRefsAt + 4 * (kRows * w + 16 * c + row)));
-          // (equal ones may both be infinite)
-          const float f = m[c] == top ? 1.0f : __builtin_amdgcn_exp2f(m[c] - top);
-          const float g = own[c] == top ? 1.0f : __builtin_amdgcn_exp2f(own[c] - top);
-          m[c] = top;
-          l[c] *= f;
-          r[c] *= f;
-          sum[c] *= g;
-          rsum[c] *= g;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) o[c][u] *= f;
-          // whole log2 units, in both exponents; 255: past every exponent, also for a
-          // difference that is NaN (infinities: the sum is NaN then)
-          const uint32_t down = __umul24((uint32_t)fminf(top - own[c], 255.0f), 0x00800080u);
-          const u32x2 p = lds_read<u32x2>(weights_at(c));
-          lds_write(weights_at(c), u32x2{sub_sat(p[0], down), sub_sat(p[1], down)});
-        }
-        lds_barrier();
-      }
-      again();
-#pragma unroll
-      for (int c = 0; c < 2; ++c) l[c] += sum[c], r[c] += rsum[c];
-      add(at);
-      x = next;
+      for (int u = 0; u < kUnits; ++u) top = fmaxf(top, ref(round, u, c));
+      advance(c, top);
     }
   }
 
-  __device__ __forceinline__ void finish(int first_row, int split) {
-    lds_barrier();
+  __device__ __forceinline__ void run(int first_row) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) m[c] = -INFINITY, l[c] = r[c] = 0.0f;
+    int parent = -2;
+    if (lane < a.nodes) parent = a.parents[(int64_t)b * a.nodes + lane];
+    int page = 0;
+    if (begin + of < end) page = page_of(begin + of);
+    load_q(first_row);
+    tree(first_row, parent);
+    lds_barrier();  // round 0's rows
+    int round = 0;
+#pragma clang loop unroll(disable)
+    for (int from = begin; from < end; from += kUnits, ++round) {
+      const int i = uniform(from + of);
+      again();
+      const Rows in = rows(round);
+      if (round > 0 && moved(round - 1)) agree(round - 1);
+      const Unit x = unit(min(i, units - 1), page);
+      if (i + kUnits < end) page = page_of(i + kUnits);
+      const float was[2] = {m[0], m[1]};
+      if (i < end) {
+        if (whole(x))
+          score<true>(x, round, in);
+        else
+          score<false>(x, round, in);
+      } else {  // the round's last units: nothing
+#pragma unroll
+        for (int c = 0; c < 2; ++c) lds_write(weights_at(round, c), u32x2{0, 0});
+        if (lane == 0) lds_write(gone_at(round), 0xffffu);
+      }
+      if (group == 0) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          lds_write(lds + kRefsAt + (round & 1) * kRefsBytes + 4 * (kRows * of + 16 * c + row),
+                    m[c]);
+      }
+      if (__ballot(m[0] != was[0] || m[1] != was[1]) != 0 && lane == 0)
+        lds_write(lds + kMovedAt + 4 * (round & 3), 1);
+      if (threadIdx.x == 0) lds_write(lds + kMovedAt + 4 * ((round + 2) & 3), 0);
+      lds_barrier();
+    }
+    if (round > 0 && moved(round - 1)) agree(round - 1);
+    // the row's sums; none of a row that sees nothing
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       l[c] = over_groups(l[c], false);
       r[c] = over_groups(r[c], false);
-      if (lane < 16) lds_write(lds + kSumsAt + 8 * (kRows * wave + 16 * c + row), f32x2{l[c], r[c]});
+      if (group == 0)
+        lds_write(lds + kSumsAt + 8 * (kRows * of + 16 * c + row),
+                  live[c] ? f32x2{l[c], r[c] * 0x1p-27f} : f32x2{0.0f, 0.0f});
     }
     lds_barrier();
+  }
+};
+
+// Coordinates 128 g .. + 127 of all query rows: two groups of 64.
+struct Adder : Tree {
+  const int g;  // and unit g's copies
+  uint32_t from[kCopies - 1];  // where the lane's piece of a copy is in the unit
+  float m[2];
+  f32x4 o[2][2][4];  // query rows 16 c + row, coordinates 128 g + 64 h + 16 u + 4 group + i
+
+  __device__ __forceinline__ Adder(const Tree& t) : Tree(t), g(wave - kScorers) {
+#pragma unroll
+    for (int n = 0; n < kCopies - 1; ++n) {
+      const uint32_t p = 64 * n + lane, r = p / 36, j = p - 36 * r;
+      from[n] = 576 * r + 16 * (j ^ turn(r));
+    }
+  }
+
+  // The rows of unit i, if there is one, in two parts: what there is to do between them can
+  // wait for LDS meanwhile.
+  template <int kPart>
+  __device__ __forceinline__ void copy(int i, int page, int round) const {
+    if (i >= end) return;
+    const uint32_t to = buffer(round) + kUnitBytes * g;
+    const Unit x = unit(i, page);
+    const uint8_t* const rows = x.page + x.in_page * kNativeDataBytes;
+    constexpr int kHalf = (kCopies - 1) / 2;
+#pragma unroll
+    for (int n = kPart * kHalf; n < (kPart ? kCopies - 1 : kHalf); ++n)
+      copy_ahead16(rows, from[n], to + 1024 * n);
+    if (kPart == 0 && lane < kUnit * kScaleBytes / 4)
+      copy_ahead4(x.page + kPageRecords * kNativeDataBytes + x.in_page * kScaleBytes, 4 * lane,
+                  buffer(round) + kScalesAt + kUnit * kScaleBytes * g);
+  }
+
+  // Eight rows of the lane's coordinate of tile u of group k, as the second product's first
+  // operand: of units 2 v and 2 v + 1, rows 4 group .. + 3 each.
+  __device__ __forceinline__ bf16x8 codes(uint32_t at, int v, int k, int u) const {
+    const int pair = row >> 1;  // the lane reads row 4 group + pair % 4 of unit pair / 4
+    const int r = 4 * group + (pair & 3);
+    const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)(uintptr_t)(
+        at + kUnitBytes * (pair >> 2) + kNativeDataBytes * r + 128 * g + 8 * (row & 1) +
+        16 * (u ^ turn(r)) + 64 * k + 2 * kUnitBytes * v));
+    return codes8((uint32_t)x[0], (uint32_t)x[1], 1.0f);
+  }
+  __device__ __forceinline__ bf16x8 tail(uint32_t at, int v, int u) const {
+    const int r = 4 * group + (row >> 2);
+    u32x2 half[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)  // pieces 28 + 2 u and + 1
+      half[k] = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)(uintptr_t)(
+                     at + kNativeDataBytes * r + kNopeDim + 8 * (row & 1) +
+                     kUnitBytes * (2 * v + k) + 64 * (u >> 1) +
+                     16 * ((2 * (u & 1) + ((row & 3) >> 1)) ^ turn(r)))));
+    return as_bf16x8(u32x4{half[0][0], half[0][1], half[1][0], half[1][1]});
+  }
+
+  // O += a round. kPlain: its units' references are all m, and all of their rows count.
+  template <bool kPlain, class F>
+  __device__ __forceinline__ void add(int round, const u32x4& gone, F between) {
+    const uint32_t at = buffer(round);
+    const uint32_t weights = lds + kWeightsAt + (round & 1) * kWeightsBytes + 16 * lane;
+    const uint32_t shifts = lds + kShiftsAt + (round & 1) * kShiftsBytes + 128 * g + 16 * group;
+    u32x4 p[2][2], keep[2];
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) p[v][c] = lds_read<u32x4>(weights + 2048 * v + 1024 * c);
+    if (!kPlain) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float own[kUnits], top = m[c];
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          own[u] = ref(round, u, c);
+          top = fmaxf(top, own[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          // whole log2 units down, in both exponents; 255: past every exponent, also for a
+          // difference that is NaN (infinities: the row's sum is NaN then)
+          const uint32_t d = __umul24((uint32_t)fminf(top - own[u], 255.0f), 0x00800080u);
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            p[u / 2][c][2 * (u % 2) + k] = sub_sat(p[u / 2][c][2 * (u % 2) + k], d);
+        }
+        const float f = m[c] == top ? 1.0f : __builtin_amdgcn_exp2f(m[c] - top);
+        m[c] = top;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) o[c][k][u] *= f;
+      }
+      // rows 4 group .. + 3 of both units, two a dword
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t two = gone[2 * v + k / 2] >> (4 * group + 2 * (k & 1));
+          keep[v][k] = (two & 1u ? 0u : 0xffffu) | (two & 2u ? 0u : 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      u32x4 shift[2];
+      bf16x8 x[2][4];
+      if (k == 0 || g < kAdders - 1) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          shift[v] = lds_read<u32x4>(shifts + 512 * v + 64 * k);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) x[v][u] = codes(at, v, k, u);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          shift[v] = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
+#pragma unroll
+          for (int u = 0; u < 4; ++u) x[v][u] = tail(at, v, u);
+        }
+      }
+      between(k);
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        if (!kPlain) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            x[v][u] = as_bf16x8(__builtin_bit_cast(u32x4, x[v][u]) & keep[v]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          u32x4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = sub_sat(p[v][c][i], shift[v][i]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            o[c][k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[v][u], as_bf16x8(w), o[c][k][u],
+                                                                 0, 0, 0);
+        }
+      }
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void add(int round, F between) {
+    const u32x4 gone = lds_read<u32x4>(lds + kGoneAt + 16 * (round & 1));
+    const int odd = lds_read<int>(lds + kMovedAt + 4 * (round & 3));
+    if (uniform((int)(gone[0] | gone[1] | gone[2] | gone[3]) | odd) == 0)
+      add<true>(round, gone, between);
+    else
+      add<false>(round, gone, between);
+  }
+
+  __device__ __forceinline__ void run(int first_row, int split) {
+    if (threadIdx.x == 64 * kScorers) lds_write(lds + kMovedAt, u32x4{0, 0, 0, 0});
+    const int i = uniform(begin + g);
+    int page = 0;
+    if (i < end) page = page_of(i);
+    copy<0>(i, page, 0);
+    copy<1>(i, page, 0);
+    if (i + kUnits < end) page = page_of(i + kUnits);
+    copy<0>(i + kUnits, page, 1);
+    copy<1>(i + kUnits, page, 1);
+    if (i + 2 * kUnits < end) page = page_of(i + 2 * kUnits);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      m[c] = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[c][k][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    landed(i + kUnits);  // round 0
+    lds_barrier();
+    int round = 0;
+#pragma clang loop unroll(disable)
+    for (int from = begin; from < end; from += kUnits, ++round) {
+      // scored: round; added: the one before; copied: the one after next
+      const int i = uniform(from + g) + 2 * kUnits;
+      if (round > 0) {
+        add(round - 1, [&](int k) {
+          if (k == 0)
+            copy<0>(i, page, round + 2);
+          else
+            copy<1>(i, page, round + 2);
+        });
+      } else {
+        copy<0>(i, page, 2);
+        copy<1>(i, page, 2);
+      }
+      if (i + kUnits < end) page = page_of(i + kUnits);
+      landed(i);
+      lds_barrier();
+    }
+    if (round > 0) add(round - 1, [](int) {});
+    lds_barrier();
+    finish(first_row, split);
+  }
+
+  // Until the copies before those of unit `last`, the latest, have landed.
+  __device__ __forceinline__ void landed(int last) const {
+    if (last < end)
+      wait_copies<kCopies>();
+    else
+      wait_copies<0>();
+  }
+
+  __device__ __forceinline__ void finish(int first_row, int split) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float sum = 0.0f, rsum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const f32x2 of = lds_read<f32x2>(lds + kSumsAt + 8 * (kRows * w + 16 * c + row));
-        sum += of[0];
-        rsum += of[1];
+      for (int u = 0; u < kUnits; ++u) {
+        const f32x2 part = lds_read<f32x2>(lds + kSumsAt + 8 * (kRows * u + 16 * c + row));
+        sum += part[0];
+        rsum += part[1];
       }
       const int at = first_row + 16 * c + row;
       if (at >= a.q_rows) continue;
-      if (!live[c]) sum = 0.0f;
       const int node = at / a.heads, h = at - node * a.heads;
       const int64_t token = (int64_t)b * a.nodes + node;
-      const int c0 = 64 * wave + 4 * group;
+      const int c0 = 128 * g + 4 * group;
       if (a.ws_o) {
         const int64_t to = (token * a.splits + split) * a.heads + h;
         const float f = sum != 0.0f ? 1.0f / rsum : 0.0f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          f32x4 x = o[c][u] * f;
+        for (int u = 0; u < 8; ++u) {
+          f32x4 x = o[c][u / 4][u % 4] * f;
           if (sum == 0.0f) x = f32x4{0.f, 0.f, 0.f, 0.f};
           __builtin_nontemporal_store(x, (f32x4*)(a.ws_o + to * kHeadDim + c0 + 16 * u));
         }
         // (NaN goes on as infinity: the combine's maximum would pass over a NaN)
-        if (wave == 0 && group == 0)
+        if (g == 0 && group == 0)
           a.ws_lse[to] = sum != sum     ? INFINITY
                          : sum != 0.0f ? m[c] + __builtin_amdgcn_logf(sum)
                                        : -INFINITY;
@@ -539,10 +735,10 @@ struct Tree {
         if (sum != 0.0f) f = sum * em / (rsum * z);
         lse = (top + __builtin_amdgcn_logf(z)) * kLn2;
       }
-      if (wave == 0 && group == 0) a.lse[token * a.heads + h] = lse;
+      if (g == 0 && group == 0) a.lse[token * a.heads + h] = lse;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        f32x4 x = o[c][u] * f;
+      for (int u = 0; u < 8; ++u) {
+        f32x4 x = o[c][u / 4][u % 4] * f;
         if (sum == 0.0f) x = f32x4{0.f, 0.f, 0.f, 0.f};
         *(u32x2*)(a.out + (token * a.heads + h) * kHeadDim + c0 + 16 * u) =
             u32x2{__builtin_bit_cast(uint32_t, bf16_pair(x[0], x[1])),
@@ -552,19 +748,22 @@ struct Tree {
   }
 };
 
-__global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * (kScorers + kAdders)) void tree_decode_kernel(TreeArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
-  const int b = (int)blockIdx.x / a.tiles;
-  const int first_row = ((int)blockIdx.x - b * a.tiles) * kRows;
-  const int split = (int)blockIdx.y;
+  // Workgroups go to the eight XCDs in turn: the tiles of one request and split, which read
+  // the same rows, go to one, so that its L2 cache serves all but the first.
+  const int at = (int)blockIdx.x >> 3;
+  const int part = at / a.tiles * 8 + ((int)blockIdx.x & 7);
+  if (part >= a.batch * a.splits) return;
+  const int b = part / a.splits, split = part - b * a.splits;
+  const int first_row = at % a.tiles * kRows;
   Tree t(a, (uint32_t)(uintptr_t)(lds_void*)lds, b);
-  t.load_q(first_row);
-  t.request();
-  t.tree(first_row);
-  const int share = ((t.units + a.splits - 1) / a.splits + kWaves - 1) / kWaves * kWaves;
-  const int begin = min(split * share, t.units);
-  t.run(begin, min(begin + share, t.units));
-  t.finish(first_row, split);
+  t.request(split);
+  if (t.wave < kScorers) {
+    Scorer(t).run(first_row);
+  } else {
+    Adder(t).run(first_row, split);
+  }
 }
 
 bool aligned(const void* p, uintptr_t al) { return ((uintptr_t)p & (al - 1)) == 0; }
@@ -635,6 +834,7 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
   if (bytes > 0 && !aligned(workspace, 16)) return RM_ERR_ALIGN;
   TreeArgs a;
   a.q = q;
+  a.batch = (int)batch;
   a.nodes = (int)nodes;
   a.heads = (int)heads;
   a.q_rows = (int)(nodes * heads);
@@ -661,8 +861,8 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
   a.ws_o = splits > 1 ? (float*)workspace : nullptr;
   a.ws_lse = splits > 1 ? (float*)workspace + (size_t)splits * rows * kHeadDim : nullptr;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(tree_decode_kernel, dim3((unsigned)(batch * a.tiles), (unsigned)splits),
-                     dim3(64 * kWaves), 0, s, a);
+  hipLaunchKernelGGL(tree_decode_kernel, dim3((unsigned)((batch * splits + 7) / 8 * 8 * a.tiles)),
+                     dim3(64 * (kScorers + kAdders)), 0, s, a);
   if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   if (splits > 1) {
     launch_combine<true>(a.ws_o, a.ws_lse, sink, splits, batch * nodes, heads, out, lse, s);
