@@ -38,30 +38,37 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 template <int kThreads>
 struct Shared {
   static constexpr int kWaves = kThreads / 64;
-  uint32_t bins[kBins];
-  uint32_t part[2 * kWaves];
+  uint32_t bins[kBins];  // later the numbers, where they fit
+  alignas(16) uint32_t part[5][kWaves];
   uint32_t pick[4];
+  uint32_t list[64];
 };
 
-__device__ __forceinline__ uint32_t wave_min(uint32_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x = min(x, (uint32_t)__shfl_xor((int)x, d, 64));
-  return x;
+// Inclusive sum over the wave's lanes up to and with this one (shifts within each row of 16,
+// then the last lanes of rows 0 and 2 to the next row, of row 1 to the upper half).
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ uint32_t plus_dpp(uint32_t x) {
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, kRowMask, 0xf, false);
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x = max(x, (uint32_t)__shfl_xor((int)x, d, 64));
-  return x;
-}
-// Inclusive sum over the wave's lanes up to and with this one.
 __device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
-  const int lane = wave_lane();
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t y = (uint32_t)__shfl_up((int)x, d, 64);
-    if (lane >= d) x += y;
-  }
-  return x;
+  x = plus_dpp<0x111, 0xf>(x);
+  x = plus_dpp<0x112, 0xf>(x);
+  x = plus_dpp<0x114, 0xf>(x);
+  x = plus_dpp<0x118, 0xf>(x);
+  x = plus_dpp<0x142, 0xa>(x);
+  return plus_dpp<0x143, 0xc>(x);
+}
+// Over the wave's lanes.
+template <class F>
+__device__ __forceinline__ uint32_t wave_all_of(uint32_t x, F op) {
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, false));
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, false));
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, false));
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, false));
+  const auto h = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = op(h[0], h[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return op(q[0], q[1]);
 }
 __device__ __forceinline__ int below(uint64_t mask) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
@@ -87,21 +94,25 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
   }
   if (count == 0) return;
   const float* const from = a.scores + row * a.stride;
-  const int turns = (length + 4 * kThreads - 1) / (4 * kThreads);
+  // a wave's scores stand together, 256 a turn, so that only totals of waves meet; shares
+  // differ by less than four scores, so that no thread goes without where others have two turns
+  const int share = ((length + 4 * S::kWaves - 1) / (4 * S::kWaves)) * 4;
+  const int begin = min(wave * share, length), end = min(begin + share, length);
+  const int turns = (share + 255) / 256;
   auto load = [&](int turn, uint32_t (&key)[4]) {
-    const int at = 4 * (turn * kThreads + tid);
+    const int at = begin + 256 * turn + 4 * lane;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.wide && at + 3 < length) {
+    if (a.wide && at + 3 < end) {
       const f32x4 v = *(const f32x4*)(from + at);
 #pragma unroll
       for (int c = 0; c < 4; ++c) x[c] = v[c];
     } else {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        if (at + c < length) x[c] = from[at + c];
+        if (at + c < end) x[c] = from[at + c];
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) key[c] = at + c < length ? key_of(x[c]) : 0u;
+    for (int c = 0; c < 4; ++c) key[c] = at + c < end ? key_of(x[c]) : 0u;
   };
   uint32_t held[kHeld > 0 ? kHeld : 1][4];
   // f(turn, keys) for every turn of the row
@@ -123,23 +134,33 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     for (int i = 0; i < kHeld; ++i)
       if (i < turns) load(i, held[i]);
   }
-  // the range of all keys
-  uint32_t lo = 0xffffffffu, hi = 0;
+  // The range: from the row's lowest key, or the lowest of the threads' highest keys (the
+  // second highest, for more than a key a thread), which enough keys reach, to its highest.
+  uint32_t lo = 0xffffffffu, hi = 0, second = 0;
   each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
+      second = max(second, min(hi, key[c]));
       hi = max(hi, key[c]);
       lo = min(lo, key[c] != 0 ? key[c] : 0xffffffffu);
     }
   });
-  lo = wave_min(lo);
-  hi = wave_max(hi);
-  if (lane == 0) s.part[wave] = lo, s.part[S::kWaves + wave] = hi;
-  __syncthreads();
+  {
+    const auto least = [](uint32_t x, uint32_t y) { return min(x, y); };
+    const auto most = [](uint32_t x, uint32_t y) { return max(x, y); };
+    uint32_t reach = count <= kThreads ? hi : count <= 2 * kThreads ? second : 0;
+    reach = wave_all_of(reach, least);
+    lo = wave_all_of(lo, least);
+    hi = wave_all_of(hi, most);
+    if (lane == 0) s.part[0][wave] = lo, s.part[1][wave] = hi, s.part[2][wave] = reach;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < S::kWaves; ++w) {
-    lo = min(lo, s.part[w]);
-    hi = max(hi, s.part[S::kWaves + w]);
+    for (int w = 0; w < S::kWaves; ++w) {
+      lo = min(lo, s.part[0][w]);
+      hi = max(hi, s.part[1][w]);
+      reach = min(reach, s.part[2][w]);
+    }
+    lo = max(lo, reach);
   }
   // need: how many of [lo, hi] are taken; those above hi are taken whole
   uint32_t need = (uint32_t)count;
@@ -148,6 +169,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     const int bits = 32 - __builtin_clz(hi - lo);
     const int shift = max(bits - 11, 0);
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+    if (tid == 0) s.pick[3] = 0;
     __syncthreads();
     each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
@@ -164,10 +186,11 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       sum += mine[i];
     }
     const uint32_t upto = wave_prefix(sum);
-    if (lane == 63) s.part[wave] = upto;
+    if (lane == 63) s.part[0][wave] = upto;
     __syncthreads();
     uint32_t before = upto - sum;
-    for (int w = 0; w < wave; ++w) before += s.part[w];
+#pragma unroll
+    for (int w = 0; w < S::kWaves; ++w) before += w < wave ? s.part[0][w] : 0u;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if (before < need && before + mine[i] >= need) {
@@ -182,48 +205,78 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     need -= s.pick[1];
     lo += bin << shift;
     hi = min(hi, lo + ((1u << shift) - 1));
-    if (held_in == need) break;  // the bin is taken whole
-    __syncthreads();             // (bins and pick are written again)
+    if (held_in == need || lo == hi) break;  // the bin is taken whole, or is one key
+    if (held_in <= 64) {  // a lane each: every wave ranks them
+      each([&](int, const uint32_t (&key)[4]) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (key[c] >= lo && key[c] <= hi) s.list[atomicAdd(&s.pick[3], 1u)] = key[c];
+      });
+      __syncthreads();
+      const uint32_t key = lane < (int)held_in ? s.list[lane] : 0u;
+      uint32_t over = 0, same = 0;
+      for (int i = 0; i < (int)held_in; ++i) {
+        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+        over += other > key;
+        same += other == key;
+      }
+      const uint64_t last = __ballot(over < need && over + same >= need);
+      const int at = __builtin_ctzll(last);
+      lo = hi = (uint32_t)__builtin_amdgcn_readlane((int)key, at);
+      need -= (uint32_t)__builtin_amdgcn_readlane((int)over, at);
+      break;
+    }
+    __syncthreads();  // (bins and pick are written again)
   }
   // Taken: keys above hi, and of [lo, hi] the first `need`. (A range that is taken whole
   // has just as many; else it is one key.)
-  __syncthreads();
-  uint32_t above = 0, ties = 0;  // of the turns before
-  each([&](int turn, const uint32_t (&key)[4]) {
-    uint64_t over[4], same[4];
+  uint32_t above = 0, ties = 0;  // of the waves before
+  {
     uint32_t n_over = 0, n_same = 0;
+    each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      over[c] = __ballot(key[c] > hi);
-      same[c] = __ballot(key[c] >= lo && key[c] <= hi);
-      n_over += __popcll(over[c]);
-      n_same += __popcll(same[c]);
-    }
-    uint32_t* const part = s.bins + (turn & 1) * 2 * S::kWaves;
-    if (lane == 0) part[2 * wave] = n_over, part[2 * wave + 1] = n_same;
+      for (int c = 0; c < 4; ++c) {
+        n_over += __popcll(__ballot(key[c] > hi));
+        n_same += __popcll(__ballot(key[c] >= lo && key[c] <= hi));
+      }
+    });
+    if (lane == 0) s.part[3][wave] = n_over, s.part[4][wave] = n_same;
     __syncthreads();
-    uint32_t a0 = above, t0 = ties;
 #pragma unroll
     for (int w = 0; w < S::kWaves; ++w) {
-      const uint32_t o = part[2 * w], e = part[2 * w + 1];
-      if (w < wave) a0 += o, t0 += e;
-      above += o;
-      ties += e;
+      above += w < wave ? s.part[3][w] : 0u;
+      ties += w < wave ? s.part[4][w] : 0u;
     }
+  }
+  auto number = [&](auto put) {
+    each([&](int turn, const uint32_t (&key)[4]) {
+      uint32_t a0 = above, t0 = ties;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      a0 += below(over[c]);
-      t0 += below(same[c]);
-    }
-    const int at = 4 * (turn * kThreads + tid);
+      for (int c = 0; c < 4; ++c) {
+        const uint64_t over = __ballot(key[c] > hi);
+        const uint64_t same = __ballot(key[c] >= lo && key[c] <= hi);
+        a0 += below(over);
+        t0 += below(same);
+        above += __popcll(over);
+        ties += __popcll(same);
+      }
+      const int at = begin + 256 * turn + 4 * lane;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const bool is_over = key[c] > hi, is_same = key[c] >= lo && key[c] <= hi;
-      if (is_over || (is_same && t0 < need)) out[a0 + min(t0, need)] = at + c;
-      a0 += is_over;
-      t0 += is_same;
-    }
-  });
+      for (int c = 0; c < 4; ++c) {
+        const bool is_over = key[c] > hi, is_same = key[c] >= lo && key[c] <= hi;
+        if (is_over || (is_same && t0 < need)) put(a0 + min(t0, need), at + c);
+        a0 += is_over;
+        t0 += is_same;
+      }
+    });
+  };
+  if (count <= kBins) {  // through LDS, to be written side by side
+    number([&](uint32_t to, int i) { s.bins[to] = (uint32_t)i; });
+    __syncthreads();
+    for (int i = tid; i < count; i += kThreads) out[i] = (int)s.bins[i];
+  } else {
+    number([&](uint32_t to, int i) { out[to] = i; });
+  }
 }
 
 bool aligned(const void* p, uintptr_t al) { return ((uintptr_t)p & (al - 1)) == 0; }

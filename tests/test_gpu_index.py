@@ -313,7 +313,7 @@ def check_topk(x, lengths, k, **kw):
     idx, counts = remnant.index_topk(x, None if lengths is None else gpu(lengths, I32), k, **kw)
     want, n = ref.topk(x.reshape(-1, x.shape[-1]).cpu().numpy(), lengths, k)
     assert np.array_equal(counts.cpu().numpy(), n)
-    assert np.array_equal(idx.reshape(-1, k).cpu().numpy(), want)
+    assert np.array_equal(idx.cpu().numpy().reshape(want.shape), want)
 
 
 WIDTHS = [1, 2, 63, 257, 1000, 2047, 2048, 2049, 8191, 8193, 20000, 32768, 32769, 100003]
