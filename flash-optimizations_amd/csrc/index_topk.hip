@@ -70,9 +70,10 @@ __device__ __forceinline__ uint32_t wave_all_of(uint32_t x, F op) {
   const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return op(q[0], q[1]);
 }
-__device__ __forceinline__ int below(uint64_t mask) {
-  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
-                                        __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+// `plus` and how many of the lanes before are in the mask.
+__device__ __forceinline__ uint32_t below(uint64_t mask, uint32_t plus) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, plus));
 }
 
 // kHeld: turns of 4 * kThreads scores that the row's keys stay in registers for; 0: a row of
@@ -99,20 +100,37 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
   const int share = ((length + 4 * S::kWaves - 1) / (4 * S::kWaves)) * 4;
   const int begin = min(wave * share, length), end = min(begin + share, length);
   const int turns = (share + 255) / 256;
-  auto load = [&](int turn, uint32_t (&key)[4]) {
+  // A turn's scores as they are (zeros where there are none), then their keys. (In two steps,
+  // so that no turn's keys wait while loads of the next are to be issued.)
+  auto load = [&](int turn, uint32_t (&x)[4]) {
     const int at = begin + 256 * turn + 4 * lane;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.wide && at + 3 < end) {
-      const f32x4 v = *(const f32x4*)(from + at);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[c] = v[c];
+    for (int c = 0; c < 4; ++c) x[c] = 0;
+    if (a.wide) {
+      if (at + 3 < end) {
+        const u32x4 v = *(const u32x4*)(from + at);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = v[c];
+      }
     } else {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        if (at + c < end) x[c] = from[at + c];
+        if (at + c < end) x[c] = f2u(from[at + c]);
+    }
+  };
+  auto keys = [&](int turn, uint32_t (&x)[4]) {
+    const int at = begin + 256 * turn + 4 * lane;
+    if (a.wide && at < end && at + 3 >= end) {  // the share's last scores
+#pragma unroll
+      for (int c = 0; c < 3; ++c)
+        if (at + c < end) x[c] = f2u(from[at + c]);
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) key[c] = at + c < end ? key_of(x[c]) : 0u;
+    for (int c = 0; c < 4; ++c) x[c] = key_of(u2f(x[c]));
+    if (begin + 256 * (turn + 1) > end) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = at + c < end ? x[c] : 0u;
+    }
   };
   uint32_t held[kHeld > 0 ? kHeld : 1][4];
   // f(turn, keys) for every turn of the row
@@ -125,6 +143,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       for (int i = 0; i < turns; ++i) {
         uint32_t key[4];
         load(i, key);
+        keys(i, key);
         f(i, key);
       }
     }
@@ -133,6 +152,9 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
       if (i < turns) load(i, held[i]);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (i < turns) keys(i, held[i]);
   }
   // The range: from the row's lowest key, or the lowest of the threads' highest keys (the
   // second highest, for more than a key a thread), which enough keys reach, to its highest.
@@ -142,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     for (int c = 0; c < 4; ++c) {
       second = max(second, min(hi, key[c]));
       hi = max(hi, key[c]);
-      lo = min(lo, key[c] != 0 ? key[c] : 0xffffffffu);
+      lo = min(lo, key[c] - 1);  // (no score: passed over)
     }
   });
   {
@@ -150,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     const auto most = [](uint32_t x, uint32_t y) { return max(x, y); };
     uint32_t reach = count <= kThreads ? hi : count <= 2 * kThreads ? second : 0;
     reach = wave_all_of(reach, least);
-    lo = wave_all_of(lo, least);
+    lo = wave_all_of(lo, least) + 1;
     hi = wave_all_of(hi, most);
     if (lane == 0) s.part[0][wave] = lo, s.part[1][wave] = hi, s.part[2][wave] = reach;
     __syncthreads();
@@ -164,6 +186,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
   }
   // need: how many of [lo, hi] are taken; those above hi are taken whole
   uint32_t need = (uint32_t)count;
+  bool whole = false;  // all of [lo, hi] are taken
   for (;;) {
     if (lo == hi) break;
     const int bits = 32 - __builtin_clz(hi - lo);
@@ -174,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        if (key[c] >= lo && key[c] <= hi) atomicAdd(&s.bins[(key[c] - lo) >> shift], 1u);
+        if (key[c] - lo <= hi - lo) atomicAdd(&s.bins[(key[c] - lo) >> shift], 1u);
     });
     __syncthreads();
     // the bin that holds the need-th from above: thread t sums bins from the top
@@ -205,12 +228,13 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     need -= s.pick[1];
     lo += bin << shift;
     hi = min(hi, lo + ((1u << shift) - 1));
-    if (held_in == need || lo == hi) break;  // the bin is taken whole, or is one key
+    whole = held_in == need;
+    if (whole || lo == hi) break;
     if (held_in <= 64) {  // a lane each: every wave ranks them
       each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          if (key[c] >= lo && key[c] <= hi) s.list[atomicAdd(&s.pick[3], 1u)] = key[c];
+          if (key[c] - lo <= hi - lo) s.list[atomicAdd(&s.pick[3], 1u)] = key[c];
       });
       __syncthreads();
       const uint32_t key = lane < (int)held_in ? s.list[lane] : 0u;
@@ -224,20 +248,22 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       const int at = __builtin_ctzll(last);
       lo = hi = (uint32_t)__builtin_amdgcn_readlane((int)key, at);
       need -= (uint32_t)__builtin_amdgcn_readlane((int)over, at);
+      whole = need == (uint32_t)__builtin_amdgcn_readlane((int)same, at);
       break;
     }
     __syncthreads();  // (bins and pick are written again)
   }
-  // Taken: keys above hi, and of [lo, hi] the first `need`. (A range that is taken whole
-  // has just as many; else it is one key.)
+  // Taken: keys from `lowest` on, and where not all of [lo, hi] are, which is one key then,
+  // the first `need` of those.
+  const uint32_t lowest = whole ? lo : hi + 1;
   uint32_t above = 0, ties = 0;  // of the waves before
   {
     uint32_t n_over = 0, n_same = 0;
     each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        n_over += __popcll(__ballot(key[c] > hi));
-        n_same += __popcll(__ballot(key[c] >= lo && key[c] <= hi));
+        n_over += __popcll(__ballot(key[c] >= lowest));
+        if (!whole) n_same += __popcll(__ballot(key[c] == lo));
       }
     });
     if (lane == 0) s.part[3][wave] = n_over, s.part[4][wave] = n_same;
@@ -250,23 +276,36 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
   }
   auto number = [&](auto put) {
     each([&](int turn, const uint32_t (&key)[4]) {
-      uint32_t a0 = above, t0 = ties;
+      const int at = begin + 256 * turn + 4 * lane;
+      uint32_t to = above;
+      uint64_t over[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const uint64_t over = __ballot(key[c] > hi);
-        const uint64_t same = __ballot(key[c] >= lo && key[c] <= hi);
-        a0 += below(over);
-        t0 += below(same);
-        above += __popcll(over);
+        over[c] = __ballot(key[c] >= lowest);
+        to = below(over[c], to);
+        above += __popcll(over[c]);
+      }
+      if (whole) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (key[c] >= lowest) put(to, at + c);
+          to += key[c] >= lowest;
+        }
+        return;
+      }
+      uint32_t tie = ties;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint64_t same = __ballot(key[c] == lo);
+        tie = below(same, tie);
         ties += __popcll(same);
       }
-      const int at = begin + 256 * turn + 4 * lane;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const bool is_over = key[c] > hi, is_same = key[c] >= lo && key[c] <= hi;
-        if (is_over || (is_same && t0 < need)) put(a0 + min(t0, need), at + c);
-        a0 += is_over;
-        t0 += is_same;
+        const bool is_over = key[c] >= lowest, is_same = key[c] == lo;
+        if (is_over || (is_same && tie < need)) put(to + min(tie, need), at + c);
+        to += is_over;
+        tie += is_same;
       }
     });
   };
