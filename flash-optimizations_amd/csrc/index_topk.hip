@@ -18,7 +18,7 @@ using namespace rm;
 namespace {
 
 constexpr int kBins = 2048;
-constexpr uint32_t kLowestKey = 0x007fffffu;  // of -inf, and of NaN; 0 is no score
+// (Keys are 0x007fffff, of -inf, and up: 0 is no score.)
 
 struct TopkArgs {
   const float* scores;
@@ -30,10 +30,12 @@ struct TopkArgs {
 };
 
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const int b = (int)f2u(x + 0.0f);  // (-0 and 0 are equal)
-  const uint32_t key = (uint32_t)(b ^ ((b >> 31) | (int)0x80000000u));
-  return x != x ? kLowestKey : key;
+  // (the sum makes -0 zero and any NaN quiet, the maximum NaN -inf)
+  const int b = (int)f2u(fmaxf(x + 0.0f, -INFINITY));
+  return (uint32_t)(b ^ ((b >> 31) | (int)0x80000000u));
 }
+__device__ __forceinline__ uint32_t least(uint32_t x, uint32_t y) { return min(x, y); }
+__device__ __forceinline__ uint32_t most(uint32_t x, uint32_t y) { return max(x, y); }
 
 template <int kThreads>
 struct Shared {
@@ -41,7 +43,7 @@ struct Shared {
   uint32_t bins[kBins];  // later the numbers, where they fit
   alignas(16) uint32_t part[5][kWaves];
   uint32_t pick[4];
-  uint32_t list[64];
+  u32x2 list[64];  // key, wave
 };
 
 // Inclusive sum over the wave's lanes up to and with this one (shifts within each row of 16,
@@ -156,37 +158,44 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     for (int i = 0; i < kHeld; ++i)
       if (i < turns) keys(i, held[i]);
   }
-  // The range: from the row's lowest key, or the lowest of the threads' highest keys (the
-  // second highest, for more than a key a thread), which enough keys reach, to its highest.
-  uint32_t lo = 0xffffffffu, hi = 0, second = 0;
+  // The range: from the lowest of the threads' highest keys (the second highest, for more
+  // than a key a thread), which enough keys reach, to the highest. Where a thread has none
+  // or more are wanted, from the row's lowest key.
+  uint32_t lo, hi = 0, second = 0;
   each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      second = max(second, min(hi, key[c]));
+      second = max(second, min(hi, key[c]));  // (hi is not below it: the middle of three)
       hi = max(hi, key[c]);
-      lo = min(lo, key[c] - 1);  // (no score: passed over)
     }
   });
-  {
-    const auto least = [](uint32_t x, uint32_t y) { return min(x, y); };
-    const auto most = [](uint32_t x, uint32_t y) { return max(x, y); };
-    uint32_t reach = count <= kThreads ? hi : count <= 2 * kThreads ? second : 0;
-    reach = wave_all_of(reach, least);
-    lo = wave_all_of(lo, least) + 1;
-    hi = wave_all_of(hi, most);
-    if (lane == 0) s.part[0][wave] = lo, s.part[1][wave] = hi, s.part[2][wave] = reach;
+  lo = wave_all_of(count <= kThreads ? hi : count <= 2 * kThreads ? second : 0u, least);
+  hi = wave_all_of(hi, most);
+  if (lane == 0) s.part[0][wave] = lo, s.part[1][wave] = hi;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < S::kWaves; ++w) {
+    lo = min(lo, s.part[0][w]);
+    hi = max(hi, s.part[1][w]);
+  }
+  if (lo == 0) {
+    lo = 0xffffffffu;
+    each([&](int, const uint32_t (&key)[4]) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) lo = min(lo, key[c] - 1);  // (no score: passed over)
+    });
+    lo = wave_all_of(lo, least);
+    if (lane == 0) s.part[2][wave] = lo;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < S::kWaves; ++w) {
-      lo = min(lo, s.part[0][w]);
-      hi = max(hi, s.part[1][w]);
-      reach = min(reach, s.part[2][w]);
-    }
-    lo = max(lo, reach);
+    for (int w = 0; w < S::kWaves; ++w) lo = min(lo, s.part[2][w]);
+    lo += 1;
   }
   // need: how many of [lo, hi] are taken; those above hi are taken whole
   uint32_t need = (uint32_t)count;
-  bool whole = false;  // all of [lo, hi] are taken
+  bool whole = false;            // all of [lo, hi] are taken
+  uint32_t above = 0, ties = 0;  // of the waves before: above hi, and in [lo, hi]
+  bool counted = false;
   for (;;) {
     if (lo == hi) break;
     const int bits = 32 - __builtin_clz(hi - lo);
@@ -228,42 +237,51 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     need -= s.pick[1];
     lo += bin << shift;
     hi = min(hi, lo + ((1u << shift) - 1));
-    whole = held_in == need;
-    if (whole || lo == hi) break;
     if (held_in <= 64) {  // a lane each: every wave ranks them
+      uint32_t n_over = 0;
       each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (key[c] - lo <= hi - lo) s.list[atomicAdd(&s.pick[3], 1u)] = key[c];
+        for (int c = 0; c < 4; ++c) {
+          n_over += __popcll(__ballot(key[c] > hi));
+          if (key[c] - lo <= hi - lo)
+            s.list[atomicAdd(&s.pick[3], 1u)] = u32x2{key[c], (uint32_t)wave};
+        }
       });
+      if (lane == 0) s.part[3][wave] = n_over;
       __syncthreads();
-      const uint32_t key = lane < (int)held_in ? s.list[lane] : 0u;
+      const u32x2 at = lane < (int)held_in ? s.list[lane] : u32x2{0u, 0xffffu};
       uint32_t over = 0, same = 0;
       for (int i = 0; i < (int)held_in; ++i) {
-        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)key, i);
-        over += other > key;
-        same += other == key;
+        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)at[0], i);
+        over += other > at[0];
+        same += other == at[0];
       }
-      const uint64_t last = __ballot(over < need && over + same >= need);
-      const int at = __builtin_ctzll(last);
-      lo = hi = (uint32_t)__builtin_amdgcn_readlane((int)key, at);
-      need -= (uint32_t)__builtin_amdgcn_readlane((int)over, at);
-      whole = need == (uint32_t)__builtin_amdgcn_readlane((int)same, at);
+      // (lanes without a key have all of the others above them)
+      const int last = __builtin_ctzll(__ballot(over < need && over + same >= need));
+      lo = hi = (uint32_t)__builtin_amdgcn_readlane((int)at[0], last);
+      need -= (uint32_t)__builtin_amdgcn_readlane((int)over, last);
+      whole = need == (uint32_t)__builtin_amdgcn_readlane((int)same, last);
+      above = __popcll(__ballot(at[0] > hi && (int)at[1] < wave));
+      ties = __popcll(__ballot(at[0] == hi && (int)at[1] < wave));
+#pragma unroll
+      for (int w = 0; w < S::kWaves; ++w) above += w < wave ? s.part[3][w] : 0u;
+      counted = true;
       break;
     }
+    whole = held_in == need;
+    if (whole || lo == hi) break;
     __syncthreads();  // (bins and pick are written again)
   }
   // Taken: keys from `lowest` on, and where not all of [lo, hi] are, which is one key then,
   // the first `need` of those.
   const uint32_t lowest = whole ? lo : hi + 1;
-  uint32_t above = 0, ties = 0;  // of the waves before
-  {
+  if (!counted) {
     uint32_t n_over = 0, n_same = 0;
     each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        n_over += __popcll(__ballot(key[c] >= lowest));
-        if (!whole) n_same += __popcll(__ballot(key[c] == lo));
+        n_over += __popcll(__ballot(key[c] > hi));
+        n_same += __popcll(__ballot(key[c] - lo <= hi - lo));
       }
     });
     if (lane == 0) s.part[3][wave] = n_over, s.part[4][wave] = n_same;
@@ -274,6 +292,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       ties += w < wave ? s.part[4][w] : 0u;
     }
   }
+  if (whole) above += ties;
   auto number = [&](auto put) {
     each([&](int turn, const uint32_t (&key)[4]) {
       const int at = begin + 256 * turn + 4 * lane;
