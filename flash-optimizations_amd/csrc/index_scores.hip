@@ -9,14 +9,21 @@
 // products as float32 does, while this card's 8-bit matrix instructions (both
 // 16x16x32 and 16x16x128, at the same and twice the rate) were 4e-5 of the result off on
 // codes of eight octaves. A wave holds its tokens' coded heads in registers as first
-// operands, 16 heads a tile, and takes its pages in turn, 16 records a tile as second
+// operands, 16 heads a tile, and takes pages in turn, 16 records a tile as second
 // operands, converted once for all of its tokens. (Which coordinate stands where in the
 // long axis is free as long as both operands agree: a lane takes coordinates 16 g .. + 15 and
 // 64 + 16 g .. + 15 of its row, two 16-byte loads of a record that together use whole
-// 64-byte pieces.) The products come out with a lane's four heads of one record beside
-// each other, so the weighted sum over heads is in the lane; the four lanes of a record
-// meet once a page, where record l of the page ends in lane l and its scale, score
-// and store are one access a wave.
+// 64-byte pieces.) A tile's registers take the next page's records as soon as they are
+// converted, so a page is in flight while one is multiplied. The products come out with a
+// lane's four heads of one record beside each other, so the weighted sum over heads is in
+// the lane; the four lanes of a record meet once a page, where record l of the page ends in
+// lane l and its scale, score and store are one access a wave.
+//
+// Bound by the matrix instructions and by memory alike from two tokens and 64 heads on
+// (128 requests of 2 tokens and 32,768 records: 145 us; 108 for the bytes at 5.1 TB/s, 115
+// for the products at 1,189 TFLOP/s, what a large product reaches), by the products alone
+// for many tokens (512 tokens, 35,840 records: 230 us, 1,310 TFLOP/s), by memory and its
+// latency for one (64 ragged requests 24 us, 17 for the bytes).
 #include <algorithm>
 
 #include "index_device.h"
@@ -27,6 +34,8 @@ using namespace rm;
 namespace {
 
 constexpr int kWaves = 4;
+
+typedef __attribute__((address_space(4))) int32_t const_i32;  // scalar loads
 
 struct ScoreArgs {
   const uint16_t* q;     // [batch, q_len, heads, 128]
@@ -42,6 +51,7 @@ struct ScoreArgs {
   float* out;  // [batch * q_len, width]
   int pages;   // of a row of out
   int groups;  // workgroups along the tokens of a request
+  int least;   // pages that a wave takes at least, if there are
 };
 
 __device__ __forceinline__ uint32_t over_groups_top(uint32_t x) {
@@ -57,126 +67,195 @@ __device__ __forceinline__ bf16x8 values_of(uint32_t lo, uint32_t hi) {
                     fp8_pair_to_bf16<false>(hi, 1.0f), fp8_pair_to_bf16<true>(hi, 1.0f)});
 }
 
+// A tile of heads as the products take it: coordinates 64 (k / 2) + 16 group + 8 (k % 2) ..
+// of head `row` in x[k], and its weight times its scale (NaN for a row with an infinity or
+// NaN, whose codes are zeros).
+struct Heads {
+  bf16x8 x[4];
+  float weight;
+};
+__device__ __forceinline__ Heads coded(const ScoreArgs& a, int64_t token, int h, int group) {
+  u32x4 x[4] = {};
+  float weight = 0.0f;
+  if (h < a.heads) {
+    const int64_t at = token * a.heads + h;
+    const u32x4* const from = (const u32x4*)(a.q + at * kIndexDim);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = from[2 * group + (k & 1) + 8 * (k >> 1)];
+    weight = a.weights[at];
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    top = top_of_pairs(top,
+                       top_of_pairs(top_of_pairs(x[k][0], x[k][1]), top_of_pairs(x[k][2], x[k][3])));
+  top = over_groups_top(max(top & 0xffffu, top >> 16));
+  const bool special = top >= 0x7f80u;
+  const float scale = exp2i(ue8m0_exponent(bf16_to_f32(top)));
+  Heads to;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t lo = index_codes(x[k][0], x[k][1], scale);
+    const uint32_t hi = index_codes(x[k][2], x[k][3], scale);
+    to.x[k] = values_of(special ? 0u : lo, special ? 0u : hi);
+  }
+  to.weight = special ? NAN : weight * scale;
+  return to;
+}
+
 // kTiles x 16 heads, kTokens tokens a wave. kApart: the waves of a workgroup take
-// different tokens and the same pages; otherwise the same tokens and pages in turn.
+// different tokens and the same pages; otherwise the same tokens and pages in turn, and
+// each codes some of the heads for all.
 template <int kTiles, int kTokens, bool kApart>
-__global__ __launch_bounds__(64 * kWaves) void index_scores_kernel(ScoreArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kTiles * kTokens >= 8 ? 2 : kTiles >= 4 ? 3 : kTokens >= 2 ? 2 : 4) void index_scores_kernel(ScoreArgs a) {
+  constexpr int kShared = kApart ? 1 : kTokens * kTiles;
+  __shared__ u32x4 coded_heads[kShared][4][64];
+  // (weights stay there: 2 x 64 heads and theirs in registers would spill)
+  __shared__ f32x4 head_weights[kApart ? kWaves : 1][kTokens * kTiles][4];
   const int lane = wave_lane(), row = lane & 15, group = lane >> 4;
   const int wave = uniform((int)(threadIdx.x >> 6));
-  const int b = (int)blockIdx.x / a.groups;
-  const int of = (int)blockIdx.x - b * a.groups;
+  const int b = (int)blockIdx.y / a.groups;
+  const int of = (int)blockIdx.y - b * a.groups;
   const int t0 = of * kTokens * (kApart ? kWaves : 1) + (kApart ? wave * kTokens : 0);
   if (t0 >= a.q_len) return;
   const int64_t first = (int64_t)b * a.q_len + t0;  // row of q, lengths and out
-  const int32_t* const table = a.block_table + b * a.bt_stride;
+  const const_i32* const table = (const const_i32*)a.block_table + b * a.bt_stride;
   int length[kTokens], most = 0;
 #pragma unroll
   for (int t = 0; t < kTokens; ++t) {
     length[t] = 0;
     if (t0 + t < a.q_len)
-      length[t] = (int)min((int64_t)max(a.lengths[first + t], 0),
+      length[t] = (int)min((int64_t)max(((const const_i32*)a.lengths)[first + t], 0),
                            min(a.width, (int64_t)a.max_blocks * kPageRecords));
     most = max(most, length[t]);
   }
   const int live = (most + kPageRecords - 1) / kPageRecords;  // pages to score
-  const int step = (int)gridDim.y * (kApart ? 1 : kWaves);
-  int p = kApart ? (int)blockIdx.y : (int)blockIdx.y * kWaves + wave;
+  // of `of_all` waves (workgroups) that take pages in turn, `working` have scores to find
+  const int of_all = (int)gridDim.x * (kApart ? 1 : kWaves);
+  const int turn = (int)((blockIdx.x + blockIdx.y) % gridDim.x);
+  const int start = kApart ? turn : turn * kWaves;
+  const int me = start + (kApart ? 0 : wave);
+  int working = of_all;
+  if (!kApart)
+    working = min(of_all, ((live + a.least - 1) / a.least + kWaves - 1) / kWaves * kWaves);
+  auto put = [&](int p, const float (&s)[kTokens]) {
+    const int64_t r = (int64_t)p * kPageRecords + lane;
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t)
+      if (t0 + t < a.q_len && r < a.width) a.out[(first + t) * a.width + r] = s[t];
+  };
+  float none[kTokens];
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) none[t] = -INFINITY;
+  for (int p = live + me; p < a.pages; p += of_all) put(p, none);
+  if (start >= min(live, working)) return;
 
-  bf16x8 q[kTokens][kTiles][4];
-  f32x4 w[kTokens][kTiles];
-  if (p < live) {
+  constexpr int kAll = kTokens * kTiles, kAtOnce = kAll < 4 ? kAll : 4;
+  bf16x8 q[kAll][4];  // tile i of token t: kTiles t + i
+  if constexpr (kApart) {
 #pragma unroll
     for (int t = 0; t < kTokens; ++t) {
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        const int h = 16 * i + row;
-        u32x4 x[4] = {};
-        float weight = 0.0f;
-        if (t0 + t < a.q_len && h < a.heads) {
-          const int64_t at = (first + t) * a.heads + h;
-          const u32x4* const from = (const u32x4*)(a.q + at * kIndexDim);
+        const Heads x = coded(a, first + t, t0 + t < a.q_len ? 16 * i + row : a.heads, group);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = from[2 * group + (k & 1) + 8 * (k >> 1)];
-          weight = a.weights[at];
-        }
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          top = top_of_pairs(top, top_of_pairs(top_of_pairs(x[k][0], x[k][1]),
-                                               top_of_pairs(x[k][2], x[k][3])));
-        top = over_groups_top(max(top & 0xffffu, top >> 16));
-        const bool special = top >= 0x7f80u;  // an infinity or NaN in the row
-        const float scale = exp2i(ue8m0_exponent(bf16_to_f32(top)));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t lo = index_codes(x[k][0], x[k][1], scale);
-          const uint32_t hi = index_codes(x[k][2], x[k][3], scale);
-          q[t][i][k] = values_of(special ? 0u : lo, special ? 0u : hi);
-        }
-        // the product's rows 4 group + c of a tile: those heads' weights
-        const float all = special ? NAN : weight * scale;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          w[t][i][c] = u2f((uint32_t)__builtin_amdgcn_ds_bpermute(4 * (4 * group + c),
-                                                                  (int)f2u(all)));
+        for (int k = 0; k < 4; ++k) q[kTiles * t + i][k] = x.x[k];
+        if (group == 0) ((float*)&head_weights[wave][kTiles * t + i][0])[row] = x.weight;
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
+  } else {
+#pragma unroll 1
+    for (int n = 0; n < kShared; n += kWaves) {
+      const int at = n + wave, t = at / kTiles, i = at - t * kTiles;
+      if (kShared % kWaves == 0 || at < kShared) {
+        const Heads x = coded(a, first + t, t0 + t < a.q_len ? 16 * i + row : a.heads, group);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) coded_heads[at][k][lane] = __builtin_bit_cast(u32x4, x.x[k]);
+        if (group == 0) ((float*)&head_weights[0][at][0])[row] = x.weight;
+      }
+    }
+    __syncthreads();
+    if (me >= min(live, working)) return;
+#pragma unroll
+    for (int i = 0; i < kAll; ++i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[i][k] = __builtin_bit_cast(bf16x8, coded_heads[i][k][lane]);
     }
   }
-  for (; p < a.pages; p += step) {
-    const int64_t r = (int64_t)p * kPageRecords + lane;
-    float s[kTokens];
+  // Records 16 i + row of a page, and the scale of record lane. (A page that is not mapped:
+  // page 0's, which nobody looks at.)
+  u32x4 raw[4][2];
+  float scale;
+  auto mapped = [&](int page) { return page >= 0 && page < a.pool_pages; };
+  auto base = [&](int page) {
+    return a.pool + (int64_t)(mapped(page) ? page : 0) * kIndexPageBytes;
+  };
+  auto fetch = [&](const uint8_t* from, int i) {
+    const u32x4* const at = (const u32x4*)(from + (16 * i + row) * kIndexDim) + group;
+    raw[i][0] = at[0];
+    raw[i][1] = at[4];
+  };
+  int page = table[me];
+  int next = me + working < live ? table[me + working] : -1;
+  {
+    const uint8_t* const from = base(page);
 #pragma unroll
-    for (int t = 0; t < kTokens; ++t) s[t] = -INFINITY;
-    const int page = p < live ? table[p] : -1;
-    if (page >= 0 && page < a.pool_pages) {
-      const uint8_t* const from = a.pool + (int64_t)page * kIndexPageBytes;
-      const float scale = *(const float*)(from + kIndexScalesAt + 4 * lane);
-      u32x4 raw[4][2];
+    for (int i = 0; i < 4; ++i) fetch(from, i);
+    scale = *(const float*)(from + kIndexScalesAt + 4 * lane);
+  }
+  for (int p = me; p < live; p += working) {
+    const int after = p + 2 * working < live ? table[p + 2 * working] : -1;
+    const uint8_t* const ahead = base(next);  // (once past the end: page 0 again)
+    // the product's rows 4 group + c of a tile: those heads' weights
+    int of_group = group;
+    asm volatile("" : "+v"(of_group));
+    float sum[kTokens][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u32x4* const at = (const u32x4*)(from + (16 * i + row) * kIndexDim) + group;
-        raw[i][0] = at[0];
-        raw[i][1] = at[4];
-      }
-      float sum[kTokens][4];
+    for (int i = 0; i < 4; ++i) {
+      bf16x8 k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        bf16x8 k[4];
+      for (int n = 0; n < 4; ++n)
+        k[n] = values_of(raw[i][n / 2][2 * (n & 1)], raw[i][n / 2][2 * (n & 1) + 1]);
+      fetch(ahead, i);
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t) sum[t][i] = 0.0f;
+#pragma unroll
+      for (int from = 0; from < kAll; from += kAtOnce) {
+        f32x4 d[kAtOnce];
+#pragma unroll
+        for (int h = 0; h < kAtOnce; ++h) d[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < 4; ++n)
-          k[n] = values_of(raw[i][n / 2][2 * (n & 1)], raw[i][n / 2][2 * (n & 1) + 1]);
 #pragma unroll
-        for (int t = 0; t < kTokens; ++t) {
-          f32x4 d[kTiles];
+          for (int h = 0; h < kAtOnce; ++h)
+            d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q[from + h][n], k[n], d[h], 0, 0, 0);
 #pragma unroll
-          for (int h = 0; h < kTiles; ++h) d[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < kAtOnce; ++h) {
+          float& all = sum[(from + h) / kTiles][i];
+          const f32x4 w = head_weights[kApart ? wave : 0][from + h][of_group];
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int h = 0; h < kTiles; ++h)
-              d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q[t][h][n], k[n], d[h], 0, 0, 0);
-          float all = 0.0f;
-#pragma unroll
-          for (int h = 0; h < kTiles; ++h)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)  // (a NaN stays one)
-              all = __builtin_fmaf(w[t][h][c], __builtin_elementwise_maximum(d[h][c], 0.0f), all);
-          sum[t][i] = all;
+          for (int c = 0; c < 4; ++c)  // (a NaN stays one)
+            all = __builtin_fmaf(w[c], __builtin_elementwise_maximum(d[h][c], 0.0f), all);
         }
       }
-#pragma unroll
-      for (int t = 0; t < kTokens; ++t) {
-        // over the four lanes of a record; lane l ends with record l
-        const auto x02 = __builtin_amdgcn_permlane32_swap(f2u(sum[t][0]), f2u(sum[t][2]), false, false);
-        const auto x13 = __builtin_amdgcn_permlane32_swap(f2u(sum[t][1]), f2u(sum[t][3]), false, false);
-        const float lo = u2f(x02[0]) + u2f(x02[1]), hi = u2f(x13[0]) + u2f(x13[1]);
-        const auto x = __builtin_amdgcn_permlane16_swap(f2u(lo), f2u(hi), false, false);
-        if (r < length[t]) s[t] = scale * (u2f(x[0]) + u2f(x[1]));
-      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    float s[kTokens];
 #pragma unroll
-    for (int t = 0; t < kTokens; ++t)
-      if (t0 + t < a.q_len && r < a.width) a.out[(first + t) * a.width + r] = s[t];
+    for (int t = 0; t < kTokens; ++t) {
+      // over the four lanes of a record; lane l ends with record l
+      const auto x02 = __builtin_amdgcn_permlane32_swap(f2u(sum[t][0]), f2u(sum[t][2]), false, false);
+      const auto x13 = __builtin_amdgcn_permlane32_swap(f2u(sum[t][1]), f2u(sum[t][3]), false, false);
+      const float lo = u2f(x02[0]) + u2f(x02[1]), hi = u2f(x13[0]) + u2f(x13[1]);
+      const auto x = __builtin_amdgcn_permlane16_swap(f2u(lo), f2u(hi), false, false);
+      s[t] = scale * (u2f(x[0]) + u2f(x[1]));
+      if (!mapped(page) || p * kPageRecords + lane >= length[t]) s[t] = -INFINITY;
+    }
+    scale = *(const float*)(ahead + kIndexScalesAt + 4 * lane);
+    put(p, s);
+    page = next;
+    next = after;
   }
 }
 
@@ -202,21 +281,28 @@ extern "C" int rm_index_scores(const uint16_t* q, int64_t batch, int64_t q_len, 
       !aligned(lengths, 4) || !aligned(out, 4))
     return RM_ERR_ALIGN;
   ScoreArgs a{q, weights, (int)q_len, (int)heads, pool, (int)pool_pages, block_table,
-              block_table_stride, (int)max_blocks, lengths, width, out,
-              (int)((width + kPageRecords - 1) / kPageRecords), 0};
+              block_table_stride, pool_pages > 0 ? (int)max_blocks : 0, lengths, width, out,
+              (int)((width + kPageRecords - 1) / kPageRecords), 0, 1};
   const int tokens = q_len > 1 && heads <= 64 ? 2 : 1;
   const bool apart = q_len >= 8 * kWaves;
   a.groups = (int)((q_len + tokens * (apart ? kWaves : 1) - 1) / (tokens * (apart ? kWaves : 1)));
   const int64_t rows = batch * a.groups;
   const int64_t turns = (a.pages + (apart ? 1 : kWaves) - 1) / (apart ? 1 : kWaves);
-  const int64_t splits = std::min<int64_t>(turns, std::max<int64_t>(1, 2048 / rows));
+  // Workgroups: two turns of what the chip holds, which is two waves a SIMD with 128 coded
+  // heads in registers and three or more with fewer (64 ragged requests: 2,048 23.6 us,
+  // 1,536 24.7, 1,024 28.9; 128 requests of 2 tokens: 1,024 145 us, 2,048 151, 512 142).
+  // A wave takes four pages at least once there are that many, as its heads cost it about
+  // as much as one (64 ragged requests, of two pages 26.9 us, of six 28.9).
+  const int64_t most = tokens * heads > 64 ? 1024 : 2048;
+  const int64_t splits = std::min<int64_t>(turns, std::max<int64_t>(1, most / rows));
+  a.least = (int)std::min<int64_t>(std::max<int64_t>(rows * a.pages / 4096, 1), 4);
   const auto pick = [&](auto one, auto two, auto more) { return apart ? more : tokens == 2 ? two : one; };
   const auto kern =
       heads <= 16   ? pick(index_scores_kernel<1, 1, false>, index_scores_kernel<1, 2, false>, index_scores_kernel<1, 2, true>)
       : heads <= 32 ? pick(index_scores_kernel<2, 1, false>, index_scores_kernel<2, 2, false>, index_scores_kernel<2, 2, true>)
       : heads <= 64 ? pick(index_scores_kernel<4, 1, false>, index_scores_kernel<4, 2, false>, index_scores_kernel<4, 2, true>)
                     : pick(index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, true>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)rows, (unsigned)splits), dim3(64 * kWaves), 0,
+  hipLaunchKernelGGL(kern, dim3((unsigned)splits, (unsigned)rows), dim3(64 * kWaves), 0,
                      (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
 }
