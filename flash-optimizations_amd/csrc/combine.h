@@ -1,8 +1,10 @@
 // Merge of split partials with the sink, shared by the decodes: partial O / l and
 // log2 l + m per (token, split, head), [tokens, splits, heads, 512] and [tokens,
 // splits, heads] floats, to out (BF16) and lse. kNatural: the partials' coordinates
-// in their own order and any number of heads (4-bit records); otherwise in
-// partial_coord() order with heads a multiple of 16 (Packed and Native).
+// in their own order and any number of heads (4-bit records, trees); otherwise in
+// partial_coord() order with heads a multiple of 16 (Packed and Native). kRagged: of the
+// slots of tokens_each tokens only the first counts[token / tokens_each] hold partials; no
+// slots: the rows are finished already.
 #pragma once
 #include "remnant_device.h"
 
@@ -59,20 +61,24 @@ __device__ __forceinline__ float lane_of(float x, int l) {
 // head from the grid instead of a division: 64 heads x 16 tokens 4.5 -> 4.1 us, 128
 // heads 5.6 -> 4.9, 16 heads x 64 tokens of four splits 4.6 unchanged; the
 // other combine, one token of 64 splits, 3.9 -> 3.4).
-template <int kWaveBatch, bool kNatural>
+template <int kWaveBatch, bool kNatural, bool kRagged>
 __global__ __launch_bounds__(256) void combine_wave_kernel(const float* __restrict__ ws_o,
                                                            const float* __restrict__ ws_lse,
                                                            const float* __restrict__ sink,
-                                                           int splits, int heads,
+                                                           int slots, int heads,
                                                            uint16_t* __restrict__ out,
-                                                           float* __restrict__ lse) {
+                                                           float* __restrict__ lse,
+                                                           const int32_t* __restrict__ counts,
+                                                           int tokens_each) {
   const int lane = wave_lane();
   // block (x, y): heads 4x .. 4x + 3 of token y (a token's heads are a multiple of 16)
   const int64_t t = blockIdx.y;
   const int h = blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6));
   if (kNatural && h >= heads) return;
+  const int splits = kRagged ? uniform(counts[t / tokens_each]) : slots;
+  if (kRagged && splits == 0) return;
   const int64_t row = t * heads + h;
-  const float* src = ws_o + (t * splits * heads + h) * kHeadDim + 8 * lane;
+  const float* src = ws_o + (t * slots * heads + h) * kHeadDim + 8 * lane;
   const int64_t step = (int64_t)heads * kHeadDim;
   f32x4 x[2 * kWaveBatch];
 #pragma unroll
@@ -81,7 +87,7 @@ __global__ __launch_bounds__(256) void combine_wave_kernel(const float* __restri
     x[2 * u] = *(const f32x4*)from;
     x[2 * u + 1] = *(const f32x4*)(from + 4);
   }
-  const float lse_at = ws_lse[(t * splits + min(lane, splits - 1)) * heads + h];
+  const float lse_at = ws_lse[(t * slots + min(lane, splits - 1)) * heads + h];
   const float ls = lane < splits ? lse_at : -INFINITY;
   const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
   const float mz = wave_all<true>(fmaxf(ls, sink2));
@@ -142,12 +148,14 @@ __global__ __launch_bounds__(256) void combine_wave_kernel(const float* __restri
 // kPerWave (4, 8 or 16) is the smallest that covers the splits; loads past the
 // last split repeat it and are left out of the sum, as in combine_wave_kernel.
 constexpr int kCombineSlices = kHeadDim / 64;
-template <int kPerWave, bool kNatural>
+template <int kPerWave, bool kNatural, bool kRagged>
 __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ ws_o,
                                                       const float* __restrict__ ws_lse,
-                                                      const float* __restrict__ sink, int splits,
+                                                      const float* __restrict__ sink, int slots,
                                                       int heads, uint16_t* __restrict__ out,
-                                                      float* __restrict__ lse) {
+                                                      float* __restrict__ lse,
+                                                      const int32_t* __restrict__ counts,
+                                                      int tokens_each) {
   __shared__ float part[4][64];
   const int lane = wave_lane();
   const int wave = uniform((int)(threadIdx.x >> 6));
@@ -155,9 +163,11 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
   const int64_t t = blockIdx.y;
   const int h = blockIdx.x / kCombineSlices;
   const int slice = blockIdx.x % kCombineSlices;
+  const int splits = kRagged ? uniform(counts[t / tokens_each]) : slots;
+  if (kRagged && splits == 0) return;
   const int64_t row = t * heads + h;
   const int64_t step = (int64_t)heads * kHeadDim;
-  const float* src = ws_o + (t * splits * heads + h) * kHeadDim + 64 * slice + lane;
+  const float* src = ws_o + (t * slots * heads + h) * kHeadDim + 64 * slice + lane;
   // issue every load first: this wave's partials and all split LSEs
   float x[kPerWave];
 #pragma unroll
@@ -165,7 +175,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
     const int s = wave + 4 * u;
     x[u] = src[min(s, splits - 1) * step];
   }
-  const float lse_at = ws_lse[(t * splits + min(lane, splits - 1)) * heads + h];
+  const float lse_at = ws_lse[(t * slots + min(lane, splits - 1)) * heads + h];
   const float ls = lane < splits ? lse_at : -INFINITY;
   const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
   const float mz = wave_all<true>(fmaxf(ls, sink2));
@@ -196,20 +206,24 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
   }
 }
 
-template <bool kNatural>
+template <bool kNatural, bool kRagged = false>
 void launch_combine(const float* ws_o, const float* ws_lse, const float* sink, int slots,
-                    int64_t tokens, int64_t heads, uint16_t* out, float* lse, hipStream_t s) {
+                    int64_t tokens, int64_t heads, uint16_t* out, float* lse, hipStream_t s,
+                    const int32_t* counts = nullptr, int64_t tokens_each = 1) {
   // rows: one workgroup per 64 coordinates of each. In natural order also where the wave
   // form would take two turns (decode of 4-bit records, 16 tokens x 16 heads, 16 splits
-  // 15.3 -> 13.1 us with it; 24 tokens, 8 splits: 16.8 with this form, 16.3 the other)
-  const bool few = tokens * heads < 256 || (kNatural && slots > 8);
-  const auto kern = few ? (slots <= 16   ? combine_kernel<4, kNatural>
-                           : slots <= 32 ? combine_kernel<8, kNatural>
-                                         : combine_kernel<16, kNatural>)
-                    : slots <= 4 ? combine_wave_kernel<4, kNatural>
-                                 : combine_wave_kernel<8, kNatural>;
+  // 15.3 -> 13.1 us with it; 24 tokens, 8 splits: 16.8 with this form, 16.3 the other), but
+  // not where most rows have fewer partials than slots
+  const bool few = tokens * heads < 256 || (kNatural && !kRagged && slots > 8);
+  const auto kern =
+      few ? (slots <= 16   ? combine_kernel<4, kNatural, kRagged>
+             : slots <= 32 ? combine_kernel<8, kNatural, kRagged>
+                           : combine_kernel<16, kNatural, kRagged>)
+      : slots <= 4 || kRagged ? combine_wave_kernel<4, kNatural, kRagged>
+                              : combine_wave_kernel<8, kNatural, kRagged>;
   const dim3 grid((unsigned)(few ? heads * kCombineSlices : (heads + 3) / 4), (unsigned)tokens);
-  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, ws_o, ws_lse, sink, slots, (int)heads, out, lse);
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, ws_o, ws_lse, sink, slots, (int)heads, out, lse,
+                     counts, (int)tokens_each);
 }
 
 }  // namespace

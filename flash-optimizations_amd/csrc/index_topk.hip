@@ -46,20 +46,6 @@ struct Shared {
   u32x2 list[64];  // key, wave
 };
 
-// Inclusive sum over the wave's lanes up to and with this one (shifts within each row of 16,
-// then the last lanes of rows 0 and 2 to the next row, of row 1 to the upper half).
-template <int kCtrl, int kRowMask>
-__device__ __forceinline__ uint32_t plus_dpp(uint32_t x) {
-  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, kRowMask, 0xf, false);
-}
-__device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
-  x = plus_dpp<0x111, 0xf>(x);
-  x = plus_dpp<0x112, 0xf>(x);
-  x = plus_dpp<0x114, 0xf>(x);
-  x = plus_dpp<0x118, 0xf>(x);
-  x = plus_dpp<0x142, 0xa>(x);
-  return plus_dpp<0x143, 0xc>(x);
-}
 // Over the wave's lanes.
 template <class F>
 __device__ __forceinline__ uint32_t wave_all_of(uint32_t x, F op) {

@@ -71,7 +71,12 @@ constexpr int kRefsBytes = kUnits * kRows * 4;
 constexpr int kGoneAt = kRefsAt + 2 * kRefsBytes;  // [4 units]: bits of rows that are left out
 constexpr int kMovedAt = kGoneAt + 2 * 16;         // [4], by round
 constexpr int kSumsAt = kMovedAt + 16;              // [4 units][32 query rows] of l, r
-constexpr int kLdsBytes = kSumsAt + kUnits * kRows * 8;
+constexpr int kStartsAt = kSumsAt + kUnits * kRows * 8;  // [requests + 1]
+constexpr int kQueriesAt = 3 * kRoundBytes;  // before a piece's fourth round is copied
+constexpr int kMaxShared = 256;   // requests whose rounds are dealt out evenly
+constexpr int kLdsBytes = kStartsAt + (kMaxShared + 1) * 4;
+// What a piece costs beyond its rounds, in rounds (about 6 us of 1.5).
+constexpr int kOverhead = 4;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr float kHeadroom = 16.0f;
 constexpr float kRounded = 0x1p-100f;  // the rounded weights' sums: times 2^127 and this
@@ -100,12 +105,15 @@ struct TreeArgs {
   const int32_t* past_lengths;
   const float* sink;
   float scale_log2;
-  int splits;
+  int parts;   // workgroups that share the rounds of a tile's requests; 0: a request each
+  int slots;   // partials that a request can have
   uint16_t* out;
   float* lse;
-  float* ws_o;  // null: one split, finish in place
+  float* ws_o;
   float* ws_lse;
+  int32_t* counts;  // [batch] partials of the request; 0: finished in place
 };
+typedef const __attribute__((address_space(4))) TreeArgs const_args;
 
 __device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
   return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * lane, (int)x);
@@ -149,10 +157,11 @@ __device__ __forceinline__ void copy_ahead4(const uint8_t* base, uint32_t offset
 
 // What both roles know.
 struct Tree {
-  const TreeArgs& a;
+  const_args* a;
   const uint32_t lds;
   int lane, row, group;
-  const int wave, b;
+  const int wave;
+  int b;
   // the request: its rows of the block tables, and the pools (the compressed records first)
   const const_i32* table[2];
   const uint8_t* pool[2];
@@ -160,33 +169,49 @@ struct Tree {
   int held, past, first, past_units, units;
   int begin, end;                            // the workgroup's units
 
-  __device__ __forceinline__ Tree(const TreeArgs& args, uint32_t at, int request)
+  int slot, of_slots;                        // the piece among its request's
+
+  __device__ __forceinline__ Tree(const_args* args, uint32_t at)
       : a(args),
         lds(at),
         lane(wave_lane()),
         row(lane & 15),
         group(lane >> 4),
-        wave(uniform((int)(threadIdx.x >> 6))),
-        b(request) {}
+        wave(uniform((int)(threadIdx.x >> 6))) {}
 
-  __device__ __forceinline__ void request(int split) {
-    held = max(min(((const const_i32*)a.lengths)[b], 0x7fffff00), 0);
-    past = 0;
-    if (a.past_lengths)
-      past = max(min(((const const_i32*)a.past_lengths)[b], a.past_blocks * kPageRecords), 0);
-    first = max(held - a.window + 1, 0) & ~(kUnit - 1);
-    const int stop = (int)min((int64_t)held + a.nodes, (int64_t)a.blocks * kPageRecords);
-    past_units = (past + kUnit - 1) / kUnit;
-    units = past_units + max((stop - first + kUnit - 1) / kUnit, 0);
-    const int share = ((units + a.splits - 1) / a.splits + kUnits - 1) / kUnits * kUnits;
-    begin = min(split * share, units);
-    end = min(begin + share, units);
-    table[0] = (const const_i32*)a.past_table + b * a.past_stride;
-    table[1] = (const const_i32*)a.table + b * a.table_stride;
-    pool[0] = a.past;
-    pool[1] = a.pool;
-    pages[0] = a.past_pages;
-    pages[1] = a.pool_pages;
+  struct Extent {
+    int held, past, first, past_units, units;
+  };
+  __device__ __forceinline__ static Extent extent(const_args* a, int length, int past_length) {
+    Extent x;
+    x.held = max(min(length, 0x7fffff00), 0);
+    x.past = max(min(past_length, a->past_blocks * kPageRecords), 0);
+    x.first = max(x.held - a->window + 1, 0) & ~(kUnit - 1);
+    const int stop = (int)min((int64_t)x.held + a->nodes, (int64_t)a->blocks * kPageRecords);
+    x.past_units = (x.past + kUnit - 1) / kUnit;
+    x.units = x.past_units + max((stop - x.first + kUnit - 1) / kUnit, 0);
+    return x;
+  }
+  __device__ __forceinline__ static int rounds(const Extent& x) {
+    return max((x.units + kUnits - 1) / kUnits, 1);
+  }
+
+  // Rounds from .. to - 1 of a request.
+  __device__ __forceinline__ void piece(int request, int from, int to) {
+    anew();
+    b = request;
+    const Extent x = extent(a, ((const const_i32*)a->lengths)[b],
+                            a->past_lengths ? ((const const_i32*)a->past_lengths)[b] : 0);
+    held = x.held, past = x.past, first = x.first, past_units = x.past_units, units = x.units;
+    begin = min(from * kUnits, units);
+    end = min(to, rounds(x)) * kUnits;
+    end = min(end, units);
+    table[0] = (const const_i32*)a->past_table + b * a->past_stride;
+    table[1] = (const const_i32*)a->table + b * a->table_stride;
+    pool[0] = a->past;
+    pool[1] = a->pool;
+    pages[0] = a->past_pages;
+    pages[1] = a->pool_pages;
     // (kept in registers: chosen between in memory, each unit would wait for them again)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -203,6 +228,10 @@ struct Tree {
   }
   // What follows from the lane is worked out again in each round: kept, it would push Q out
   // of the registers.
+  __device__ __forceinline__ void anew() {
+    asm volatile("" : "+s"(a));
+    again();
+  }
   __device__ __forceinline__ void again() {
     asm volatile("" : "+v"(lane));
     row = lane & 15;
@@ -249,27 +278,36 @@ struct Scorer : Tree {
 
   __device__ __forceinline__ Scorer(const Tree& t) : Tree(t), of(wave) {}
 
+  // Rows 8 wave .. + 7 of Q to LDS. Piece j of row r goes to place j ^ (r & 15) there, so that
+  // sixteen lanes reading one piece of sixteen rows meet every bank once.
+  __device__ __forceinline__ void copy_q(int first_row) const {
+    const uint8_t* const from =
+        (const uint8_t*)(a->q + ((int64_t)b * a->q_rows + first_row) * kHeadDim);
+#pragma unroll
+    for (int n = 0; n < kRows / kScorers; ++n) {
+      const int r = kRows / kScorers * of + n;
+      copy_ahead16(from, 2 * kHeadDim * min(r, a->q_rows - 1 - first_row) + 16 * (lane ^ (r & 15)),
+                   lds + kQueriesAt + 2 * kHeadDim * r);
+    }
+  }
   // Coordinates 64 s + 16 group .. + 15 as two operands, then the tail's 32 t + 8 group.
-  __device__ __forceinline__ void load_q(int first_row) {
+  __device__ __forceinline__ void load_q() {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int at = min(first_row + 16 * c + row, a.q_rows - 1);
-      const uint16_t* const from = a.q + ((int64_t)b * a.q_rows + at) * kHeadDim;
+      const uint32_t at = lds + kQueriesAt + 2 * kHeadDim * (16 * c + row);
 #pragma unroll
-      for (int s = 0; s < 7; ++s) {
-        q[c][2 * s] = *(const u32x4*)(from + 64 * s + 16 * group);
-        q[c][2 * s + 1] = *(const u32x4*)(from + 64 * s + 16 * group + 8);
-      }
+      for (int s = 0; s < 14; ++s)
+        q[c][s] = lds_read<u32x4>(at + 16 * ((8 * (s / 2) + 2 * group + (s & 1)) ^ row));
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        q[c][14 + t] = *(const u32x4*)(from + kNopeDim + 32 * t + 8 * group);
+        q[c][14 + t] = lds_read<u32x4>(at + 16 * ((56 + 4 * t + group) ^ row));
     }
   }
 
   // Lane j works out node j's path (parent: of node lane); each lane then takes its query
   // row's node.
   __device__ __forceinline__ void tree(int first_row, int parent) {
-    bool bad = lane >= a.nodes || parent < -1 || parent >= lane;
+    bool bad = lane >= a->nodes || parent < -1 || parent >= lane;
     int up = bad ? -1 : parent;
     uint64_t seen = 1ull << lane;
     // twice as many steps up each time
@@ -287,23 +325,23 @@ struct Scorer : Tree {
     }
     const int depth = __popcll(seen) - 1;
     // ancestors before the window (a path's nodes are in the order of their numbers)
-    for (int n = depth + 1; n > a.window; --n) seen &= seen - 1;
+    for (int n = depth + 1; n > a->window; --n) seen &= seen - 1;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int at = first_row + 16 * c + row;
-      const int node = min(at / a.heads, a.nodes - 1);
+      const int node = min(at / a->heads, a->nodes - 1);
       const uint32_t padding = from_lane(bad, node);  // (every lane takes part)
-      live[c] = at < a.q_rows && !padding;
+      live[c] = at < a->q_rows && !padding;
       path[c][0] = from_lane((uint32_t)seen, node);
       path[c][1] = from_lane((uint32_t)(seen >> 32), node);
-      lowest[c] = held + (int)from_lane((uint32_t)depth, node) - a.window + 1;
+      lowest[c] = held + (int)from_lane((uint32_t)depth, node) - a->window + 1;
     }
   }
 
   // Whether every live query row sees all of the unit.
   __device__ __forceinline__ bool whole(const Unit& x) const {
     return x.mapped & (x.at + kUnit <= (x.past ? past : held)) &
-           (x.past | (x.at >= held + a.nodes - a.window));
+           (x.past | (x.at >= held + a->nodes - a->window));
   }
   __device__ __forceinline__ uint32_t weights_at(int round, int c) const {
     return lds + kWeightsAt + (round & 1) * kWeightsBytes + 2048 * (of >> 1) + 1024 * c +
@@ -333,7 +371,7 @@ struct Scorer : Tree {
   __device__ __forceinline__ void score(const Unit& x, int round, const Rows& in) {
     const u32x2 bytes = in.bytes;
     // rows of the unit that count
-    const int stop = min(x.past ? past - x.at : held + a.nodes - x.at, kUnit);
+    const int stop = min(x.past ? past - x.at : held + a->nodes - x.at, kUnit);
     uint32_t odd = 0, gone = 0;  // rows with an infinity or NaN, and with those nobody sees
     if (!kWhole) {
       // row `row`, pieces 9 group .. + 8: an infinity or NaN in it?
@@ -388,7 +426,7 @@ struct Scorer : Tree {
     // value i is row 4 group + i of the unit
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      f32x4 s = (acc[c][0] + acc[c][1]) * a.scale_log2;
+      f32x4 s = (acc[c][0] + acc[c][1]) * a->scale_log2;
       if (!kWhole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -439,12 +477,15 @@ struct Scorer : Tree {
 #pragma unroll
     for (int c = 0; c < 2; ++c) m[c] = -INFINITY, l[c] = r[c] = 0.0f;
     int parent = -2;
-    if (lane < a.nodes) parent = a.parents[(int64_t)b * a.nodes + lane];
+    if (lane < a->nodes) parent = a->parents[(int64_t)b * a->nodes + lane];
     int page = 0;
     if (begin + of < end) page = page_of(begin + of);
-    load_q(first_row);
+    asm volatile("" : "+v"(parent));  // (to be waited for before there are copies)
+    copy_q(first_row);
     tree(first_row, parent);
-    lds_barrier();  // round 0's rows
+    wait_copies<0>();
+    lds_barrier();  // round 0's rows, and Q
+    load_q();
     int round = 0;
 #pragma clang loop unroll(disable)
     for (int from = begin; from < end; from += kUnits, ++round) {
@@ -640,7 +681,7 @@ struct Adder : Tree {
       add<false>(round, gone, between);
   }
 
-  __device__ __forceinline__ void run(int first_row, int split) {
+  __device__ __forceinline__ void run(int first_row) {
     if (threadIdx.x == 64 * kScorers) lds_write(lds + kMovedAt, u32x4{0, 0, 0, 0});
     const int i = uniform(begin + g);
     int page = 0;
@@ -683,7 +724,8 @@ struct Adder : Tree {
     }
     if (round > 0) add(round - 1, [](int) {});
     lds_barrier();
-    finish(first_row, split);
+    anew();
+    finish(first_row);
   }
 
   // Until the copies before those of unit `last`, the latest, have landed.
@@ -694,7 +736,7 @@ struct Adder : Tree {
       wait_copies<0>();
   }
 
-  __device__ __forceinline__ void finish(int first_row, int split) {
+  __device__ __forceinline__ void finish(int first_row) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float sum = 0.0f, rsum = 0.0f;
@@ -705,27 +747,27 @@ struct Adder : Tree {
         rsum += part[1];
       }
       const int at = first_row + 16 * c + row;
-      if (at >= a.q_rows) continue;
-      const int node = at / a.heads, h = at - node * a.heads;
-      const int64_t token = (int64_t)b * a.nodes + node;
+      if (at >= a->q_rows) continue;
+      const int node = at / a->heads, h = at - node * a->heads;
+      const int64_t token = (int64_t)b * a->nodes + node;
       const int c0 = 128 * g + 4 * group;
-      if (a.ws_o) {
-        const int64_t to = (token * a.splits + split) * a.heads + h;
+      if (of_slots > 1) {
+        const int64_t to = (token * a->slots + slot) * a->heads + h;
         const float f = sum != 0.0f ? 1.0f / rsum : 0.0f;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           f32x4 x = o[c][u / 4][u % 4] * f;
           if (sum == 0.0f) x = f32x4{0.f, 0.f, 0.f, 0.f};
-          __builtin_nontemporal_store(x, (f32x4*)(a.ws_o + to * kHeadDim + c0 + 16 * u));
+          __builtin_nontemporal_store(x, (f32x4*)(a->ws_o + to * kHeadDim + c0 + 16 * u));
         }
         // (NaN goes on as infinity: the combine's maximum would pass over a NaN)
         if (g == 0 && group == 0)
-          a.ws_lse[to] = sum != sum     ? INFINITY
+          a->ws_lse[to] = sum != sum     ? INFINITY
                          : sum != 0.0f ? m[c] + __builtin_amdgcn_logf(sum)
                                        : -INFINITY;
         continue;
       }
-      const float sink2 = a.sink ? a.sink[h] * kLog2e : -INFINITY;
+      const float sink2 = a->sink ? a->sink[h] * kLog2e : -INFINITY;
       const float top = fmaxf(sum != 0.0f ? m[c] : -INFINITY, sink2);
       float f = 0.0f, lse = -INFINITY;
       if (top != -INFINITY || sum != 0.0f) {
@@ -735,12 +777,12 @@ struct Adder : Tree {
         if (sum != 0.0f) f = sum * em / (rsum * z);
         lse = (top + __builtin_amdgcn_logf(z)) * kLn2;
       }
-      if (g == 0 && group == 0) a.lse[token * a.heads + h] = lse;
+      if (g == 0 && group == 0) a->lse[token * a->heads + h] = lse;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         f32x4 x = o[c][u / 4][u % 4] * f;
         if (sum == 0.0f) x = f32x4{0.f, 0.f, 0.f, 0.f};
-        *(u32x2*)(a.out + (token * a.heads + h) * kHeadDim + c0 + 16 * u) =
+        *(u32x2*)(a->out + (token * a->heads + h) * kHeadDim + c0 + 16 * u) =
             u32x2{__builtin_bit_cast(uint32_t, bf16_pair(x[0], x[1])),
                   __builtin_bit_cast(uint32_t, bf16_pair(x[2], x[3]))};
       }
@@ -748,22 +790,90 @@ struct Adder : Tree {
   }
 };
 
-__global__ __launch_bounds__(64 * (kScorers + kAdders)) void tree_decode_kernel(TreeArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
-  // Workgroups go to the eight XCDs in turn: the tiles of one request and split, which read
-  // the same rows, go to one, so that its L2 cache serves all but the first.
-  const int at = (int)blockIdx.x >> 3;
-  const int part = at / a.tiles * 8 + ((int)blockIdx.x & 7);
-  if (part >= a.batch * a.splits) return;
-  const int b = part / a.splits, split = part - b * a.splits;
-  const int first_row = at % a.tiles * kRows;
-  Tree t(a, (uint32_t)(uintptr_t)(lds_void*)lds, b);
-  t.request(split);
-  if (t.wave < kScorers) {
-    Scorer(t).run(first_row);
-  } else {
-    Adder(t).run(first_row, split);
+// The rounds of all requests stand on one axis, each request's followed by kOverhead, and a
+// part takes an equal piece of it: b's rounds from `start` on, of which several parts can have
+// some. Starts go to LDS.
+struct Share {
+  int first;  // request
+  int begin, end, size;
+};
+__device__ __forceinline__ Share deal(const Tree& t, int part) {
+  constexpr int kEach = kMaxShared / 64;
+  const_args* const a = t.a;
+  int rounds[kEach], sum = 0, most = 0;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = kEach * t.lane + k;
+    rounds[k] = -kOverhead;  // (past the last request: nothing)
+    if (i < a->batch)
+      rounds[k] = Tree::rounds(
+          Tree::extent(a, a->lengths[i], a->past_lengths ? a->past_lengths[i] : 0));
+    most = max(most, rounds[k]);
+    sum += rounds[k] + kOverhead;
   }
+  const int upto = (int)wave_prefix((uint32_t)sum);
+  const int total = __builtin_amdgcn_readlane(upto, 63) - kOverhead;
+  most = uniform((int)wave_all<true>((float)most));
+  Share x;
+  // (and no request in more pieces than there are slots; one can begin inside a part, but for
+  // the first)
+  const int cuts = max(a->slots - (a->batch > 1 ? 1 : 0), 1);
+  x.size = max(max((total + a->parts - 1) / a->parts, (most + cuts - 1) / cuts), 1);
+  x.begin = part * x.size;
+  x.end = x.begin + x.size;
+  x.first = 0;
+  int start = upto - sum;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = kEach * t.lane + k;
+    x.first += __popcll(__ballot(i < a->batch && start + rounds[k] <= x.begin));
+    if (t.wave == 0 && i <= a->batch) lds_write(t.lds + kStartsAt + 4 * i, start);
+    start += rounds[k] + kOverhead;
+  }
+  if (t.wave == 0 && kEach * (t.lane + 1) == a->batch && t.lane == 63)
+    lds_write(t.lds + kStartsAt + 4 * a->batch, start);
+  lds_barrier();
+  return x;
+}
+
+__global__ __launch_bounds__(64 * (kScorers + kAdders)) void tree_decode_kernel(TreeArgs) {
+  const_args* a = (const_args*)__builtin_amdgcn_kernarg_segment_ptr();
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
+  // Workgroups go to the eight XCDs in turn: the tiles of one part, which read the same rows,
+  // go to one, so that its L2 cache serves all but the first.
+  const int at = (int)blockIdx.x >> 3;
+  const int part = at / a->tiles * 8 + ((int)blockIdx.x & 7);
+  const int tile = at % a->tiles, first_row = tile * kRows;
+  Tree t(a, (uint32_t)(uintptr_t)(lds_void*)lds);
+  if (part >= (a->parts > 0 ? a->parts : a->batch)) return;
+  Share share = {part, 0, 0, 0};
+  if (a->parts > 0) share = deal(t, part);
+  const int last = a->parts > 0 ? a->batch : part + 1;
+  const auto start = [&](int i) { return uniform(lds_read<int>(t.lds + kStartsAt + 4 * i)); };
+  const auto each = [&](auto run) {
+#pragma clang loop unroll(disable)
+    for (int b = uniform(share.first); b < last; ++b) {
+      int from = 0, to = 0x7fffffff / kUnits;
+      t.slot = 0, t.of_slots = 1;
+      if (a->parts > 0) {
+        const int at = start(b), rounds = start(b + 1) - kOverhead - at;
+        if (at >= share.end) break;
+        from = max(share.begin - at, 0), to = min(share.end - at, rounds);
+        t.slot = part - at / share.size;
+        t.of_slots = (at + rounds - 1) / share.size - at / share.size + 1;
+        if (a->counts && tile == 0 && t.slot == t.of_slots - 1 && threadIdx.x == 0)
+          a->counts[b] = t.of_slots > 1 ? t.of_slots : 0;
+      }
+      t.piece(b, from, to);
+      int row = first_row;
+      asm volatile("" : "+s"(row));
+      run(row);
+    }
+  };
+  if (t.wave < kScorers)
+    each([&](int row) { Scorer(t).run(row); });
+  else
+    each([&](int row) { Adder(t).run(row); });
 }
 
 bool aligned(const void* p, uintptr_t al) { return ((uintptr_t)p & (al - 1)) == 0; }
@@ -775,17 +885,36 @@ bool bad_sizes(int64_t batch, int64_t nodes, int64_t heads, int64_t blocks, int6
          window < 0 || window > 0x7fffffff || past_blocks < 0 || past_blocks > (1 << 24);
 }
 
-int plan(int64_t batch, int64_t nodes, int64_t heads, int64_t blocks, int64_t window,
-         int64_t past_blocks) {
-  const int64_t tiles = std::max<int64_t>(batch * ((nodes * heads + kRows - 1) / kRows), 1);
+struct Plan {
+  int parts, slots;
+  size_t counts_at, bytes;
+};
+// Parts: as many as fill the chip with one turn of workgroups (one a CU, for its LDS), four
+// turns where a turn could not be filled well. With four turns of whole requests or more, a
+// request each, as in any order they fill it.
+Plan plan(int64_t batch, int64_t nodes, int64_t heads, int64_t blocks, int64_t window,
+          int64_t past_blocks) {
+  const int64_t tiles = std::max<int64_t>((nodes * heads + kRows - 1) / kRows, 1);
   int64_t rows = blocks * kPageRecords;
   if (window > 0) rows = std::min(rows, window + nodes + kUnit);
-  const int64_t rounds = (rows + past_blocks * kPageRecords + kRound - 1) / kRound;
-  const int64_t most = std::min<int64_t>({256 / tiles, rounds, kMaxSplits});
-  return (int)std::max<int64_t>(most, 1);
-}
-size_t ws_bytes(int64_t splits, int64_t rows) {
-  return splits > 1 ? (size_t)(splits * rows) * (kHeadDim + 1) * sizeof(float) : 0;
+  const int64_t rounds =
+      std::max<int64_t>((rows + past_blocks * kPageRecords + kRound - 1) / kRound, 1);
+  Plan p = {0, 1, 0, 0};
+  if (batch > kMaxShared || batch * tiles >= 1024 || rounds >= (1 << 22)) return p;
+  const int64_t most = std::max<int64_t>(batch * rounds, 1);
+  p.parts = (int)std::min<int64_t>(std::max<int64_t>((tiles <= 64 ? 256 : 1024) / tiles, 1), most);
+  if (batch <= 1) {
+    const int64_t share = (rounds + p.parts - 1) / p.parts;
+    p.slots = (int)((rounds + share - 1) / share);
+  } else {  // four times an even share's
+    p.slots = (int)std::min<int64_t>(4 * ((p.parts + batch - 1) / batch) + 1, p.parts);
+  }
+  p.slots = std::min(p.slots, kMaxSplits);
+  if (p.slots > 1) {
+    p.counts_at = (size_t)(p.slots * batch * nodes * heads) * (kHeadDim + 1) * sizeof(float);
+    p.bytes = p.counts_at + (size_t)batch * sizeof(int32_t);
+  }
+  return p;
 }
 
 }  // namespace
@@ -794,9 +923,9 @@ extern "C" int rm_tree_decode_workspace(int64_t batch, int64_t nodes, int64_t he
                                         int64_t max_blocks, int64_t window, int64_t history_blocks,
                                         int32_t* num_splits, size_t* workspace_bytes) {
   if (bad_sizes(batch, nodes, heads, max_blocks, window, history_blocks)) return RM_ERR_SHAPE;
-  const int splits = plan(batch, nodes, heads, max_blocks, window, history_blocks);
-  if (num_splits) *num_splits = splits;
-  if (workspace_bytes) *workspace_bytes = ws_bytes(splits, batch * nodes * heads);
+  const Plan p = plan(batch, nodes, heads, max_blocks, window, history_blocks);
+  if (num_splits) *num_splits = p.slots;
+  if (workspace_bytes) *workspace_bytes = p.bytes;
   return RM_OK;
 }
 
@@ -828,10 +957,9 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
                         (const void*)sink, (const void*)lse})
     if (!aligned(p, 4)) return RM_ERR_ALIGN;
   const int64_t rows = batch * nodes * heads;
-  const int splits = plan(batch, nodes, heads, max_blocks, window, history_blocks);
-  const size_t bytes = ws_bytes(splits, rows);
-  if (bytes > 0 && (!workspace || workspace_bytes < bytes)) return RM_ERR_WORKSPACE;
-  if (bytes > 0 && !aligned(workspace, 16)) return RM_ERR_ALIGN;
+  const Plan p = plan(batch, nodes, heads, max_blocks, window, history_blocks);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return RM_ERR_WORKSPACE;
+  if (p.bytes > 0 && !aligned(workspace, 16)) return RM_ERR_ALIGN;
   TreeArgs a;
   a.q = q;
   a.batch = (int)batch;
@@ -855,17 +983,20 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
   a.past_lengths = history_blocks > 0 && history_pages > 0 ? history_lengths : nullptr;
   a.sink = sink;
   a.scale_log2 = softmax_scale * kLog2e;
-  a.splits = splits;
+  a.parts = p.parts;
+  a.slots = p.slots;
   a.out = out;
   a.lse = lse;
-  a.ws_o = splits > 1 ? (float*)workspace : nullptr;
-  a.ws_lse = splits > 1 ? (float*)workspace + (size_t)splits * rows * kHeadDim : nullptr;
+  a.ws_o = (float*)workspace;
+  a.ws_lse = (float*)workspace + (size_t)p.slots * rows * kHeadDim;
+  a.counts = p.slots > 1 ? (int32_t*)((uint8_t*)workspace + p.counts_at) : nullptr;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(tree_decode_kernel, dim3((unsigned)((batch * splits + 7) / 8 * 8 * a.tiles)),
+  hipLaunchKernelGGL(tree_decode_kernel, dim3((unsigned)((p.parts > 0 ? p.parts : batch) + 7) / 8 * 8 * a.tiles),
                      dim3(64 * (kScorers + kAdders)), 0, s, a);
   if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
-  if (splits > 1) {
-    launch_combine<true>(a.ws_o, a.ws_lse, sink, splits, batch * nodes, heads, out, lse, s);
+  if (p.slots > 1) {
+    launch_combine<true, true>(a.ws_o, a.ws_lse, sink, p.slots, batch * nodes, heads, out, lse, s,
+                               a.counts, nodes);
     if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   }
   return RM_OK;
