@@ -68,9 +68,8 @@ constexpr int kShiftsAt = kWeightsAt + 2 * kWeightsBytes;  // [2][8 groups][4][8
 constexpr int kShiftsBytes = 2 * 8 * 64;
 constexpr int kRefsAt = kShiftsAt + 2 * kShiftsBytes;  // [4 units][32 query rows] float
 constexpr int kRefsBytes = kUnits * kRows * 4;
-constexpr int kGoneAt = kRefsAt + 2 * kRefsBytes;  // [4 units]: bits of rows that are left out
-constexpr int kMovedAt = kGoneAt + 2 * 16;         // [4], by round
-constexpr int kSumsAt = kMovedAt + 16;              // [4 units][32 query rows] of l, r
+constexpr int kStateAt = kRefsAt + 2 * kRefsBytes;  // [4 units]: bits of rows left out, kMoved
+constexpr int kSumsAt = kStateAt + 2 * 16;          // [4 units][32 query rows] of l, r
 constexpr int kStartsAt = kSumsAt + kUnits * kRows * 8;  // [requests + 1]
 constexpr int kQueriesAt = 3 * kRoundBytes;  // before a piece's fourth round is copied
 constexpr int kMaxShared = 256;   // requests whose rounds are dealt out evenly
@@ -78,6 +77,7 @@ constexpr int kLdsBytes = kStartsAt + (kMaxShared + 1) * 4;
 // What a piece costs beyond its rounds, in rounds (about 6 us of 1.5).
 constexpr int kOverhead = 4;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
+constexpr uint32_t kMoved = 1u << 16;  // the unit took references of its own
 constexpr float kHeadroom = 16.0f;
 constexpr float kRounded = 0x1p-100f;  // the rounded weights' sums: times 2^127 and this
 
@@ -147,6 +147,18 @@ __device__ __forceinline__ void copy_ahead16(const uint8_t* base, uint32_t offse
                :
                : "v"(offset), "s"(base), "s"(lds)
                : "memory", "m0");
+}
+// Four of them, each 1,024 bytes after the one before in both.
+__device__ __forceinline__ void copy_ahead16x4(const uint8_t* base, uint32_t o0, uint32_t o1,
+                                               uint32_t o2, uint32_t o3, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
+      "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+      "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
+      "global_load_lds_dwordx4 %3, %4 offset:3072"
+      :
+      : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds)
+      : "memory", "m0");
 }
 __device__ __forceinline__ void copy_ahead4(const uint8_t* base, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
@@ -257,12 +269,12 @@ struct Tree {
   __device__ __forceinline__ uint32_t buffer(int round) const {
     return lds + (round & (kBuffers - 1)) * kRoundBytes;
   }
-  __device__ __forceinline__ float ref(int round, int unit, int c) const {
-    return lds_read<float>(lds + kRefsAt + (round & 1) * kRefsBytes +
-                           4 * (kRows * unit + 16 * c + row));
+  __device__ __forceinline__ uint32_t ref_at(int round, int unit, int c) const {
+    return lds + kRefsAt + (round & 1) * kRefsBytes + 4 * (kRows * unit + 16 * c + row);
   }
-  __device__ __forceinline__ bool moved(int round) const {
-    return uniform(lds_read<int>(lds + kMovedAt + 4 * (round & 3))) != 0;
+  // Of a round's units.
+  __device__ __forceinline__ u32x4 state(int round) const {
+    return lds_read<u32x4>(lds + kStateAt + 16 * (round & 1));
   }
 };
 
@@ -348,10 +360,6 @@ struct Scorer : Tree {
            16 * lane + 8 * (of & 1);
   }
 
-  __device__ __forceinline__ uint32_t gone_at(int round) const {
-    return lds + kGoneAt + 16 * (round & 1) + 4 * of;
-  }
-
   // The unit of a round: weights to LDS, their sums to l and r, m to the references that they
   // were taken against.
   struct Rows {
@@ -399,9 +407,8 @@ struct Scorer : Tree {
                           128 * group + 16 * (row >> 2) + 2 * (4 * (of & 1) + (row & 3));
       lds_write<uint16_t>(to, (uint16_t)((254u - (two & 0xffu)) << 7));
       lds_write<uint16_t>(to + 64, (uint16_t)((254u - ((two >> 8) & 0xffu)) << 7));
-      if (lane == 0) lds_write(gone_at(round), gone);
     }
-    f32x4 acc[2][2] = {};
+    f32x4 acc[2] = {};
 #pragma unroll
     for (int s = 0; s < 7; ++s) {
       const float f = u2f(((bytes[s / 4] >> (8 * (s % 4))) & 0xffu) << 23);
@@ -409,24 +416,26 @@ struct Scorer : Tree {
       const bf16x8 k0 = codes8(v[0], v[1], f), k1 = codes8(v[2], v[3], f);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        acc[c][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, as_bf16x8(q[c][2 * s]), acc[c][0],
-                                                            0, 0, 0);
-        acc[c][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, as_bf16x8(q[c][2 * s + 1]),
-                                                            acc[c][1], 0, 0, 0);
+        acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, as_bf16x8(q[c][2 * s]), acc[c], 0, 0, 0);
       }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, as_bf16x8(q[c][2 * s + 1]), acc[c], 0, 0,
+                                                         0);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const bf16x8 k = as_bf16x8(in.key[7 + t]);
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, as_bf16x8(q[c][14 + t]), acc[c][t],
-                                                            0, 0, 0);
+        acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, as_bf16x8(q[c][14 + t]), acc[c], 0, 0, 0);
     }
     // value i is row 4 group + i of the unit
+    f32x4 s[2];
+    float top[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      f32x4 s = (acc[c][0] + acc[c][1]) * a->scale_log2;
+      s[c] = acc[c] * a->scale_log2;
       if (!kWhole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -435,16 +444,28 @@ struct Scorer : Tree {
           const bool on_path = ((word >> (node & 31)) & 1u) != 0;
           const bool see = live[c] & x.mapped & (n < stop) &
                            (x.past | (node < 0 ? p >= lowest[c] : on_path));
-          s[i] = (odd >> n) & 1u ? NAN : s[i];
-          s[i] = see ? s[i] : -INFINITY;
+          s[c][i] = (odd >> n) & 1u ? NAN : s[c][i];
+          s[c][i] = see ? s[c][i] : -INFINITY;
         }
       }
-      const float top = over_groups(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), true);
-      if (__ballot(top > m[c]) != 0) advance(c, top > m[c] ? ceilf(top) + kHeadroom : m[c]);
+      top[c] = over_groups(fmaxf(fmaxf(s[c][0], s[c][1]), fmaxf(s[c][2], s[c][3])), true);
+    }
+    uint32_t moved = 0;
+    if (__ballot((top[0] > m[0]) | (top[1] > m[1])) != 0) {
+      moved = kMoved;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        advance(c, top[c] > m[c] ? ceilf(top[c]) + kHeadroom : m[c]);
+        if (group == 0) lds_write(ref_at(round, of, c), m[c]);
+      }
+    }
+    if (lane == 0) lds_write(lds + kStateAt + 16 * (round & 1) + 4 * of, gone | moved);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
       const float ref = m[c] == -INFINITY ? 0.0f : m[c];
       f32x4 p;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[c][i] - ref);
       l[c] += (p[0] + p[1]) + (p[2] + p[3]);
       p *= 0x1p127f;
       const bf16x2 lo = bf16_pair(p[0], p[1]), hi = bf16_pair(p[2], p[3]), one = {(__bf16)kRounded,
@@ -462,15 +483,20 @@ struct Scorer : Tree {
     r[c] *= f;
     m[c] = to;
   }
-  // The highest reference of a round's units.
-  __device__ __forceinline__ void agree(int round) {
+  // The highest reference of a round's units. (Those that did not move have the one that all
+  // had before.)
+  __device__ __forceinline__ void agree(int round, const u32x4& was) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float top = m[c];
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) top = fmaxf(top, ref(round, u, c));
+      for (int u = 0; u < kUnits; ++u)
+        if (uniform((int)(was[u] & kMoved))) top = fmaxf(top, lds_read<float>(ref_at(round, u, c)));
       advance(c, top);
     }
+  }
+  __device__ __forceinline__ static bool any_moved(const u32x4& was) {
+    return (uniform((int)(was[0] | was[1] | was[2] | was[3])) & (int)kMoved) != 0;
   }
 
   __device__ __forceinline__ void run(int first_row) {
@@ -491,11 +517,11 @@ struct Scorer : Tree {
     for (int from = begin; from < end; from += kUnits, ++round) {
       const int i = uniform(from + of);
       again();
+      const u32x4 was = state(round - 1);
       const Rows in = rows(round);
-      if (round > 0 && moved(round - 1)) agree(round - 1);
+      if (round > 0 && any_moved(was)) agree(round - 1, was);
       const Unit x = unit(min(i, units - 1), page);
       if (i + kUnits < end) page = page_of(i + kUnits);
-      const float was[2] = {m[0], m[1]};
       if (i < end) {
         if (whole(x))
           score<true>(x, round, in);
@@ -504,20 +530,14 @@ struct Scorer : Tree {
       } else {  // the round's last units: nothing
 #pragma unroll
         for (int c = 0; c < 2; ++c) lds_write(weights_at(round, c), u32x2{0, 0});
-        if (lane == 0) lds_write(gone_at(round), 0xffffu);
+        if (lane == 0) lds_write(lds + kStateAt + 16 * (round & 1) + 4 * of, 0xffffu);
       }
-      if (group == 0) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          lds_write(lds + kRefsAt + (round & 1) * kRefsBytes + 4 * (kRows * of + 16 * c + row),
-                    m[c]);
-      }
-      if (__ballot(m[0] != was[0] || m[1] != was[1]) != 0 && lane == 0)
-        lds_write(lds + kMovedAt + 4 * (round & 3), 1);
-      if (threadIdx.x == 0) lds_write(lds + kMovedAt + 4 * ((round + 2) & 3), 0);
       lds_barrier();
     }
-    if (round > 0 && moved(round - 1)) agree(round - 1);
+    if (round > 0) {
+      const u32x4 was = state(round - 1);
+      if (any_moved(was)) agree(round - 1, was);
+    }
     // the row's sums; none of a row that sees nothing
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -534,7 +554,7 @@ struct Scorer : Tree {
 // Coordinates 128 g .. + 127 of all query rows: two groups of 64.
 struct Adder : Tree {
   const int g;  // and unit g's copies
-  uint32_t from[kCopies - 1];  // where the lane's piece of a copy is in the unit
+  uint32_t from[kCopies - 1];  // where the lane's piece of copy n is in the unit, less 1,024 n
   float m[2];
   f32x4 o[2][2][4];  // query rows 16 c + row, coordinates 128 g + 64 h + 16 u + 4 group + i
 
@@ -542,7 +562,7 @@ struct Adder : Tree {
 #pragma unroll
     for (int n = 0; n < kCopies - 1; ++n) {
       const uint32_t p = 64 * n + lane, r = p / 36, j = p - 36 * r;
-      from[n] = 576 * r + 16 * (j ^ turn(r));
+      from[n] = 576 * r + 16 * (j ^ turn(r)) - 1024 * n;
     }
   }
 
@@ -554,13 +574,15 @@ struct Adder : Tree {
     const uint32_t to = buffer(round) + kUnitBytes * g;
     const Unit x = unit(i, page);
     const uint8_t* const rows = x.page + x.in_page * kNativeDataBytes;
-    constexpr int kHalf = (kCopies - 1) / 2;
-#pragma unroll
-    for (int n = kPart * kHalf; n < (kPart ? kCopies - 1 : kHalf); ++n)
-      copy_ahead16(rows, from[n], to + 1024 * n);
-    if (kPart == 0 && lane < kUnit * kScaleBytes / 4)
-      copy_ahead4(x.page + kPageRecords * kNativeDataBytes + x.in_page * kScaleBytes, 4 * lane,
-                  buffer(round) + kScalesAt + kUnit * kScaleBytes * g);
+    constexpr int n = 4 * kPart;
+    copy_ahead16x4(rows + 1024 * n, from[n], from[n + 1], from[n + 2], from[n + 3], to + 1024 * n);
+    if (kPart == 0) {
+      if (lane < kUnit * kScaleBytes / 4)
+        copy_ahead4(x.page + kPageRecords * kNativeDataBytes + x.in_page * kScaleBytes, 4 * lane,
+                    buffer(round) + kScalesAt + kUnit * kScaleBytes * g);
+    } else {
+      copy_ahead16(rows + 8192, from[8], to + 8192);
+    }
   }
 
   // Eight rows of the lane's coordinate of tile u of group k, as the second product's first
@@ -586,24 +608,53 @@ struct Adder : Tree {
     return as_bf16x8(u32x4{half[0][0], half[0][1], half[1][0], half[1][1]});
   }
 
-  // O += a round. kPlain: its units' references are all m, and all of their rows count.
-  template <bool kPlain, class F>
-  __device__ __forceinline__ void add(int round, const u32x4& gone, F between) {
+  // Eight rows of the lane's coordinates of group k, as the second product's first operands,
+  // and the shifts of their scales.
+  struct Codes {
+    u32x4 shift[2];
+    bf16x8 x[2][4];
+  };
+  __device__ __forceinline__ Codes all_codes(int round, int k) const {
     const uint32_t at = buffer(round);
-    const uint32_t weights = lds + kWeightsAt + (round & 1) * kWeightsBytes + 16 * lane;
     const uint32_t shifts = lds + kShiftsAt + (round & 1) * kShiftsBytes + 128 * g + 16 * group;
-    u32x4 p[2][2], keep[2];
+    Codes in;
+    int mine = g;  // (compared again each time: kept, the result takes a register too many)
+    asm volatile("" : "+s"(mine));
+    if (k == 0 || mine < kAdders - 1) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        in.shift[v] = lds_read<u32x4>(shifts + 512 * v + 64 * k);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) in.x[v][u] = codes(at, v, k, u);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        in.shift[v] = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
+#pragma unroll
+        for (int u = 0; u < 4; ++u) in.x[v][u] = tail(at, v, u);
+      }
+    }
+    return in;
+  }
+
+  // O += a round. Plain rounds: their units' references are all m, and all of their rows count.
+  template <bool plain, class F>
+  __device__ __forceinline__ void add(int round, const u32x4& was, F between) {
+    const uint32_t weights = lds + kWeightsAt + (round & 1) * kWeightsBytes + 16 * lane;
+    u32x4 p[2][2];
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int c = 0; c < 2; ++c) p[v][c] = lds_read<u32x4>(weights + 2048 * v + 1024 * c);
-    if (!kPlain) {
+    if (!plain) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float own[kUnits], top = m[c];
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
-          own[u] = ref(round, u, c);
+          const float ref = lds_read<float>(ref_at(round, u, c));
+          own[u] = was[u] & kMoved ? ref : m[c];
           top = fmaxf(top, own[u]);
         }
 #pragma unroll
@@ -622,67 +673,51 @@ struct Adder : Tree {
 #pragma unroll
           for (int u = 0; u < 4; ++u) o[c][k][u] *= f;
       }
-      // rows 4 group .. + 3 of both units, two a dword
-#pragma unroll
-      for (int v = 0; v < 2; ++v)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t two = gone[2 * v + k / 2] >> (4 * group + 2 * (k & 1));
-          keep[v][k] = (two & 1u ? 0u : 0xffffu) | (two & 2u ? 0u : 0xffff0000u);
-        }
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      u32x4 shift[2];
-      bf16x8 x[2][4];
-      if (k == 0 || g < kAdders - 1) {
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          shift[v] = lds_read<u32x4>(shifts + 512 * v + 64 * k);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) x[v][u] = codes(at, v, k, u);
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          shift[v] = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
-#pragma unroll
-          for (int u = 0; u < 4; ++u) x[v][u] = tail(at, v, u);
-        }
-      }
+      Codes in = all_codes(round, k);
       between(k);
+      if (!plain) {
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        if (!kPlain) {
+        for (int v = 0; v < 2; ++v) {
+          u32x4 keep;  // rows 4 group .. + 3 of both units, two a dword
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t two = was[2 * v + n / 2] >> (4 * group + 2 * (n & 1));
+            keep[n] = (two & 1u ? 0u : 0xffffu) | (two & 2u ? 0u : 0xffff0000u);
+          }
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            x[v][u] = as_bf16x8(__builtin_bit_cast(u32x4, x[v][u]) & keep[v]);
+            in.x[v][u] = as_bf16x8(__builtin_bit_cast(u32x4, in.x[v][u]) & keep);
         }
+      }
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           u32x4 w;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = sub_sat(p[v][c][i], shift[v][i]);
+          for (int i = 0; i < 4; ++i) w[i] = sub_sat(p[v][c][i], in.shift[v][i]);
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            o[c][k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[v][u], as_bf16x8(w), o[c][k][u],
-                                                                 0, 0, 0);
+            o[c][k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(in.x[v][u], as_bf16x8(w),
+                                                                 o[c][k][u], 0, 0, 0);
         }
       }
     }
   }
+
   template <class F>
   __device__ __forceinline__ void add(int round, F between) {
-    const u32x4 gone = lds_read<u32x4>(lds + kGoneAt + 16 * (round & 1));
-    const int odd = lds_read<int>(lds + kMovedAt + 4 * (round & 3));
-    if (uniform((int)(gone[0] | gone[1] | gone[2] | gone[3]) | odd) == 0)
-      add<true>(round, gone, between);
+    const u32x4 was = state(round);
+    if (uniform((int)(was[0] | was[1] | was[2] | was[3])) == 0)
+      add<true>(round, was, between);
     else
-      add<false>(round, gone, between);
+      add<false>(round, was, between);
   }
 
   __device__ __forceinline__ void run(int first_row) {
-    if (threadIdx.x == 64 * kScorers) lds_write(lds + kMovedAt, u32x4{0, 0, 0, 0});
     const int i = uniform(begin + g);
     int page = 0;
     if (i < end) page = page_of(i);
@@ -857,10 +892,12 @@ __global__ __launch_bounds__(64 * (kScorers + kAdders)) void tree_decode_kernel(
       t.slot = 0, t.of_slots = 1;
       if (a->parts > 0) {
         const int at = start(b), rounds = start(b + 1) - kOverhead - at;
+        int size = share.size;  // (nor is its reciprocal kept)
+        asm volatile("" : "+s"(size));
         if (at >= share.end) break;
         from = max(share.begin - at, 0), to = min(share.end - at, rounds);
-        t.slot = part - at / share.size;
-        t.of_slots = (at + rounds - 1) / share.size - at / share.size + 1;
+        t.slot = part - at / size;
+        t.of_slots = (at + rounds - 1) / size - at / size + 1;
         if (a->counts && tile == 0 && t.slot == t.of_slots - 1 && threadIdx.x == 0)
           a->counts[b] = t.of_slots > 1 ? t.of_slots : 0;
       }

