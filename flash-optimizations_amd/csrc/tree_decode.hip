@@ -143,28 +143,28 @@ __device__ __forceinline__ float over_groups(float x, bool is_max) {
 // waited for all copies in flight before each transposed read and at each barrier (16 x 16
 // nodes 316 us with the builtin, 292 so, both then). wait_copies() and the barriers order them here.
 __device__ __forceinline__ void copy_ahead16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :
-               : "v"(offset), "s"(base), "s"(lds)
-               : "memory", "m0");
+               : "v"(offset), "s"(base), "{m0}"(lds)
+               : "memory");
 }
 // Four of them, each 1,024 bytes after the one before in both.
 __device__ __forceinline__ void copy_ahead16x4(const uint8_t* base, uint32_t o0, uint32_t o1,
                                                uint32_t o2, uint32_t o3, uint32_t lds) {
   asm volatile(
-      "s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
+      "s_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
       "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
       "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
       "global_load_lds_dwordx4 %3, %4 offset:3072"
       :
-      : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds)
-      : "memory", "m0");
+      : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "{m0}"(lds)
+      : "memory");
 }
 __device__ __forceinline__ void copy_ahead4(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1"
                :
-               : "v"(offset), "s"(base), "s"(lds)
-               : "memory", "m0");
+               : "v"(offset), "s"(base), "{m0}"(lds)
+               : "memory");
 }
 
 // What both roles know.
@@ -566,36 +566,32 @@ struct Adder : Tree {
     }
   }
 
-  // The rows of unit i, if there is one, in two parts: what there is to do between them can
-  // wait for LDS meanwhile.
-  template <int kPart>
+  // The rows of unit i, if there is one.
   __device__ __forceinline__ void copy(int i, int page, int round) const {
     if (i >= end) return;
     const uint32_t to = buffer(round) + kUnitBytes * g;
     const Unit x = unit(i, page);
     const uint8_t* const rows = x.page + x.in_page * kNativeDataBytes;
-    constexpr int n = 4 * kPart;
-    copy_ahead16x4(rows + 1024 * n, from[n], from[n + 1], from[n + 2], from[n + 3], to + 1024 * n);
-    if (kPart == 0) {
-      if (lane < kUnit * kScaleBytes / 4)
-        copy_ahead4(x.page + kPageRecords * kNativeDataBytes + x.in_page * kScaleBytes, 4 * lane,
-                    buffer(round) + kScalesAt + kUnit * kScaleBytes * g);
-    } else {
-      copy_ahead16(rows + 8192, from[8], to + 8192);
-    }
+    copy_ahead16x4(rows, from[0], from[1], from[2], from[3], to);
+    copy_ahead16x4(rows + 4096, from[4], from[5], from[6], from[7], to + 4096);
+    copy_ahead16(rows + 8192, from[8], to + 8192);
+    if (lane < kUnit * kScaleBytes / 4)
+      copy_ahead4(x.page + kPageRecords * kNativeDataBytes + x.in_page * kScaleBytes, 4 * lane,
+                  buffer(round) + kScalesAt + kUnit * kScaleBytes * g);
   }
 
-  // Eight rows of the lane's coordinate of tile u of group k, as the second product's first
-  // operand: of units 2 v and 2 v + 1, rows 4 group .. + 3 each.
-  __device__ __forceinline__ bf16x8 codes(uint32_t at, int v, int k, int u) const {
+  // Eight codes of the lane's coordinate of tile u of group k: of units 2 v and 2 v + 1, rows
+  // 4 group .. + 3 each, as the second product's first operand takes them.
+  __device__ __forceinline__ u32x2 codes(uint32_t at, int v, int k, int u) const {
     const int pair = row >> 1;  // the lane reads row 4 group + pair % 4 of unit pair / 4
     const int r = 4 * group + (pair & 3);
-    const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)(uintptr_t)(
-        at + kUnitBytes * (pair >> 2) + kNativeDataBytes * r + 128 * g + 8 * (row & 1) +
-        16 * (u ^ turn(r)) + 64 * k + 2 * kUnitBytes * v));
-    return codes8((uint32_t)x[0], (uint32_t)x[1], 1.0f);
+    return __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_void*)(uintptr_t)(
+                   at + kUnitBytes * (pair >> 2) + kNativeDataBytes * r + 128 * g +
+                   8 * (row & 1) + 16 * (u ^ turn(r)) + 64 * k + 2 * kUnitBytes * v)));
   }
-  __device__ __forceinline__ bf16x8 tail(uint32_t at, int v, int u) const {
+  // The same of the tail, which is BF16.
+  __device__ __forceinline__ u32x4 tail(uint32_t at, int v, int u) const {
     const int r = 4 * group + (row >> 2);
     u32x2 half[2];
 #pragma unroll
@@ -605,49 +601,54 @@ struct Adder : Tree {
                      at + kNativeDataBytes * r + kNopeDim + 8 * (row & 1) +
                      kUnitBytes * (2 * v + k) + 64 * (u >> 1) +
                      16 * ((2 * (u & 1) + ((row & 3) >> 1)) ^ turn(r)))));
-    return as_bf16x8(u32x4{half[0][0], half[0][1], half[1][0], half[1][1]});
+    return u32x4{half[0][0], half[0][1], half[1][0], half[1][1]};
+  }
+  // (asked again each time: kept, the answer takes a register too many)
+  __device__ __forceinline__ bool with_tail() const {
+    int mine = g;
+    asm volatile("" : "+s"(mine));
+    return mine == kAdders - 1;
   }
 
-  // Eight rows of the lane's coordinates of group k, as the second product's first operands,
-  // and the shifts of their scales.
-  struct Codes {
-    u32x4 shift[2];
-    bf16x8 x[2][4];
-  };
-  __device__ __forceinline__ Codes all_codes(int round, int k) const {
+  // O += a round, in one stretch for all rounds, with everything asked for from LDS at once and
+  // `between` while it comes. A round whose units took references of their own, or that leaves
+  // rows out, only sets its operands right first.
+  template <class F>
+  __device__ __forceinline__ void add(int round, F between) {
     const uint32_t at = buffer(round);
+    const u32x4 was = state(round);
+    const uint32_t weights = lds + kWeightsAt + (round & 1) * kWeightsBytes + 16 * lane;
     const uint32_t shifts = lds + kShiftsAt + (round & 1) * kShiftsBytes + 128 * g + 16 * group;
-    Codes in;
-    int mine = g;  // (compared again each time: kept, the result takes a register too many)
-    asm volatile("" : "+s"(mine));
-    if (k == 0 || mine < kAdders - 1) {
+    u32x4 p[2][2], shift[2][2], second[2][4];
+    u32x2 first[2][4];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) p[v][c] = lds_read<u32x4>(weights + 2048 * v + 1024 * c);
+      shift[0][v] = lds_read<u32x4>(shifts + 512 * v);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) first[v][u] = codes(at, v, 0, u);
+    }
+    if (!with_tail()) {
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        in.shift[v] = lds_read<u32x4>(shifts + 512 * v + 64 * k);
+        shift[1][v] = lds_read<u32x4>(shifts + 512 * v + 64);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) in.x[v][u] = codes(at, v, k, u);
+        for (int u = 0; u < 4; ++u) {
+          const u32x2 x = codes(at, v, 1, u);
+          second[v][u] = u32x4{x[0], x[1], 0u, 0u};
+        }
       }
     } else {
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        in.shift[v] = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
+        shift[1][v] = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
 #pragma unroll
-        for (int u = 0; u < 4; ++u) in.x[v][u] = tail(at, v, u);
+        for (int u = 0; u < 4; ++u) second[v][u] = tail(at, v, u);
       }
     }
-    return in;
-  }
-
-  // O += a round. Plain rounds: their units' references are all m, and all of their rows count.
-  template <bool plain, class F>
-  __device__ __forceinline__ void add(int round, const u32x4& was, F between) {
-    const uint32_t weights = lds + kWeightsAt + (round & 1) * kWeightsBytes + 16 * lane;
-    u32x4 p[2][2];
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) p[v][c] = lds_read<u32x4>(weights + 2048 * v + 1024 * c);
-    if (!plain) {
+    const uint32_t any = (uint32_t)uniform((int)(was[0] | was[1] | was[2] | was[3]));
+    if (any & kMoved) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float own[kUnits], top = m[c];
@@ -674,58 +675,64 @@ struct Adder : Tree {
           for (int u = 0; u < 4; ++u) o[c][k][u] *= f;
       }
     }
+    if (any & (kMoved - 1)) {
+#pragma unroll
+      for (int n = 0; n < kUnits; ++n) {  // rows 4 group .. + 3 of unit n
+        const uint32_t four = was[n] >> (4 * group);
+        const uint32_t lo = (four & 1u ? 0u : 0xffffu) | (four & 2u ? 0u : 0xffff0000u);
+        const uint32_t hi = (four & 4u ? 0u : 0xffffu) | (four & 8u ? 0u : 0xffff0000u);
+        const uint32_t bytes = (lo & 0xffu) | (lo >> 8 & 0xff00u) | (hi << 16 & 0xff0000u) |
+                               (hi & 0xff000000u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          first[n / 2][u][n % 2] &= bytes;
+          if (!with_tail()) {
+            second[n / 2][u][n % 2] &= bytes;
+          } else {
+            second[n / 2][u][2 * (n % 2)] &= lo;
+            second[n / 2][u][2 * (n % 2) + 1] &= hi;
+          }
+        }
+      }
+    }
+    between();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      Codes in = all_codes(round, k);
-      between(k);
-      if (!plain) {
+      if (k == 1 && !with_tail()) {
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          u32x4 keep;  // rows 4 group .. + 3 of both units, two a dword
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const uint32_t two = was[2 * v + n / 2] >> (4 * group + 2 * (n & 1));
-            keep[n] = (two & 1u ? 0u : 0xffffu) | (two & 2u ? 0u : 0xffff0000u);
-          }
+        for (int v = 0; v < 2; ++v)
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            in.x[v][u] = as_bf16x8(__builtin_bit_cast(u32x4, in.x[v][u]) & keep);
-        }
+            second[v][u] =
+                __builtin_bit_cast(u32x4, codes8(second[v][u][0], second[v][u][1], 1.0f));
       }
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
+        bf16x8 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          x[u] = k == 0 ? codes8(first[v][u][0], first[v][u][1], 1.0f) : as_bf16x8(second[v][u]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           u32x4 w;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = sub_sat(p[v][c][i], in.shift[v][i]);
+          for (int i = 0; i < 4; ++i) w[i] = sub_sat(p[v][c][i], shift[k][v][i]);
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            o[c][k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(in.x[v][u], as_bf16x8(w),
-                                                                 o[c][k][u], 0, 0, 0);
+            o[c][k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], as_bf16x8(w), o[c][k][u],
+                                                                 0, 0, 0);
         }
       }
     }
-  }
-
-  template <class F>
-  __device__ __forceinline__ void add(int round, F between) {
-    const u32x4 was = state(round);
-    if (uniform((int)(was[0] | was[1] | was[2] | was[3])) == 0)
-      add<true>(round, was, between);
-    else
-      add<false>(round, was, between);
   }
 
   __device__ __forceinline__ void run(int first_row) {
     const int i = uniform(begin + g);
     int page = 0;
     if (i < end) page = page_of(i);
-    copy<0>(i, page, 0);
-    copy<1>(i, page, 0);
+    copy(i, page, 0);
     if (i + kUnits < end) page = page_of(i + kUnits);
-    copy<0>(i + kUnits, page, 1);
-    copy<1>(i + kUnits, page, 1);
+    copy(i + kUnits, page, 1);
     if (i + 2 * kUnits < end) page = page_of(i + 2 * kUnits);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -737,28 +744,23 @@ struct Adder : Tree {
     }
     landed(i + kUnits);  // round 0
     lds_barrier();
-    int round = 0;
+    // scored: round; added: the one before; copied: the one after next
+    if (begin < end) {
+      const int i = uniform(begin + g) + 2 * kUnits;
+      copy(i, page, 2);
+      if (i + kUnits < end) page = page_of(i + kUnits);
+      landed(i);
+    }
+    lds_barrier();
+    int round = 1;
 #pragma clang loop unroll(disable)
     for (int from = begin; from < end; from += kUnits, ++round) {
-      // scored: round; added: the one before; copied: the one after next
-      const int i = uniform(from + g) + 2 * kUnits;
-      if (round > 0) {
-        add(round - 1, [&](int k) {
-          if (k == 0)
-            copy<0>(i, page, round + 2);
-          else
-            copy<1>(i, page, round + 2);
-        });
-      } else {
-        copy<0>(i, page, 2);
-        copy<1>(i, page, 2);
-      }
+      const int i = uniform(from + g) + 3 * kUnits;
+      add(round - 1, [&] { copy(i, page, round + 2); });
       if (i + kUnits < end) page = page_of(i + kUnits);
       landed(i);
       lds_barrier();
     }
-    if (round > 0) add(round - 1, [](int) {});
-    lds_barrier();
     anew();
     finish(first_row);
   }
