@@ -39,6 +39,7 @@
 // sees, and for rows with an infinity or NaN, whose scores are NaN where they are seen: a
 // zero weight must not meet them.
 #include <algorithm>
+#include <cmath>
 
 #include "combine.h"
 #include "lds.h"
@@ -79,7 +80,7 @@ constexpr int kOverhead = 4;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr uint32_t kMoved = 1u << 16;  // the unit took references of its own
 constexpr float kHeadroom = 16.0f;
-constexpr float kRounded = 0x1p-100f;  // the rounded weights' sums: times 2^127 and this
+constexpr float kUnit27 = 0x1p-100f;  // sums of the weights, which are times 2^127, in 2^27
 
 typedef __attribute__((address_space(4))) int32_t const_i32;  // scalar loads
 
@@ -104,7 +105,8 @@ struct TreeArgs {
   int past_blocks;
   const int32_t* past_lengths;
   const float* sink;
-  float scale_log2;
+  float scale_log2;  // not below zero
+  bool negated;      // and q times -1
   int parts;   // workgroups that share the rounds of a tile's requests; 0: a request each
   int slots;   // partials that a request can have
   uint16_t* out;
@@ -313,6 +315,10 @@ struct Scorer : Tree {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         q[c][14 + t] = lds_read<u32x4>(at + 16 * ((56 + 4 * t + group) ^ row));
+      if (a->negated) {
+#pragma unroll
+        for (int s = 0; s < 16; ++s) q[c][s] ^= 0x80008000u;
+      }
     }
   }
 
@@ -375,38 +381,37 @@ struct Scorer : Tree {
     for (int s = 0; s < 9; ++s) x.key[s] = lds_read<u32x4>(k_at + 64 * s);
     return x;
   }
+  // Bits of the unit's rows with an infinity or NaN.
+  __device__ __forceinline__ uint32_t odd_rows(int round, const u32x2& bytes) const {
+    // row `row`, pieces 9 group .. + 8
+    const uint32_t mine = buffer(round) + kUnitBytes * of + kNativeDataBytes * row + 144 * group;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int n = 0; n < 9; ++n) {
+      const u32x4 v = lds_read<u32x4>(mine + 16 * n);
+      // (pieces 28 and up are the tail)
+      const bool tail = 9 * group + n >= 28;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) bad |= special(v[k], tail);
+      if (n % 3 == 2) __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int g = 0; g < 7; ++g) bad |= ((bytes[g / 4] >> (8 * (g % 4))) & 0xffu) == 0xffu;
+    const uint64_t found = __ballot(bad != 0);
+    return (uint32_t)(found | found >> 16 | found >> 32 | found >> 48) & 0xffffu;
+  }
   template <bool kWhole>
   __device__ __forceinline__ void score(const Unit& x, int round, const Rows& in) {
     const u32x2 bytes = in.bytes;
     // rows of the unit that count
     const int stop = min(x.past ? past - x.at : held + a->nodes - x.at, kUnit);
-    uint32_t odd = 0, gone = 0;  // rows with an infinity or NaN, and with those nobody sees
-    if (!kWhole) {
-      // row `row`, pieces 9 group .. + 8: an infinity or NaN in it?
-      const uint32_t mine = buffer(round) + kUnitBytes * of + kNativeDataBytes * row + 144 * group;
-      uint32_t bad = 0;
-#pragma unroll
-      for (int n = 0; n < 9; ++n) {
-        const u32x4 v = lds_read<u32x4>(mine + 16 * n);
-        // (pieces 28 and up are the tail)
-        const bool tail = 9 * group + n >= 28;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) bad |= special(v[k], tail);
-        if (n % 3 == 2) __builtin_amdgcn_sched_barrier(0);
-      }
-#pragma unroll
-      for (int g = 0; g < 7; ++g)
-        bad |= ((bytes[g / 4] >> (8 * (g % 4))) & 0xffu) == 0xffu;
-      const uint64_t found = __ballot(bad != 0);
-      odd = (uint32_t)(found | found >> 16 | found >> 32 | found >> 48) & 0xffffu;
-      gone = x.mapped ? odd | (0xffffu << stop & 0xffffu) : 0xffffu;
-    }
     {  // shifts of row `row` for groups 2 group and 2 group + 1
       const uint32_t two = (group >= 2 ? bytes[1] : bytes[0]) >> (16 * (group & 1));
       const uint32_t to = lds + kShiftsAt + (round & 1) * kShiftsBytes + 512 * (of >> 1) +
                           128 * group + 16 * (row >> 2) + 2 * (4 * (of & 1) + (row & 3));
-      lds_write<uint16_t>(to, (uint16_t)((254u - (two & 0xffu)) << 7));
-      lds_write<uint16_t>(to + 64, (uint16_t)((254u - ((two >> 8) & 0xffu)) << 7));
+      const uint32_t both = (0x00fe00feu - ((two & 0xffu) | (two << 8 & 0xff0000u))) << 7;
+      lds_write<uint16_t>(to, (uint16_t)both);
+      lds_write<uint16_t>(to + 64, (uint16_t)(both >> 16));
     }
     f32x4 acc[2] = {};
 #pragma unroll
@@ -431,11 +436,21 @@ struct Scorer : Tree {
         acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, as_bf16x8(q[c][14 + t]), acc[c], 0, 0, 0);
     }
     // value i is row 4 group + i of the unit
-    f32x4 s[2];
+    uint32_t odd = 0, gone = 0;  // rows with an infinity or NaN, and with those nobody sees
+    if (!kWhole) {
+      // (a row with an infinity or NaN has a score like it with any query row: without one
+      // no row is looked through)
+      float none = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) none = __builtin_fmaf(acc[c][i], 0.0f, none);
+      if (__ballot(none != 0.0f) != 0) odd = odd_rows(round, bytes);
+      gone = x.mapped ? odd | (0xffffu << stop & 0xffffu) : 0xffffu;
+    }
     float top[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      s[c] = acc[c] * a->scale_log2;
       if (!kWhole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -444,11 +459,14 @@ struct Scorer : Tree {
           const bool on_path = ((word >> (node & 31)) & 1u) != 0;
           const bool see = live[c] & x.mapped & (n < stop) &
                            (x.past | (node < 0 ? p >= lowest[c] : on_path));
-          s[c][i] = (odd >> n) & 1u ? NAN : s[c][i];
-          s[c][i] = see ? s[c][i] : -INFINITY;
+          acc[c][i] *= a->scale_log2;
+          acc[c][i] = (odd >> n) & 1u ? NAN : acc[c][i];
+          acc[c][i] = see ? acc[c][i] : -INFINITY;
         }
       }
-      top[c] = over_groups(fmaxf(fmaxf(s[c][0], s[c][1]), fmaxf(s[c][2], s[c][3])), true);
+      top[c] = over_groups(
+          fmaxf(fmaxf(acc[c][0], acc[c][1]), fmaxf(acc[c][2], acc[c][3])), true);
+      if (kWhole) top[c] *= a->scale_log2;
     }
     uint32_t moved = 0;
     if (__ballot((top[0] > m[0]) | (top[1] > m[1])) != 0) {
@@ -462,14 +480,16 @@ struct Scorer : Tree {
     if (lane == 0) lds_write(lds + kStateAt + 16 * (round & 1) + 4 * of, gone | moved);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const float ref = m[c] == -INFINITY ? 0.0f : m[c];
+      const float ref = m[c] == -INFINITY ? 0.0f : m[c] - 127.0f;
       f32x4 p;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[c][i] - ref);
-      l[c] += (p[0] + p[1]) + (p[2] + p[3]);
-      p *= 0x1p127f;
-      const bf16x2 lo = bf16_pair(p[0], p[1]), hi = bf16_pair(p[2], p[3]), one = {(__bf16)kRounded,
-                                                                                  (__bf16)kRounded};
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(
+            kWhole ? __builtin_fmaf(acc[c][i], a->scale_log2, -ref) : acc[c][i] - ref);
+        l[c] = __builtin_fmaf(p[i], kUnit27, l[c]);
+      }
+      const bf16x2 lo = bf16_pair(p[0], p[1]), hi = bf16_pair(p[2], p[3]), one = {(__bf16)kUnit27,
+                                                                                  (__bf16)kUnit27};
       r[c] = __builtin_amdgcn_fdot2_f32_bf16(lo, one, r[c], false);
       r[c] = __builtin_amdgcn_fdot2_f32_bf16(hi, one, r[c], false);
       const u32x2 d = {__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
@@ -545,7 +565,7 @@ struct Scorer : Tree {
       r[c] = over_groups(r[c], false);
       if (group == 0)
         lds_write(lds + kSumsAt + 8 * (kRows * of + 16 * c + row),
-                  live[c] ? f32x2{l[c], r[c] * 0x1p-27f} : f32x2{0.0f, 0.0f});
+                  live[c] ? f32x2{l[c] * 0x1p-27f, r[c] * 0x1p-27f} : f32x2{0.0f, 0.0f});
     }
     lds_barrier();
   }
@@ -619,8 +639,8 @@ struct Adder : Tree {
     const u32x4 was = state(round);
     const uint32_t weights = lds + kWeightsAt + (round & 1) * kWeightsBytes + 16 * lane;
     const uint32_t shifts = lds + kShiftsAt + (round & 1) * kShiftsBytes + 128 * g + 16 * group;
-    u32x4 p[2][2], shift[2][2], second[2][4];
-    u32x2 first[2][4];
+    u32x4 p[2][2], shift[2][2], last[2][4];
+    u32x2 first[2][4], second[2][4];
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
 #pragma unroll
@@ -634,17 +654,14 @@ struct Adder : Tree {
       for (int v = 0; v < 2; ++v) {
         shift[1][v] = lds_read<u32x4>(shifts + 512 * v + 64);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const u32x2 x = codes(at, v, 1, u);
-          second[v][u] = u32x4{x[0], x[1], 0u, 0u};
-        }
+        for (int u = 0; u < 4; ++u) second[v][u] = codes(at, v, 1, u);
       }
     } else {
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
         shift[1][v] = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // 127 << 7
 #pragma unroll
-        for (int u = 0; u < 4; ++u) second[v][u] = tail(at, v, u);
+        for (int u = 0; u < 4; ++u) last[v][u] = tail(at, v, u);
       }
     }
     const uint32_t any = (uint32_t)uniform((int)(was[0] | was[1] | was[2] | was[3]));
@@ -689,8 +706,8 @@ struct Adder : Tree {
           if (!with_tail()) {
             second[n / 2][u][n % 2] &= bytes;
           } else {
-            second[n / 2][u][2 * (n % 2)] &= lo;
-            second[n / 2][u][2 * (n % 2) + 1] &= hi;
+            last[n / 2][u][2 * (n % 2)] &= lo;
+            last[n / 2][u][2 * (n % 2) + 1] &= hi;
           }
         }
       }
@@ -703,7 +720,7 @@ struct Adder : Tree {
         for (int v = 0; v < 2; ++v)
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            second[v][u] =
+            last[v][u] =
                 __builtin_bit_cast(u32x4, codes8(second[v][u][0], second[v][u][1], 1.0f));
       }
 #pragma unroll
@@ -711,7 +728,7 @@ struct Adder : Tree {
         bf16x8 x[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          x[u] = k == 0 ? codes8(first[v][u][0], first[v][u][1], 1.0f) : as_bf16x8(second[v][u]);
+          x[u] = k == 0 ? codes8(first[v][u][0], first[v][u][1], 1.0f) : as_bf16x8(last[v][u]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           u32x4 w;
@@ -835,41 +852,35 @@ struct Share {
   int begin, end, size;
 };
 __device__ __forceinline__ Share deal(const Tree& t, int part) {
-  constexpr int kEach = kMaxShared / 64;
   const_args* const a = t.a;
-  int rounds[kEach], sum = 0, most = 0;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = kEach * t.lane + k;
-    rounds[k] = -kOverhead;  // (past the last request: nothing)
+  int total = 0, most = 0;
+  for (int i0 = 0; i0 < a->batch; i0 += 64) {
+    const int i = i0 + t.lane;
+    int cost = 0;
     if (i < a->batch)
-      rounds[k] = Tree::rounds(
-          Tree::extent(a, a->lengths[i], a->past_lengths ? a->past_lengths[i] : 0));
-    most = max(most, rounds[k]);
-    sum += rounds[k] + kOverhead;
+      cost = kOverhead + Tree::rounds(Tree::extent(
+                             a, a->lengths[i], a->past_lengths ? a->past_lengths[i] : 0));
+    const int upto = (int)wave_prefix((uint32_t)cost);
+    // (each wave writes all of them: it waits for nobody)
+    if (i <= a->batch) lds_write(t.lds + kStartsAt + 4 * i, total + upto - cost);
+    total += __builtin_amdgcn_readlane(upto, 63);
+    most = max(most, cost - kOverhead);
   }
-  const int upto = (int)wave_prefix((uint32_t)sum);
-  const int total = __builtin_amdgcn_readlane(upto, 63) - kOverhead;
+  if (a->batch % 64 == 0) lds_write(t.lds + kStartsAt + 4 * a->batch, total);
   most = uniform((int)wave_all<true>((float)most));
   Share x;
   // (and no request in more pieces than there are slots; one can begin inside a part, but for
   // the first)
   const int cuts = max(a->slots - (a->batch > 1 ? 1 : 0), 1);
-  x.size = max(max((total + a->parts - 1) / a->parts, (most + cuts - 1) / cuts), 1);
+  x.size = max(max((total - kOverhead + a->parts - 1) / a->parts, (most + cuts - 1) / cuts), 1);
   x.begin = part * x.size;
   x.end = x.begin + x.size;
   x.first = 0;
-  int start = upto - sum;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = kEach * t.lane + k;
-    x.first += __popcll(__ballot(i < a->batch && start + rounds[k] <= x.begin));
-    if (t.wave == 0 && i <= a->batch) lds_write(t.lds + kStartsAt + 4 * i, start);
-    start += rounds[k] + kOverhead;
+  for (int i0 = 0; i0 < a->batch; i0 += 64) {
+    const int i = i0 + t.lane;
+    const int next = lds_read<int>(t.lds + kStartsAt + 4 * min(i + 1, a->batch));
+    x.first += __popcll(__ballot(i < a->batch && next - kOverhead <= x.begin));
   }
-  if (t.wave == 0 && kEach * (t.lane + 1) == a->batch && t.lane == 63)
-    lds_write(t.lds + kStartsAt + 4 * a->batch, start);
-  lds_barrier();
   return x;
 }
 
@@ -1021,7 +1032,8 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
   a.past_blocks = (int)history_blocks;
   a.past_lengths = history_blocks > 0 && history_pages > 0 ? history_lengths : nullptr;
   a.sink = sink;
-  a.scale_log2 = softmax_scale * kLog2e;
+  a.scale_log2 = std::fabs(softmax_scale) * kLog2e;
+  a.negated = softmax_scale < 0.0f;
   a.parts = p.parts;
   a.slots = p.slots;
   a.out = out;
