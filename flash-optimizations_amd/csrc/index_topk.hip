@@ -43,7 +43,8 @@ struct Shared {
   uint32_t bins[kBins];  // later the numbers, where they fit
   alignas(16) uint32_t part[5][kWaves];
   uint32_t pick[4];
-  u32x2 list[64];  // key, wave
+  u32x2 list[64];        // key, wave
+  uint32_t rank[2][64];  // list keys above it, and equal
 };
 
 // Over the wave's lanes.
@@ -188,6 +189,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     const int shift = max(bits - 11, 0);
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
     if (tid == 0) s.pick[3] = 0;
+    if (tid < 128) s.rank[tid >> 6][tid & 63] = 0;
     __syncthreads();
     each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     need -= s.pick[1];
     lo += bin << shift;
     hi = min(hi, lo + ((1u << shift) - 1));
-    if (held_in <= 64) {  // a lane each: every wave ranks them
+    if (held_in <= 64) {  // a lane each, ranked by all waves
       uint32_t n_over = 0;
       each([&](int, const uint32_t (&key)[4]) {
 #pragma unroll
@@ -237,11 +239,15 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       __syncthreads();
       const u32x2 at = lane < (int)held_in ? s.list[lane] : u32x2{0u, 0xffffu};
       uint32_t over = 0, same = 0;
-      for (int i = 0; i < (int)held_in; ++i) {
+      for (int i = wave; i < (int)held_in; i += S::kWaves) {
         const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)at[0], i);
         over += other > at[0];
         same += other == at[0];
       }
+      atomicAdd(&s.rank[0][lane], over);
+      atomicAdd(&s.rank[1][lane], same);
+      __syncthreads();
+      over = s.rank[0][lane], same = s.rank[1][lane];
       // (lanes without a key have all of the others above them)
       const int last = __builtin_ctzll(__ballot(over < need && over + same >= need));
       lo = hi = (uint32_t)__builtin_amdgcn_readlane((int)at[0], last);
