@@ -80,7 +80,7 @@ constexpr int kOverhead = 4;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr uint32_t kMoved = 1u << 16;  // the unit took references of its own
 constexpr float kHeadroom = 16.0f;
-constexpr float kUnit27 = 0x1p-100f;  // sums of the weights, which are times 2^127, in 2^27
+constexpr float kUnit27 = 0x1p-100f;  // of weights times 2^127, for their sum times 2^27
 
 typedef __attribute__((address_space(4))) int32_t const_i32;  // scalar loads
 
@@ -480,14 +480,14 @@ struct Scorer : Tree {
     if (lane == 0) lds_write(lds + kStateAt + 16 * (round & 1) + 4 * of, gone | moved);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const float ref = m[c] == -INFINITY ? 0.0f : m[c] - 127.0f;
+      const float ref = m[c] == -INFINITY ? 0.0f : m[c];
       f32x4 p;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4; ++i)
         p[i] = __builtin_amdgcn_exp2f(
             kWhole ? __builtin_fmaf(acc[c][i], a->scale_log2, -ref) : acc[c][i] - ref);
-        l[c] = __builtin_fmaf(p[i], kUnit27, l[c]);
-      }
+      l[c] += (p[0] + p[1]) + (p[2] + p[3]);
+      p *= 0x1p127f;  // (in the exponent of exp2 it would cost the argument three bits)
       const bf16x2 lo = bf16_pair(p[0], p[1]), hi = bf16_pair(p[2], p[3]), one = {(__bf16)kUnit27,
                                                                                   (__bf16)kUnit27};
       r[c] = __builtin_amdgcn_fdot2_f32_bf16(lo, one, r[c], false);
@@ -565,7 +565,7 @@ struct Scorer : Tree {
       r[c] = over_groups(r[c], false);
       if (group == 0)
         lds_write(lds + kSumsAt + 8 * (kRows * of + 16 * c + row),
-                  live[c] ? f32x2{l[c] * 0x1p-27f, r[c] * 0x1p-27f} : f32x2{0.0f, 0.0f});
+                  live[c] ? f32x2{l[c], r[c] * 0x1p-27f} : f32x2{0.0f, 0.0f});
     }
     lds_barrier();
   }
@@ -1038,8 +1038,8 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
   a.slots = p.slots;
   a.out = out;
   a.lse = lse;
-  a.ws_o = (float*)workspace;
-  a.ws_lse = (float*)workspace + (size_t)p.slots * rows * kHeadDim;
+  a.ws_o = p.slots > 1 ? (float*)workspace : nullptr;
+  a.ws_lse = p.slots > 1 ? a.ws_o + (size_t)p.slots * rows * kHeadDim : nullptr;
   a.counts = p.slots > 1 ? (int32_t*)((uint8_t*)workspace + p.counts_at) : nullptr;
   hipStream_t s = (hipStream_t)stream;
   hipLaunchKernelGGL(tree_decode_kernel, dim3((unsigned)((p.parts > 0 ? p.parts : batch) + 7) / 8 * 8 * a.tiles),
