@@ -129,6 +129,55 @@ def test_batches(batch):
     check(case.run(), case.want())
 
 
+class Ragged(Tree):
+    """A tree with given committed lengths, and histories."""
+
+    def __init__(self, lengths, *, nodes=2, heads=4, window=None, past=None, seed=0):
+        super().__init__(nodes, heads, batch=len(lengths), context=1, window=window, seed=seed)
+        self.lengths = np.asarray(lengths)
+        self.table, pages = syn.paged_requests([int(n) + nodes for n in lengths], seed, None)
+        self.pool = ref.random_native(pages + 1, seed)
+        if past is not None:
+            table, pages = syn.paged_requests([max(int(c), 1) for c in past], seed + 1, None)
+            self.past = [ref.random_native(pages + 1, seed + 5), table, np.asarray(past)]
+
+
+@pytest.mark.parametrize("batch", [2, 5, 63, 64, 65, 129, 255, 256, 257, 300])
+def test_ragged_batches(batch):
+    """Rounds of all requests are dealt out to the workgroups: shares that begin and end
+    anywhere in a request, several requests a share, and more requests than are dealt."""
+    banner(f"{batch} ragged requests")
+    rng = np.random.default_rng(batch)
+    most = 30000 // batch
+    case = Ragged(rng.integers(0, most, batch), seed=batch)
+    check(case.run(), case.want())
+    case = Ragged(rng.integers(0, most, batch), window=100, past=rng.integers(0, most, batch),
+                  nodes=3, heads=3, seed=batch + 1)
+    check(case.run(), case.want())
+
+
+@pytest.mark.parametrize("batch", [2, 7, 30])
+@pytest.mark.parametrize("at", [0, -1])
+def test_a_long_request_among_short_ones(batch, at):
+    """More shares than the workspace has places for a request's partials."""
+    banner(f"one long of {batch}, at {at}")
+    lengths = np.arange(batch) % 4
+    lengths[at] = 20000
+    case = Ragged(lengths, seed=batch)
+    check(case.run(), case.want())
+    window = Ragged(lengths[:, None].repeat(2, 1).reshape(-1)[:batch], window=64,
+                    past=lengths[::-1], seed=batch)
+    check(window.run(), window.want())
+
+
+@pytest.mark.parametrize("nodes, heads", [(1, 1024), (20, 100), (64, 33), (64, 128)])
+def test_many_tiles(nodes, heads):
+    """More tiles of query rows than fill one turn of the chip: fewer shares, down to one."""
+    banner(f"{nodes} x {heads}")
+    case = Ragged([0, 333, 100], nodes=nodes, heads=heads, window=90, past=[70, 3, 0], seed=heads)
+    check(case.run(), case.want())
+
+
 def test_padding_and_roots():
     """Padding by any number that is no parent, its descendants, trees of roots alone; a
     request without a live node."""
