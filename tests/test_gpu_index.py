@@ -240,6 +240,17 @@ def test_scores_of_many_requests():
     check_scores(case.run(), case.want())
 
 
+@pytest.mark.parametrize("heads, q_len, batch", [(64, 1, 45), (20, 3, 21), (100, 2, 13)])
+def test_scores_of_ragged_requests(heads, q_len, batch):
+    """Long and short requests in one call, where a wave takes several pages at least and
+    most waves of the short ones have none."""
+    banner(f"scores ragged {heads} heads, {q_len} queries")
+    case = Scored(heads, 21000, batch=batch, q_len=q_len, seed=batch)
+    case.lengths[q_len:] = np.minimum(case.lengths[q_len:],
+                                      np.arange(case.lengths.size - q_len) * 97 % 1500 - 3)
+    check_scores(case.run(), case.want())
+
+
 @pytest.mark.parametrize("width", [1, 63, 65, 127, 200, 700])
 def test_scores_width(width):
     """Columns fewer than the table's records, more, and no whole pages; what stands
