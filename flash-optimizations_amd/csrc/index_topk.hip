@@ -89,34 +89,36 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
   const int share = ((length + 4 * S::kWaves - 1) / (4 * S::kWaves)) * 4;
   const int begin = min(wave * share, length), end = min(begin + share, length);
   const int turns = (share + 255) / 256;
-  // A turn's scores as they are (zeros where there are none), then their keys. (In two steps,
-  // so that no turn's keys wait while loads of the next are to be issued.)
+  // A turn's scores as they are, then their keys: in two steps, and with no load left out
+  // where there is no score (the row's last whole four instead), so that the keys of one
+  // turn need not wait for the loads of another. The row's last scores that are no four
+  // (`odd`, from `rest` on) are loaded apart.
+  const bool wide = a.wide && length >= 4;
+  const int rest = wide ? length & ~3 : 0x7fffffff;
+  uint32_t odd[3];
+#pragma unroll
+  for (int c = 0; c < 3; ++c) odd[c] = f2u(from[min((length & ~3) + c, length - 1)]);
   auto load = [&](int turn, uint32_t (&x)[4]) {
     const int at = begin + 256 * turn + 4 * lane;
+    if (wide) {
+      const u32x4 v = *(const u32x4*)(from + min(at, (length - 4) & ~3));
 #pragma unroll
-    for (int c = 0; c < 4; ++c) x[c] = 0;
-    if (a.wide) {
-      if (at + 3 < end) {
-        const u32x4 v = *(const u32x4*)(from + at);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = v[c];
-      }
+      for (int c = 0; c < 4; ++c) x[c] = v[c];
     } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (at + c < end) x[c] = f2u(from[at + c]);
+      for (int c = 0; c < 4; ++c) x[c] = f2u(from[min(at + c, length - 1)]);
     }
   };
   auto keys = [&](int turn, uint32_t (&x)[4]) {
     const int at = begin + 256 * turn + 4 * lane;
-    if (a.wide && at < end && at + 3 >= end) {  // the share's last scores
+    const bool last = begin + 256 * (turn + 1) > end;
+    if (last && at == rest) {
 #pragma unroll
-      for (int c = 0; c < 3; ++c)
-        if (at + c < end) x[c] = f2u(from[at + c]);
+      for (int c = 0; c < 3; ++c) x[c] = odd[c];
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c) x[c] = key_of(u2f(x[c]));
-    if (begin + 256 * (turn + 1) > end) {
+    if (last) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) x[c] = at + c < end ? x[c] : 0u;
     }
@@ -137,25 +139,28 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       }
     }
   };
-  if constexpr (kHeld > 0) {
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (i < turns) load(i, held[i]);
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (i < turns) keys(i, held[i]);
-  }
   // The range: from the lowest of the threads' highest keys (the second highest, for more
   // than a key a thread), which enough keys reach, to the highest. Where a thread has none
   // or more are wanted, from the row's lowest key.
   uint32_t lo, hi = 0, second = 0;
-  each([&](int, const uint32_t (&key)[4]) {
+  const auto range = [&](int, const uint32_t (&key)[4]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       second = max(second, min(hi, key[c]));  // (hi is not below it: the middle of three)
       hi = max(hi, key[c]);
     }
-  });
+  };
+  if constexpr (kHeld > 0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) load(i, held[i]);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      keys(i, held[i]);
+      range(i, held[i]);
+    }
+  } else {
+    each(range);
+  }
   lo = wave_all_of(count <= kThreads ? hi : count <= 2 * kThreads ? second : 0u, least);
   hi = wave_all_of(hi, most);
   if (lane == 0) s.part[0][wave] = lo, s.part[1][wave] = hi;
