@@ -132,12 +132,16 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi, float scale) 
                          fp8_pair_to_bf16<false>(hi, scale), fp8_pair_to_bf16<true>(hi, scale)});
 }
 
+// (NaN if either is: fmaxf first quiets both, an instruction each)
+__device__ __forceinline__ float higher(float x, float y) {
+  return __builtin_elementwise_maximum(x, y);
+}
 // Over the four lanes that share lane % 16.
 __device__ __forceinline__ float over_groups(float x, bool is_max) {
   const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
-  x = is_max ? fmaxf(u2f(a[0]), u2f(a[1])) : u2f(a[0]) + u2f(a[1]);
+  x = is_max ? higher(u2f(a[0]), u2f(a[1])) : u2f(a[0]) + u2f(a[1]);
   const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
-  return is_max ? fmaxf(u2f(b[0]), u2f(b[1])) : u2f(b[0]) + u2f(b[1]);
+  return is_max ? higher(u2f(b[0]), u2f(b[1])) : u2f(b[0]) + u2f(b[1]);
 }
 
 // Copies memory -> LDS of 16 or 4 bytes a lane, from base + offset to lds + 16 or 4 lane. As
@@ -464,8 +468,9 @@ struct Scorer : Tree {
           acc[c][i] = see ? acc[c][i] : -INFINITY;
         }
       }
+      // (a NaN, whose row leaves this query row NaN, moves no reference)
       top[c] = over_groups(
-          fmaxf(fmaxf(acc[c][0], acc[c][1]), fmaxf(acc[c][2], acc[c][3])), true);
+          higher(higher(acc[c][0], acc[c][1]), higher(acc[c][2], acc[c][3])), true);
       if (kWhole) top[c] *= a->scale_log2;
     }
     uint32_t moved = 0;
