@@ -3,8 +3,8 @@
 // splits, heads] floats, to out (BF16) and lse. kNatural: the partials' coordinates
 // in their own order and any number of heads (4-bit records, trees); otherwise in
 // partial_coord() order with heads a multiple of 16 (Packed and Native). kRagged: of the
-// slots of tokens_each tokens only the first counts[token / tokens_each] hold partials; no
-// slots: the rows are finished already.
+// slots of request r's tokens only the first counts[r] hold partials; none: its rows are
+// finished already.
 #pragma once
 #include "remnant_device.h"
 
@@ -68,14 +68,13 @@ __global__ __launch_bounds__(256) void combine_wave_kernel(const float* __restri
                                                            int slots, int heads,
                                                            uint16_t* __restrict__ out,
                                                            float* __restrict__ lse,
-                                                           const int32_t* __restrict__ counts,
-                                                           int tokens_each) {
+                                                           const int32_t* __restrict__ counts) {
   const int lane = wave_lane();
-  // block (x, y): heads 4x .. 4x + 3 of token y (a token's heads are a multiple of 16)
-  const int64_t t = blockIdx.y;
+  // block (x, y, z): heads 4x .. 4x + 3 of token y (of request z, where they are ragged)
+  const int64_t t = kRagged ? blockIdx.z * gridDim.y + blockIdx.y : blockIdx.y;
   const int h = blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6));
   if (kNatural && h >= heads) return;
-  const int splits = kRagged ? uniform(counts[t / tokens_each]) : slots;
+  const int splits = kRagged ? counts[blockIdx.z] : slots;
   if (kRagged && splits == 0) return;
   const int64_t row = t * heads + h;
   const float* src = ws_o + (t * slots * heads + h) * kHeadDim + 8 * lane;
@@ -154,16 +153,15 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
                                                       const float* __restrict__ sink, int slots,
                                                       int heads, uint16_t* __restrict__ out,
                                                       float* __restrict__ lse,
-                                                      const int32_t* __restrict__ counts,
-                                                      int tokens_each) {
+                                                      const int32_t* __restrict__ counts) {
   __shared__ float part[4][64];
   const int lane = wave_lane();
   const int wave = uniform((int)(threadIdx.x >> 6));
-  // block (x, y): head x / 8 and slice x % 8 of token y
-  const int64_t t = blockIdx.y;
+  // block (x, y, z): head x / 8 and slice x % 8 of token y (of request z)
+  const int64_t t = kRagged ? blockIdx.z * gridDim.y + blockIdx.y : blockIdx.y;
   const int h = blockIdx.x / kCombineSlices;
   const int slice = blockIdx.x % kCombineSlices;
-  const int splits = kRagged ? uniform(counts[t / tokens_each]) : slots;
+  const int splits = kRagged ? counts[blockIdx.z] : slots;
   if (kRagged && splits == 0) return;
   const int64_t row = t * heads + h;
   const int64_t step = (int64_t)heads * kHeadDim;
@@ -209,7 +207,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
 template <bool kNatural, bool kRagged = false>
 void launch_combine(const float* ws_o, const float* ws_lse, const float* sink, int slots,
                     int64_t tokens, int64_t heads, uint16_t* out, float* lse, hipStream_t s,
-                    const int32_t* counts = nullptr, int64_t tokens_each = 1) {
+                    const int32_t* counts = nullptr, int64_t requests = 1) {
   // rows: one workgroup per 64 coordinates of each. In natural order also where the wave
   // form would take two turns (decode of 4-bit records, 16 tokens x 16 heads, 16 splits
   // 15.3 -> 13.1 us with it; 24 tokens, 8 splits: 16.8 with this form, 16.3 the other), but
@@ -221,9 +219,10 @@ void launch_combine(const float* ws_o, const float* ws_lse, const float* sink, i
                            : combine_kernel<16, kNatural, kRagged>)
       : slots <= 4 || kRagged ? combine_wave_kernel<4, kNatural, kRagged>
                               : combine_wave_kernel<8, kNatural, kRagged>;
-  const dim3 grid((unsigned)(few ? heads * kCombineSlices : (heads + 3) / 4), (unsigned)tokens);
+  const dim3 grid((unsigned)(few ? heads * kCombineSlices : (heads + 3) / 4),
+                  (unsigned)(tokens / requests), (unsigned)requests);
   hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, ws_o, ws_lse, sink, slots, (int)heads, out, lse,
-                     counts, (int)tokens_each);
+                     counts);
 }
 
 }  // namespace

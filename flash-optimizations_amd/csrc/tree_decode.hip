@@ -1052,7 +1052,7 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
   if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   if (p.slots > 1) {
     launch_combine<true, true>(a.ws_o, a.ws_lse, sink, p.slots, batch * nodes, heads, out, lse, s,
-                               a.counts, nodes);
+                               a.counts, batch);
     if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   }
   return RM_OK;
