@@ -65,10 +65,16 @@ __device__ __forceinline__ uint32_t below(uint64_t mask, uint32_t plus) {
                                    __builtin_amdgcn_mbcnt_lo((uint32_t)mask, plus));
 }
 
-// kHeld: turns of 4 * kThreads scores that the row's keys stay in registers for; 0: a row of
-// any length, read again for each pass.
-template <int kThreads, int kHeld>
+// A row's keys stay in registers for kHeld turns of 4 * kThreads scores. kLong: rows longer
+// than that, with kInLds turns in LDS and what is longer still read again for each pass (64
+// rows of 65,536 scores 23.6 us, 38.4 when each pass read them; 256 rows of 32,768 18.1 from
+// registers and 24.5 read). Widths up to 2,048 and 8,192 have variants of their own, whose
+// fewer turns are less code to fetch (64 rows of 8,192: 7.8 us and 9.4 with half the threads;
+// 64 rows of 2,000: 5.9, and 8.0 read).
+constexpr int kInLds = 8;
+template <int kThreads, int kHeld, bool kLong>
 __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
+  __shared__ u32x4 kept[kLong ? kInLds : 1][kLong ? kThreads : 1];
   using S = Shared<kThreads>;
   __shared__ S s;
   const int tid = (int)threadIdx.x, lane = wave_lane(), wave = uniform(tid >> 6);
@@ -123,15 +129,19 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       for (int c = 0; c < 4; ++c) x[c] = at + c < end ? x[c] : 0u;
     }
   };
-  uint32_t held[kHeld > 0 ? kHeld : 1][4];
+  uint32_t held[kHeld][4];
   // f(turn, keys) for every turn of the row
   auto each = [&](auto f) {
-    if constexpr (kHeld > 0) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i)
-        if (i < turns) f(i, held[i]);
-    } else {
-      for (int i = 0; i < turns; ++i) {
+    for (int i = 0; i < kHeld; ++i)
+      if (i < turns) f(i, held[i]);
+    if constexpr (kLong) {
+      for (int i = kHeld; i < min(turns, kHeld + kInLds); ++i) {
+        const u32x4 x = kept[i - kHeld][tid];
+        const uint32_t key[4] = {x[0], x[1], x[2], x[3]};
+        f(i, key);
+      }
+      for (int i = kHeld + kInLds; i < turns; ++i) {
         uint32_t key[4];
         load(i, key);
         keys(i, key);
@@ -150,16 +160,28 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       hi = max(hi, key[c]);
     }
   };
-  if constexpr (kHeld > 0) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) load(i, held[i]);
+  for (int i = 0; i < kHeld; ++i) load(i, held[i]);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      keys(i, held[i]);
-      range(i, held[i]);
+  for (int i = 0; i < kHeld; ++i) {
+    keys(i, held[i]);
+    range(i, held[i]);
+  }
+  if constexpr (kLong) {
+    uint32_t key[kInLds][4];
+#pragma unroll
+    for (int i = 0; i < kInLds; ++i) load(kHeld + i, key[i]);
+#pragma unroll
+    for (int i = 0; i < kInLds; ++i) {
+      keys(kHeld + i, key[i]);
+      range(kHeld + i, key[i]);
+      kept[i][tid] = u32x4{key[i][0], key[i][1], key[i][2], key[i][3]};
     }
-  } else {
-    each(range);
+    for (int i = kHeld + kInLds; i < turns; ++i) {
+      load(i, key[0]);
+      keys(i, key[0]);
+      range(i, key[0]);
+    }
   }
   lo = wave_all_of(count <= kThreads ? hi : count <= 2 * kThreads ? second : 0u, least);
   hi = wave_all_of(hi, most);
@@ -350,10 +372,10 @@ extern "C" int rm_index_topk(const float* scores, int64_t row_stride, const int3
     return RM_ERR_ALIGN;
   const TopkArgs a{scores, row_stride, lengths, (int)width, (int)k,
                    aligned(scores, 16) && (rows == 1 || row_stride % 4 == 0), indices, counts};
-  const auto kern = width <= 2048    ? index_topk_kernel<256, 2>
-                    : width <= 8192  ? index_topk_kernel<1024, 2>
-                    : width <= 32768 ? index_topk_kernel<1024, 8>
-                                     : index_topk_kernel<1024, 0>;
+  const auto kern = width <= 2048    ? index_topk_kernel<256, 2, false>
+                    : width <= 8192  ? index_topk_kernel<1024, 2, false>
+                    : width <= 32768 ? index_topk_kernel<1024, 8, false>
+                                     : index_topk_kernel<1024, 8, true>;
   hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(width <= 2048 ? 256 : 1024), 0,
                      (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;

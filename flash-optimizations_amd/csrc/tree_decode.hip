@@ -108,6 +108,7 @@ struct TreeArgs {
   float scale_log2;  // not below zero
   bool negated;      // and q times -1
   int parts;   // workgroups that share the rounds of a tile's requests; 0: a request each
+  bool each_eighth;  // an XCD takes every eighth part, not one after the other
   int slots;   // partials that a request can have
   uint16_t* out;
   float* lse;
@@ -893,10 +894,15 @@ __global__ __launch_bounds__(64 * (kScorers + kAdders)) void tree_decode_kernel(
   const_args* a = (const_args*)__builtin_amdgcn_kernarg_segment_ptr();
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
   // Workgroups go to the eight XCDs in turn: the tiles of one part, which read the same rows,
-  // go to one, so that its L2 cache serves all but the first.
-  const int at = (int)blockIdx.x >> 3;
-  const int part = at / a->tiles * 8 + ((int)blockIdx.x & 7);
-  const int tile = at % a->tiles, first_row = tile * kRows;
+  // go to one, so that its L2 cache serves all but the first. An XCD takes every eighth part if
+  // that fills none with more than its 32 CUs hold, or if there are many requests, which may
+  // come in the order of their lengths; otherwise parts that follow each other, all XCDs as
+  // many tiles (5 requests x 62 tiles: 27 us so, 50 with every eighth).
+  const int xcd = (int)blockIdx.x & 7, turn = (int)blockIdx.x >> 3;
+  const int at = a->each_eighth ? (turn / a->tiles * 8 + xcd) * a->tiles + turn % a->tiles
+                                : xcd * ((int)gridDim.x >> 3) + turn;
+  const int part = at / a->tiles;
+  const int tile = at - part * a->tiles, first_row = tile * kRows;
   Tree t(a, (uint32_t)(uintptr_t)(lds_void*)lds);
   if (part >= (a->parts > 0 ? a->parts : a->batch)) return;
   Share share = {part, 0, 0, 0};
@@ -946,7 +952,9 @@ struct Plan {
 };
 // Parts: as many as fill the chip with one turn of workgroups (one a CU, for its LDS), four
 // turns where a turn could not be filled well. With four turns of whole requests or more, a
-// request each, as in any order they fill it.
+// request each, as in any order they fill it; and with requests of few rounds, as a piece and
+// the combine cost what 6 rounds take.
+constexpr int64_t kWhole = 6;
 Plan plan(int64_t batch, int64_t nodes, int64_t heads, int64_t blocks, int64_t window,
           int64_t past_blocks) {
   const int64_t tiles = std::max<int64_t>((nodes * heads + kRows - 1) / kRows, 1);
@@ -955,7 +963,8 @@ Plan plan(int64_t batch, int64_t nodes, int64_t heads, int64_t blocks, int64_t w
   const int64_t rounds =
       std::max<int64_t>((rows + past_blocks * kPageRecords + kRound - 1) / kRound, 1);
   Plan p = {0, 1, 0, 0};
-  if (batch > kMaxShared || batch * tiles >= 1024 || rounds >= (1 << 22)) return p;
+  if (batch > kMaxShared || batch * tiles >= 1024 || rounds <= kWhole || rounds >= (1 << 22))
+    return p;
   const int64_t most = std::max<int64_t>(batch * rounds, 1);
   p.parts = (int)std::min<int64_t>(std::max<int64_t>((tiles <= 64 ? 256 : 1024) / tiles, 1), most);
   if (batch <= 1) {
@@ -1040,14 +1049,18 @@ extern "C" int rm_tree_decode_fwd(const uint16_t* q, int64_t batch, int64_t node
   a.scale_log2 = std::fabs(softmax_scale) * kLog2e;
   a.negated = softmax_scale < 0.0f;
   a.parts = p.parts;
+  a.each_eighth = p.parts > 0 ? (p.parts + 7) / 8 * a.tiles <= 32 : batch >= 64;
   a.slots = p.slots;
   a.out = out;
   a.lse = lse;
   a.ws_o = p.slots > 1 ? (float*)workspace : nullptr;
   a.ws_lse = p.slots > 1 ? a.ws_o + (size_t)p.slots * rows * kHeadDim : nullptr;
   a.counts = p.slots > 1 ? (int32_t*)((uint8_t*)workspace + p.counts_at) : nullptr;
+  const int64_t parts = p.parts > 0 ? p.parts : batch;
+  const int64_t groups = a.each_eighth ? (parts + 7) / 8 * 8 * a.tiles
+                                       : (parts * a.tiles + 7) / 8 * 8;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(tree_decode_kernel, dim3((unsigned)((p.parts > 0 ? p.parts : batch) + 7) / 8 * 8 * a.tiles),
+  hipLaunchKernelGGL(tree_decode_kernel, dim3((unsigned)groups),
                      dim3(64 * (kScorers + kAdders)), 0, s, a);
   if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
   if (p.slots > 1) {
