@@ -283,8 +283,14 @@ extern "C" int rm_index_scores(const uint16_t* q, int64_t batch, int64_t q_len, 
   ScoreArgs a{q, weights, (int)q_len, (int)heads, pool, (int)pool_pages, block_table,
               block_table_stride, pool_pages > 0 ? (int)max_blocks : 0, lengths, width, out,
               (int)((width + kPageRecords - 1) / kPageRecords), 0, 1};
-  const int tokens = q_len > 1 && heads <= 64 ? 2 : 1;
-  const bool apart = q_len >= 8 * kWaves;
+  // Tokens of a wave: as many as make eight tiles of heads, as each page is converted for all
+  // of them at once (3 x 257 tokens of 32 heads, 25,286 records: 156 us; 185 with two), or two
+  // if there is not that much to do (4 tokens of 32 heads, 999 records: 5.7 us; 7.3 with four).
+  const int tiles = heads <= 16 ? 1 : heads <= 32 ? 2 : heads <= 64 ? 4 : 8;
+  const int full = 8 / tiles;
+  const bool much = batch * q_len * a.pages >= 16384;
+  const int tokens = q_len >= full && (much || full <= 2) ? full : q_len > 1 ? 2 : 1;
+  const bool apart = q_len >= 8 * kWaves && tokens == full;
   a.groups = (int)((q_len + tokens * (apart ? kWaves : 1) - 1) / (tokens * (apart ? kWaves : 1)));
   const int64_t rows = batch * a.groups;
   const int64_t turns = (a.pages + (apart ? 1 : kWaves) - 1) / (apart ? 1 : kWaves);
@@ -292,16 +298,24 @@ extern "C" int rm_index_scores(const uint16_t* q, int64_t batch, int64_t q_len, 
   // heads in registers and three or more with fewer (64 ragged requests: 2,048 23.6 us,
   // 1,536 24.7, 1,024 28.9; 128 requests of 2 tokens: 1,024 145 us, 2,048 151, 512 142).
   // A wave takes four pages at least once there are that many, as its heads cost it about
-  // as much as one (64 ragged requests, of two pages 26.9 us, of six 28.9).
-  const int64_t most = tokens * heads > 64 ? 1024 : 2048;
-  const int64_t splits = std::min<int64_t>(turns, std::max<int64_t>(1, most / rows));
-  a.least = (int)std::min<int64_t>(std::max<int64_t>(rows * a.pages / 4096, 1), 4);
-  const auto pick = [&](auto one, auto two, auto more) { return apart ? more : tokens == 2 ? two : one; };
+  // as much as one (64 ragged requests, of two pages 26.9 us, of six 28.9), and where it codes
+  // all of them itself as much as three (3 x 257 tokens, 333 records: 19.0 us; 25.4 of one).
+  const int64_t most = tokens * tiles >= 8 ? 1024 : 2048;
+  int64_t splits = std::min<int64_t>(turns, std::max<int64_t>(1, most / rows));
+  a.least = (int)std::min<int64_t>(std::max<int64_t>(rows * a.pages / (apart ? 256 : 4096), 1), 4);
+  if (apart) splits = std::min<int64_t>(splits, std::max<int64_t>(1, a.pages / a.least));
+  const auto pick = [&](auto one, auto two, auto more, auto many) {
+    return apart ? many : tokens > 2 ? more : tokens == 2 ? two : one;
+  };
   const auto kern =
-      heads <= 16   ? pick(index_scores_kernel<1, 1, false>, index_scores_kernel<1, 2, false>, index_scores_kernel<1, 2, true>)
-      : heads <= 32 ? pick(index_scores_kernel<2, 1, false>, index_scores_kernel<2, 2, false>, index_scores_kernel<2, 2, true>)
-      : heads <= 64 ? pick(index_scores_kernel<4, 1, false>, index_scores_kernel<4, 2, false>, index_scores_kernel<4, 2, true>)
-                    : pick(index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, true>);
+      tiles == 1   ? pick(index_scores_kernel<1, 1, false>, index_scores_kernel<1, 2, false>,
+                          index_scores_kernel<1, 8, false>, index_scores_kernel<1, 8, true>)
+      : tiles == 2 ? pick(index_scores_kernel<2, 1, false>, index_scores_kernel<2, 2, false>,
+                          index_scores_kernel<2, 4, false>, index_scores_kernel<2, 4, true>)
+      : tiles == 4 ? pick(index_scores_kernel<4, 1, false>, index_scores_kernel<4, 2, false>,
+                          index_scores_kernel<4, 2, false>, index_scores_kernel<4, 2, true>)
+                   : pick(index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, false>,
+                          index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, true>);
   hipLaunchKernelGGL(kern, dim3((unsigned)splits, (unsigned)rows), dim3(64 * kWaves), 0,
                      (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
