@@ -1,13 +1,19 @@
 // Selection of the k highest of each row's first length scores, as ascending record
 // numbers: equal scores go to the lowest records, NaN counts as -inf.
 //
-// A workgroup takes a row. Scores become keys whose unsigned order is theirs. The k-th
-// highest key lies in [lo, hi], at first the row's smallest and largest; a histogram of
-// that range in 2,048 equal bins (in LDS) finds its bin, which is the next range, until
-// the bin is taken whole or is one key: at most three histograms, as each leaves 11 bits
-// fewer. Range by range and not by fixed digits, since scores of one query share most of
-// their leading bits. Then every wave counts what it takes of each turn of 256 scores,
-// a scan over turns and waves gives the places, and the numbers are written in order.
+// A workgroup takes a row. Scores become keys whose unsigned order is theirs, held in
+// registers (and LDS, for long rows): the row is read once. The k-th highest key lies in
+// [lo, hi]: from the lowest of the threads' highest or second highest keys, which enough
+// keys reach (it leaves a quarter of a row of ordinary scores), to the highest. A histogram of
+// that range in 2,048 equal bins (in LDS) finds its bin; a bin of up to 64 keys is listed
+// and ranked, a larger one is the next range: at most three histograms, as each leaves 11
+// bits fewer. Range by range and not by fixed digits, since scores of one query share most
+// of their leading bits. A wave's scores stand together, so that each wave knows its places
+// from one count a wave; numbers are put in order in LDS and written side by side.
+//
+// Bound by vector operations, about thirty a key of which seven make it and find the range
+// while the row comes (256 rows of 32,768: 16.5 us, of which 3.3 are loads; 64 such ragged
+// rows 11.9, on 64 of 256 CUs; one of 8,192 6.3, a launch and six barriers).
 #include <algorithm>
 
 #include "remnant_device.h"
