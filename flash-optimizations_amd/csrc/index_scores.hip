@@ -52,6 +52,7 @@ struct ScoreArgs {
   int pages;   // of a row of out
   int groups;  // workgroups along the tokens of a request
   int least;   // pages that a wave takes at least, if there are
+  int splits;  // workgroups of a row of them
 };
 
 __device__ __forceinline__ uint32_t over_groups_top(uint32_t x) {
@@ -114,8 +115,10 @@ __global__ __launch_bounds__(64 * kWaves, kTiles * kTokens >= 8 ? 2 : kTiles >= 
   __shared__ f32x4 head_weights[kApart ? kWaves : 1][kTokens * kTiles][4];
   const int lane = wave_lane(), row = lane & 15, group = lane >> 4;
   const int wave = uniform((int)(threadIdx.x >> 6));
-  const int b = (int)blockIdx.y / a.groups;
-  const int of = (int)blockIdx.y - b * a.groups;
+  const int row_of_groups = (int)(blockIdx.x / (uint32_t)a.splits);
+  const int split = (int)blockIdx.x - row_of_groups * a.splits;
+  const int b = row_of_groups / a.groups;
+  const int of = row_of_groups - b * a.groups;
   const int t0 = of * kTokens * (kApart ? kWaves : 1) + (kApart ? wave * kTokens : 0);
   if (t0 >= a.q_len) return;
   const int64_t first = (int64_t)b * a.q_len + t0;  // row of q, lengths and out
@@ -131,8 +134,8 @@ __global__ __launch_bounds__(64 * kWaves, kTiles * kTokens >= 8 ? 2 : kTiles >= 
   }
   const int live = (most + kPageRecords - 1) / kPageRecords;  // pages to score
   // of `of_all` waves (workgroups) that take pages in turn, `working` have scores to find
-  const int of_all = (int)gridDim.x * (kApart ? 1 : kWaves);
-  const int turn = (int)((blockIdx.x + blockIdx.y) % gridDim.x);
+  const int of_all = a.splits * (kApart ? 1 : kWaves);
+  const int turn = (split + row_of_groups) % a.splits;
   const int start = kApart ? turn : turn * kWaves;
   const int me = start + (kApart ? 0 : wave);
   int working = of_all;
@@ -282,7 +285,7 @@ extern "C" int rm_index_scores(const uint16_t* q, int64_t batch, int64_t q_len, 
     return RM_ERR_ALIGN;
   ScoreArgs a{q, weights, (int)q_len, (int)heads, pool, (int)pool_pages, block_table,
               block_table_stride, pool_pages > 0 ? (int)max_blocks : 0, lengths, width, out,
-              (int)((width + kPageRecords - 1) / kPageRecords), 0, 1};
+              (int)((width + kPageRecords - 1) / kPageRecords), 0, 1, 1};
   // Tokens of a wave: as many as make eight tiles of heads, as each page is converted for all
   // of them at once (3 x 257 tokens of 32 heads, 25,286 records: 156 us; 185 with two), or two
   // if there is not that much to do (4 tokens of 32 heads, 999 records: 5.7 us; 7.3 with four).
@@ -304,6 +307,7 @@ extern "C" int rm_index_scores(const uint16_t* q, int64_t batch, int64_t q_len, 
   int64_t splits = std::min<int64_t>(turns, std::max<int64_t>(1, most / rows));
   a.least = (int)std::min<int64_t>(std::max<int64_t>(rows * a.pages / (apart ? 256 : 4096), 1), 4);
   if (apart) splits = std::min<int64_t>(splits, std::max<int64_t>(1, a.pages / a.least));
+  a.splits = (int)splits;
   const auto pick = [&](auto one, auto two, auto more, auto many) {
     return apart ? many : tokens > 2 ? more : tokens == 2 ? two : one;
   };
@@ -316,7 +320,7 @@ extern "C" int rm_index_scores(const uint16_t* q, int64_t batch, int64_t q_len, 
                           index_scores_kernel<4, 2, false>, index_scores_kernel<4, 2, true>)
                    : pick(index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, false>,
                           index_scores_kernel<8, 1, false>, index_scores_kernel<8, 1, true>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)splits, (unsigned)rows), dim3(64 * kWaves), 0,
+  hipLaunchKernelGGL(kern, dim3((unsigned)(splits * rows)), dim3(64 * kWaves), 0,
                      (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
 }

@@ -251,6 +251,24 @@ def test_scores_of_ragged_requests(heads, q_len, batch):
     check_scores(case.run(), case.want())
 
 
+def test_scores_of_more_tokens_than_a_grid_dimension():
+    """33,000 requests of 3 tokens are 66,000 rows of workgroups."""
+    banner("scores 33,000 requests")
+    batch, q_len = 33000, 3
+    rng = np.random.default_rng(4)
+    pool = random_pool(3, 4)
+    q = (torch.randn(batch, q_len, 1, KEY, generator=torch.Generator().manual_seed(4)) * 2).bfloat16()
+    weights = rng.standard_normal((batch, q_len, 1)).astype(np.float32)
+    table = rng.integers(0, 3, (batch, 1))
+    lengths = rng.integers(0, 6, batch * q_len)
+    got = remnant.index_scores(q.to(DEV), gpu(weights), gpu(pool), gpu(table, I32),
+                               gpu(lengths, I32), out=torch.empty(batch, q_len, 5, device=DEV))
+    some = np.concatenate([np.arange(40), rng.integers(40, batch, 200), np.arange(batch - 40, batch)])
+    want = ref.scores(q[some], weights[some], pool, table[some],
+                      lengths.reshape(batch, q_len)[some].reshape(-1), 5)
+    check_scores(got[torch.from_numpy(some).to(DEV)], want)
+
+
 @pytest.mark.parametrize("width", [1, 63, 65, 127, 200, 700])
 def test_scores_width(width):
     """Columns fewer than the table's records, more, and no whole pages; what stands
