@@ -167,16 +167,17 @@ __device__ __forceinline__ void copy_ahead16(const uint8_t* base, uint32_t offse
                : "v"(offset), "s"(base), "{m0}"(lds)
                : "memory");
 }
-// Four of them, each 1,024 bytes after the one before in both.
+// Four of them, each 1,024 bytes after the one before (an instruction's offset counts in both).
 __device__ __forceinline__ void copy_ahead16x4(const uint8_t* base, uint32_t o0, uint32_t o1,
                                                uint32_t o2, uint32_t o3, uint32_t lds) {
   asm volatile(
       "s_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
-      "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
-      "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
-      "global_load_lds_dwordx4 %3, %4 offset:3072"
+      "global_load_lds_dwordx4 %1, %4 offset:%6\n\t"
+      "global_load_lds_dwordx4 %2, %4 offset:%7\n\t"
+      "global_load_lds_dwordx4 %3, %4 offset:%8"
       :
-      : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "{m0}"(lds)
+      : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "{m0}"(lds), "n"(1024), "n"(2 * 1024),
+        "n"(3 * 1024)
       : "memory");
 }
 __device__ __forceinline__ void copy_ahead4(const uint8_t* base, uint32_t offset, uint32_t lds) {
