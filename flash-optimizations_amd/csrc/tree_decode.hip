@@ -594,7 +594,7 @@ struct Scorer : Tree {
 struct Adder : Tree {
   const int g;  // and unit g's copies
   uint32_t from[kCopies - 1];  // where the lane's piece of copy n is in the unit, less 1,024 n
-  float m[2];
+  float m[2], sink[2];
   f32x4 o[2][2][4];  // query rows 16 c + row, coordinates 128 g + 64 h + 16 u + 4 group + i
 
   __device__ __forceinline__ Adder(const Tree& t) : Tree(t), g(wave - kScorers) {
@@ -778,7 +778,14 @@ struct Adder : Tree {
 #pragma unroll
         for (int u = 0; u < 4; ++u) o[c][k][u] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    landed(i + kUnits);  // round 0
+    // (for the end, so that it need not wait for them: 7 trees of 5 nodes 13.0 us, 12.6 so)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      sink[c] = -INFINITY;
+      const int at = first_row + 16 * c + row;
+      if (a->sink && of_slots == 1 && at < a->q_rows) sink[c] = a->sink[at % a->heads];
+    }
+    landed(i + kUnits);  // round 0 (and what was asked for besides counts as round 1's)
     lds_barrier();
     // scored: round; added: the one before; copied: the one after next
     if (begin < end) {
@@ -840,7 +847,7 @@ struct Adder : Tree {
                                        : -INFINITY;
         continue;
       }
-      const float sink2 = a->sink ? a->sink[h] * kLog2e : -INFINITY;
+      const float sink2 = sink[c] * kLog2e;
       const float top = fmaxf(sum != 0.0f ? m[c] : -INFINITY, sink2);
       float f = 0.0f, lse = -INFINITY;
       if (top != -INFINITY || sum != 0.0f) {
