@@ -42,6 +42,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ uint32_t least(uint32_t x, uint32_t y) { return min(x, y); }
 __device__ __forceinline__ uint32_t most(uint32_t x, uint32_t y) { return max(x, y); }
+__device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y) { return x + y; }
 
 template <int kThreads>
 struct Shared {
@@ -53,13 +54,17 @@ struct Shared {
   uint32_t rank[2][64];  // list keys above it, and equal
 };
 
-// Over the wave's lanes.
+// Over each row of 16 lanes, and over the wave's lanes.
 template <class F>
-__device__ __forceinline__ uint32_t wave_all_of(uint32_t x, F op) {
+__device__ __forceinline__ uint32_t row_all_of(uint32_t x, F op) {
   x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, false));
   x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, false));
   x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, false));
-  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, false));
+  return op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, false));
+}
+template <class F>
+__device__ __forceinline__ uint32_t wave_all_of(uint32_t x, F op) {
+  x = row_all_of(x, op);
   const auto h = __builtin_amdgcn_permlane16_swap(x, x, false, false);
   x = op(h[0], h[1]);
   const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
@@ -193,11 +198,11 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
   hi = wave_all_of(hi, most);
   if (lane == 0) s.part[0][wave] = lo, s.part[1][wave] = hi;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < S::kWaves; ++w) {
-    lo = min(lo, s.part[0][w]);
-    hi = max(hi, s.part[1][w]);
-  }
+  const int other = lane & (S::kWaves - 1);  // a wave a lane, in each row of 16
+  const bool earlier = other < wave && (lane & 15) < S::kWaves;
+  static_assert(S::kWaves <= 16, "a row of lanes");
+  lo = uniform((int)row_all_of(s.part[0][other], least));
+  hi = uniform((int)row_all_of(s.part[1][other], most));
   if (lo == 0) {
     lo = 0xffffffffu;
     each([&](int, const uint32_t (&key)[4]) {
@@ -207,9 +212,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     lo = wave_all_of(lo, least);
     if (lane == 0) s.part[2][wave] = lo;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < S::kWaves; ++w) lo = min(lo, s.part[2][w]);
-    lo += 1;
+    lo = uniform((int)row_all_of(s.part[2][other], least)) + 1;
   }
   // need: how many of [lo, hi] are taken; those above hi are taken whole
   uint32_t need = (uint32_t)count;
@@ -241,9 +244,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     const uint32_t upto = wave_prefix(sum);
     if (lane == 63) s.part[0][wave] = upto;
     __syncthreads();
-    uint32_t before = upto - sum;
-#pragma unroll
-    for (int w = 0; w < S::kWaves; ++w) before += w < wave ? s.part[0][w] : 0u;
+    uint32_t before = upto - sum + row_all_of(earlier ? s.part[0][other] : 0u, plus);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if (before < need && before + mine[i] >= need) {
@@ -288,8 +289,7 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
       whole = need == (uint32_t)__builtin_amdgcn_readlane((int)same, last);
       above = __popcll(__ballot(at[0] > hi && (int)at[1] < wave));
       ties = __popcll(__ballot(at[0] == hi && (int)at[1] < wave));
-#pragma unroll
-      for (int w = 0; w < S::kWaves; ++w) above += w < wave ? s.part[3][w] : 0u;
+      above += row_all_of(earlier ? s.part[3][other] : 0u, plus);
       counted = true;
       break;
     }
@@ -311,11 +311,8 @@ __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
     });
     if (lane == 0) s.part[3][wave] = n_over, s.part[4][wave] = n_same;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < S::kWaves; ++w) {
-      above += w < wave ? s.part[3][w] : 0u;
-      ties += w < wave ? s.part[4][w] : 0u;
-    }
+    above += row_all_of(earlier ? s.part[3][other] : 0u, plus);
+    ties += row_all_of(earlier ? s.part[4][other] : 0u, plus);
   }
   if (whole) above += ties;
   auto number = [&](auto put) {
