@@ -12,8 +12,8 @@
 // from one count a wave; numbers are put in order in LDS and written side by side.
 //
 // Bound by vector operations, about thirty a key of which seven make it and find the range
-// while the row comes (256 rows of 32,768: 16.5 us, of which 3.3 are loads; 64 such ragged
-// rows 11.9, on 64 of 256 CUs; one of 8,192 6.3, a launch and six barriers).
+// while the row comes (256 rows of 32,768: 16.1 us, of which 3.3 are loads; 64 such ragged
+// rows 11.5, on 64 of 256 CUs; one of 8,192 6.0, a launch and six barriers).
 #include <algorithm>
 
 #include "remnant_device.h"
@@ -76,12 +76,11 @@ __device__ __forceinline__ uint32_t below(uint64_t mask, uint32_t plus) {
                                    __builtin_amdgcn_mbcnt_lo((uint32_t)mask, plus));
 }
 
-// A row's keys stay in registers for kHeld turns of 4 * kThreads scores. kLong: rows longer
-// than that, with kInLds turns in LDS and what is longer still read again for each pass (64
-// rows of 65,536 scores 23.6 us, 38.4 when each pass read them; 256 rows of 32,768 18.1 from
-// registers and 24.5 read). Widths up to 2,048 and 8,192 have variants of their own, whose
-// fewer turns are less code to fetch (64 rows of 8,192: 7.8 us and 9.4 with half the threads;
-// 64 rows of 2,000: 5.9, and 8.0 read).
+// A row's keys stay in registers for kHeld turns of 4 * kThreads scores: as few as hold the
+// width, as a turn more is code to fetch and keys to make (1,430 rows of 16,384: 35 us with
+// four turns, 65 with eight). kLong: longer rows, with kInLds turns in LDS and what is longer
+// still read again for each pass (64 rows of 65,536 23.6 us, 38.4 when each pass read them;
+// 256 rows of 32,768 18.1 from registers and 24.5 read).
 constexpr int kInLds = 8;
 template <int kThreads, int kHeld, bool kLong>
 __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {
@@ -375,11 +374,19 @@ extern "C" int rm_index_topk(const float* scores, int64_t row_stride, const int3
     return RM_ERR_ALIGN;
   const TopkArgs a{scores, row_stride, lengths, (int)width, (int)k,
                    aligned(scores, 16) && (rows == 1 || row_stride % 4 == 0), indices, counts};
+  // Threads: a wave's own work (scans, barriers) is most of a short row's, so that fewer are
+  // better for short rows and, once the chip is full, for longer ones, as long as two keys a
+  // thread reach k (one row of 4,096, k = 512: 4.7 us with half of the threads, 6.3 with all;
+  // 1,430 rows of 8,192, 512 of each: 18.2 and 21.6, 2,048 of each: 26.9 and 23.3).
+  const bool half = k <= 1024 && (width <= 4096 || (rows >= 1024 && width <= 8192));
   const auto kern = width <= 2048    ? index_topk_kernel<256, 2, false>
+                    : half           ? width <= 4096 ? index_topk_kernel<512, 2, false>
+                                                     : index_topk_kernel<512, 4, false>
                     : width <= 8192  ? index_topk_kernel<1024, 2, false>
+                    : width <= 16384 ? index_topk_kernel<1024, 4, false>
                     : width <= 32768 ? index_topk_kernel<1024, 8, false>
                                      : index_topk_kernel<1024, 8, true>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(width <= 2048 ? 256 : 1024), 0,
+  hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(width <= 2048 ? 256 : half ? 512 : 1024), 0,
                      (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
 }

@@ -359,6 +359,26 @@ def test_topk_sizes(width):
     check_topk(x, None, min(64, width))
 
 
+@pytest.mark.parametrize("width", [4095, 4096, 4097, 8192, 16384, 16385, 65536, 65537])
+def test_topk_around_the_threads_and_turns(width):
+    """Both sides of the widths and of the k that other numbers of threads, turns and places
+    for the keys begin at."""
+    banner(f"topk around {width}")
+    rng = np.random.default_rng(width)
+    x = gpu(rng.standard_normal((3, width)).astype(np.float32))
+    lengths = np.array([width, width - 1, width // 3])
+    for k in (1, 512, 1024, 1025, 2048, 2049):
+        check_topk(x, lengths, k)
+
+
+@pytest.mark.parametrize("rows", [1023, 1024])
+def test_topk_of_a_full_chip(rows):
+    banner(f"topk of {rows} rows of 5,000")
+    rng = np.random.default_rng(rows)
+    x = gpu(rng.standard_normal((rows, 5000)).astype(np.float32))
+    check_topk(x, rng.integers(0, 5001, rows), 300)
+
+
 def shapes(rng, n):
     """Rows that a histogram of equal bins finds hard."""
     x = np.zeros((20, n), np.float32)
