@@ -86,9 +86,9 @@ constexpr int kStartsAt = kSumsAt + kUnits * kRows * 8;  // [requests + 1]
 constexpr int kQueriesAt = 3 * kRoundBytes;  // before a piece's fourth round is copied
 constexpr int kMaxShared = 256;   // requests whose rounds are dealt out evenly
 constexpr int kLdsBytes = kStartsAt + (kMaxShared + 1) * 4;
-// What a piece costs beyond its rounds, in rounds (about 6 us; window trees 36.8 us with two,
-// 35.3 with four, 34.6 with six, large ones the same).
-constexpr int kOverhead = 4;
+// What a piece costs beyond its rounds, in rounds (about 7 us of 1.35; window trees 36.8 us
+// with two, 35.3 with four, 34.6 with six, large ones the same).
+constexpr int kOverhead = 6;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr uint32_t kMoved = 1u << 16;  // the unit took references of its own
 constexpr float kHeadroom = 16.0f;
