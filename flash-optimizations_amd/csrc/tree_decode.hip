@@ -22,7 +22,7 @@
 //     Weights stand as P * 2^127 in BF16, and (254 - scale byte) << 7 is subtracted as
 //     integers, saturating at zero: exact for every byte but 255, whose row has NaN scores;
 //     what falls below 2^-126 becomes zero. The adders also copy the rows of the round after
-//     next to LDS as they are stored (global_load_lds), in between their products.
+//     next to LDS as they are stored (global_load_lds), while a round's operands come.
 // One barrier a round. m is a whole number of log2 units, kept 16 above the largest score of
 // the round that set it, so that it hardly ever moves again; a unit with a score above it
 // takes its own for that round. After it the scorers go on from the highest of the units',
