@@ -160,9 +160,11 @@ __device__ __forceinline__ float over_groups(float x, bool is_max) {
 // Copies memory -> LDS of 16 or 4 bytes a lane, from base + offset to lds + 16 or 4 lane. As
 // assembly, because the compiler orders the builtin's writes to LDS by waits of its own: it
 // waited for all copies in flight before each transposed read and at each barrier (16 x 16
-// nodes 316 us with the builtin, 292 so, both then). wait_copies() and the barriers order them here.
+// nodes 316 us with the builtin, 292 so, both then). wait_copies() and the barriers order
+// them here. (s_nop 4: a base that a vector instruction wrote, as one that was spilled is, may
+// be read five wait states later; the compiler counts them for its own instructions only.)
 __device__ __forceinline__ void copy_ahead16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                :
                : "v"(offset), "s"(base), "{m0}"(lds)
                : "memory");
@@ -171,7 +173,7 @@ __device__ __forceinline__ void copy_ahead16(const uint8_t* base, uint32_t offse
 __device__ __forceinline__ void copy_ahead16x4(const uint8_t* base, uint32_t o0, uint32_t o1,
                                                uint32_t o2, uint32_t o3, uint32_t lds) {
   asm volatile(
-      "s_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
+      "s_nop 4\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
       "global_load_lds_dwordx4 %1, %4 offset:%6\n\t"
       "global_load_lds_dwordx4 %2, %4 offset:%7\n\t"
       "global_load_lds_dwordx4 %3, %4 offset:%8"
@@ -181,7 +183,7 @@ __device__ __forceinline__ void copy_ahead16x4(const uint8_t* base, uint32_t o0,
       : "memory");
 }
 __device__ __forceinline__ void copy_ahead4(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1"
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1"
                :
                : "v"(offset), "s"(base), "{m0}"(lds)
                : "memory");
