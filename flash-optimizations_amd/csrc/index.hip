@@ -19,6 +19,9 @@ using namespace rm;
 namespace {
 
 constexpr int kWaves = 4;
+// Rows of a launch of the store. A launch has fewer than 2^32 threads (2^28 rows): with more
+// the count wraps, without an error.
+constexpr int64_t kLaunchRows = (int64_t)1 << 27;
 
 template <int kCtrl>
 __device__ __forceinline__ float dpp(float x) {
@@ -202,12 +205,18 @@ extern "C" int rm_index_store_rows(const void* x, int x_dtype, int64_t x_row_str
       !aligned(pool, 16) || !aligned(weight, 16) || !aligned(freqs, 16) || !aligned(dst_slot, 4) ||
       !aligned(position, 4))
     return RM_ERR_ALIGN;
-  const StoreArgs a{x, x_row_stride, weight, eps, dst_slot, position, freqs, freq_rows, n, pool,
-                    pool_pages * kPageRecords, (uint32_t)ratio};
-  const unsigned blocks = (unsigned)((n + 4 * kWaves - 1) / (4 * kWaves));
-  hipLaunchKernelGGL(x_dtype == RM_BF16 ? index_store_kernel<true> : index_store_kernel<false>,
-                     dim3(blocks), dim3(64 * kWaves), 0, (hipStream_t)stream, a);
-  return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
+  const int64_t row_bytes = x_row_stride * (x_dtype == RM_BF16 ? 2 : 4);
+  for (int64_t at = 0; at < n; at += kLaunchRows) {
+    const int64_t rows = std::min(n - at, kLaunchRows);
+    const StoreArgs a{(const uint8_t*)x + at * row_bytes, x_row_stride, weight, eps, dst_slot + at,
+                      freqs ? position + at : nullptr, freqs, freq_rows, rows, pool,
+                      pool_pages * kPageRecords, (uint32_t)ratio};
+    const unsigned blocks = (unsigned)((rows + 4 * kWaves - 1) / (4 * kWaves));
+    hipLaunchKernelGGL(x_dtype == RM_BF16 ? index_store_kernel<true> : index_store_kernel<false>,
+                       dim3(blocks), dim3(64 * kWaves), 0, (hipStream_t)stream, a);
+    if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
+  }
+  return RM_OK;
 }
 
 extern "C" int rm_index_gather_bf16(const uint8_t* pool, int64_t pool_pages, const int32_t* slots,

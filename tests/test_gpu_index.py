@@ -141,6 +141,26 @@ def test_store_and_reader_past_4_gib():
     check_scores(got, ref.scores(q, w.numpy(), small, np.array([[0, 1]]), [84], 128))
 
 
+def test_store_of_more_rows_than_a_launch():
+    """2^28 rows, 16 a workgroup of 256 threads, likewise; most have no slot."""
+    banner("store 2^28 + 21 rows")
+    rows = (1 << 28) + 21
+    x = torch.empty(rows, KEY, dtype=torch.bfloat16, device=DEV)  # 69 GB
+    slots = torch.full((rows,), -1, dtype=I32, device=DEV)
+    at = [0, 1, (1 << 27) - 1, 1 << 27, (1 << 28) - 1, 1 << 28, rows - 1]
+    some = keys(len(at), 8, torch.bfloat16)
+    for i, row in enumerate(at):
+        x[row] = some[i].to(DEV)
+        slots[row] = 3 * i
+    pool = remnant.LatentPool(1, fmt="index", device=DEV)
+    pool.buffer.fill_(0x5A)
+    remnant.index_store_rows(x, torch.ones(KEY, device=DEV), 1e-6, slots, None, None, pool)
+    got = pool.layer().cpu().numpy()
+    del x, slots
+    torch.cuda.empty_cache()
+    assert np.array_equal(got, expect(some, np.arange(len(at)) * 3, 1))
+
+
 # ---- reader ----
 
 @pytest.mark.parametrize("queries,k", [(1, 1), (1, 700), (3, 37), (5, 5), (2, 20000), (70000, 1)])
