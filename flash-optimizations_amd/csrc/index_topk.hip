@@ -372,8 +372,7 @@ extern "C" int rm_index_topk(const float* scores, int64_t row_stride, const int3
   if (!counts || (width > 0 && !scores) || (k > 0 && !indices)) return RM_ERR_NULL;
   if (!aligned(scores, 4) || !aligned(lengths, 4) || !aligned(indices, 4) || !aligned(counts, 4))
     return RM_ERR_ALIGN;
-  const TopkArgs a{scores, row_stride, lengths, (int)width, (int)k,
-                   aligned(scores, 16) && (rows == 1 || row_stride % 4 == 0), indices, counts};
+  const bool wide = aligned(scores, 16) && (rows == 1 || row_stride % 4 == 0);
   // Threads: a wave's own work (scans, barriers) is most of a short row's, so that fewer are
   // better for short rows and, once the chip is full, for longer ones, as long as two keys a
   // thread reach k (one row of 4,096, k = 512: 4.7 us with half of the threads, 6.3 with all;
@@ -386,7 +385,16 @@ extern "C" int rm_index_topk(const float* scores, int64_t row_stride, const int3
                     : width <= 16384 ? index_topk_kernel<1024, 4, false>
                     : width <= 32768 ? index_topk_kernel<1024, 8, false>
                                      : index_topk_kernel<1024, 8, true>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(width <= 2048 ? 256 : half ? 512 : 1024), 0,
-                     (hipStream_t)stream, a);
-  return hipGetLastError() == hipSuccess ? RM_OK : RM_ERR_LAUNCH;
+  const int threads = width <= 2048 ? 256 : half ? 512 : 1024;
+  // A launch has fewer than 2^32 threads: with more the count wraps, without an error.
+  constexpr int64_t kLaunchRows = (int64_t)1 << 21;
+  for (int64_t at = 0; at < rows; at += kLaunchRows) {
+    const TopkArgs a{scores ? scores + at * row_stride : nullptr, row_stride,
+                     lengths ? lengths + at : nullptr, (int)width, (int)k, wide,
+                     indices ? indices + at * k : nullptr, counts + at};
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(rows - at, kLaunchRows)), dim3(threads), 0,
+                       (hipStream_t)stream, a);
+    if (hipGetLastError() != hipSuccess) return RM_ERR_LAUNCH;
+  }
+  return RM_OK;
 }

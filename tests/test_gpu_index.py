@@ -482,6 +482,15 @@ def test_topk_of_many_rows_and_no_rows():
     assert (idx == -1).all() and (counts == 0).all()
 
 
+def test_topk_of_more_rows_than_a_launch():
+    """2^24 rows of 256 threads are as many threads as a launch cannot have."""
+    banner("topk 2^24 + 5 rows")
+    rows = (1 << 24) + 5
+    x = torch.randn(rows, 2, device=DEV, generator=torch.Generator(DEV).manual_seed(6))
+    idx, counts = remnant.index_topk(x, None, 1)
+    assert torch.equal(idx[:, 0], (x[:, 1] > x[:, 0]).to(I32)) and (counts == 1).all()
+
+
 # ---- host cache ----
 
 def test_host_cache_round_trip():
