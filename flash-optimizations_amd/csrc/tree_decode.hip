@@ -149,6 +149,9 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi, float scale) 
 __device__ __forceinline__ float higher(float x, float y) {
   return __builtin_elementwise_maximum(x, y);
 }
+__device__ __forceinline__ float lower(float x, float y) {
+  return __builtin_elementwise_minimum(x, y);
+}
 // Over the four lanes that share lane % 16.
 __device__ __forceinline__ float over_groups(float x, bool is_max) {
   const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
@@ -420,8 +423,11 @@ struct Scorer : Tree {
     const uint64_t found = __ballot(bad != 0);
     return (uint32_t)(found | found >> 16 | found >> 32 | found >> 48) & 0xffffu;
   }
+  // False, before any weight or sum, for a whole unit that has to go by row: a row with an
+  // infinity can have a score of -inf, which would weigh nothing (and its infinity, taken by the
+  // adders, would make one coordinate NaN).
   template <bool kWhole>
-  __device__ __forceinline__ void score(const Unit& x, int round, const Rows& in) {
+  __device__ __forceinline__ bool score(const Unit& x, int round, const Rows& in) {
     const u32x2 bytes = in.bytes;
     // rows of the unit that count
     const int stop = min(x.past ? past - x.at : held + a->nodes - x.at, kUnit);
@@ -456,6 +462,13 @@ struct Scorer : Tree {
         acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, as_bf16x8(q[c][14 + t]), acc[c], 0, 0, 0);
     }
     // value i is row 4 group + i of the unit
+    if (kWhole) {
+      float least[2];  // (a NaN leaves its query row NaN, whatever the unit's others are)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        least[c] = lower(lower(acc[c][0], acc[c][1]), lower(acc[c][2], acc[c][3]));
+      if (__ballot((least[0] == -INFINITY) | (least[1] == -INFINITY)) != 0) return false;
+    }
     uint32_t odd = 0, gone = 0;  // rows with an infinity or NaN, and with those nobody sees
     if (!kWhole) {
       // (a row with an infinity or NaN has a score like it with any query row: without one
@@ -516,6 +529,7 @@ struct Scorer : Tree {
       const u32x2 d = {__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
       lds_write(weights_at(round, c), d);
     }
+    return true;
   }
   // The sums go on against `to`. (Equal references may both be infinite.)
   __device__ __forceinline__ void advance(int c, float to) {
@@ -559,15 +573,17 @@ struct Scorer : Tree {
       const int i = uniform(from + of);
       again();
       const u32x4 was = state(round - 1);
-      const Rows in = rows(round);
+      Rows in = rows(round);
       if (round > 0 && any_moved(was)) agree(round - 1, was);
       const Unit x = unit(min(i, units - 1), page);
       if (i + kUnits < end) page = page_of(i + kUnits);
       if (i < end) {
-        if (whole(x))
-          score<true>(x, round, in);
-        else
-          score<false>(x, round, in);
+        bool by_row = !whole(x);
+        if (!by_row && !score<true>(x, round, in)) {
+          by_row = true;
+          in = rows(round);
+        }
+        if (by_row) score<false>(x, round, in);
       } else {  // the round's last units: nothing
 #pragma unroll
         for (int c = 0; c < 2; ++c) lds_write(weights_at(round, c), u32x2{0, 0});

@@ -309,6 +309,44 @@ def test_whole_units_pass_nan_on():
         check((out[1:], lse[1:]), [x[1:] for x in want], how)
 
 
+def test_infinities_in_whole_units():
+    """An infinity that every node of a request sees, at rows of every unit: NaN for all of
+    the request's outputs and sums, whatever its sign and the query rows' (half of the
+    scores are -inf) and wherever the row lies in a unit; padding nodes stay zero, also
+    with NaN queries; the other requests stay as they are."""
+    banner("infinities seen by all")
+    parents = np.array([[-1, 0, 0, -2, 1]] * 3)
+    for window, past in ((None, 0), (None, 150), (128, 150)):
+        case = Tree(5, 16, batch=3, context=300, window=window, past=past, parents=parents, seed=21)
+        case.lengths[:] = 300
+        case.table = np.arange(15).reshape(3, 5)
+        case.pool = ref.random_native(15, 21)
+        want = case.want()
+        case.q[:, 3] = torch.nan
+        clean = [t.clone() for t in case.run()]
+        check(clean, want)
+        spots = [(case.pool, case.table, p) for p in ((180, 255, 285, 299) if window else
+                                                      (0, 70, 143, 160, 255, 287, 295, 299))]
+        if past:
+            case.past[2][:] = 150
+            case.past[1] = np.arange(9).reshape(3, 3)
+            case.past[0] = ref.random_native(9, 22)
+            want = case.want()
+            spots += [(case.past[0], case.past[1], p) for p in (0, 17, 100, 149)]
+        live = [0, 1, 2, 4]
+        for pool, table, p in spots:
+            for bits in (0x7F80, 0xFF80):
+                page, at = int(table[1, p // 64]), (p % 64) * 576 + 448 + 2 * (p % 64)
+                held = pool[page, at:at + 2].copy()
+                pool[page, at:at + 2] = np.array([bits], np.uint16).view(np.uint8)
+                out, lse = case.run()
+                where = (window, past, p, hex(bits))
+                assert torch.isnan(out[1, live]).all() and torch.isnan(lse[1, live]).all(), where
+                assert (out[1, 3] == 0).all() and torch.isfinite(lse[1, 3]).all(), where
+                check((out[::2], lse[::2]), [x[::2] for x in want], where)
+                pool[page, at:at + 2] = held
+
+
 @pytest.mark.parametrize("sigma", [2.0 ** -12, 2.0 ** 20, 2.0 ** 60])
 def test_small_and_large_rows(sigma):
     """Scales far from one: exponents of the weights, not values, carry them."""
