@@ -236,7 +236,9 @@ PyObject* store_rows(PyObject* const* v, Py_ssize_t count, const Format& format,
     freq_rows = freqs->numel() / ((RM_HEAD_DIM - RM_NOPE_DIM) / 2);
   }
   if (rows == 0 || (freqs && freq_rows == 0)) return none();
-  launch(one_device(x, &weight, &loc, positions, freqs, &pool.buffer), name, entry, x.const_data_ptr(), bf16 ? (int)RM_BF16 : (int)RM_F32, x.stride(0),
+  // (one row has no distance to a next one: whatever the tensor says)
+  launch(one_device(x, &weight, &loc, positions, freqs, &pool.buffer), name, entry,
+         x.const_data_ptr(), bf16 ? (int)RM_BF16 : (int)RM_F32, rows > 1 ? x.stride(0) : format.dim,
          (const float*)weight.const_data_ptr(), eps, i32(loc), i32(positions),
          freqs ? (const float*)freqs->const_data_ptr() : nullptr, freq_rows, ratio, rows, pool.at,
          pool.pages);

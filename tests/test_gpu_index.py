@@ -118,6 +118,20 @@ def test_store_special_rows():
                 assert np.array_equal(a, b, equal_nan=True), eps
 
 
+def test_store_of_one_row_of_any_stride():
+    """The distance to a next row is nobody's business where there is none."""
+    banner("store one row")
+    x = keys(1, 12)
+    wide = torch.zeros(3, 129, device=DEV)
+    wide[0, :KEY] = x[0].to(DEV)
+    want = expect(x, [5], 1)
+    for one in (x.to(DEV).t().contiguous().t(), wide[:1, :KEY], x.to(DEV).expand(4, KEY)[1:2]):
+        assert one.shape == (1, KEY)
+        assert np.array_equal(store(one, [5], 1), want), one.stride()
+        assert np.array_equal(store(one.bfloat16().as_strided((1, KEY), (1, 1)), [5], 1),
+                              expect(x.bfloat16(), [5], 1))
+
+
 def test_store_and_reader_past_4_gib():
     banner("store far slots")
     pages = 520000  # 4.4 GB
