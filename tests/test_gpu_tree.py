@@ -178,6 +178,26 @@ def test_many_tiles(nodes, heads):
     check(case.run(), case.want())
 
 
+@pytest.mark.parametrize("nodes, heads, batch", [(16, 16, 3), (63, 32, 3), (64, 32, 4), (40, 52, 3),
+                                                 (64, 128, 3), (60, 160, 2), (64, 300, 1)])
+def test_many_tiles_share_rounds(nodes, heads, batch):
+    """8, 63, 64, 65, 256, 300 and 600 tiles of query rows whose requests' rounds are dealt
+    out, to as many shares as there are for that many tiles (the last: one)."""
+    banner(f"{nodes} x {heads} x {batch}, rounds dealt out")
+    lengths = [1500, 0, 700, 90][:batch]
+    for case in (Ragged(lengths, nodes=nodes, heads=heads, seed=heads),
+                 Ragged(lengths, nodes=nodes, heads=heads, window=90, past=[900, 70, 0, 1200][:batch],
+                        seed=heads + 1)):
+        splits, need = remnant.get_tree_decode_metadata(
+            batch, nodes, heads, case.table.shape[1], window=case.window,
+            history_blocks=case.past[1].shape[1] if case.past else 0)
+        assert (splits > 1 and need > 0) or nodes * heads > 512 * 32
+        got = case.run()
+        check(got, case.want())
+        for a, b in zip(case.run(), got):
+            assert torch.equal(a, b)
+
+
 def test_padding_and_roots():
     """Padding by any number that is no parent, its descendants, trees of roots alone; a
     request without a live node."""
