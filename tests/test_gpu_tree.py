@@ -590,6 +590,66 @@ def test_graphs_replay_with_new_inputs():
                 assert torch.equal(a, b), turn
 
 
+def test_graphs_deal_by_the_lengths_of_the_replay():
+    """Two captured calls, each with a workspace of its own that holds anything before a
+    replay: lengths from none to the tables' capacity, so that a request is now finished by
+    one workgroup, now split over many."""
+    banner("graphs with other lengths")
+    batch, nodes, heads, columns = 3, 4, 16, 20
+    splits, need = remnant.get_tree_decode_metadata(batch, nodes, heads, columns, history_blocks=4)
+    assert splits > 1 and need > 0
+    rng = np.random.default_rng(7)
+    full = columns * 64 - nodes
+    turns = [([0, 0, 0], [0, 0, 0]), ([full, 1, 64], [0, 256, 3]), ([5, full, 700], [256] * 3),
+             ([full] * 3, [256, 0, 9]), ([64, 0, 3], [0] * 3), ([full + nodes, 900, 17], [1, 2, 3]),
+             ([0, 130, full], [0] * 3)]
+
+    def feed(seed, turn):
+        g = torch.Generator().manual_seed(100 * seed + turn)
+        lengths, past = turns[turn]
+        return [(torch.randn(batch, nodes, heads, 512, generator=g) * 0.5).bfloat16().to(DEV),
+                gpu(lengths, I32), gpu(random_parents(rng, batch, nodes), I32), gpu(past, I32)]
+
+    sides = []
+    for seed in range(2):
+        pool, old = ref.random_native(batch * columns, seed), ref.random_native(12, seed + 9)
+        table = rng.permutation(batch * columns).reshape(batch, columns)
+        past_table = rng.permutation(12).reshape(batch, 4)
+        sink = rng.standard_normal(heads).astype(np.float32)
+        on = [gpu(pool), gpu(table, I32), gpu(old), gpu(past_table, I32), gpu(sink)]
+
+        def call(q, lengths, parents, past, on=on, workspace=None):
+            return remnant.tree_decode_fwd(q, on[0], on[1], lengths, parents, history_pool=on[2],
+                                           history_table=on[3], history_lengths=past, sink=on[4],
+                                           workspace=workspace)
+
+        static, ws = feed(seed, 1), torch.empty(need, dtype=torch.uint8, device=DEV)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(*static, workspace=ws)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = call(*static, workspace=ws)
+        sides.append((seed, (pool, table, old, past_table, sink), call, static, ws, graph, outs))
+    for turn in range(len(turns)):
+        for seed, (pool, table, old, past_table, sink), call, static, ws, graph, outs in sides:
+            fresh = feed(seed, turn)
+            for s, f in zip(static, fresh):
+                s.copy_(f)
+            ws.fill_(0xFF)
+            graph.replay()
+            if turn % 2:
+                torch.cuda.synchronize()
+            eager = call(*fresh)
+            for a, b in zip(outs, eager):
+                assert torch.equal(a, b), turn
+            lengths, past = turns[turn]
+            check(outs, ref.tree(fresh[0].cpu(), pool, table, lengths, fresh[2].cpu().numpy(), None,
+                                 old, past_table, past, sink=sink), (turn, seed))
+
+
 def test_two_streams_at_once():
     banner("two streams")
     cases = [Tree(8, 16, batch=2, context=3000, seed=30), Tree(16, 8, context=300, past=500, seed=31)]
