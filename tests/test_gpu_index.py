@@ -303,6 +303,26 @@ def test_scores_of_more_tokens_than_a_grid_dimension():
     check_scores(got[torch.from_numpy(some).to(DEV)], want)
 
 
+@pytest.mark.parametrize("heads, q_len, batch, context", [
+    (128, 33, 2, 700), (65, 130, 1, 900),                             # eight tiles, tokens apart
+    (32, 5, 11, 20000), (24, 31, 2, 20000),                           # two tiles, four tokens a wave
+    (32, 67, 1, 20000), (17, 130, 1, 9000),                           # the same, apart
+    (1, 9, 6, 20000), (16, 31, 2, 20000), (16, 8, 7, 19999),          # one tile, eight tokens
+    (3, 35, 1, 31000), (64, 34, 1, 700), (40, 7, 3, 900)])
+def test_scores_of_many_tokens(heads, q_len, batch, context):
+    """Tokens that are no multiple of what a wave or workgroup takes, at sizes where those
+    take as many as they can; lengths that differ widely between the tokens of a wave, and
+    pages that are not mapped."""
+    banner(f"scores {heads} heads, {q_len} tokens of {batch} x {context}")
+    case = Scored(heads, context, batch=batch, q_len=q_len, seed=heads + q_len)
+    rng = np.random.default_rng(q_len)
+    case.lengths = np.where(rng.random(case.lengths.size) < 0.3,
+                            rng.integers(-2, context + 1, case.lengths.size), case.lengths)
+    case.lengths[0] = context
+    case.table[:, 1] = -1
+    check_scores(case.run(), case.want())
+
+
 @pytest.mark.parametrize("width", [1, 63, 65, 127, 200, 700])
 def test_scores_width(width):
     """Columns fewer than the table's records, more, and no whole pages; what stands
