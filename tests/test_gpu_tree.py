@@ -329,38 +329,42 @@ def test_whole_units_pass_nan_on():
         check((out[1:], lse[1:]), [x[1:] for x in want], how)
 
 
-def test_infinities_in_whole_units():
+@pytest.mark.parametrize("context, window, past, split", [
+    (300, None, 0, False), (300, None, 150, True), (300, 128, 150, False), (1300, None, 150, True)])
+def test_infinities_in_whole_units(context, window, past, split):
     """An infinity that every node of a request sees, at rows of every unit: NaN for all of
     the request's outputs and sums, whatever its sign and the query rows' (half of the
     scores are -inf) and wherever the row lies in a unit; padding nodes stay zero, also
     with NaN queries; the other requests stay as they are."""
-    banner("infinities seen by all")
+    banner(f"infinities seen by all, {context} committed, window {window}, history {past}")
     parents = np.array([[-1, 0, 0, -2, 1]] * 3)
-    for window, past in ((None, 0), (None, 150), (128, 150)):
-        case = Tree(5, 16, batch=3, context=300, window=window, past=past, parents=parents, seed=21)
-        case.lengths[:] = 300
-        case.table = np.arange(15).reshape(3, 5)
-        case.pool = ref.random_native(15, 21)
+    columns = (context + 5) // 64 + 1
+    case = Tree(5, 16, batch=3, context=context, window=window, past=past, parents=parents, seed=21)
+    case.lengths[:] = context
+    case.table = np.arange(3 * columns).reshape(3, columns)
+    case.pool = ref.random_native(3 * columns, 21)
+    if past:
+        case.past = [ref.random_native(9, 22), np.arange(9).reshape(3, 3), np.array([past] * 3)]
+    splits = remnant.get_tree_decode_metadata(3, 5, 16, columns, window=window,
+                                              history_blocks=3 if past else 0)[0]
+    assert (splits > 1) == split
+    spots = [(case.pool, case.table, p) for p in (0, 70, 143, 160, 180, 255, 285, 287, 295, 299, 640,
+                                                  1023, 1290)
+             if (context - 120 if window else 0) <= p < context]
+    if past:
+        spots += [(case.past[0], case.past[1], p) for p in (0, 17, 100, 149)]
+    live = [0, 1, 2, 4]
+    for filler in (1.0, torch.nan):
+        case.q[:, 3] = filler
         want = case.want()
-        case.q[:, 3] = torch.nan
-        clean = [t.clone() for t in case.run()]
-        check(clean, want)
-        spots = [(case.pool, case.table, p) for p in ((180, 255, 285, 299) if window else
-                                                      (0, 70, 143, 160, 255, 287, 295, 299))]
-        if past:
-            case.past[2][:] = 150
-            case.past[1] = np.arange(9).reshape(3, 3)
-            case.past[0] = ref.random_native(9, 22)
-            want = case.want()
-            spots += [(case.past[0], case.past[1], p) for p in (0, 17, 100, 149)]
-        live = [0, 1, 2, 4]
+        check(case.run(), want)
         for pool, table, p in spots:
             for bits in (0x7F80, 0xFF80):
                 page, at = int(table[1, p // 64]), (p % 64) * 576 + 448 + 2 * (p % 64)
                 held = pool[page, at:at + 2].copy()
                 pool[page, at:at + 2] = np.array([bits], np.uint16).view(np.uint8)
                 out, lse = case.run()
-                where = (window, past, p, hex(bits))
+                where = (filler, p, hex(bits))
                 assert torch.isnan(out[1, live]).all() and torch.isnan(lse[1, live]).all(), where
                 assert (out[1, 3] == 0).all() and torch.isfinite(lse[1, 3]).all(), where
                 check((out[::2], lse[::2]), [x[::2] for x in want], where)
