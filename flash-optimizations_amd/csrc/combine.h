@@ -213,12 +213,12 @@ void launch_combine(const float* ws_o, const float* ws_lse, const float* sink, i
   // 15.3 -> 13.1 us with it; 24 tokens, 8 splits: 16.8 with this form, 16.3 the other), but
   // not where most rows have fewer partials than slots
   const bool few = tokens * heads < 256 || (kNatural && !kRagged && slots > 8);
-  const auto kern =
-      few ? (slots <= 16   ? combine_kernel<4, kNatural, kRagged>
-             : slots <= 32 ? combine_kernel<8, kNatural, kRagged>
-                           : combine_kernel<16, kNatural, kRagged>)
-      : slots <= 4 || kRagged ? combine_wave_kernel<4, kNatural, kRagged>
-                              : combine_wave_kernel<8, kNatural, kRagged>;
+  const auto wave = slots <= 4 || kRagged ? combine_wave_kernel<4, kNatural, kRagged>
+                                          : combine_wave_kernel<kRagged ? 4 : 8, kNatural, kRagged>;
+  const auto kern = !few          ? wave
+                    : slots <= 16 ? combine_kernel<4, kNatural, kRagged>
+                    : slots <= 32 ? combine_kernel<8, kNatural, kRagged>
+                                  : combine_kernel<16, kNatural, kRagged>;
   const dim3 grid((unsigned)(few ? heads * kCombineSlices : (heads + 3) / 4),
                   (unsigned)(tokens / requests), (unsigned)requests);
   hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, ws_o, ws_lse, sink, slots, (int)heads, out, lse,
