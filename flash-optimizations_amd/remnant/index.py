@@ -49,8 +49,10 @@ def index_scores(q: torch.Tensor, weights: torch.Tensor, pool, block_table: torc
     ``q`` bfloat16 [batch, q_len, heads <= 128, 128], ``weights`` float32 [batch, q_len,
     heads]; ``lengths`` int32, an entry for each of the batch * q_len tokens: the records
     it may see, the first of its request's row of ``block_table``. Returns float32 [batch,
-    q_len, records]: sum over heads of weight times max(0, q . key), heads and keys both
-    as E4M3 with a scale a row, -inf past a token's length and where no page is mapped.
+    q_len, records]: the record's scale times the sum over heads of weight * scale of q *
+    max(0, codes of q . codes of the key), heads being coded as the store codes a key; for
+    scales above zero, as the store's, that is the sum of weight * max(0, q . key) of the
+    coded values. -inf past a token's length and where no page is mapped.
     ``out`` sets the number of records (without it the block table's capacity). A scale
     that belongs in the scores goes into ``weights``."""
     return _lib.ops().scores(q, weights, pool, block_table, lengths, out, layer_id)
