@@ -19,11 +19,11 @@
 // the lane; the four lanes of a record meet once a page, where record l of the page ends in
 // lane l and its scale, score and store are one access a wave.
 //
-// Bound by the matrix instructions and by memory alike from two tokens and 64 heads on
-// (128 requests of 2 tokens and 32,768 records: 145 us; 108 for the bytes at 5.1 TB/s, 115
-// for the products at 1,189 TFLOP/s, what a large product reaches), by the products alone
-// for many tokens (512 tokens, 35,840 records: 230 us, 1,310 TFLOP/s), by memory and its
-// latency for one (64 ragged requests 24 us, 17 for the bytes).
+// Bound by the products for many tokens (512 tokens, 35,840 records: 231 us, 1,310 TFLOP/s; a
+// large library product reaches 1,189), by the matrix instructions and by memory alike for
+// two tokens of 64 heads (128 requests of 32,768 records: 145 us; 108 for the bytes at 5.1 TB/s,
+// 105 for the products at 1,310 TFLOP/s), by memory and its latency for one (64 ragged
+// requests 24 us, 17 for the bytes).
 #include <algorithm>
 
 #include "index_device.h"
@@ -107,8 +107,12 @@ __device__ __forceinline__ Heads coded(const ScoreArgs& a, int64_t token, int h,
 // kTiles x 16 heads, kTokens tokens a wave. kApart: the waves of a workgroup take
 // different tokens and the same pages; otherwise the same tokens and pages in turn, and
 // each codes some of the heads for all.
+constexpr int waves_a_simd(int tiles, int tokens) {
+  return tiles * tokens >= 8 ? 2 : tiles >= 4 ? 3 : tokens >= 2 ? 2 : 4;
+}
 template <int kTiles, int kTokens, bool kApart>
-__global__ __launch_bounds__(64 * kWaves, kTiles * kTokens >= 8 ? 2 : kTiles >= 4 ? 3 : kTokens >= 2 ? 2 : 4) void index_scores_kernel(ScoreArgs a) {
+__global__ __launch_bounds__(64 * kWaves, waves_a_simd(kTiles, kTokens)) void index_scores_kernel(
+    ScoreArgs a) {
   constexpr int kShared = kApart ? 1 : kTokens * kTiles;
   __shared__ u32x4 coded_heads[kShared][4][64];
   // (weights stay there: 2 x 64 heads and theirs in registers would spill)

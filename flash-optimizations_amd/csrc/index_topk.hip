@@ -11,9 +11,11 @@
 // of their leading bits. A wave's scores stand together, so that each wave knows its places
 // from one count a wave; numbers are put in order in LDS and written side by side.
 //
-// Bound by vector operations, about thirty a key of which seven make it and find the range
-// while the row comes (256 rows of 32,768: 16.1 us, of which 3.3 are loads; 64 such ragged
-// rows 11.5, on 64 of 256 CUs; one of 8,192 6.0, a launch and six barriers).
+// Bound by one workgroup a CU, whose phases wait for each other: loads, then about thirty vector
+// operations a key (seven make it and find the range while the row comes) in passes with a
+// barrier between them. Vector instructions are issued in half of the busy cycles (256 rows of
+// 32,768: 16.2 us, 512 rows 30.3; 512 of 35,840 39.3; 64 ragged rows of up to 32,768 11.5, on 64
+// of 256 CUs; one of 8,192 6.0, a launch and six barriers).
 #include <algorithm>
 
 #include "remnant_device.h"
@@ -80,7 +82,7 @@ __device__ __forceinline__ uint32_t below(uint64_t mask, uint32_t plus) {
 // width, as a turn more is code to fetch and keys to make (1,430 rows of 16,384: 35 us with
 // four turns, 65 with eight). kLong: longer rows, with kInLds turns in LDS and what is longer
 // still read again for each pass (64 rows of 65,536 23.6 us, 38.4 when each pass read them;
-// 256 rows of 32,768 18.1 from registers and 24.5 read).
+// 256 rows of 32,768 then 6.4 us more when each pass read them).
 constexpr int kInLds = 8;
 template <int kThreads, int kHeld, bool kLong>
 __global__ __launch_bounds__(kThreads) void index_topk_kernel(TopkArgs a) {

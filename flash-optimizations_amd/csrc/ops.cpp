@@ -1,7 +1,7 @@
 // Argument checks and launches of the 4-bit and index operators, the tree attention and
-// the slot maps, for remnant/mx4.py, index.py, tree.py and slots.py (module remnant_ops). Small calls are bound by
-// the host: a launch takes 3.2 us, and the same checks in Python, with ctypes, took 4 to
-// 8 more (a call of a window list 8.2 us, 6.1 here; the slot map of a step 10.0 and 6.3;
+// the slot maps, for remnant/mx4.py, index.py, tree.py and slots.py (module remnant_ops).
+// Small calls are bound by the host: a launch takes 3.2 us, and the same checks in Python,
+// with ctypes, took 4 to 8 more (a call of a window list 8.2 us, 6.1 here; the slot map of a step 10.0 and 6.3;
 // a decode of one launch with window rows 12.4 and 6.8, of two launches 14.6 and 9.3).
 // Shape and type mistakes raise ValueError before anything is launched (TypeError where a
 // tensor or a number is something else altogether); work goes to the current stream of the

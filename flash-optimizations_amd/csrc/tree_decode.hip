@@ -28,16 +28,19 @@
 // takes its own for that round. After it the scorers go on from the highest of the units',
 // and the adders lower that round's weights (integer subtractions on their exponents) and O.
 // The output is divided by the sum of the weights as they were rounded, and lse takes the
-// sum of the exact ones: roundings that a row's weights have in common cancel.
+// sum of the exact ones: roundings that a row's weights have in common cancel. The weights are
+// the one thing held in fewer bits, as the matrix instruction takes them: outputs are up to
+// 0.0020 off, 0.0017 by their own rounding to BF16.
 //
 // LDS holds a row's 36 pieces of 16 bytes in a row, with the order in each four of them
 // turned by the row's number (the copies choose their source), so that eight lanes reading
 // one piece of eight rows meet every bank once.
 //
-// Bound by vector issue beside the matrix pipes: a round is 1,024 cycles of matrix
-// instructions a SIMD and about 1,600 of vector ones (480 convert codes), and takes 1.35 us
-// (16 requests of 256 query rows, 4,096 to 16,384 records: 117 us, 640 TFLOP/s; a large
-// product reaches 1,189). 32 query rows, as the queries and outputs of more do not fit the
+// Bound by the two roles' waits for each other, one barrier a round: a round is 1,024 cycles of
+// matrix instructions a SIMD and about 1,600 of vector ones (480 convert codes), and takes
+// 1.35 us, some 3,200 cycles; vector issue takes 49 % of all cycles, the matrix pipes are
+// busy in 32 % (16 requests of 256 query rows, 4,096 to 16,384 records: 117 us, 640 TFLOP/s; a
+// large product reaches 1,189). 32 query rows, as the queries and outputs of more do not fit the
 // registers of two waves a SIMD; 64 rows a round, as four rounds fill LDS. Small calls are
 // their start and end: 8 x 16 query rows over 8,192 records take 18.4 us, of which three
 // rounds are 4, the combine 4 and the launches 5.
@@ -86,8 +89,8 @@ constexpr int kStartsAt = kSumsAt + kUnits * kRows * 8;  // [requests + 1]
 constexpr int kQueriesAt = 3 * kRoundBytes;  // before a piece's fourth round is copied
 constexpr int kMaxShared = 256;   // requests whose rounds are dealt out evenly
 constexpr int kLdsBytes = kStartsAt + (kMaxShared + 1) * 4;
-// What a piece costs beyond its rounds, in rounds (about 7 us of 1.35; window trees 36.8 us
-// with two, 35.3 with four, 34.6 with six, large ones the same).
+// What a piece costs beyond its rounds, in rounds (about 8 us at 1.35 a round; window trees
+// 36.8 us with two, 35.3 with four, 34.6 with six, large ones the same).
 constexpr int kOverhead = 6;
 static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 constexpr uint32_t kMoved = 1u << 16;  // the unit took references of its own

@@ -233,7 +233,8 @@ int rm_packed_to_native_planes(const uint8_t* values, const uint64_t* bitmaps,
  * Packed record (codes, bitmap and scales together; format RM_FORMAT_PACKED
  * with its keep_count) or the Native data row and scale row
  * (RM_FORMAT_NATIVE) or the 4-bit record (RM_FORMAT_MX4) or the index row and its
- * scale (RM_FORMAT_INDEX); keep_count is looked at for Packed records alone. Pairs with a slot < 0 or beyond its pool are skipped.
+ * scale (RM_FORMAT_INDEX); keep_count is looked at for Packed records alone. Pairs with a
+ * slot < 0 or beyond its pool are skipped.
  * Layer l of a pool starts l * layer_bytes after its base. Either pool may be
  * device memory or pinned host memory (hipHostMalloc). 8-byte alignment. */
 int rm_copy_records(const uint8_t* src, int64_t src_pages, int64_t src_layer_bytes,
